@@ -7,12 +7,14 @@
  * the host before anything was launched. No exceptions cross this boundary. Per-row run-time conditions
  * (all-masked row, candidate overflow, draw within tolerance of a boundary) are reported in device `flags`.
  *
- * Two groups of entry points:
+ * Three groups of entry points:
  *  (1) one launcher per reference kernel, same argument order and output layout as the kernel the reference
  *      resolves by name (citations at each declaration), with the launch geometry chosen here;
  *      the gfx950 code object whirl_sampling_gfx950.co exports the same `extern "C" __global__` names for callers
  *      that use hipModuleGetFunction (block = 1024 threads, grid = rows, no dynamic LDS);
- *  (2) the batched fused sampler and the classic speculative verify, which the reference does not have.
+ *  (2) the batched fused sampler and the classic speculative verify, which the reference does not have;
+ *  (3) log-probabilities of the tokens a model answered with, and the losses that train it on them, forwards and backwards,
+ *      which the reference does not have either.
  */
 #ifndef WHIRL_SAMPLING_ABI_H
 #define WHIRL_SAMPLING_ABI_H
@@ -539,6 +541,102 @@ typedef struct ws_spec_verify {
 
 uint64_t ws_spec_verify_workspace(const ws_spec_verify* v);
 int ws_spec_verify_classic(void* stream, const ws_spec_verify* v);
+
+/* ---- (3) log-probabilities of answered tokens, losses over them ------------------------------------------- */
+
+/* Rows of logits, each with a token it answered with (a sampled one, a given one), and what was applied to the logits when it was drawn:
+ * temperature and allow mask, as in ws_batch (penalties and bias: ws_adjust_rows first). With m = max x_v over the allowed tokens,
+ * S = sum exp((x_v - m) * inv_t) and p_v = exp((x_v - m) * inv_t) / S:
+ *   logprob = (x_y - m) * inv_t - ln S of the row's token y,    entropy = -sum p_v ln p_v.
+ * A row whose token id lies outside [0, vocab) - -1 by custom - has no token: its logprob is 0 and nothing is derived from it.
+ * Logits that are not allowed count as -inf, whatever they hold. A row where nothing is left (every allowed logit -inf, or none
+ * allowed) has stats {-inf, 0}, entropy 0 and, if it has a token, logprob -inf, and its derivatives are 0. A token that is not allowed
+ * has logprob -inf and its row the derivatives of the others. An allowed logit of +inf or NaN, or an inv_t that is
+ * not a positive finite number, makes everything of its row NaN. Results are the same bits on every run.
+ * rows and vocab: at most 1048575 each. */
+typedef struct ws_loss_rows {
+    const void* logits; /* device, [rows][row_stride] of dtype, aligned to its elements */
+    int32_t dtype;      /* WS_DTYPE_* */
+    uint32_t rows;      /* 0: nothing is launched but what an empty sum takes */
+    uint32_t vocab;
+    uint64_t row_stride;    /* elements between rows (>= vocab) */
+    const int32_t* ids;     /* device [rows] (NULL: no row has a token) */
+    const float* inv_t;     /* device [rows], 1 / temperature (NULL: 1) */
+    const uint32_t* allow;  /* bitmap as in ws_batch (NULL: all) */
+    uint64_t allow_stride;  /* 32-bit words between rows (>= (vocab + 31) / 32) */
+} ws_loss_rows;
+
+/* Log-probabilities and entropies. stats[row] = {m, S}, the layout of ws_batch.stats: what ws_token_logprobs_grad needs of the forward
+ * pass. workspace: device memory of ws_token_logprobs_workspace() bytes (0: none is needed), 8-byte aligned, of any
+ * contents, nobody else's until the launch is done (few rows are shared by up to 64 workgroups each, which meet there; a captured
+ * launch may be replayed). Without it every row is one workgroup's: slower, the sums in another order. */
+uint64_t ws_token_logprobs_workspace(const ws_loss_rows* r, int want_entropy);
+int ws_token_logprobs(void* stream, const ws_loss_rows* r, float* logprob, float* stats, float* entropy /* may be NULL */, void* workspace,
+                      uint64_t workspace_bytes);
+
+/* Their gradient: with g = d_logprob[row] (NULL: 0; a row without a token: 0) and h = d_entropy[row] (NULL: 0) the derivatives of some loss by
+ * the row's logprob and entropy, d_logits[row][v] = inv_t * (g * (1[v = y] - p_v) - h * p_v * (ln p_v + entropy[row])), in the
+ * logits' dtype. stats, entropy: what ws_token_logprobs wrote (entropy only with d_entropy). A row with g = h = 0 is not read and
+ * gets zeros. d_logits: [rows][d_stride], the first vocab of a row are written; it may be the logits themselves (same address and stride), but not
+ * overlap them otherwise. */
+int ws_token_logprobs_grad(void* stream, const ws_loss_rows* r, const float* stats, const float* d_logprob, const float* entropy,
+                           const float* d_entropy, void* d_logits, uint64_t d_stride);
+
+/* The clipped policy loss with a KL term and an entropy bonus. Per token, with ratio = exp(logprob - old_logprob) and advantage A:
+ *   gain = min(ratio * A, clip(ratio, 1 - clip_low, 1 + clip_high) * A), and with dual_clip and A < 0 at least dual_clip * A;
+ *   kl   = exp(ref - logprob) - (ref - logprob) - 1;
+ *   loss = sum of weight * (-gain + kl_coef * kl - entropy_coef * entropy).
+ * A token of weight 0 counts for nothing, whatever its other entries hold. Where the clip holds the gain, it has no derivative. */
+typedef struct ws_policy {
+    const float* old_logprob; /* device [rows]: of the model that drew the tokens */
+    const float* ref_logprob; /* device [rows] (NULL: no KL term, kl_coef must be 0) */
+    const float* advantage;   /* device [rows] */
+    const float* weight;      /* device [rows] (NULL: 1 / rows each) */
+    double clip_low;          /* 0 .. 1 */
+    double clip_high;         /* >= 0 */
+    double dual_clip;         /* 0: off; else > 1 */
+    double kl_coef;
+    double entropy_coef;
+} ws_policy;
+/* sums: loss, sum of weight * -gain, of weight * kl, of weight * entropy, and the weight of the tokens whose gain a clip holds */
+enum { WS_POLICY_LOSS = 0, WS_POLICY_SURROGATE = 1, WS_POLICY_KL = 2, WS_POLICY_ENTROPY = 3, WS_POLICY_CLIPPED = 4, WS_POLICY_SUMS = 5 };
+
+/* The loss over log-probabilities the caller has, and its derivatives by them. entropy: device [rows] (NULL: none, entropy_coef must be 0);
+ * d_entropy may be NULL. workspace as above, of ws_policy_loss_workspace() bytes; required where that is not 0. */
+uint64_t ws_policy_loss_workspace(uint32_t rows);
+int ws_policy_loss(void* stream, uint32_t rows, const ws_policy* p, const float* logprob, const float* entropy, float* sums, float* d_logprob,
+                   float* d_entropy, void* workspace, uint64_t workspace_bytes);
+
+/* The loss from the logits, and its gradient by them: what ws_token_logprobs, ws_policy_loss and ws_token_logprobs_grad do together,
+ * with a row read once where the registers hold it. Rows without a token and rows of weight 0 count for nothing: they are not read, their
+ * logprob and entropy are 0, their gradient is zero. Without `weight` every row weighs 1 / rows, those without a token too. entropy: out (may be
+ * NULL, entropy_coef must be 0 then). d_logits as in ws_token_logprobs_grad. workspace as above, of
+ * ws_policy_loss_rows_workspace() bytes; required. */
+uint64_t ws_policy_loss_rows_workspace(const ws_loss_rows* r, const ws_policy* p, int want_entropy);
+int ws_policy_loss_rows(void* stream, const ws_loss_rows* r, const ws_policy* p, float* sums, float* logprob, float* entropy, void* d_logits,
+                        uint64_t d_stride, void* workspace, uint64_t workspace_bytes);
+
+/* The loss of paired log ratios: answers 2 p (preferred) and 2 p + 1 of pair p are the rows seq_off[2 p] .. seq_off[2 p + 1] and
+ * seq_off[2 p + 1] .. seq_off[2 p + 2]; with s their sums of logprob - ref_logprob and h = beta * (s_preferred - s_other)
+ *   pair_loss = (1 - label_smoothing) * ln(1 + exp(-h)) + label_smoothing * ln(1 + exp(h)),    loss = sum of weight * pair_loss,
+ * reward[p] = beta * s of the two. Answers may be empty. seq_off ascends; offsets beyond `rows` end there. d_logprob is written for all rows, 0 for those
+ * of no answer. A pair of weight 0 counts for nothing. workspace as above, of ws_preference_loss_workspace() bytes; required where that is
+ * not 0. */
+typedef struct ws_preference {
+    uint32_t rows, pairs;
+    const uint32_t* seq_off;  /* device [2 * pairs + 1] */
+    const float* logprob;     /* device [rows] */
+    const float* ref_logprob; /* device [rows] (NULL: 0) */
+    const float* weight;      /* device [pairs] (NULL: 1 / pairs each) */
+    double beta;
+    double label_smoothing; /* 0 .. 1 */
+    float* loss;            /* out, device [1] */
+    float* pair_loss;       /* out, device [pairs] */
+    float* reward;          /* out, device [pairs][2] */
+    float* d_logprob;       /* out, device [rows] */
+} ws_preference;
+uint64_t ws_preference_loss_workspace(uint32_t pairs);
+int ws_preference_loss(void* stream, const ws_preference* p, void* workspace, uint64_t workspace_bytes);
 
 #ifdef __cplusplus
 }

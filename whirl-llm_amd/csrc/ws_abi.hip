@@ -12,6 +12,7 @@
 #include "ws_adjust.h"
 #include "ws_common.h"
 #include "ws_draft.h"
+#include "ws_loss.h"
 #include "ws_pick.h"
 #include "ws_sample.h"
 #include "ws_spec.h"
@@ -59,6 +60,14 @@ int launch_draft_shared(hipStream_t stream, const float* x, int n, int* ctl_all,
 int launch_argmax_shared(hipStream_t stream, int mode, const float* x, int n, int* out, const void* dst, int* ids, int* pos, int advance, unsigned rows,
                          unsigned parts, unsigned long long* scratch, unsigned long long tag);
 int prepare_top();
+// ws_loss.hip: log-probabilities, losses over them and their gradients
+int launch_score(hipStream_t stream, int dtype, const ScoreArgs& a, bool policy);
+int launch_grad(hipStream_t stream, int dtype, const GradArgs& a);
+int launch_policy_rows(hipStream_t stream, int dtype, const RowsArgs& b, bool slope);
+int launch_policy(hipStream_t stream, const PolicyArgs& a, unsigned groups);
+int launch_preference(hipStream_t stream, const PreferenceArgs& a, unsigned groups);
+uint32_t loss_threads();
+uint32_t loss_grad_chunks(int dtype, uint32_t vocab);
 }  // namespace ws
 
 namespace {
@@ -1069,5 +1078,208 @@ int ws_history_stage(void* stream, const ws_history_stage_args* b) {
 uint64_t ws_spec_verify_workspace(const ws_spec_verify* v) { return ws::spec_workspace(v, compute_units()); }
 
 int ws_spec_verify_classic(void* stream, const ws_spec_verify* v) { return ws::spec_launch(S(stream), v, compute_units()); }
+
+// ---- log-probabilities, losses over them
+namespace {
+constexpr uint32_t kMostLossRows = 1048575u;
+
+uint64_t elem_bytes(int dtype) { return dtype == WS_DTYPE_F32 ? 4u : 2u; }
+bool aligned(const void* p, uint64_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+bool loss_rows_ok(const ws_loss_rows* r) {
+    if (!r || (r->dtype != WS_DTYPE_F32 && r->dtype != WS_DTYPE_BF16) || r->vocab == 0 || r->vocab > 1048575u || r->rows > kMostLossRows) return false;
+    if (r->rows && (!r->logits || !aligned(r->logits, elem_bytes(r->dtype)))) return false;
+    if (r->row_stride < r->vocab || (r->allow && r->allow_stride < (r->vocab + 31u) / 32u)) return false;
+    return true;
+}
+// bytes from a matrix's first element to behind its last
+uint64_t extent(uint32_t rows, uint32_t vocab, uint64_t stride, uint64_t each) { return rows ? ((rows - 1u) * stride + vocab) * each : 0u; }
+// d_logits: the logits themselves, or memory of its own
+bool gradient_ok(const ws_loss_rows* r, const void* d, uint64_t stride) {
+    if (!r->rows) return true;
+    const uint64_t e = elem_bytes(r->dtype);
+    if (!d || !aligned(d, e) || stride < r->vocab) return false;
+    if (d == r->logits && stride == r->row_stride) return true;
+    const uintptr_t a = reinterpret_cast<uintptr_t>(r->logits), b = reinterpret_cast<uintptr_t>(d);
+    return a + extent(r->rows, r->vocab, r->row_stride, e) <= b || b + extent(r->rows, r->vocab, stride, e) <= a;
+}
+ws::LossRows loss_rows(const ws_loss_rows* r) {
+    return ws::LossRows{static_cast<const unsigned char*>(r->logits), r->row_stride * elem_bytes(r->dtype), r->rows, r->vocab, r->ids, r->inv_t, r->allow, r->allow_stride};
+}
+// workgroups a row of the log-probabilities: some four a compute unit, each with two vectors a thread at least
+uint32_t score_parts(const ws_loss_rows* r) {
+    const uint32_t want = 4u * static_cast<uint32_t>(compute_units()), vectors = r->vocab / (r->dtype == WS_DTYPE_F32 ? 4u : 8u);
+    uint32_t parts = r->rows ? want / r->rows : 1u;
+    const uint32_t most = vectors / (2u * ws::loss_threads());
+    if (parts > most) parts = most;
+    return parts < 2u ? 1u : (parts > 64u ? 64u : parts);
+}
+uint64_t meet_bytes(uint32_t rows, uint32_t parts, bool entropy) { return parts > 1u ? uint64_t{rows} * parts * (entropy ? 32u : 16u) : 0u; }
+bool workspace_ok(const void* w, uint64_t bytes, uint64_t need) { return need == 0 || (w && bytes >= need && aligned(w, 8u)); }
+
+bool policy_ok(const ws_policy* p, uint32_t rows, bool entropy) {
+    if (!p || (rows && (!p->old_logprob || !p->advantage))) return false;
+    if (!(p->clip_low >= 0.0 && p->clip_low <= 1.0) || !(p->clip_high >= 0.0) || !(p->dual_clip == 0.0 || p->dual_clip > 1.0)) return false;
+    return p->kl_coef == p->kl_coef && p->entropy_coef == p->entropy_coef && (p->ref_logprob || p->kl_coef == 0.0) && (entropy || p->entropy_coef == 0.0);
+}
+ws::PolicyIn policy_in(const ws_policy* p, uint32_t rows) {
+    return ws::PolicyIn{p->old_logprob, p->ref_logprob, p->advantage, p->weight, rows ? 1.0 / rows : 0.0, p->clip_low, p->clip_high, p->dual_clip, p->kl_coef, p->entropy_coef};
+}
+// workgroups of a sum over tokens
+uint32_t policy_groups(uint32_t rows) {
+    const uint32_t n = (rows + 511u) / 512u;
+    return n < 1u ? 1u : (n > 64u ? 64u : n);
+}
+uint64_t policy_meet_bytes(uint32_t rows) { return policy_groups(rows) > 1u ? uint64_t{policy_groups(rows)} * ws::kPolicySums * 16u : 0u; }
+uint32_t preference_groups(uint32_t pairs) { return pairs > 256u ? 256u : pairs; }
+
+// the workspace of ws_policy_loss_rows, in this order: the rows' terms, meeting places, and for rows of two launches stats and derivatives
+struct RowsPlan {
+    bool held;  // one launch, a workgroup a row
+    uint32_t parts;
+    uint64_t terms, sums_meet, meet, stats, d_logprob, d_entropy, bytes;
+};
+RowsPlan rows_plan(const ws_loss_rows* r, const ws_policy* p, bool entropy) {
+    RowsPlan n{};
+    n.held = 2u * r->rows >= static_cast<uint32_t>(compute_units());
+    n.parts = n.held ? 1u : score_parts(r);
+    n.sums_meet = uint64_t{r->rows} * ws::kPolicySums * 8u;
+    n.meet = n.sums_meet + policy_meet_bytes(r->rows);
+    n.stats = n.meet + meet_bytes(r->rows, n.parts, entropy);
+    n.d_logprob = n.stats + (n.held ? 0u : uint64_t{r->rows} * 8u);
+    n.d_entropy = n.d_logprob + (n.held ? 0u : uint64_t{r->rows} * 4u);
+    n.bytes = n.d_entropy + (n.held || p->entropy_coef == 0.0 ? 0u : uint64_t{r->rows} * 4u);
+    return n;
+}
+int grad_on(void* stream, const ws_loss_rows* r, const float* stats, const float* d_logprob, const float* entropy, const float* d_entropy, void* d_logits, uint64_t d_stride) {
+    ws::GradArgs a{};
+    a.R = loss_rows(r);
+    a.stats = stats;
+    a.entropy = entropy;
+    a.d_logprob = d_logprob;
+    a.d_entropy = d_entropy;
+    a.out = static_cast<unsigned char*>(d_logits);
+    a.out_bytes = d_stride * elem_bytes(r->dtype);
+    a.chunks = ws::loss_grad_chunks(r->dtype, r->vocab);
+    if (uint64_t{r->rows} * a.chunks * ws::loss_threads() >= uint64_t{1} << 32) return WS_E_UNSUPPORTED;  // (more than a launch has threads)
+    return ws::launch_grad(S(stream), r->dtype, a);
+}
+}  // namespace
+
+uint64_t ws_token_logprobs_workspace(const ws_loss_rows* r, int want_entropy) { return loss_rows_ok(r) ? meet_bytes(r->rows, score_parts(r), want_entropy != 0) : 0u; }
+
+int ws_token_logprobs(void* stream, const ws_loss_rows* r, float* logprob, float* stats, float* entropy, void* workspace, uint64_t workspace_bytes) {
+    if (!loss_rows_ok(r)) return WS_E_INVALID;
+    if (r->rows == 0) return WS_OK;
+    if (!logprob || !stats) return WS_E_INVALID;
+    ws::ScoreArgs a{};
+    a.R = loss_rows(r);
+    a.logprob = logprob;
+    a.stats = stats;
+    a.entropy = entropy;
+    a.parts = score_parts(r);
+    if (a.parts > 1u) {
+        if (workspace && workspace_ok(workspace, workspace_bytes, meet_bytes(r->rows, a.parts, entropy != nullptr))) {
+            a.meet = static_cast<unsigned long long*>(workspace);
+            a.tag = launch_tag();
+        } else {
+            a.parts = 1u;
+        }
+    }
+    return ws::launch_score(S(stream), r->dtype, a, false);
+}
+
+int ws_token_logprobs_grad(void* stream, const ws_loss_rows* r, const float* stats, const float* d_logprob, const float* entropy, const float* d_entropy, void* d_logits,
+                           uint64_t d_stride) {
+    if (!loss_rows_ok(r) || !gradient_ok(r, d_logits, d_stride)) return WS_E_INVALID;
+    if (r->rows == 0) return WS_OK;
+    if (!stats || (d_entropy && !entropy)) return WS_E_INVALID;
+    return grad_on(stream, r, stats, d_logprob, entropy, d_entropy, d_logits, d_stride);
+}
+
+uint64_t ws_policy_loss_workspace(uint32_t rows) { return policy_meet_bytes(rows); }
+
+int ws_policy_loss(void* stream, uint32_t rows, const ws_policy* p, const float* logprob, const float* entropy, float* sums, float* d_logprob, float* d_entropy, void* workspace,
+                   uint64_t workspace_bytes) {
+    if (!policy_ok(p, rows, entropy != nullptr) || !sums || (rows && (!logprob || !d_logprob)) || rows > (1u << 30)) return WS_E_INVALID;
+    if (!workspace_ok(workspace, workspace_bytes, policy_meet_bytes(rows))) return WS_E_WORKSPACE;
+    ws::PolicyArgs a{};
+    a.P = policy_in(p, rows);
+    a.rows = rows;
+    a.logprob = logprob;
+    a.entropy = entropy;
+    a.d_logprob = d_logprob;
+    a.d_entropy = d_entropy;
+    a.sums = sums;
+    a.meet = static_cast<unsigned long long*>(workspace);
+    a.tag = launch_tag();
+    return ws::launch_policy(S(stream), a, policy_groups(rows));
+}
+
+uint64_t ws_policy_loss_rows_workspace(const ws_loss_rows* r, const ws_policy* p, int want_entropy) {
+    return loss_rows_ok(r) && p ? rows_plan(r, p, want_entropy != 0).bytes : 0u;
+}
+
+int ws_policy_loss_rows(void* stream, const ws_loss_rows* r, const ws_policy* p, float* sums, float* logprob, float* entropy, void* d_logits, uint64_t d_stride, void* workspace,
+                        uint64_t workspace_bytes) {
+    if (!loss_rows_ok(r) || !policy_ok(p, r->rows, entropy != nullptr) || !gradient_ok(r, d_logits, d_stride) || !sums) return WS_E_INVALID;
+    if (r->rows && (!r->ids || !logprob)) return WS_E_INVALID;
+    const RowsPlan n = rows_plan(r, p, entropy != nullptr);
+    if (!workspace_ok(workspace, workspace_bytes, n.bytes)) return WS_E_WORKSPACE;
+    unsigned char* work = static_cast<unsigned char*>(workspace);
+    if (r->rows) {
+        ws::ScoreArgs a{};
+        a.R = loss_rows(r);
+        a.logprob = logprob;
+        a.entropy = entropy;
+        a.parts = n.parts;
+        a.P = policy_in(p, r->rows);
+        a.terms = reinterpret_cast<double*>(work);
+        if (n.held) {
+            if (const int e = ws::launch_policy_rows(S(stream), r->dtype, ws::RowsArgs{a, static_cast<unsigned char*>(d_logits), d_stride * elem_bytes(r->dtype)}, p->entropy_coef != 0.0); e != 0)
+                return e;
+        } else {
+            a.stats = reinterpret_cast<float*>(work + n.stats);
+            a.d_logprob = reinterpret_cast<float*>(work + n.d_logprob);
+            a.d_entropy = p->entropy_coef != 0.0 ? reinterpret_cast<float*>(work + n.d_entropy) : nullptr;
+            a.meet = reinterpret_cast<unsigned long long*>(work + n.meet);
+            a.tag = launch_tag();
+            if (const int e = ws::launch_score(S(stream), r->dtype, a, true); e != 0) return e;
+            if (const int e = grad_on(stream, r, a.stats, a.d_logprob, entropy, a.d_entropy, d_logits, d_stride); e != 0) return e;
+        }
+    }
+    ws::PolicyArgs a{};
+    a.rows = r->rows;
+    a.terms = reinterpret_cast<const double*>(work);
+    a.sums = sums;
+    a.meet = reinterpret_cast<unsigned long long*>(work + n.sums_meet);
+    a.tag = launch_tag();
+    return ws::launch_policy(S(stream), a, policy_groups(r->rows));
+}
+
+uint64_t ws_preference_loss_workspace(uint32_t pairs) { return preference_groups(pairs) > 1u ? uint64_t{preference_groups(pairs)} * 16u : 0u; }
+
+int ws_preference_loss(void* stream, const ws_preference* p, void* workspace, uint64_t workspace_bytes) {
+    if (!p || p->pairs == 0 || p->pairs > (1u << 30) || p->rows > (1u << 30) || !p->seq_off || !p->loss || !p->pair_loss || !p->reward) return WS_E_INVALID;
+    if ((p->rows && (!p->logprob || !p->d_logprob)) || p->beta != p->beta || !(p->label_smoothing >= 0.0 && p->label_smoothing <= 1.0)) return WS_E_INVALID;
+    if (!workspace_ok(workspace, workspace_bytes, ws_preference_loss_workspace(p->pairs))) return WS_E_WORKSPACE;
+    ws::PreferenceArgs a{};
+    a.rows = p->rows;
+    a.pairs = p->pairs;
+    a.seq_off = p->seq_off;
+    a.logprob = p->logprob;
+    a.ref_logprob = p->ref_logprob;
+    a.weight = p->weight;
+    a.weight_all = 1.0 / p->pairs;
+    a.beta = p->beta;
+    a.smoothing = p->label_smoothing;
+    a.loss = p->loss;
+    a.pair_loss = p->pair_loss;
+    a.reward = p->reward;
+    a.d_logprob = p->d_logprob;
+    a.meet = static_cast<unsigned long long*>(workspace);
+    a.tag = launch_tag();
+    return ws::launch_preference(S(stream), a, preference_groups(p->pairs));
+}
 
 }  // extern "C"
