@@ -570,7 +570,7 @@ typedef struct ws_loss_rows {
  * pass. workspace: device memory of ws_token_logprobs_workspace() bytes (0: none is needed), 8-byte aligned, of any
  * contents, nobody else's until the launch is done (few rows are shared by up to 64 workgroups each, which meet there; a captured
  * launch may be replayed). Without it every row is one workgroup's: slower, the sums in another order. */
-uint64_t ws_token_logprobs_workspace(const ws_loss_rows* r, int want_entropy);
+uint64_t ws_token_logprobs_workspace(const ws_loss_rows* r);
 int ws_token_logprobs(void* stream, const ws_loss_rows* r, float* logprob, float* stats, float* entropy /* may be NULL */, void* workspace,
                       uint64_t workspace_bytes);
 
@@ -612,7 +612,7 @@ int ws_policy_loss(void* stream, uint32_t rows, const ws_policy* p, const float*
  * logprob and entropy are 0, their gradient is zero. Without `weight` every row weighs 1 / rows, those without a token too. entropy: out (may be
  * NULL, entropy_coef must be 0 then). d_logits as in ws_token_logprobs_grad. workspace as above, of
  * ws_policy_loss_rows_workspace() bytes; required. */
-uint64_t ws_policy_loss_rows_workspace(const ws_loss_rows* r, const ws_policy* p, int want_entropy);
+uint64_t ws_policy_loss_rows_workspace(const ws_loss_rows* r);
 int ws_policy_loss_rows(void* stream, const ws_loss_rows* r, const ws_policy* p, float* sums, float* logprob, float* entropy, void* d_logits,
                         uint64_t d_stride, void* workspace, uint64_t workspace_bytes);
 

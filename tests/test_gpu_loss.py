@@ -231,9 +231,8 @@ def test_policy_loss_of_no_tokens():
     assert m.token_logprobs_grad(logits, torch.empty(0, dtype=torch.int32, device=DEV), stats).shape == (0, 100)
 
 
-# few rows go through two launches, from half as many rows as compute units on a workgroup a row with the row in registers: 256, 512 and 1024 threads,
-# and rows beyond what they hold
-ROWS = [(1, 1), (1, 129), (7, 1000), (16, 50257), (3, 151936), (5, 262144), (130, 3), (140, 1001), (130, 20480), (129, 20485), (128, 40961), (130, 50257), (128, 81921), (128, 151936),
+# rows of one workgroup and of several, of both builds (shares of up to 1024 and 3072 vectors), up to 512 rows in one launch, more in two
+ROWS = [(600, 777), (520, 12400), (513, 25001), (1, 1), (1, 129), (7, 1000), (16, 50257), (3, 151936), (5, 262144), (130, 3), (140, 1001), (130, 20480), (129, 20485), (128, 40961), (130, 50257), (128, 81921), (128, 151936),
         (128, 160007)]
 
 

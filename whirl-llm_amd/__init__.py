@@ -179,14 +179,14 @@ ABI = {
     "ws_history_stage": (C.c_int, [C.c_void_p, C.POINTER(HistoryStage)]),
     "ws_spec_verify_workspace": (C.c_uint64, [C.POINTER(SpecVerify)]),
     "ws_spec_verify_classic": (C.c_int, [C.c_void_p, C.POINTER(SpecVerify)]),
-    "ws_token_logprobs_workspace": (C.c_uint64, [C.POINTER(LossRows), C.c_int]),
+    "ws_token_logprobs_workspace": (C.c_uint64, [C.POINTER(LossRows)]),
     "ws_token_logprobs": (C.c_int, [C.c_void_p, C.POINTER(LossRows), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64]),
     "ws_token_logprobs_grad": (C.c_int, [C.c_void_p, C.POINTER(LossRows), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                          C.c_uint64]),
     "ws_policy_loss_workspace": (C.c_uint64, [C.c_uint32]),
     "ws_policy_loss": (C.c_int, [C.c_void_p, C.c_uint32, C.POINTER(Policy), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                  C.c_void_p, C.c_uint64]),
-    "ws_policy_loss_rows_workspace": (C.c_uint64, [C.POINTER(LossRows), C.POINTER(Policy), C.c_int]),
+    "ws_policy_loss_rows_workspace": (C.c_uint64, [C.POINTER(LossRows)]),
     "ws_policy_loss_rows": (C.c_int, [C.c_void_p, C.POINTER(LossRows), C.POINTER(Policy), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                       C.c_uint64, C.c_void_p, C.c_uint64]),
     "ws_preference_loss_workspace": (C.c_uint64, [C.c_uint32]),
@@ -569,57 +569,71 @@ def spec_verify_classic(p, q, draft, seed, step0, rng=RNG_PHILOX, tol=0.0, works
 # ---------------------------------------------------------------------------------------------------------------------
 # log-probabilities of answered tokens, losses over them and their gradients
 
-def _vector(name, t, dtype, n, dev, optional=True):
-    """The address of a contiguous device vector of n entries (None: NULL)."""
+_LOSS_DTYPES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}
+_F32, _I32 = torch.float32, torch.int32
+
+
+def _vector(name, t, dtype, n, at):
+    """The address of a contiguous vector of n entries on device number `at` (None: NULL)."""
     if t is None:
-        if optional:
-            return None
-        raise WsError(f"{name}: missing")
-    if t.dtype != dtype or t.device != dev or t.numel() != n or not t.is_contiguous():
-        raise WsError(f"{name}: contiguous {str(dtype)[6:]} tensor of {n} entries on {dev}")
+        return None
+    if t.dtype is not dtype or t.get_device() != at or t.numel() != n or not t.is_contiguous():
+        raise WsError(f"{name}: contiguous {str(dtype)[6:]} tensor of {n} entries on cuda:{at} expected, got {str(t.dtype)[6:]} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _on_current(dev):
-    if dev.type != "cuda":
-        raise WsError(f"device tensors expected, got {dev}")
-    if dev.index != torch._C._cuda_getDevice():  # (the launch goes to the current device's stream)
-        raise WsError(f"tensors on the current device (cuda:{torch._C._cuda_getDevice()}) expected, got {dev}")
+def _given(name, t):
+    if t is None:
+        raise WsError(f"{name}: missing")
+    return t
 
 
-def _matrix(name, t, dtypes):
-    if t.dim() != 2 or t.dtype not in dtypes or (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
-        raise WsError(f"{name}: [rows, vocab] float32 / bfloat16 device tensor with unit inner stride, rows that do not overlap")
+def _device_of(name, t):
+    """The number of the tensor's device, which has to be the current one: launches go to the current device's stream."""
+    at = t.get_device()
+    if at < 0 or at != torch._C._cuda_getDevice():
+        raise WsError(f"{name}: a tensor on the current device expected, got {t.device}")
+    return at
+
+
+def _rows_stride(name, t):
+    """(rows, vocab, elements between rows) of a matrix."""
+    if t.dim() != 2 or t.dtype not in _LOSS_DTYPES:
+        raise WsError(f"{name}: [rows, vocab] float32 / bfloat16 device tensor")
+    (rows, vocab), (stride, inner) = t.shape, t.stride()
+    if rows < 2:
+        stride = vocab
+    if (inner != 1 and vocab > 1) or stride < vocab:
+        raise WsError(f"{name}: unit inner stride and rows that do not overlap")
+    return rows, vocab, stride
 
 
 def _loss_rows(logits, ids, inv_t, allow):
-    _matrix("logits", logits, (torch.float32, torch.bfloat16))
-    dev = logits.device
-    _on_current(dev)
-    rows, vocab = logits.shape
-    r = LossRows(logits=logits.data_ptr(), dtype=DTYPE_F32 if logits.dtype == torch.float32 else DTYPE_BF16, rows=rows, vocab=vocab,
-                 row_stride=logits.stride(0) if rows > 1 else vocab, ids=_vector("ids", ids, torch.int32, rows, dev),
-                 inv_t=_vector("inv_t", inv_t, torch.float32, rows, dev))
+    rows, vocab, stride = _rows_stride("logits", logits)
+    at = _device_of("logits", logits)
+    r = LossRows(logits.data_ptr(), _LOSS_DTYPES[logits.dtype], rows, vocab, stride, _vector("ids", ids, _I32, rows, at), _vector("inv_t", inv_t, _F32, rows, at))
     if allow is not None:
-        if allow.dim() != 2 or allow.dtype != torch.int32 or allow.device != dev or allow.shape[0] != rows or allow.shape[1] < (vocab + 31) // 32 or allow.stride(1) != 1:
-            raise WsError("allow: [rows, (vocab + 31) / 32] int32 device tensor with unit inner stride")
+        if allow.dim() != 2 or allow.dtype is not _I32 or allow.get_device() != at or allow.shape[0] != rows or allow.shape[1] < (vocab + 31) // 32 or allow.stride(1) != 1:
+            raise WsError("allow: [rows, (vocab + 31) / 32] int32 tensor with unit inner stride on the logits' device")
         r.allow, r.allow_stride = allow.data_ptr(), allow.stride(0) if rows > 1 else allow.shape[1]
-    return r, rows, vocab, dev
+    return r, rows, vocab, at
 
 
-def _gradient_for(logits, out):
+def _gradient_for(logits, out, vocab):
+    """(the gradient's matrix, elements between its rows)"""
     if out is None:
-        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    _matrix("out", out, (logits.dtype,))
-    if out.shape != logits.shape or out.device != logits.device:
-        raise WsError("out: of the logits' shape, on their device")
-    return out
+        return logits.new_empty(logits.shape), vocab  # (half the host time of torch.empty with a dtype and a device)
+    if out.shape != logits.shape or out.dtype is not logits.dtype or out.get_device() != logits.get_device():
+        raise WsError("out: of the logits' shape and dtype, on their device")
+    return out, _rows_stride("out", out)[2]
 
 
-def _scratch(need, dev):
-    """Workspace of any contents for one call: asked for with every call, as the greedy picks' (torch's allocator hands memory out in the order
-    of the stream), so that every stream, thread and captured graph has its own."""
-    return torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+def _with_work(words, need, dev):
+    """A float32 result of `words` entries with the call's workspace behind it, and where that is: memory of any contents, asked for with every call as the
+    greedy picks' is, so that every stream, thread and captured graph has its own. The result is cut to its size when the call is made."""
+    first = (words + 1) & ~1
+    t = torch.empty(first + (need + 3) // 4, dtype=_F32, device=dev)
+    return t, t.data_ptr() + 4 * first
 
 
 def token_logprobs(logits, ids, inv_t=None, allow=None, want_entropy=False):
@@ -627,34 +641,32 @@ def token_logprobs(logits, ids, inv_t=None, allow=None, want_entropy=False):
     [rows], an id outside [0, vocab) (-1) = no token, logprob 0; inv_t: float32 [rows] (1 / temperature); allow: int32 bitmap
     [rows, (vocab + 31) / 32]. Returns (logprob float32 [rows], stats float32 [rows, 2] = maximum and sum of the row, which
     token_logprobs_grad takes, entropy float32 [rows] or None)."""
-    r, rows, vocab, dev = _loss_rows(logits, ids, inv_t, allow)
-    logprob = torch.empty(rows, dtype=torch.float32, device=dev)
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev)
-    entropy = torch.empty(rows, dtype=torch.float32, device=dev) if want_entropy else None
-    need = lib().ws_token_logprobs_workspace(C.byref(r), int(want_entropy))
-    work = _scratch(need, dev)
-    check(lib().ws_token_logprobs(_stream(), C.byref(r), _p(logprob), _p(stats), _p(entropy), _p(work), need), "ws_token_logprobs")
-    return logprob, stats, entropy
+    r, rows, vocab, at = _loss_rows(logits, ids, inv_t, allow)
+    dev, call, ref = logits.device, lib(), C.byref(r)
+    need = call.ws_token_logprobs_workspace(ref)
+    stats, work = _with_work(2 * rows, need, dev)
+    logprob = torch.empty(rows, dtype=_F32, device=dev)
+    entropy = torch.empty(rows, dtype=_F32, device=dev) if want_entropy else None
+    check(call.ws_token_logprobs(_stream(), ref, logprob.data_ptr(), stats.data_ptr(), _p(entropy), work, need), "ws_token_logprobs")
+    return logprob, stats.resize_(rows, 2), entropy
 
 
 def token_logprobs_grad(logits, ids, stats, d_logprob=None, entropy=None, d_entropy=None, inv_t=None, allow=None, out=None):
     """Gradient with respect to the logits of a loss whose derivatives by token_logprobs' logprob and entropy are d_logprob and d_entropy (float32
     [rows], None: 0), in the logits' dtype (ws_token_logprobs_grad). stats, entropy: what token_logprobs returned for the same logits,
     ids, inv_t and allow. out: where to write it; it may be `logits`. A row whose derivatives are 0 is not read."""
-    r, rows, vocab, dev = _loss_rows(logits, ids, inv_t, allow)
-    out = _gradient_for(logits, out)
-    check(lib().ws_token_logprobs_grad(_stream(), C.byref(r), _vector("stats", stats, torch.float32, 2 * rows, dev, False),
-                                       _vector("d_logprob", d_logprob, torch.float32, rows, dev), _vector("entropy", entropy, torch.float32, rows, dev),
-                                       _vector("d_entropy", d_entropy, torch.float32, rows, dev), _p(out), out.stride(0) if rows > 1 else vocab),
+    r, rows, vocab, at = _loss_rows(logits, ids, inv_t, allow)
+    out, stride = _gradient_for(logits, out, vocab)
+    check(lib().ws_token_logprobs_grad(_stream(), C.byref(r), _vector("stats", _given("stats", stats), _F32, 2 * rows, at), _vector("d_logprob", d_logprob, _F32, rows, at),
+                                       _vector("entropy", entropy, _F32, rows, at), _vector("d_entropy", d_entropy, _F32, rows, at), out.data_ptr(), stride),
           "ws_token_logprobs_grad")
     return out
 
 
-def _policy(old_logprob, advantage, ref_logprob, weight, rows, dev, clip_low, clip_high, dual_clip, kl_coef, entropy_coef):
-    return Policy(old_logprob=_vector("old_logprob", old_logprob, torch.float32, rows, dev, False),
-                  ref_logprob=_vector("ref_logprob", ref_logprob, torch.float32, rows, dev),
-                  advantage=_vector("advantage", advantage, torch.float32, rows, dev, False), weight=_vector("weight", weight, torch.float32, rows, dev),
-                  clip_low=clip_low, clip_high=clip_high, dual_clip=dual_clip, kl_coef=kl_coef, entropy_coef=entropy_coef)
+def _policy(old_logprob, advantage, ref_logprob, weight, rows, at, clip_low, clip_high, dual_clip, kl_coef, entropy_coef):
+    return Policy(_vector("old_logprob", _given("old_logprob", old_logprob), _F32, rows, at), _vector("ref_logprob", ref_logprob, _F32, rows, at),
+                  _vector("advantage", _given("advantage", advantage), _F32, rows, at), _vector("weight", weight, _F32, rows, at),
+                  clip_low, clip_high, dual_clip, kl_coef, entropy_coef)
 
 
 def policy_loss(logprob, old_logprob, advantage, ref_logprob=None, entropy=None, weight=None, clip_low=0.2, clip_high=0.2, dual_clip=0.0, kl_coef=0.0,
@@ -662,17 +674,16 @@ def policy_loss(logprob, old_logprob, advantage, ref_logprob=None, entropy=None,
     """The clipped policy loss over float32 [rows] log-probabilities (ws_policy_loss). weight: float32 [rows], 0 = the token counts for nothing (None:
     1 / rows each). Returns (sums float32 [5] = loss, surrogate, KL, entropy, clipped weight; d_logprob float32 [rows]; d_entropy float32
     [rows], or None without entropy)."""
-    rows, dev = logprob.numel(), logprob.device
-    _on_current(dev)
-    p = _policy(old_logprob, advantage, ref_logprob, weight, rows, dev, clip_low, clip_high, dual_clip, kl_coef, entropy_coef)
-    sums = torch.empty(5, dtype=torch.float32, device=dev)
-    d_logprob = torch.empty(rows, dtype=torch.float32, device=dev)
-    d_entropy = torch.empty(rows, dtype=torch.float32, device=dev) if entropy is not None else None
-    need = lib().ws_policy_loss_workspace(rows)
-    work = _scratch(need, dev)
-    check(lib().ws_policy_loss(_stream(), rows, C.byref(p), _vector("logprob", logprob, torch.float32, rows, dev, False),
-                               _vector("entropy", entropy, torch.float32, rows, dev), _p(sums), _p(d_logprob), _p(d_entropy), _p(work), need), "ws_policy_loss")
-    return sums, d_logprob, d_entropy
+    rows, at, dev = logprob.numel(), _device_of("logprob", logprob), logprob.device
+    p = _policy(old_logprob, advantage, ref_logprob, weight, rows, at, clip_low, clip_high, dual_clip, kl_coef, entropy_coef)
+    call = lib()
+    need = call.ws_policy_loss_workspace(rows)
+    sums, work = _with_work(5, need, dev)
+    d_logprob = torch.empty(rows, dtype=_F32, device=dev)
+    d_entropy = torch.empty(rows, dtype=_F32, device=dev) if entropy is not None else None
+    check(call.ws_policy_loss(_stream(), rows, C.byref(p), _vector("logprob", logprob, _F32, rows, at), _vector("entropy", entropy, _F32, rows, at), sums.data_ptr(),
+                              d_logprob.data_ptr(), _p(d_entropy), work, need), "ws_policy_loss")
+    return sums.resize_(5), d_logprob, d_entropy
 
 
 def policy_loss_rows(logits, ids, old_logprob, advantage, ref_logprob=None, weight=None, inv_t=None, allow=None, clip_low=0.2, clip_high=0.2,
@@ -680,38 +691,37 @@ def policy_loss_rows(logits, ids, old_logprob, advantage, ref_logprob=None, weig
     """The clipped policy loss from the logits and its gradient by them (ws_policy_loss_rows): token_logprobs, policy_loss and token_logprobs_grad in
     one. Rows without a token and rows of weight 0 count for nothing and are not read. out: where to write the gradient; it may be
     `logits`. Returns (sums float32 [5], logprob float32 [rows], entropy float32 [rows] or None, d_logits)."""
-    r, rows, vocab, dev = _loss_rows(logits, ids, inv_t, allow)
-    p = _policy(old_logprob, advantage, ref_logprob, weight, rows, dev, clip_low, clip_high, dual_clip, kl_coef, entropy_coef)
-    out = _gradient_for(logits, out)
-    sums = torch.empty(5, dtype=torch.float32, device=dev)
-    logprob = torch.empty(rows, dtype=torch.float32, device=dev)
-    entropy = torch.empty(rows, dtype=torch.float32, device=dev) if want_entropy or entropy_coef != 0.0 else None
-    need = lib().ws_policy_loss_rows_workspace(C.byref(r), C.byref(p), int(entropy is not None))
-    work = _scratch(need, dev)
-    check(lib().ws_policy_loss_rows(_stream(), C.byref(r), C.byref(p), _p(sums), _p(logprob), _p(entropy), _p(out), out.stride(0) if rows > 1 else vocab,
-                                    _p(work), need), "ws_policy_loss_rows")
-    return sums, logprob, entropy, out
+    r, rows, vocab, at = _loss_rows(logits, _given("ids", ids), inv_t, allow)
+    p = _policy(old_logprob, advantage, ref_logprob, weight, rows, at, clip_low, clip_high, dual_clip, kl_coef, entropy_coef)
+    out, stride = _gradient_for(logits, out, vocab)
+    dev, call, ref = logits.device, lib(), C.byref(r)
+    need = call.ws_policy_loss_rows_workspace(ref)
+    sums, work = _with_work(5, need, dev)
+    logprob = torch.empty(rows, dtype=_F32, device=dev)
+    entropy = torch.empty(rows, dtype=_F32, device=dev) if want_entropy or entropy_coef != 0.0 else None
+    check(call.ws_policy_loss_rows(_stream(), ref, C.byref(p), sums.data_ptr(), logprob.data_ptr(), _p(entropy), out.data_ptr(), stride, work, need), "ws_policy_loss_rows")
+    return sums.resize_(5), logprob, entropy, out
 
 
 def preference_loss(logprob, seq_off, ref_logprob=None, weight=None, beta=0.1, label_smoothing=0.0):
     """The loss of paired log ratios over float32 [rows] log-probabilities (ws_preference_loss). seq_off: int32 [2 * pairs + 1], ascending: rows
     seq_off[2 p] .. seq_off[2 p + 1] are the preferred answer of pair p, the next ones the other. weight: float32 [pairs] (None: 1 / pairs
     each). Returns (loss float32 [1], pair_loss float32 [pairs], reward float32 [pairs, 2], d_logprob float32 [rows])."""
-    rows, dev = logprob.numel(), logprob.device
-    _on_current(dev)
+    rows, at, dev = logprob.numel(), _device_of("logprob", logprob), logprob.device
     pairs = (seq_off.numel() - 1) // 2
-    loss = torch.empty(1, dtype=torch.float32, device=dev)
-    pair_loss = torch.empty(max(pairs, 0), dtype=torch.float32, device=dev)
-    reward = torch.empty((max(pairs, 0), 2), dtype=torch.float32, device=dev)
-    d_logprob = torch.empty(rows, dtype=torch.float32, device=dev)
-    a = Preference(rows=rows, pairs=max(pairs, 0), seq_off=_vector("seq_off", seq_off, torch.int32, 2 * pairs + 1, dev, False),
-                   logprob=_vector("logprob", logprob, torch.float32, rows, dev, False), ref_logprob=_vector("ref_logprob", ref_logprob, torch.float32, rows, dev),
-                   weight=_vector("weight", weight, torch.float32, pairs, dev), beta=beta, label_smoothing=label_smoothing, loss=_p(loss),
-                   pair_loss=_p(pair_loss), reward=_p(reward), d_logprob=_p(d_logprob))
-    need = lib().ws_preference_loss_workspace(pairs) if pairs > 0 else 0
-    work = _scratch(need, dev)
-    check(lib().ws_preference_loss(_stream(), C.byref(a), _p(work), need), "ws_preference_loss")
-    return loss, pair_loss, reward, d_logprob
+    if pairs < 1:
+        raise WsError("seq_off: 2 * pairs + 1 offsets of one pair at least")
+    call = lib()
+    need = call.ws_preference_loss_workspace(pairs)
+    loss, work = _with_work(1, need, dev)
+    pair_loss = torch.empty(pairs, dtype=_F32, device=dev)
+    reward = torch.empty((pairs, 2), dtype=_F32, device=dev)
+    d_logprob = torch.empty(rows, dtype=_F32, device=dev)
+    a = Preference(rows, pairs, _vector("seq_off", seq_off, _I32, 2 * pairs + 1, at), _vector("logprob", logprob, _F32, rows, at),
+                   _vector("ref_logprob", ref_logprob, _F32, rows, at), _vector("weight", weight, _F32, pairs, at), beta, label_smoothing, loss.data_ptr(),
+                   pair_loss.data_ptr(), reward.data_ptr(), d_logprob.data_ptr())
+    check(call.ws_preference_loss(_stream(), C.byref(a), work, need), "ws_preference_loss")
+    return loss.resize_(1), pair_loss, reward, d_logprob
 
 
 # ---------------------------------------------------------------------------------------------------------------------

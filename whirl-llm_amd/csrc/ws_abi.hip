@@ -61,12 +61,13 @@ int launch_argmax_shared(hipStream_t stream, int mode, const float* x, int n, in
                          unsigned parts, unsigned long long* scratch, unsigned long long tag);
 int prepare_top();
 // ws_loss.hip: log-probabilities, losses over them and their gradients
-int launch_score(hipStream_t stream, int dtype, const ScoreArgs& a, bool policy);
+int launch_score(hipStream_t stream, int dtype, const ScoreArgs& a);
 int launch_grad(hipStream_t stream, int dtype, const GradArgs& a);
-int launch_policy_rows(hipStream_t stream, int dtype, const RowsArgs& b, bool slope);
+int launch_policy_rows(hipStream_t stream, int dtype, const RowsArgs& a, bool slope);
 int launch_policy(hipStream_t stream, const PolicyArgs& a, unsigned groups);
 int launch_preference(hipStream_t stream, const PreferenceArgs& a, unsigned groups);
 uint32_t loss_threads();
+uint32_t loss_most_share();  // vectors of a row that a workgroup of policy_rows_kernel holds
 uint32_t loss_grad_chunks(int dtype, uint32_t vocab);
 }  // namespace ws
 
@@ -1106,15 +1107,17 @@ bool gradient_ok(const ws_loss_rows* r, const void* d, uint64_t stride) {
 ws::LossRows loss_rows(const ws_loss_rows* r) {
     return ws::LossRows{static_cast<const unsigned char*>(r->logits), r->row_stride * elem_bytes(r->dtype), r->rows, r->vocab, r->ids, r->inv_t, r->allow, r->allow_stride};
 }
-// workgroups a row of the log-probabilities: some four a compute unit, each with two vectors a thread at least
+uint32_t row_vectors(const ws_loss_rows* r) { return r->vocab / (r->dtype == WS_DTYPE_F32 ? 4u : 8u); }
+uint32_t share_of(uint32_t vectors, uint32_t parts) { return (vectors + parts - 1u) / parts; }
+// Workgroups a row of the log-probabilities: of 1536 vectors (six a thread), or of fewer where rows are few, 512 vectors at least, four a compute unit.
 uint32_t score_parts(const ws_loss_rows* r) {
-    const uint32_t want = 4u * static_cast<uint32_t>(compute_units()), vectors = r->vocab / (r->dtype == WS_DTYPE_F32 ? 4u : 8u);
-    uint32_t parts = r->rows ? want / r->rows : 1u;
-    const uint32_t most = vectors / (2u * ws::loss_threads());
+    const uint32_t vectors = row_vectors(r), most = vectors / 512u;
+    uint32_t parts = r->rows ? 4u * static_cast<uint32_t>(compute_units()) / r->rows : 1u;
     if (parts > most) parts = most;
+    if (parts < vectors / 1536u) parts = vectors / 1536u;
     return parts < 2u ? 1u : (parts > 64u ? 64u : parts);
 }
-uint64_t meet_bytes(uint32_t rows, uint32_t parts, bool entropy) { return parts > 1u ? uint64_t{rows} * parts * (entropy ? 32u : 16u) : 0u; }
+uint64_t meet_bytes(uint32_t rows, uint32_t parts, uint32_t words) { return parts > 1u ? uint64_t{rows} * parts * words * 8u : 0u; }
 bool workspace_ok(const void* w, uint64_t bytes, uint64_t need) { return need == 0 || (w && bytes >= need && aligned(w, 8u)); }
 
 bool policy_ok(const ws_policy* p, uint32_t rows, bool entropy) {
@@ -1127,28 +1130,35 @@ ws::PolicyIn policy_in(const ws_policy* p, uint32_t rows) {
 }
 // workgroups of a sum over tokens
 uint32_t policy_groups(uint32_t rows) {
-    const uint32_t n = (rows + 511u) / 512u;
+    const uint32_t n = (rows + 1023u) / 1024u;
     return n < 1u ? 1u : (n > 64u ? 64u : n);
 }
-uint64_t policy_meet_bytes(uint32_t rows) { return policy_groups(rows) > 1u ? uint64_t{policy_groups(rows)} * ws::kPolicySums * 16u : 0u; }
+uint64_t policy_meet_bytes(uint32_t slots) { return uint64_t{slots} * ws::kPolicySums * 16u; }
 uint32_t preference_groups(uint32_t pairs) { return pairs > 256u ? 256u : pairs; }
 
-// the workspace of ws_policy_loss_rows, in this order: the rows' terms, meeting places, and for rows of two launches stats and derivatives
+// The workspace of ws_policy_loss_rows: the words of the sum's workgroups or rows, those of the rows' parts, the rows' terms. One launch where rows are few,
+// a second one adds up the terms of more (policy_rows_kernel).
+constexpr uint32_t kOneLaunchRows = 64u;
 struct RowsPlan {
-    bool held;  // one launch, a workgroup a row
-    uint32_t parts;
-    uint64_t terms, sums_meet, meet, stats, d_logprob, d_entropy, bytes;
+    uint32_t parts, groups;
+    bool one;
+    uint64_t words, meet, terms, bytes;
 };
-RowsPlan rows_plan(const ws_loss_rows* r, const ws_policy* p, bool entropy) {
+RowsPlan rows_plan(const ws_loss_rows* r) {
     RowsPlan n{};
-    n.held = 2u * r->rows >= static_cast<uint32_t>(compute_units());
-    n.parts = n.held ? 1u : score_parts(r);
-    n.sums_meet = uint64_t{r->rows} * ws::kPolicySums * 8u;
-    n.meet = n.sums_meet + policy_meet_bytes(r->rows);
-    n.stats = n.meet + meet_bytes(r->rows, n.parts, entropy);
-    n.d_logprob = n.stats + (n.held ? 0u : uint64_t{r->rows} * 8u);
-    n.d_entropy = n.d_logprob + (n.held ? 0u : uint64_t{r->rows} * 4u);
-    n.bytes = n.d_entropy + (n.held || p->entropy_coef == 0.0 ? 0u : uint64_t{r->rows} * 4u);
+    const uint32_t vectors = row_vectors(r), least = share_of(vectors, ws::loss_most_share());
+    uint32_t parts = r->rows ? 2u * static_cast<uint32_t>(compute_units()) / r->rows : 1u;
+    if (parts > vectors / 256u) parts = vectors / 256u;
+    if (parts > 64u) parts = 64u;
+    if (parts < least) parts = least;
+    n.parts = parts < 1u ? 1u : parts;
+    n.one = r->rows != 0u && r->rows <= kOneLaunchRows;
+    n.words = meet_bytes(r->rows, n.parts, ws::kPartWords + (n.one ? 2u : 0u));
+    const uint64_t groups = r->rows / 1024u + n.words / 32768u + 1u;  // (of the second launch, which also clears the words)
+    n.groups = groups > 64u ? 64u : static_cast<uint32_t>(groups);
+    n.meet = policy_meet_bytes(n.one ? r->rows : n.groups);
+    n.terms = n.meet + n.words;
+    n.bytes = n.terms + (n.one ? 0u : uint64_t{r->rows} * ws::kPolicySums * 8u);
     return n;
 }
 int grad_on(void* stream, const ws_loss_rows* r, const float* stats, const float* d_logprob, const float* entropy, const float* d_entropy, void* d_logits, uint64_t d_stride) {
@@ -1161,12 +1171,11 @@ int grad_on(void* stream, const ws_loss_rows* r, const float* stats, const float
     a.out = static_cast<unsigned char*>(d_logits);
     a.out_bytes = d_stride * elem_bytes(r->dtype);
     a.chunks = ws::loss_grad_chunks(r->dtype, r->vocab);
-    if (uint64_t{r->rows} * a.chunks * ws::loss_threads() >= uint64_t{1} << 32) return WS_E_UNSUPPORTED;  // (more than a launch has threads)
     return ws::launch_grad(S(stream), r->dtype, a);
 }
 }  // namespace
 
-uint64_t ws_token_logprobs_workspace(const ws_loss_rows* r, int want_entropy) { return loss_rows_ok(r) ? meet_bytes(r->rows, score_parts(r), want_entropy != 0) : 0u; }
+uint64_t ws_token_logprobs_workspace(const ws_loss_rows* r) { return loss_rows_ok(r) ? meet_bytes(r->rows, score_parts(r), ws::kPartWords) : 0u; }
 
 int ws_token_logprobs(void* stream, const ws_loss_rows* r, float* logprob, float* stats, float* entropy, void* workspace, uint64_t workspace_bytes) {
     if (!loss_rows_ok(r)) return WS_E_INVALID;
@@ -1179,14 +1188,15 @@ int ws_token_logprobs(void* stream, const ws_loss_rows* r, float* logprob, float
     a.entropy = entropy;
     a.parts = score_parts(r);
     if (a.parts > 1u) {
-        if (workspace && workspace_ok(workspace, workspace_bytes, meet_bytes(r->rows, a.parts, entropy != nullptr))) {
+        if (workspace && workspace_ok(workspace, workspace_bytes, meet_bytes(r->rows, a.parts, ws::kPartWords))) {
             a.meet = static_cast<unsigned long long*>(workspace);
             a.tag = launch_tag();
         } else {
             a.parts = 1u;
         }
     }
-    return ws::launch_score(S(stream), r->dtype, a, false);
+    a.per = share_of(row_vectors(r), a.parts);
+    return ws::launch_score(S(stream), r->dtype, a);
 }
 
 int ws_token_logprobs_grad(void* stream, const ws_loss_rows* r, const float* stats, const float* d_logprob, const float* entropy, const float* d_entropy, void* d_logits,
@@ -1197,12 +1207,12 @@ int ws_token_logprobs_grad(void* stream, const ws_loss_rows* r, const float* sta
     return grad_on(stream, r, stats, d_logprob, entropy, d_entropy, d_logits, d_stride);
 }
 
-uint64_t ws_policy_loss_workspace(uint32_t rows) { return policy_meet_bytes(rows); }
+uint64_t ws_policy_loss_workspace(uint32_t rows) { return policy_groups(rows) > 1u ? policy_meet_bytes(policy_groups(rows)) : 0u; }
 
 int ws_policy_loss(void* stream, uint32_t rows, const ws_policy* p, const float* logprob, const float* entropy, float* sums, float* d_logprob, float* d_entropy, void* workspace,
                    uint64_t workspace_bytes) {
     if (!policy_ok(p, rows, entropy != nullptr) || !sums || (rows && (!logprob || !d_logprob)) || rows > (1u << 30)) return WS_E_INVALID;
-    if (!workspace_ok(workspace, workspace_bytes, policy_meet_bytes(rows))) return WS_E_WORKSPACE;
+    if (!workspace_ok(workspace, workspace_bytes, ws_policy_loss_workspace(rows))) return WS_E_WORKSPACE;
     ws::PolicyArgs a{};
     a.P = policy_in(p, rows);
     a.rows = rows;
@@ -1216,45 +1226,45 @@ int ws_policy_loss(void* stream, uint32_t rows, const ws_policy* p, const float*
     return ws::launch_policy(S(stream), a, policy_groups(rows));
 }
 
-uint64_t ws_policy_loss_rows_workspace(const ws_loss_rows* r, const ws_policy* p, int want_entropy) {
-    return loss_rows_ok(r) && p ? rows_plan(r, p, want_entropy != 0).bytes : 0u;
-}
+uint64_t ws_policy_loss_rows_workspace(const ws_loss_rows* r) { return loss_rows_ok(r) ? rows_plan(r).bytes : 0u; }
 
 int ws_policy_loss_rows(void* stream, const ws_loss_rows* r, const ws_policy* p, float* sums, float* logprob, float* entropy, void* d_logits, uint64_t d_stride, void* workspace,
                         uint64_t workspace_bytes) {
     if (!loss_rows_ok(r) || !policy_ok(p, r->rows, entropy != nullptr) || !gradient_ok(r, d_logits, d_stride) || !sums) return WS_E_INVALID;
     if (r->rows && (!r->ids || !logprob)) return WS_E_INVALID;
-    const RowsPlan n = rows_plan(r, p, entropy != nullptr);
+    const RowsPlan n = rows_plan(r);
     if (!workspace_ok(workspace, workspace_bytes, n.bytes)) return WS_E_WORKSPACE;
     unsigned char* work = static_cast<unsigned char*>(workspace);
+    ws::PolicyArgs sum{};
     if (r->rows) {
-        ws::ScoreArgs a{};
+        ws::RowsArgs a{};
         a.R = loss_rows(r);
+        a.P = policy_in(p, r->rows);
         a.logprob = logprob;
         a.entropy = entropy;
-        a.parts = n.parts;
-        a.P = policy_in(p, r->rows);
-        a.terms = reinterpret_cast<double*>(work);
-        if (n.held) {
-            if (const int e = ws::launch_policy_rows(S(stream), r->dtype, ws::RowsArgs{a, static_cast<unsigned char*>(d_logits), d_stride * elem_bytes(r->dtype)}, p->entropy_coef != 0.0); e != 0)
-                return e;
+        a.out = static_cast<unsigned char*>(d_logits);
+        a.out_bytes = d_stride * elem_bytes(r->dtype);
+        if (n.one) {
+            a.sums_meet = reinterpret_cast<unsigned long long*>(work);
+            a.sums = sums;
         } else {
-            a.stats = reinterpret_cast<float*>(work + n.stats);
-            a.d_logprob = reinterpret_cast<float*>(work + n.d_logprob);
-            a.d_entropy = p->entropy_coef != 0.0 ? reinterpret_cast<float*>(work + n.d_entropy) : nullptr;
-            a.meet = reinterpret_cast<unsigned long long*>(work + n.meet);
-            a.tag = launch_tag();
-            if (const int e = ws::launch_score(S(stream), r->dtype, a, true); e != 0) return e;
-            if (const int e = grad_on(stream, r, a.stats, a.d_logprob, entropy, a.d_entropy, d_logits, d_stride); e != 0) return e;
+            a.terms = reinterpret_cast<double*>(work + n.terms);
         }
+        a.parts = n.parts;
+        a.per = share_of(row_vectors(r), n.parts);
+        a.meet = reinterpret_cast<unsigned long long*>(work + n.meet);
+        a.tag = launch_tag();
+        if (const int e = ws::launch_policy_rows(S(stream), r->dtype, a, p->entropy_coef != 0.0); e != 0) return e;
+        if (n.one) return WS_OK;
+        sum.words = a.meet;
+        sum.n_words = n.words / 8u;
     }
-    ws::PolicyArgs a{};
-    a.rows = r->rows;
-    a.terms = reinterpret_cast<const double*>(work);
-    a.sums = sums;
-    a.meet = reinterpret_cast<unsigned long long*>(work + n.sums_meet);
-    a.tag = launch_tag();
-    return ws::launch_policy(S(stream), a, policy_groups(r->rows));
+    sum.rows = r->rows;
+    sum.terms = reinterpret_cast<const double*>(work + n.terms);
+    sum.sums = sums;
+    sum.meet = reinterpret_cast<unsigned long long*>(work);
+    sum.tag = launch_tag();
+    return ws::launch_policy(S(stream), sum, n.groups);
 }
 
 uint64_t ws_preference_loss_workspace(uint32_t pairs) { return preference_groups(pairs) > 1u ? uint64_t{preference_groups(pairs)} * 16u : 0u; }

@@ -41,13 +41,20 @@ struct PolicyToken {
     double sum[kPolicySums];
 };
 
+struct PolicyRow {  // a token's entries
+    float old_logprob, ref_logprob, advantage;
+    double weight;
+};
 __device__ __forceinline__ double policy_weight(const PolicyIn& P, uint32_t row) { return P.weight ? static_cast<double>(P.weight[row]) : P.weight_all; }
+__device__ __forceinline__ PolicyRow policy_row(const PolicyIn& P, uint32_t row) {
+    return PolicyRow{P.old_logprob[row], P.ref_logprob ? P.ref_logprob[row] : 0.f, P.advantage[row], policy_weight(P, row)};
+}
 
 // gain = min(r A, clip(r) A) with r = exp(lp - old); for A < 0 not below dual_clip * A. Where the clip holds it there is no
 // derivative, so the comparison is made in 64 bits: rounded to 32, one token in some million would fall on the other side.
-__device__ __forceinline__ PolicyToken policy_token(const PolicyIn& P, uint32_t row, double w, double lp, double H) {
+__device__ __forceinline__ PolicyToken policy_token(const PolicyIn& P, const PolicyRow& T, double lp, double H) {
     PolicyToken o;
-    const double A = static_cast<double>(P.advantage[row]), r = exp(lp - static_cast<double>(P.old_logprob[row]));
+    const double w = T.weight, A = static_cast<double>(T.advantage), r = exp(lp - static_cast<double>(T.old_logprob));
     const double free = r * A, held = fmin(fmax(r, 1.0 - P.clip_low), 1.0 + P.clip_high) * A;
     double gain = held < free ? held : free;
     bool clipped = held < free;
@@ -57,7 +64,7 @@ __device__ __forceinline__ PolicyToken policy_token(const PolicyIn& P, uint32_t 
     }
     double kl = 0.0, back = 0.0;
     if (P.ref_logprob) {  // exp(b) - b - 1 with b = ref - lp, never negative
-        const double b = static_cast<double>(P.ref_logprob[row]) - lp;
+        const double b = static_cast<double>(T.ref_logprob) - lp;
         back = expm1(b);
         kl = back - b;
     }
@@ -73,20 +80,78 @@ __device__ __forceinline__ PolicyToken policy_token(const PolicyIn& P, uint32_t 
 
 // ---- workgroups that meet in memory of any contents, as argmax_shared does (ws_top.h): every word is left twice, once mixed with a
 // tag that no other launch has; whoever finds all pairs together goes on, the one whose words come last does, others may and
-// write the same. The pairs are then broken, for a captured launch has its tag again at every replay.
-__device__ __forceinline__ void leave_word(unsigned long long* at, unsigned long long v, unsigned long long tag) {
+// write the same. The pairs are then broken, for a captured launch has its tag again at every replay. `apart`: words between the two of
+// a pair, with the same word of the other workgroups between them: everybody looks at everybody's, past the caches, and a look at words
+// side by side is an eighth of the requests (64 parts of a row of 151936, their words 32 bytes apart: 8.3 us, the launch without them 5.8).
+__device__ __forceinline__ void leave_word(unsigned long long* at, uint32_t apart, unsigned long long v, unsigned long long tag) {
     __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __hip_atomic_store(at + 1, v ^ tag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(at + apart, v ^ tag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ bool find_word(const unsigned long long* at, unsigned long long tag, unsigned long long& v) {
+__device__ __forceinline__ bool find_word(const unsigned long long* at, uint32_t apart, unsigned long long tag, unsigned long long& v) {
     v = __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    return (v ^ __hip_atomic_load(at + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) == tag;
+    return (v ^ __hip_atomic_load(at + apart, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) == tag;
 }
-__device__ __forceinline__ void break_word(unsigned long long* at) {
+__device__ __forceinline__ void break_word(unsigned long long* at, uint32_t apart) {
     __hip_atomic_store(at, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __hip_atomic_store(at + 1, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(at + apart, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 __device__ __forceinline__ void words_arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// `slots` workgroups that add up K sums each, by their first waves: each leaves its own (lane 0's), and when they have arrived gathers everybody's, added up in the same
+// order whoever does it; false where somebody is still to come. meet: [K][2][slots]. (The last slots' first sum is looked at first: they come
+// last. Several looks are on their way together: one after the other a sum of five over 256 slots took 14 us.)
+template <int K>
+__device__ __forceinline__ void leave_sums(unsigned long long* meet, uint32_t slots, uint32_t slot, const double (&sum)[K], unsigned long long tag) {
+#pragma unroll
+    for (uint32_t k = 0; k < K; ++k) leave_word(meet + static_cast<size_t>(2u * k) * slots + slot, slots, static_cast<unsigned long long>(__double_as_longlong(sum[k])), tag);
+}
+template <int K>
+__device__ __forceinline__ bool gather_sums(unsigned long long* meet, uint32_t slots, double (&sum)[K], unsigned long long tag) {
+    const uint32_t lane = lane_id();
+    constexpr uint32_t kB = 4u;  // slots of a lane on their way together
+    auto word = [&](uint32_t p, uint32_t k) { return meet + static_cast<size_t>(2u * k) * slots + p; };
+    const uint32_t last = (slots - 1u) / (64u * kB) * (64u * kB);
+    double all[K] = {};
+    for (uint32_t p0 = last;; p0 -= 64u * kB) {
+        bool here = true;
+        unsigned long long v[kB];
+#pragma unroll
+        for (uint32_t b = 0; b < kB; ++b) {
+            const uint32_t p = p0 + b * 64u + lane;
+            v[b] = 0ull;
+            if (p < slots) here = find_word(word(p, 0u), slots, tag, v[b]) && here;
+        }
+        if (__ballot(!here) != 0ull) return false;
+#pragma unroll
+        for (uint32_t b = 0; b < kB; ++b) all[0] += __longlong_as_double(static_cast<long long>(v[b]));
+        if (p0 == 0u) break;
+    }
+    if (K > 1) {
+        bool here = true;
+        for (uint32_t p = lane; p < slots; p += 64u) {
+            unsigned long long v[K];
+#pragma unroll
+            for (uint32_t k = 1; k < K; ++k) here = find_word(word(p, k), slots, tag, v[k]) && here;
+#pragma unroll
+            for (uint32_t k = 1; k < K; ++k) all[k] += __longlong_as_double(static_cast<long long>(v[k]));
+        }
+        if (__ballot(!here) != 0ull) return false;
+    }
+    for (uint32_t p = lane; p < slots; p += 64u) {
+#pragma unroll
+        for (uint32_t k = 0; k < K; ++k) break_word(word(p, k), slots);
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < K; ++k) sum[k] = wave_sum(all[k]);
+    return true;
+}
+
+// a launch of `parts` workgroups a row: the parts in x, the rows in y and z (dispatched in this order, a row's parts one after the other)
+constexpr uint32_t kGridRows = 32768u;
+__device__ __forceinline__ uint32_t grid_row() { return blockIdx.z * kGridRows + blockIdx.y; }
+inline dim3 grid_of(uint32_t parts, uint32_t rows) {
+    return rows <= kGridRows ? dim3(parts, rows) : dim3(parts, kGridRows, (rows + kGridRows - 1u) / kGridRows);
+}
 
 // ---- a row's logits
 template <int DT>
@@ -148,11 +213,15 @@ __device__ __forceinline__ void store_logit(unsigned char* row, uint32_t i, floa
     else reinterpret_cast<uint16_t*>(row)[i] = static_cast<uint16_t>(pack_bf16(v, v));
 }
 
-// the row's bitmap: bit i, and the bits of a vector that begins at token i (it may lie across two words)
+// the row's bitmap: bit i, and the bits of a vector that begins at token i, from the two bytes that they lie in (or the row's last two). One load instead of two
+// words': 200 masked rows of 50257 fp32 MASK_US.
+struct __attribute__((packed, aligned(1))) LooseBits {
+    uint16_t v;
+};
 __device__ __forceinline__ bool allowed(const uint32_t* allow, uint32_t i) { return (allow[i >> 5] >> (i & 31u)) & 1u; }
-__device__ __forceinline__ uint32_t allowed_from(const uint32_t* allow, uint32_t i, uint32_t last_word) {
-    const uint32_t w = i >> 5;
-    return __builtin_amdgcn_alignbit(allow[min(w + 1u, last_word)], allow[w], i & 31u);
+__device__ __forceinline__ uint32_t allowed_from(const uint32_t* allow, uint32_t i, uint32_t last_byte) {
+    const uint32_t at = min(i >> 3, last_byte - 1u);
+    return static_cast<uint32_t>(reinterpret_cast<const LooseBits*>(reinterpret_cast<const unsigned char*>(allow) + at)->v) >> (i - 8u * at);
 }
 // what is not allowed becomes -inf, whatever it was
 template <int DT>
@@ -173,6 +242,27 @@ __device__ __forceinline__ uint4 only_allowed(const uint4& q, uint32_t bits) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// the vectors [j0, j1) of a row that a workgroup works on, `base` where the row begins. Loads go to the last of them where a thread has none
+// (a load behind a branch would be waited for there); what it read then counts as -inf.
+template <int DT, bool MASK, int T>
+struct Share {
+    const unsigned char* base;
+    const uint32_t* allow;
+    uint32_t head, last_byte, j0, j1;
+    __device__ __forceinline__ uint4 load(uint32_t j) const {
+        const uint32_t i = head + min(j, j1 - 1u) * Elem<DT>::kPer;
+        const uint4 q = load_loose(base + static_cast<size_t>(i) * Elem<DT>::kBytes);
+        if constexpr (MASK) return only_allowed<DT>(q, allowed_from(allow, i, last_byte));
+        return q;
+    }
+    // the vector of round jb .. jb + T, for a thread that may have none in it
+    __device__ __forceinline__ uint4 own(const uint4& q, uint32_t jb) const {
+        constexpr uint32_t none = Elem<DT>::kNone;
+        if (jb + T <= j1) return q;  // (uniform)
+        return jb + threadIdx.x < j1 ? q : make_uint4(none, none, none, none);
+    }
+};
+
 // ---- exponentials: (x - m) t log2(e), the factor as hi + lo with lo > 0 (so that a difference of -inf stays -inf)
 struct Scale {
     float hi, lo;
@@ -183,7 +273,7 @@ struct Scale {
         hi = inv_t > 0.f && inv_t < INFINITY ? h : __builtin_nanf("");  // (a temperature that is none makes the row NaN)
         lo = fmaxf(static_cast<float>(c - static_cast<double>(h)), FLT_MIN);
     }
-    __device__ __forceinline__ float of(float d) const { return fmaf(d, hi, d * lo); }
+    __device__ __forceinline__ float of(float d) const { return fmaf(d, hi, __fmul_rn(d, lo)); }
 };
 __device__ __forceinline__ float exp2_fast(float a) { return __builtin_amdgcn_exp2f(a); }  // (below 2^-126: 0)
 // two more values into a maximum. (Written out: of fmaxf the compiler makes another instruction a value, to quiet NaN.)
@@ -209,15 +299,15 @@ struct Running {
 #pragma unroll
         for (int k = 0; k < N; k += 2) {
             const float a = c.of(x[k] - M), b = c.of(x[k + 1] - M), ea = exp2_fast(a), eb = exp2_fast(b);
-            s0 += ea;
-            s1 += eb;
+            s0 = __fadd_rn(s0, ea);
+            s1 = __fadd_rn(s1, eb);
             if constexpr (ENT) {
                 t0 = fmaf(ea, fmaxf(a, kFarBelow), t0);
                 t1 = fmaf(eb, fmaxf(b, kFarBelow), t1);
             }
         }
-        s += s0 + s1;
-        if constexpr (ENT) t += t0 + t1;
+        s = __fadd_rn(s, __fadd_rn(s0, s1));
+        if constexpr (ENT) t = __fadd_rn(t, __fadd_rn(t0, t1));
     }
     __device__ __forceinline__ void take1(float x, const Scale& c) {
         const float two[2] = {x, -INFINITY};
@@ -226,8 +316,8 @@ struct Running {
     // against the maximum M >= m
     __device__ __forceinline__ void move(float M, const Scale& c) {
         const float a = c.of(m - M), e = exp2_fast(a);
-        if constexpr (ENT) t = e * fmaf(s, fmaxf(a, kFarBelow), t);
-        s *= e;
+        if constexpr (ENT) t = __fmul_rn(e, fmaf(s, fmaxf(a, kFarBelow), t));
+        s = __fmul_rn(s, e);
         m = M;
     }
 };
@@ -280,130 +370,128 @@ __device__ __forceinline__ RowSums block_sums(Running<ENT>& a, const Scale& c, f
     return r;
 }
 
+// ---- the parts of a row: what each leaves for the others, and what they make of it (in the order of the parts, whoever does)
+struct PartSums {
+    float m, s, t, x;  // x: the logit of the row's token, from the part that has it
+};
+constexpr uint32_t kPartWords = 4u;  // 64-bit words a part: two, each twice
+__device__ __forceinline__ unsigned long long two_floats(float lo, float hi) { return (static_cast<unsigned long long>(__float_as_uint(hi)) << 32) | __float_as_uint(lo); }
+__device__ __forceinline__ float low_float(unsigned long long v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float high_float(unsigned long long v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+// part p's words among those of `parts`: m and s, t and x (BOTH: where somebody asks for them)
+template <bool BOTH>
+__device__ __forceinline__ void leave_part(unsigned long long* meet, uint32_t parts, uint32_t p, const PartSums& w, unsigned long long tag) {
+    leave_word(meet + p, parts, two_floats(w.m, w.s), tag);
+    if (BOTH) leave_word(meet + 2u * parts + p, parts, two_floats(w.t, w.x), tag);
+}
+template <bool BOTH>
+__device__ __forceinline__ bool find_part(const unsigned long long* meet, uint32_t parts, uint32_t p, unsigned long long tag, PartSums& w) {
+    unsigned long long ms, tx = 0ull;
+    const bool a = find_word(meet + p, parts, tag, ms), b = !BOTH || find_word(meet + 2u * parts + p, parts, tag, tx);
+    w = PartSums{low_float(ms), high_float(ms), low_float(tx), high_float(tx)};
+    return a && b;
+}
+template <bool BOTH>
+__device__ __forceinline__ void break_part(unsigned long long* meet, uint32_t parts, uint32_t p) {
+    break_word(meet + p, parts);
+    if (BOTH) break_word(meet + 2u * parts + p, parts);
+}
+template <bool ENT>
+__device__ __forceinline__ PartSums part_sums(const RowSums& r, float x) {
+    return PartSums{r.m, static_cast<float>(r.s), ENT ? static_cast<float>(r.t) : 0.f, x};
+}
+// a wave, a lane a part
+template <bool ENT>
+__device__ __forceinline__ RowSums join_parts(bool in, const PartSums& w, const Scale& c) {
+    RowSums r{};
+    const float m = in ? w.m : -FLT_MAX;
+    const double s = in ? static_cast<double>(w.s) : 0.0;
+    r.m = wave_max(m);
+    const float d = c.of(m - r.m);
+    const double e = static_cast<double>(exp2_fast(d));
+    r.s = wave_sum(s * e);
+    if (ENT) r.t = wave_sum(e * ((in ? static_cast<double>(w.t) : 0.0) + s * static_cast<double>(fmaxf(d, kFarBelow))));
+    return r;
+}
+
 // ---- log-probabilities: a workgroup a row, or `parts` of them
 struct ScoreArgs {
     LossRows R;
     float* logprob;
     float* stats;
     float* entropy;
-    uint32_t parts;
-    unsigned long long* meet;  // parts > 1: [rows][parts][4 or 2] words
+    uint32_t parts, per;       // workgroups a row, vectors each
+    unsigned long long* meet;  // parts > 1: [rows][parts][kPartWords], broken again by whoever joins them
     unsigned long long tag;
-    // with a policy loss
-    PolicyIn P;
-    float* d_logprob;
-    float* d_entropy;
-    double* terms;  // [rows][kPolicySums]
 };
 
-template <bool POLICY>
-__device__ __forceinline__ void write_row(const ScoreArgs& A, uint32_t row, const RowSums& r, float inv_t, bool has_id, float x_id) {
-    const RowValue v = row_value(r, inv_t, has_id, x_id);
-    A.stats[2 * static_cast<size_t>(row)] = v.any ? r.m : -INFINITY;
-    A.stats[2 * static_cast<size_t>(row) + 1] = static_cast<float>(r.s);
-    A.logprob[row] = static_cast<float>(v.lp);
-    if (A.entropy) A.entropy[row] = static_cast<float>(v.H);
-    if constexpr (POLICY) {
-        const PolicyToken o = policy_token(A.P, row, policy_weight(A.P, row), v.lp, A.entropy ? v.H : 0.0);
-        A.d_logprob[row] = static_cast<float>(o.g);
-        if (A.d_entropy) A.d_entropy[row] = static_cast<float>(o.h);
-#pragma unroll
-        for (uint32_t k = 0; k < kPolicySums; ++k) A.terms[static_cast<size_t>(row) * kPolicySums + k] = o.sum[k];
-    }
-}
-// a row that counts for nothing
-__device__ __forceinline__ void write_no_row(const ScoreArgs& A, uint32_t row) {
-    A.logprob[row] = 0.f;
-    if (A.entropy) A.entropy[row] = 0.f;
-    if (A.d_logprob) A.d_logprob[row] = 0.f;
-    if (A.d_entropy) A.d_entropy[row] = 0.f;
-#pragma unroll
-    for (uint32_t k = 0; k < kPolicySums; ++k) A.terms[static_cast<size_t>(row) * kPolicySums + k] = 0.0;
-}
-
-template <int DT, bool ENT, bool MASK, bool POLICY, int T>
+template <int DT, bool ENT, bool MASK, int T>
 __global__ void __launch_bounds__(T) score_rows_kernel(ScoreArgs A) {
     constexpr uint32_t kPer = Elem<DT>::kPer, kU = 4u;  // vectors of a thread on their way together
     __shared__ float red_m[T / 64];
     __shared__ double red_s[T / 64], red_t[T / 64];
-    const uint32_t row = blockIdx.x / A.parts, part = blockIdx.x % A.parts, t = threadIdx.x, V = A.R.vocab;
+    const uint32_t row = grid_row(), part = blockIdx.x, t = threadIdx.x, V = A.R.vocab;
+    if (row >= A.R.rows) return;
+    const unsigned char* base = A.R.logits + row * A.R.row_bytes;
+    const RowSpan<DT> span(base, V);
+    const uint32_t j0 = min(part * A.per, span.vectors), j1 = min(j0 + A.per, span.vectors);
+    const Share<DT, MASK, T> share{base, MASK ? A.R.allow + row * A.R.allow_stride : nullptr, span.head, ((V + 31u) >> 5) * 4u - 1u, j0, j1};
+    uint4 q[kU];
+    if (j0 < j1) {
+#pragma unroll
+        for (uint32_t u = 0; u < kU; ++u) q[u] = share.load(j0 + u * T + t);
+    }
+    // (the row's own entries come while its logits do)
     const int32_t id = A.R.ids ? A.R.ids[row] : -1;
     const bool has_id = static_cast<uint32_t>(id) < V;
-    if constexpr (POLICY) {
-        if (!has_id || policy_weight(A.P, row) == 0.0) {  // (uniform)
-            if (part == 0u && t == 0u) write_no_row(A, row);
-            return;
-        }
-    }
-    const unsigned char* base = A.R.logits + row * A.R.row_bytes;
-    const uint32_t* allow = MASK ? A.R.allow + row * A.R.allow_stride : nullptr;
-    const uint32_t last_word = (V - 1u) >> 5;
     const float inv_t = A.R.inv_t ? A.R.inv_t[row] : 1.f;
     float x_id = -INFINITY;
-    if (has_id && (!MASK || allowed(allow, static_cast<uint32_t>(id)))) x_id = load_logit<DT>(base, static_cast<uint32_t>(id));
+    if (t < 64u && has_id && (!MASK || allowed(share.allow, static_cast<uint32_t>(id)))) x_id = load_logit<DT>(base, static_cast<uint32_t>(id));
     const Scale c(inv_t);
-    const RowSpan<DT> span(base, V);
-    const uint32_t per = (span.vectors + A.parts - 1u) / A.parts, j0 = min(part * per, span.vectors), j1 = min(j0 + per, span.vectors);
     Running<ENT> a;
-    auto get = [&](uint32_t j) {
-        uint4 q = *reinterpret_cast<const uint4*>(base + static_cast<size_t>(span.index(j)) * Elem<DT>::kBytes);
-        if constexpr (MASK) q = only_allowed<DT>(q, allowed_from(allow, span.index(j), last_word));
-        return q;
-    };
-    uint32_t j = j0 + t;
-    for (; j + (kU - 1u) * T < j1; j += kU * T) {
-        uint4 q[kU];
+    for (uint32_t jb = j0; jb < j1; jb += kU * T) {
+        uint4 next[kU];
+        const bool more = jb + kU * T < j1;
+        if (more) {
 #pragma unroll
-        for (uint32_t u = 0; u < kU; ++u) q[u] = get(j + u * T);
+            for (uint32_t u = 0; u < kU; ++u) next[u] = share.load(jb + (kU + u) * T + t);
+        }
 #pragma unroll
         for (uint32_t u = 0; u < kU; ++u) {
-            float x[kPer];
-            unpack<DT>(q[u], x);
-            a.take(x, c);
+            if (jb + u * T < j1) {  // (uniform)
+                float x[kPer];
+                unpack<DT>(share.own(q[u], jb + u * T), x);
+                a.take(x, c);
+            }
         }
-    }
-    for (; j < j1; j += T) {
-        float x[kPer];
-        unpack<DT>(get(j), x);
-        a.take(x, c);
+        if (more) {
+#pragma unroll
+            for (uint32_t u = 0; u < kU; ++u) q[u] = next[u];
+        }
     }
     if (part == 0u && t < span.rest) {
         const uint32_t i = span.rest_index(t);
-        if (!MASK || allowed(allow, i)) a.take1(load_logit<DT>(base, i), c);
+        if (!MASK || allowed(share.allow, i)) a.take1(load_logit<DT>(base, i), c);
     }
     RowSums r = block_sums<ENT, T>(a, c, red_m, red_s, red_t);
     if (t >= 64u) return;
     if (A.parts > 1u) {  // (at most 64)
-        constexpr uint32_t kWords = ENT ? 2u : 1u;
-        unsigned long long* meet = A.meet + static_cast<size_t>(row) * A.parts * (2u * kWords);
-        auto word = [&](uint32_t p, uint32_t k) { return meet + (p * kWords + k) * 2u; };
-        if (t == 0u) {
-            const float s = static_cast<float>(r.s);
-            leave_word(word(part, 0u), (static_cast<unsigned long long>(__float_as_uint(s)) << 32) | __float_as_uint(r.m), A.tag);
-            if (ENT) leave_word(word(part, kWords - 1u), static_cast<unsigned long long>(__double_as_longlong(r.t)), A.tag);
-        }
+        unsigned long long* meet = A.meet + static_cast<size_t>(row) * A.parts * kPartWords;
+        if (t == 0u) leave_part<ENT>(meet, A.parts, part, part_sums<ENT>(r, 0.f), A.tag);
         words_arrived();
         const bool in = t < A.parts;
-        unsigned long long ms = 0ull, tt = 0ull;
-        bool here = true;
-        if (in) {
-            here = find_word(word(t, 0u), A.tag, ms);
-            if (ENT) here = find_word(word(t, kWords - 1u), A.tag, tt) && here;
-        }
+        PartSums w{};
+        const bool here = !in || find_part<ENT>(meet, A.parts, t, A.tag, w);
         if (__ballot(!here) != 0ull) return;  // somebody is still to come
-        if (in) {
-            break_word(word(t, 0u));
-            if (ENT) break_word(word(t, kWords - 1u));
-        }
-        const float m = in ? __uint_as_float(static_cast<uint32_t>(ms)) : -FLT_MAX;
-        const double s = in ? static_cast<double>(__uint_as_float(static_cast<uint32_t>(ms >> 32))) : 0.0;
-        r.m = wave_max(m);
-        const float d = c.of(m - r.m);
-        const double e = static_cast<double>(exp2_fast(d));
-        r.s = wave_sum(s * e);
-        if (ENT) r.t = wave_sum(e * ((in ? __longlong_as_double(static_cast<long long>(tt)) : 0.0) + s * static_cast<double>(fmaxf(d, kFarBelow))));
+        if (in) break_part<ENT>(meet, A.parts, t);
+        r = join_parts<ENT>(in, w, c);
     }
-    if (t == 0u) write_row<POLICY>(A, row, r, inv_t, has_id, x_id);
+    if (t != 0u) return;
+    const RowValue v = row_value(r, inv_t, has_id, x_id);
+    A.stats[2 * static_cast<size_t>(row)] = v.any ? r.m : -INFINITY;
+    A.stats[2 * static_cast<size_t>(row) + 1] = static_cast<float>(r.s);
+    A.logprob[row] = static_cast<float>(v.lp);
+    if (ENT) A.entropy[row] = static_cast<float>(v.H);
 }
 
 // ---- the gradient
@@ -456,12 +544,15 @@ __device__ __forceinline__ uint4 slope_vector(const uint4& q, uint32_t first, co
 
 template <int DT, bool ENT, bool MASK, int T, int U>
 __global__ void __launch_bounds__(T) grad_rows_kernel(GradArgs A) {
-    const uint32_t row = blockIdx.x / A.chunks, chunk = blockIdx.x % A.chunks, t = threadIdx.x, V = A.R.vocab;
+    uint32_t row = grid_row();
+    if (row >= A.R.rows) return;
+    row = A.R.rows - 1u - row;
+    const uint32_t chunk = blockIdx.x, t = threadIdx.x, V = A.R.vocab;
     const unsigned char* base = A.R.logits + row * A.R.row_bytes;
     unsigned char* out = A.out + row * A.out_bytes;
     const RowSpan<DT> span(out, V);
     const uint32_t* allow = MASK ? A.R.allow + row * A.R.allow_stride : nullptr;
-    const uint32_t last_word = (V - 1u) >> 5;
+    const uint32_t last_byte = ((V + 31u) >> 5) * 4u - 1u;
     const float inv_t = A.R.inv_t ? A.R.inv_t[row] : 1.f;
     const int32_t id = A.R.ids ? A.R.ids[row] : -1;
     const bool has_id = static_cast<uint32_t>(id) < V;
@@ -483,7 +574,7 @@ __global__ void __launch_bounds__(T) grad_rows_kernel(GradArgs A) {
         const uint32_t j = j0 + u * T;
         if (j < span.vectors) {
             q[u] = load_loose(base + static_cast<size_t>(span.index(j)) * Elem<DT>::kBytes);
-            if constexpr (MASK) q[u] = only_allowed<DT>(q[u], allowed_from(allow, span.index(j), last_word));
+            if constexpr (MASK) q[u] = only_allowed<DT>(q[u], allowed_from(allow, span.index(j), last_byte));
         }
     }
     if (chunk == 0u && t < span.rest) {
@@ -500,132 +591,233 @@ __global__ void __launch_bounds__(T) grad_rows_kernel(GradArgs A) {
     }
 }
 
-// ---- the policy loss from logits to its gradient, a workgroup a row: what of the row the registers hold (NV vectors a thread) is read
-// once, the rest of a longer row a second time.
+// ---- the policy loss from logits to its gradient in one pass: the parts of a row (one, or up to 64 workgroups) keep their share in registers, NV vectors
+// a thread, leave their sums for each other, wait for the others' and write the share's gradient. The wait is bounded, since nothing says
+// that all parts run at once: a part that does not find another's words in time works that part's sums out itself, in the
+// same order and so to the same bits. (Where the gradient goes over the logits: a part writes only after its words have arrived. So logits
+// read before a look that still finds no words are the logits, and the token's logit goes with the words, not to be read
+// by a part that comes late.) The words stay until every part has seen them. Few rows' terms meet in this launch, and the parts leave a mark each when they
+// are through: whoever sees all marks of a row breaks its words. Of more rows a second launch adds up the terms and breaks the words: it costs 5 us, and a
+// wave that looks at all rows' words as much from some 500 rows on.
 struct RowsArgs {
-    ScoreArgs S;
+    LossRows R;
+    PolicyIn P;
+    float* logprob;
+    float* entropy;
     unsigned char* out;
     uint64_t out_bytes;
+    double* terms;             // [kPolicySums][rows], or:
+    unsigned long long* sums_meet;  // [kPolicySums][2][rows], for rows that meet in this launch
+    float* sums;
+    uint32_t parts, per;       // workgroups a row, vectors each
+    unsigned long long* meet;  // parts > 1: [rows][kPartWords][parts]; of rows that meet in this launch [rows][kPartWords + 2][parts], the last two the parts' marks
+    unsigned long long tag;
 };
-template <int DT, bool ENT, bool SLOPE, bool MASK, int T, int NV>
-__global__ void __launch_bounds__(T) policy_rows_kernel(RowsArgs B) {
+constexpr uint32_t kLooks = 256u;  // some 0.3 ms; the others usually come within microseconds
+
+template <int DT, bool ENT, bool SLOPE, bool MASK, int T, int NV, int WAVES>  // WAVES: a SIMD's at least
+__global__ void __launch_bounds__(T, WAVES) policy_rows_kernel(RowsArgs A) {
     constexpr uint32_t kPer = Elem<DT>::kPer;
     __shared__ float red_m[T / 64];
     __shared__ double red_s[T / 64], red_t[T / 64];
     __shared__ RowSlope shared_slope;
-    const ScoreArgs& A = B.S;
-    const uint32_t row = blockIdx.x, t = threadIdx.x, V = A.R.vocab;
+    __shared__ unsigned long long missing;
+    __shared__ PartSums found[64];
+    const uint32_t row = grid_row(), part = blockIdx.x, t = threadIdx.x, V = A.R.vocab, per = A.per;
+    if (row >= A.R.rows) return;
     const unsigned char* base = A.R.logits + row * A.R.row_bytes;
-    unsigned char* out = B.out + row * B.out_bytes;
+    unsigned char* out = A.out + row * A.out_bytes;
     const RowSpan<DT> span(out, V);
+    const uint32_t j0 = min(part * per, span.vectors), j1 = min(j0 + per, span.vectors);
     const int32_t id = A.R.ids[row];
     const bool has_id = static_cast<uint32_t>(id) < V;
+    const double weight = policy_weight(A.P, row);
+    const bool rest = part == 0u && t < span.rest;
+    const uint32_t rest_i = rest ? span.rest_index(t) : 0u;
     auto store = [&](uint32_t j, const uint4& q) { *reinterpret_cast<uint4*>(out + static_cast<size_t>(span.index(j)) * Elem<DT>::kBytes) = q; };
     auto nothing = [&]() {
-        for (uint32_t j = t; j < span.vectors; j += T) store(j, make_uint4(0u, 0u, 0u, 0u));
-        if (t < span.rest) store_logit<DT>(out, span.rest_index(t), 0.f);
+        for (uint32_t j = j0 + t; j < j1; j += T) store(j, make_uint4(0u, 0u, 0u, 0u));
+        if (rest) store_logit<DT>(out, rest_i, 0.f);
     };
-    if (!has_id || policy_weight(A.P, row) == 0.0) {  // (uniform) not read
+    unsigned long long* meet = A.meet + static_cast<size_t>(row) * A.parts * (A.terms ? kPartWords : kPartWords + 2u);
+    double terms[kPolicySums] = {};
+    auto leave_terms = [&]() {  // the row's, by the first thread of its first part
+        if (!A.terms) return leave_sums(A.sums_meet, A.R.rows, row, terms, A.tag);
+#pragma unroll
+        for (uint32_t k = 0; k < kPolicySums; ++k) A.terms[static_cast<size_t>(k) * A.R.rows + row] = terms[k];
+    };
+    auto finish = [&]() {  // by its first wave, when everything else is done
+        if (A.terms || !gather_sums(A.sums_meet, A.R.rows, terms, A.tag)) return;
+#pragma unroll
+        for (uint32_t k = 0; k < kPolicySums; ++k)
+            if (t == 0u) A.sums[k] = static_cast<float>(terms[k]);
+    };
+    if (!has_id || weight == 0.0) {  // (uniform) counts for nothing: not read
+        if (part == 0u && t == 0u) {
+            A.logprob[row] = 0.f;
+            if (A.entropy) A.entropy[row] = 0.f;
+            leave_terms();
+        }
         nothing();
-        if (t == 0u) write_no_row(A, row);
+        if (part == 0u && t < 64u) {
+            words_arrived();
+            finish();
+        }
         return;
     }
     const uint32_t* allow = MASK ? A.R.allow + row * A.R.allow_stride : nullptr;
-    const uint32_t last_word = (V - 1u) >> 5;
-    const float inv_t = A.R.inv_t ? A.R.inv_t[row] : 1.f;
-    auto get = [&](uint32_t j) {
-        uint4 q = load_loose(base + static_cast<size_t>(span.index(j)) * Elem<DT>::kBytes);
-        if constexpr (MASK) q = only_allowed<DT>(q, allowed_from(allow, span.index(j), last_word));
-        return q;
-    };
+    const Share<DT, MASK, T> share{base, allow, span.head, ((V + 31u) >> 5) * 4u - 1u, j0, j1};
     uint4 q[NV];
+    if (j0 < j1) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const uint32_t j = k * T + t;
-        q[k] = make_uint4(Elem<DT>::kNone, Elem<DT>::kNone, Elem<DT>::kNone, Elem<DT>::kNone);
-        if (j < span.vectors) q[k] = get(j);
+        for (int k = 0; k < NV; ++k)
+            if (k == 0 || j0 + k * T < j1) q[k] = share.load(j0 + k * T + t);  // (uniform)
     }
-    float x_id = -INFINITY;
-    if (t == 0u && (!MASK || allowed(allow, static_cast<uint32_t>(id)))) x_id = load_logit<DT>(base, static_cast<uint32_t>(id));
     float x_rest = -INFINITY;
-    if (t < span.rest) {
-        const uint32_t i = span.rest_index(t);
-        if (!MASK || allowed(allow, i)) x_rest = load_logit<DT>(base, i);
+    if (rest && (!MASK || allowed(allow, rest_i))) x_rest = load_logit<DT>(base, rest_i);
+    const float inv_t = A.R.inv_t ? A.R.inv_t[row] : 1.f;
+    // the part that has the row's token, and its logit
+    const uint32_t id_at = static_cast<uint32_t>(id) - span.head, id_part = id_at / kPer < span.vectors ? id_at / kPer / per : 0u;
+    auto token_logit = [&]() { return !MASK || allowed(allow, static_cast<uint32_t>(id)) ? load_logit<DT>(base, static_cast<uint32_t>(id)) : -INFINITY; };
+    PolicyRow token{};
+    float x_id = 0.f;
+    if (t < 64u) {  // (uniform for the wave)
+        token = policy_row(A.P, row);
+        if (part == id_part) x_id = token_logit();
     }
     const Scale c(inv_t);
     Running<ENT> a;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        if (k * T < span.vectors) {  // (uniform)
+        if (j0 + k * T < j1) {  // (uniform)
             float x[kPer];
-            unpack<DT>(q[k], x);
+            unpack<DT>(share.own(q[k], j0 + k * T), x);
             a.take(x, c);
         }
     }
-    for (uint32_t j = NV * T + t; j < span.vectors; j += T) {
-        float x[kPer];
-        unpack<DT>(get(j), x);
-        a.take(x, c);
+    if (rest) a.take1(x_rest, c);
+    RowSums r = block_sums<ENT, T>(a, c, red_m, red_s, red_t);
+    if (A.parts > 1u) {
+        if (t < 64u) {
+            if (t == 0u) leave_part<true>(meet, A.parts, part, part_sums<ENT>(r, x_id), A.tag);
+            words_arrived();
+            const bool in = t < A.parts;
+            PartSums w{};
+            bool here = !in;
+            for (uint32_t look = 0; look < kLooks; ++look) {
+                if (!here) here = find_part<true>(meet, A.parts, t, A.tag, w);
+                if (__ballot(!here) == 0ull) break;
+                __builtin_amdgcn_s_sleep(4);
+            }
+            const unsigned long long late = __ballot(!here);
+            found[t] = w;
+            if (t == 0u) missing = late;
+        }
+        __syncthreads();
+        for (unsigned long long late = missing; late; late &= late - 1ull) {  // (uniform)
+            const uint32_t p = static_cast<uint32_t>(__ffsll(late) - 1), p0 = min(p * per, span.vectors), p1 = min(p0 + per, span.vectors);
+            const Share<DT, MASK, T> theirs{base, allow, span.head, share.last_byte, p0, p1};
+            Running<ENT> b;
+            for (uint32_t jb = p0; jb < p1; jb += T) {
+                float x[kPer];
+                unpack<DT>(theirs.own(theirs.load(jb + t), jb), x);
+                b.take(x, c);
+            }
+            if (p == 0u && t < span.rest) {
+                const uint32_t i = span.rest_index(t);
+                b.take1(!MASK || allowed(allow, i) ? load_logit<DT>(base, i) : -INFINITY, c);
+            }
+            const float x_late = t == 0u && p == id_part ? token_logit() : 0.f;
+            __syncthreads();
+            const RowSums o = block_sums<ENT, T>(b, c, red_m, red_s, red_t);
+            if (t == 0u) {  // (everybody's logits have come: the barrier in block_sums)
+                PartSums w = part_sums<ENT>(o, x_late), came{};
+                words_arrived();
+                if (find_part<true>(meet, A.parts, p, A.tag, came)) w = came;
+                found[p] = w;
+            }
+        }
+        if (t < 64u) {
+            __builtin_amdgcn_wave_barrier();  // (one wave: its LDS stores are done before its loads)
+            r = join_parts<ENT>(t < A.parts, found[t], c);
+            x_id = found[id_part].x;
+            if (t == 0u && !A.terms) leave_word(meet + kPartWords * A.parts + part, A.parts, 0ull, A.tag);  // (the mark)
+        }
     }
-    if (t < span.rest) a.take1(x_rest, c);
-    const RowSums r = block_sums<ENT, T>(a, c, red_m, red_s, red_t);
     if (t == 0u) {
         const RowValue v = row_value(r, inv_t, true, x_id);
-        A.logprob[row] = static_cast<float>(v.lp);
-        if (A.entropy) A.entropy[row] = static_cast<float>(v.H);
-        const PolicyToken o = policy_token(A.P, row, policy_weight(A.P, row), v.lp, ENT ? v.H : 0.0);
-#pragma unroll
-        for (uint32_t k = 0; k < kPolicySums; ++k) A.terms[static_cast<size_t>(row) * kPolicySums + k] = o.sum[k];
+        const PolicyToken o = policy_token(A.P, token, v.lp, ENT ? v.H : 0.0);
         shared_slope = row_slope<SLOPE>(r.m, static_cast<float>(r.s), inv_t, static_cast<float>(o.g), static_cast<float>(o.h), static_cast<float>(v.H));
+        if (part == 0u) {
+            A.logprob[row] = static_cast<float>(v.lp);
+            if (ENT) A.entropy[row] = static_cast<float>(v.H);
+#pragma unroll
+            for (uint32_t k = 0; k < kPolicySums; ++k) terms[k] = o.sum[k];
+            leave_terms();
+        }
     }
     __syncthreads();
     const RowSlope s = shared_slope;
-    if (s.none) {
+    if (s.none) {  // (uniform)
         nothing();
-        return;
-    }
+    } else {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const uint32_t j = k * T + t;
-        if (j < span.vectors) store(j, slope_vector<DT, SLOPE>(q[k], span.index(j), s, c, static_cast<uint32_t>(id)));
+        for (int k = 0; k < NV; ++k) {
+            const uint32_t j = j0 + k * T + t;
+            if (j < j1) store(j, slope_vector<DT, SLOPE>(q[k], span.index(j), s, c, static_cast<uint32_t>(id)));
+        }
+        if (rest) {
+            float y = slope_at<SLOPE>(x_rest, s, c);
+            if (rest_i == static_cast<uint32_t>(id) && x_rest != -INFINITY) y += s.at_id;
+            store_logit<DT>(out, rest_i, y);
+        }
     }
-    for (uint32_t j = NV * T + t; j < span.vectors; j += T) store(j, slope_vector<DT, SLOPE>(get(j), span.index(j), s, c, static_cast<uint32_t>(id)));
-    if (t < span.rest) {
-        const uint32_t i = span.rest_index(t);
-        float y = slope_at<SLOPE>(x_rest, s, c);
-        if (i == static_cast<uint32_t>(id) && x_rest != -INFINITY) y += s.at_id;
-        store_logit<DT>(out, i, y);
+    if (t >= 64u || A.terms) return;
+    words_arrived();
+    if (A.parts > 1u) {
+        unsigned long long* marks = meet + kPartWords * A.parts;
+        unsigned long long mark;
+        const bool in = t < A.parts, here = !in || find_word(marks + t, A.parts, A.tag, mark);
+        if (__ballot(!here) == 0ull && in) {  // everybody is through
+            break_part<true>(meet, A.parts, t);
+            break_word(marks + t, A.parts);
+        }
     }
+    if (part == 0u) finish();
 }
 
-// ---- sums of a batch's tokens: at most 64 workgroups, whose partial sums meet
+// ---- the loss over log-probabilities, or the sum of rows' terms: the workgroups' sums meet
 struct PolicyArgs {
     PolicyIn P;
     uint32_t rows;
     const float* logprob;
     const float* entropy;
-    const double* terms;  // the rows' terms, already worked out (then nothing else is read or written but the sums)
+    const double* terms;  // [kPolicySums][rows]: worked out already (then only they are read, and only the sums written)
     float* d_logprob;
     float* d_entropy;
     float* sums;
-    unsigned long long* meet;  // [workgroups][kPolicySums][2]
+    unsigned long long* meet;  // [kPolicySums][2][workgroups]
     unsigned long long tag;
+    unsigned long long* words;  // the rows' parts' words, to be broken
+    uint64_t n_words;
 };
 
 template <int T>
 __global__ void __launch_bounds__(T) policy_kernel(PolicyArgs A) {
     __shared__ double red[kPolicySums][T / 64];
     const uint32_t t = threadIdx.x, groups = gridDim.x;
+    for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * T + t; i < A.n_words; i += static_cast<uint64_t>(groups) * T) A.words[i] = 0ull;
     double sum[kPolicySums] = {};
     for (uint32_t row = blockIdx.x * T + t; row < A.rows; row += groups * T) {
         if (A.terms) {
 #pragma unroll
-            for (uint32_t k = 0; k < kPolicySums; ++k) sum[k] += A.terms[static_cast<size_t>(row) * kPolicySums + k];
+            for (uint32_t k = 0; k < kPolicySums; ++k) sum[k] += A.terms[static_cast<size_t>(k) * A.rows + row];
             continue;
         }
-        const double w = policy_weight(A.P, row);
+        const PolicyRow token = policy_row(A.P, row);
+        const double lp = static_cast<double>(A.logprob[row]), H = A.entropy ? static_cast<double>(A.entropy[row]) : 0.0;
         PolicyToken o{};
-        if (w != 0.0) o = policy_token(A.P, row, w, static_cast<double>(A.logprob[row]), A.entropy ? static_cast<double>(A.entropy[row]) : 0.0);
+        if (token.weight != 0.0) o = policy_token(A.P, token, lp, H);
         A.d_logprob[row] = static_cast<float>(o.g);
         if (A.d_entropy) A.d_entropy[row] = static_cast<float>(o.h);
 #pragma unroll
@@ -641,25 +833,9 @@ __global__ void __launch_bounds__(T) policy_kernel(PolicyArgs A) {
 #pragma unroll
     for (uint32_t k = 0; k < kPolicySums; ++k) sum[k] = wave_sum(t < T / 64u ? red[k][t] : 0.0);
     if (groups > 1u) {
-        auto word = [&](uint32_t p, uint32_t k) { return A.meet + (static_cast<size_t>(p) * kPolicySums + k) * 2u; };
-        if (t == 0u) {
-#pragma unroll
-            for (uint32_t k = 0; k < kPolicySums; ++k) leave_word(word(blockIdx.x, k), static_cast<unsigned long long>(__double_as_longlong(sum[k])), A.tag);
-        }
+        if (t == 0u) leave_sums(A.meet, groups, blockIdx.x, sum, A.tag);
         words_arrived();
-        bool here = true;
-        unsigned long long v[kPolicySums] = {};
-        if (t < groups) {
-#pragma unroll
-            for (uint32_t k = 0; k < kPolicySums; ++k) here = find_word(word(t, k), A.tag, v[k]) && here;
-        }
-        if (__ballot(!here) != 0ull) return;
-        if (t < groups) {
-#pragma unroll
-            for (uint32_t k = 0; k < kPolicySums; ++k) break_word(word(t, k));
-        }
-#pragma unroll
-        for (uint32_t k = 0; k < kPolicySums; ++k) sum[k] = wave_sum(t < groups ? __longlong_as_double(static_cast<long long>(v[k])) : 0.0);
+        if (!gather_sums(A.meet, groups, sum, A.tag)) return;
     }
     if (t == 0u) {
 #pragma unroll
@@ -679,7 +855,7 @@ struct PreferenceArgs {
     float* pair_loss;
     float* reward;
     float* d_logprob;
-    unsigned long long* meet;  // [workgroups][2]
+    unsigned long long* meet;  // [2][workgroups]
     unsigned long long tag;
 };
 __device__ __forceinline__ double softplus(double v) { return fmax(v, 0.0) + log1p(exp(-fabs(v))); }
@@ -726,21 +902,13 @@ __global__ void __launch_bounds__(T) preference_kernel(PreferenceArgs A) {
     for (uint32_t row = blockIdx.x * T + t; row < first; row += groups * T) A.d_logprob[row] = 0.f;
     for (uint32_t row = behind + blockIdx.x * T + t; row < A.rows; row += groups * T) A.d_logprob[row] = 0.f;
     if (t >= 64u) return;
+    double sum[1] = {mine};
     if (groups > 1u) {
-        if (t == 0u) leave_word(A.meet + 2u * blockIdx.x, static_cast<unsigned long long>(__double_as_longlong(mine)), A.tag);
+        if (t == 0u) leave_sums(A.meet, groups, blockIdx.x, sum, A.tag);
         words_arrived();
-        bool here = true;
-        double all = 0.0;
-        for (uint32_t p = t; p < groups; p += 64u) {
-            unsigned long long v;
-            here = find_word(A.meet + 2u * p, A.tag, v) && here;
-            all += __longlong_as_double(static_cast<long long>(v));
-        }
-        if (__ballot(!here) != 0ull) return;
-        for (uint32_t p = t; p < groups; p += 64u) break_word(A.meet + 2u * p);
-        mine = wave_sum(all);
+        if (!gather_sums(A.meet, groups, sum, A.tag)) return;
     }
-    if (t == 0u) A.loss[0] = static_cast<float>(mine);
+    if (t == 0u) A.loss[0] = static_cast<float>(sum[0]);
 }
 
 }  // namespace ws

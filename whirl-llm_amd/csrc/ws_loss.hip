@@ -5,23 +5,41 @@
 namespace ws {
 
 namespace {
-constexpr uint32_t kScoreThreads = 256u, kGradThreads = 256u, kGradVectors = 4u;
+constexpr uint32_t kScoreThreads = 256u, kGradThreads = 256u, kGradVectors = 4u, kPolicyThreads = 1024u;
 
-template <int DT, bool ENT, bool MASK, bool POLICY>
-void score(hipStream_t stream, const ScoreArgs& a) {
-    hipLaunchKernelGGL((score_rows_kernel<DT, ENT, MASK, POLICY, kScoreThreads>), dim3(a.R.rows * a.parts), dim3(kScoreThreads), 0, stream, a);
+template <int DT, bool ENT, bool MASK>
+struct Score {
+    static void go(hipStream_t s, const ScoreArgs& a) {
+        hipLaunchKernelGGL((score_rows_kernel<DT, ENT, MASK, kScoreThreads>), grid_of(a.parts, a.R.rows), dim3(kScoreThreads), 0, s, a);
+    }
+};
+template <int DT, bool ENT, bool MASK>
+struct Grad {
+    static void go(hipStream_t s, const GradArgs& a) {
+        hipLaunchKernelGGL((grad_rows_kernel<DT, ENT, MASK, kGradThreads, kGradVectors>), grid_of(a.chunks, a.R.rows), dim3(kGradThreads), 0, s, a);
+    }
+};
+// the builds of policy_rows_kernel: threads, vectors a thread
+constexpr uint32_t kSmallShare = 4u * 256u, kMostShare = 12u * 256u;
+template <int DT, bool ENT, bool SLOPE, bool MASK, int T, int NV, int WAVES>
+void rows(hipStream_t s, const RowsArgs& a) {
+    hipLaunchKernelGGL((policy_rows_kernel<DT, ENT, SLOPE, MASK, T, NV, WAVES>), grid_of(a.parts, a.R.rows), dim3(T), 0, s, a);
 }
 template <int DT, bool ENT, bool MASK>
-void grad(hipStream_t stream, const GradArgs& a) {
-    hipLaunchKernelGGL((grad_rows_kernel<DT, ENT, MASK, kGradThreads, kGradVectors>), dim3(a.R.rows * a.chunks), dim3(kGradThreads), 0, stream, a);
-}
-template <int DT, bool ENT, bool SLOPE, bool MASK>
-void rows(hipStream_t stream, const RowsArgs& b) {
-    const uint32_t vectors = b.S.R.vocab / Elem<DT>::kPer;
-    if (vectors <= 20u * 256u) hipLaunchKernelGGL((policy_rows_kernel<DT, ENT, SLOPE, MASK, 256, 20>), dim3(b.S.R.rows), dim3(256), 0, stream, b);
-    else if (vectors <= 20u * 512u) hipLaunchKernelGGL((policy_rows_kernel<DT, ENT, SLOPE, MASK, 512, 20>), dim3(b.S.R.rows), dim3(512), 0, stream, b);
-    else hipLaunchKernelGGL((policy_rows_kernel<DT, ENT, SLOPE, MASK, 1024, 19>), dim3(b.S.R.rows), dim3(1024), 0, stream, b);
-}
+struct Rows {
+    template <bool SLOPE>
+    static void of_size(hipStream_t s, const RowsArgs& a) {
+        const uint32_t share = a.per;
+        if (share <= kSmallShare) rows<DT, ENT, SLOPE, MASK, 256, 4, 6>(s, a);
+        else rows<DT, ENT, SLOPE, MASK, 256, 12, 5>(s, a);
+    }
+    static void go(hipStream_t s, const RowsArgs& a, bool slope) {
+        if constexpr (ENT) {
+            if (slope) return of_size<true>(s, a);
+        }
+        of_size<false>(s, a);
+    }
+};
 template <template <int, bool, bool> class F, class... A>
 void by_kind(int dtype, bool ent, bool mask, A&&... a) {
     if (dtype == 0) {
@@ -32,27 +50,6 @@ void by_kind(int dtype, bool ent, bool mask, A&&... a) {
         else mask ? F<1, false, true>::go(a...) : F<1, false, false>::go(a...);
     }
 }
-template <int DT, bool ENT, bool MASK>
-struct Score {
-    static void go(hipStream_t s, const ScoreArgs& a) { score<DT, ENT, MASK, false>(s, a); }
-};
-template <int DT, bool ENT, bool MASK>
-struct ScorePolicy {
-    static void go(hipStream_t s, const ScoreArgs& a) { score<DT, ENT, MASK, true>(s, a); }
-};
-template <int DT, bool ENT, bool MASK>
-struct Grad {
-    static void go(hipStream_t s, const GradArgs& a) { grad<DT, ENT, MASK>(s, a); }
-};
-template <int DT, bool ENT, bool MASK>
-struct Rows {
-    static void go(hipStream_t s, const RowsArgs& b, bool slope) {
-        if constexpr (ENT) {
-            if (slope) return rows<DT, true, true, MASK>(s, b);
-        }
-        rows<DT, ENT, false, MASK>(s, b);
-    }
-};
 }  // namespace
 
 uint32_t loss_grad_chunks(int dtype, uint32_t vocab) {
@@ -60,10 +57,10 @@ uint32_t loss_grad_chunks(int dtype, uint32_t vocab) {
     return vectors ? (vectors + each - 1u) / each : 1u;
 }
 uint32_t loss_threads() { return kScoreThreads; }
+uint32_t loss_most_share() { return kMostShare; }
 
-int launch_score(hipStream_t stream, int dtype, const ScoreArgs& a, bool policy) {
-    if (policy) by_kind<ScorePolicy>(dtype, a.entropy != nullptr, a.R.allow != nullptr, stream, a);
-    else by_kind<Score>(dtype, a.entropy != nullptr, a.R.allow != nullptr, stream, a);
+int launch_score(hipStream_t stream, int dtype, const ScoreArgs& a) {
+    by_kind<Score>(dtype, a.entropy != nullptr, a.R.allow != nullptr, stream, a);
     return static_cast<int>(hipGetLastError());
 }
 
@@ -72,13 +69,13 @@ int launch_grad(hipStream_t stream, int dtype, const GradArgs& a) {
     return static_cast<int>(hipGetLastError());
 }
 
-int launch_policy_rows(hipStream_t stream, int dtype, const RowsArgs& b, bool slope) {
-    by_kind<Rows>(dtype, b.S.entropy != nullptr, b.S.R.allow != nullptr, stream, b, slope);
+int launch_policy_rows(hipStream_t stream, int dtype, const RowsArgs& a, bool slope) {
+    by_kind<Rows>(dtype, a.entropy != nullptr, a.R.allow != nullptr, stream, a, slope);
     return static_cast<int>(hipGetLastError());
 }
 
 int launch_policy(hipStream_t stream, const PolicyArgs& a, unsigned groups) {
-    hipLaunchKernelGGL(policy_kernel<512>, dim3(groups), dim3(512), 0, stream, a);
+    hipLaunchKernelGGL(policy_kernel<kPolicyThreads>, dim3(groups), dim3(kPolicyThreads), 0, stream, a);
     return static_cast<int>(hipGetLastError());
 }
 
