@@ -193,7 +193,7 @@ def tokens(n, seed, with_ref=True, with_weight=True):
     return t
 
 
-@pytest.mark.parametrize("n", [1, 2, 63, 64, 65, 511, 512, 513, 5000, 32768, 70001])
+@pytest.mark.parametrize("n", [1, 2, 63, 64, 65, 511, 512, 513, 1024, 1025, 5000, 32768, 70001, 300000])
 @pytest.mark.parametrize("kind", ["plain", "all"])
 def test_policy_loss(n, kind):
     """Everything in 64 bits and rounded once: half a step each."""
@@ -231,14 +231,15 @@ def test_policy_loss_of_no_tokens():
     assert m.token_logprobs_grad(logits, torch.empty(0, dtype=torch.int32, device=DEV), stats).shape == (0, 100)
 
 
-# rows of one workgroup and of several, of both builds (shares of up to 1024 and 3072 vectors), up to 512 rows in one launch, more in two
-ROWS = [(600, 777), (520, 12400), (513, 25001), (1, 1), (1, 129), (7, 1000), (16, 50257), (3, 151936), (5, 262144), (130, 3), (140, 1001), (130, 20480), (129, 20485), (128, 40961), (130, 50257), (128, 81921), (128, 151936),
+# rows of one workgroup and of several, of all builds (shares of up to 256, 1024 and 3072 vectors); sums over up to 64, 1024 and 4096 rows, and over more in a second launch
+ROWS = [(600, 777), (520, 12400), (513, 25001), (1030, 1100), (4096, 261), (4097, 300), (1, 1), (1, 129), (7, 1000), (16, 50257), (3, 151936), (5, 262144), (130, 3), (140, 1001), (130, 20480), (129, 20485), (128, 40961), (130, 50257), (128, 81921), (128, 151936),
         (128, 160007)]
 
 
-@pytest.mark.parametrize("rows,V", ROWS)
-@pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("kind", ["plain", "entropy", "bonus", "masked"])
+POLICY_CASES = [(rows, V, dtype, kind) for rows, V in ROWS for dtype in (F32, BF16) for kind in ("plain", "entropy", "bonus", "masked")] + [(4100, 12500, F32, "bonus")]
+
+
+@pytest.mark.parametrize("rows,V,dtype,kind", POLICY_CASES)
 def test_policy_loss_rows(rows, V, dtype, kind):
     m = gc.pkg()
     c = make(rows, V, dtype, 13 * rows + V, kind == "masked", 0 if kind == "plain" else 3, 0 if kind == "plain" else 1)

@@ -66,9 +66,7 @@ int launch_grad(hipStream_t stream, int dtype, const GradArgs& a);
 int launch_policy_rows(hipStream_t stream, int dtype, const RowsArgs& a, bool slope);
 int launch_policy(hipStream_t stream, const PolicyArgs& a, unsigned groups);
 int launch_preference(hipStream_t stream, const PreferenceArgs& a, unsigned groups);
-uint32_t loss_threads();
 uint32_t loss_most_share();  // vectors of a row that a workgroup of policy_rows_kernel holds
-uint32_t loss_grad_chunks(int dtype, uint32_t vocab);
 }  // namespace ws
 
 namespace {
@@ -1107,8 +1105,9 @@ bool gradient_ok(const ws_loss_rows* r, const void* d, uint64_t stride) {
 ws::LossRows loss_rows(const ws_loss_rows* r) {
     return ws::LossRows{static_cast<const unsigned char*>(r->logits), r->row_stride * elem_bytes(r->dtype), r->rows, r->vocab, r->ids, r->inv_t, r->allow, r->allow_stride};
 }
-uint32_t row_vectors(const ws_loss_rows* r) { return r->vocab / (r->dtype == WS_DTYPE_F32 ? 4u : 8u); }
-uint32_t share_of(uint32_t vectors, uint32_t parts) { return (vectors + parts - 1u) / parts; }
+// the most vectors of 16 bytes of a row, counted from a boundary of 128 bytes (RowSpan), and a share of them, whole lines
+uint32_t row_vectors(const ws_loss_rows* r) { return r->vocab / (r->dtype == WS_DTYPE_F32 ? 4u : 8u) + 7u; }
+uint32_t share_of(uint32_t vectors, uint32_t parts) { return ((vectors + parts - 1u) / parts + 7u) & ~7u; }
 // Workgroups a row of the log-probabilities: of 1536 vectors (six a thread), or of fewer where rows are few, 512 vectors at least, four a compute unit.
 uint32_t score_parts(const ws_loss_rows* r) {
     const uint32_t vectors = row_vectors(r), most = vectors / 512u;
@@ -1118,6 +1117,15 @@ uint32_t score_parts(const ws_loss_rows* r) {
     return parts < 2u ? 1u : (parts > 64u ? 64u : parts);
 }
 uint64_t meet_bytes(uint32_t rows, uint32_t parts, uint32_t words) { return parts > 1u ? uint64_t{rows} * parts * words * 8u : 0u; }
+// From which row on the gradient goes past the caches. The kernels take the rows from the last to the first, since logits that a product has just made are still in the memory-side cache (256 MiB)
+// at their end, and whoever reads the gradient begins at its front: of that, half the cache's size is left there, what is written before would be gone by then and only
+// drive out logits. A pass alone over three sets of inputs in turn, and what it adds between a copy that makes the logits and a reader of the gradient, us: everything past the caches,
+// everything through them, this: the policy step on 600 x 128256 bf16 72 / 61, 74 / 48, 71 / 45; on 3000 x 50257 131 / 125, 136 / 97, 134 / 102; on 4000 x 151936 456 / 433, 466 / 412,
+// 457 / 408; scores and their gradient of 1400 x 128256 194 / 177, 206 / 155, 204 / 154 (rows from the first to the last, through the caches: 209 / 206).
+uint32_t past_row(const ws_loss_rows* r) {
+    const uint64_t row = uint64_t{r->vocab} * elem_bytes(r->dtype), rows = (128u << 20) / row;
+    return rows < r->rows ? static_cast<uint32_t>(rows) : r->rows;
+}
 bool workspace_ok(const void* w, uint64_t bytes, uint64_t need) { return need == 0 || (w && bytes >= need && aligned(w, 8u)); }
 
 bool policy_ok(const ws_policy* p, uint32_t rows, bool entropy) {
@@ -1128,17 +1136,11 @@ bool policy_ok(const ws_policy* p, uint32_t rows, bool entropy) {
 ws::PolicyIn policy_in(const ws_policy* p, uint32_t rows) {
     return ws::PolicyIn{p->old_logprob, p->ref_logprob, p->advantage, p->weight, rows ? 1.0 / rows : 0.0, p->clip_low, p->clip_high, p->dual_clip, p->kl_coef, p->entropy_coef};
 }
-// workgroups of a sum over tokens
-uint32_t policy_groups(uint32_t rows) {
-    const uint32_t n = (rows + 1023u) / 1024u;
-    return n < 1u ? 1u : (n > 64u ? 64u : n);
-}
-uint64_t policy_meet_bytes(uint32_t slots) { return uint64_t{slots} * ws::kPolicySums * 16u; }
+// workgroups of a sum over tokens, of one over pairs
+uint32_t policy_groups(uint32_t rows) { return rows <= 1024u ? 1u : (rows > (256u << 10) ? 256u : (rows + 1023u) / 1024u); }
 uint32_t preference_groups(uint32_t pairs) { return pairs > 256u ? 256u : pairs; }
 
-// The workspace of ws_policy_loss_rows: the words of the sum's workgroups or rows, those of the rows' parts, the rows' terms. One launch where rows are few,
-// a second one adds up the terms of more (policy_rows_kernel).
-constexpr uint32_t kOneLaunchRows = 64u;
+// The workspace of ws_policy_loss_rows: the words of the sum's workgroups or rows, those of the rows' parts, the rows' terms (policy_rows_kernel).
 struct RowsPlan {
     uint32_t parts, groups;
     bool one;
@@ -1146,17 +1148,16 @@ struct RowsPlan {
 };
 RowsPlan rows_plan(const ws_loss_rows* r) {
     RowsPlan n{};
-    const uint32_t vectors = row_vectors(r), least = share_of(vectors, ws::loss_most_share());
+    const uint32_t vectors = row_vectors(r), least = (vectors + ws::loss_most_share() - 1u) / ws::loss_most_share();
     uint32_t parts = r->rows ? 2u * static_cast<uint32_t>(compute_units()) / r->rows : 1u;
     if (parts > vectors / 256u) parts = vectors / 256u;
     if (parts > 64u) parts = 64u;
     if (parts < least) parts = least;
     n.parts = parts < 1u ? 1u : parts;
-    n.one = r->rows != 0u && r->rows <= kOneLaunchRows;
+    n.one = r->rows != 0u && r->rows <= ws::kMostSlots;
     n.words = meet_bytes(r->rows, n.parts, ws::kPartWords + (n.one ? 2u : 0u));
-    const uint64_t groups = r->rows / 1024u + n.words / 32768u + 1u;  // (of the second launch, which also clears the words)
-    n.groups = groups > 64u ? 64u : static_cast<uint32_t>(groups);
-    n.meet = policy_meet_bytes(n.one ? r->rows : n.groups);
+    n.groups = r->rows < 64u * 1024u ? r->rows / 1024u + 1u : 64u;  // (of the second launch)
+    n.meet = ws::sums_bytes(n.one ? r->rows : n.groups, ws::kPolicySums);
     n.terms = n.meet + n.words;
     n.bytes = n.terms + (n.one ? 0u : uint64_t{r->rows} * ws::kPolicySums * 8u);
     return n;
@@ -1170,7 +1171,7 @@ int grad_on(void* stream, const ws_loss_rows* r, const float* stats, const float
     a.d_entropy = d_entropy;
     a.out = static_cast<unsigned char*>(d_logits);
     a.out_bytes = d_stride * elem_bytes(r->dtype);
-    a.chunks = ws::loss_grad_chunks(r->dtype, r->vocab);
+    a.past_row = past_row(r);
     return ws::launch_grad(S(stream), r->dtype, a);
 }
 }  // namespace
@@ -1207,7 +1208,7 @@ int ws_token_logprobs_grad(void* stream, const ws_loss_rows* r, const float* sta
     return grad_on(stream, r, stats, d_logprob, entropy, d_entropy, d_logits, d_stride);
 }
 
-uint64_t ws_policy_loss_workspace(uint32_t rows) { return policy_groups(rows) > 1u ? policy_meet_bytes(policy_groups(rows)) : 0u; }
+uint64_t ws_policy_loss_workspace(uint32_t rows) { return ws::sums_bytes(policy_groups(rows), ws::kPolicySums); }
 
 int ws_policy_loss(void* stream, uint32_t rows, const ws_policy* p, const float* logprob, const float* entropy, float* sums, float* d_logprob, float* d_entropy, void* workspace,
                    uint64_t workspace_bytes) {
@@ -1244,6 +1245,7 @@ int ws_policy_loss_rows(void* stream, const ws_loss_rows* r, const ws_policy* p,
         a.entropy = entropy;
         a.out = static_cast<unsigned char*>(d_logits);
         a.out_bytes = d_stride * elem_bytes(r->dtype);
+        a.past_row = past_row(r);
         if (n.one) {
             a.sums_meet = reinterpret_cast<unsigned long long*>(work);
             a.sums = sums;
@@ -1267,7 +1269,7 @@ int ws_policy_loss_rows(void* stream, const ws_loss_rows* r, const ws_policy* p,
     return ws::launch_policy(S(stream), sum, n.groups);
 }
 
-uint64_t ws_preference_loss_workspace(uint32_t pairs) { return preference_groups(pairs) > 1u ? uint64_t{preference_groups(pairs)} * 16u : 0u; }
+uint64_t ws_preference_loss_workspace(uint32_t pairs) { return ws::sums_bytes(preference_groups(pairs), 1u); }
 
 int ws_preference_loss(void* stream, const ws_preference* p, void* workspace, uint64_t workspace_bytes) {
     if (!p || p->pairs == 0 || p->pairs > (1u << 30) || p->rows > (1u << 30) || !p->seq_off || !p->loss || !p->pair_loss || !p->reward) return WS_E_INVALID;

@@ -97,58 +97,60 @@ __device__ __forceinline__ void break_word(unsigned long long* at, uint32_t apar
 }
 __device__ __forceinline__ void words_arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-// `slots` workgroups that add up K sums each, by their first waves: each leaves its own (lane 0's), and when they have arrived gathers everybody's, added up in the same
-// order whoever does it; false where somebody is still to come. meet: [K][2][slots]. (The last slots' first sum is looked at first: they come
-// last. Several looks are on their way together: one after the other a sum of five over 256 slots took 14 us.)
+// `slots` workgroups (kMostSlots at most) that add up K sums each, by their first waves: each leaves its own (lane 0's), and when they have arrived gathers everybody's, added up in
+// the same order whoever does it; false where somebody is still to come. meet: [K][2][slots], and behind them for more than 64 slots [K][2][64]: then 16 or 64
+// neighbours meet first, one of them - who takes the first pair apart - leaves their sum for the next meeting. (With everybody looking at everybody's words
+// 256 slots take 14 us, their requests go to the same few places.)
+constexpr uint32_t kMostSlots = 4096u;
+__device__ __host__ constexpr uint32_t slot_group(uint32_t slots) { return slots <= 1024u ? 16u : 64u; }
 template <int K>
 __device__ __forceinline__ void leave_sums(unsigned long long* meet, uint32_t slots, uint32_t slot, const double (&sum)[K], unsigned long long tag) {
 #pragma unroll
     for (uint32_t k = 0; k < K; ++k) leave_word(meet + static_cast<size_t>(2u * k) * slots + slot, slots, static_cast<unsigned long long>(__double_as_longlong(sum[k])), tag);
 }
-template <int K>
-__device__ __forceinline__ bool gather_sums(unsigned long long* meet, uint32_t slots, double (&sum)[K], unsigned long long tag) {
+template <int K, bool ALONE>  // n slots (64 at most) from `first`; ALONE: one wave at most gets true
+__device__ __forceinline__ bool take_sums(unsigned long long* meet, uint32_t slots, uint32_t first, uint32_t n, double (&sum)[K], unsigned long long tag) {
     const uint32_t lane = lane_id();
-    constexpr uint32_t kB = 4u;  // slots of a lane on their way together
-    auto word = [&](uint32_t p, uint32_t k) { return meet + static_cast<size_t>(2u * k) * slots + p; };
-    const uint32_t last = (slots - 1u) / (64u * kB) * (64u * kB);
-    double all[K] = {};
-    for (uint32_t p0 = last;; p0 -= 64u * kB) {
-        bool here = true;
-        unsigned long long v[kB];
+    auto word = [&](uint32_t k) { return meet + static_cast<size_t>(2u * k) * slots + first + lane; };
+    bool here = true;
+    unsigned long long v[K] = {};
+    if (lane < n) {
 #pragma unroll
-        for (uint32_t b = 0; b < kB; ++b) {
-            const uint32_t p = p0 + b * 64u + lane;
-            v[b] = 0ull;
-            if (p < slots) here = find_word(word(p, 0u), slots, tag, v[b]) && here;
+        for (uint32_t k = 0; k < K; ++k) here = find_word(word(k), slots, tag, v[k]) && here;
+    }
+    if (__ballot(!here) != 0ull) return false;
+    if (ALONE) {
+        bool won = false;
+        if (lane == 0u) {
+            unsigned long long was = v[0] ^ tag;
+            won = __hip_atomic_compare_exchange_strong(word(0u) + slots, &was, 0ull, __ATOMIC_RELAXED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-        if (__ballot(!here) != 0ull) return false;
-#pragma unroll
-        for (uint32_t b = 0; b < kB; ++b) all[0] += __longlong_as_double(static_cast<long long>(v[b]));
-        if (p0 == 0u) break;
+        if (__ballot(won) == 0ull) return false;
     }
-    if (K > 1) {
-        bool here = true;
-        for (uint32_t p = lane; p < slots; p += 64u) {
-            unsigned long long v[K];
+    if (lane < n) {
 #pragma unroll
-            for (uint32_t k = 1; k < K; ++k) here = find_word(word(p, k), slots, tag, v[k]) && here;
-#pragma unroll
-            for (uint32_t k = 1; k < K; ++k) all[k] += __longlong_as_double(static_cast<long long>(v[k]));
-        }
-        if (__ballot(!here) != 0ull) return false;
-    }
-    for (uint32_t p = lane; p < slots; p += 64u) {
-#pragma unroll
-        for (uint32_t k = 0; k < K; ++k) break_word(word(p, k), slots);
+        for (uint32_t k = 0; k < K; ++k) break_word(word(k), slots);
     }
 #pragma unroll
-    for (uint32_t k = 0; k < K; ++k) sum[k] = wave_sum(all[k]);
+    for (uint32_t k = 0; k < K; ++k) sum[k] = wave_sum(__longlong_as_double(static_cast<long long>(v[k])));
     return true;
+}
+template <int K>
+__device__ __forceinline__ bool gather_sums(unsigned long long* meet, uint32_t slots, uint32_t slot, double (&sum)[K], unsigned long long tag) {
+    if (slots <= 64u) return take_sums<K, false>(meet, slots, 0u, slots, sum, tag);
+    const uint32_t group = slot_group(slots), g = slot / group, first = g * group;
+    if (!take_sums<K, true>(meet, slots, first, min(group, slots - first), sum, tag)) return false;
+    unsigned long long* next = meet + static_cast<size_t>(2 * K) * slots;
+    if (lane_id() == 0u) leave_sums(next, 64u, g, sum, tag);
+    words_arrived();
+    return take_sums<K, false>(next, 64u, 0u, (slots + group - 1u) / group, sum, tag);
 }
 
 // a launch of `parts` workgroups a row: the parts in x, the rows in y and z (dispatched in this order, a row's parts one after the other)
 constexpr uint32_t kGridRows = 32768u;
 __device__ __forceinline__ uint32_t grid_row() { return blockIdx.z * kGridRows + blockIdx.y; }
+// bytes of the words of `slots` workgroups that add up K sums
+inline uint64_t sums_bytes(uint32_t slots, uint32_t K) { return slots < 2u ? 0u : (uint64_t{slots} + (slots > 64u ? 64u : 0u)) * K * 16u; }
 inline dim3 grid_of(uint32_t parts, uint32_t rows) {
     return rows <= kGridRows ? dim3(parts, rows) : dim3(parts, kGridRows, (rows + kGridRows - 1u) / kGridRows);
 }
@@ -160,23 +162,34 @@ struct Elem {
     static constexpr uint32_t kNone = DT == 0 ? 0xff800000u : 0xff80ff80u;      // -inf
 };
 
-// a row as whole vectors between the 16-byte boundaries of `at`, and the up to 2 (kPer - 1) logits before and behind them
+// a row as whole vectors between the 16-byte boundaries of `at`, numbered from the last boundary of 128 bytes before them ([first, end), so that 8 vectors of
+// a round are one line, and the up to 2 (kPer - 1) logits before and behind them
 template <int DT>
 struct RowSpan {
-    uint32_t head, vectors, rest;
+    uint32_t head, first, end, rest;
     __device__ __forceinline__ RowSpan(const void* at, uint32_t V) {
-        const uint32_t off = (16u - (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(at)) & 15u)) & 15u;
+        const uint32_t addr = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(at)), off = (16u - (addr & 15u)) & 15u;
         head = min(off / Elem<DT>::kBytes, V);
-        vectors = (V - head) / Elem<DT>::kPer;
+        first = ((addr + off) >> 4) & 7u;
+        const uint32_t vectors = (V - head) / Elem<DT>::kPer;
+        end = first + vectors;
         rest = V - vectors * Elem<DT>::kPer;
     }
-    __device__ __forceinline__ uint32_t rest_index(uint32_t i) const { return i < head ? i : vectors * Elem<DT>::kPer + i; }
-    __device__ __forceinline__ uint32_t index(uint32_t j) const { return head + j * Elem<DT>::kPer; }
+    __device__ __forceinline__ uint32_t rest_index(uint32_t i) const { return i < head ? i : (end - first) * Elem<DT>::kPer + i; }
+    __device__ __forceinline__ uint32_t index(uint32_t j) const { return head + (j - first) * Elem<DT>::kPer; }
+    __device__ __forceinline__ bool has(uint32_t j) const { return j - first < end - first; }
 };
 
 __device__ __forceinline__ uint4 load_loose(const unsigned char* at) {
     const LooseVec v = *reinterpret_cast<const LooseVec*>(at);
     return make_uint4(v.x, v.y, v.z, v.w);
+}
+// a gradient's vector, `past` the caches or through them. (The first written out: the compiler makes one store of the two, the second.)
+__device__ __forceinline__ void store_vector(unsigned char* at, const uint4& q, bool past) {
+    typedef uint32_t four __attribute__((ext_vector_type(4)));
+    const four v{q.x, q.y, q.z, q.w};
+    if (past) asm volatile("global_store_dwordx4 %0, %1, off nt" ::"v"(at), "v"(v) : "memory");
+    else *reinterpret_cast<four*>(at) = v;
 }
 template <int DT>
 __device__ __forceinline__ float load_logit(const unsigned char* row, uint32_t i) {
@@ -214,7 +227,7 @@ __device__ __forceinline__ void store_logit(unsigned char* row, uint32_t i, floa
 }
 
 // the row's bitmap: bit i, and the bits of a vector that begins at token i, from the two bytes that they lie in (or the row's last two). One load instead of two
-// words': 200 masked rows of 50257 fp32 MASK_US.
+// words': 200 masked rows of 50257 fp32 13.8 us, and 13.2.
 struct __attribute__((packed, aligned(1))) LooseBits {
     uint16_t v;
 };
@@ -242,24 +255,32 @@ __device__ __forceinline__ uint4 only_allowed(const uint4& q, uint32_t bits) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// the vectors [j0, j1) of a row that a workgroup works on, `base` where the row begins. Loads go to the last of them where a thread has none
+// the vectors [j0, j1) of a row that a workgroup works on, `base` where the row begins. Loads go to the nearest of them where a thread has none
 // (a load behind a branch would be waited for there); what it read then counts as -inf.
 template <int DT, bool MASK, int T>
 struct Share {
     const unsigned char* base;
     const uint32_t* allow;
-    uint32_t head, last_byte, j0, j1;
-    __device__ __forceinline__ uint4 load(uint32_t j) const {
-        const uint32_t i = head + min(j, j1 - 1u) * Elem<DT>::kPer;
-        const uint4 q = load_loose(base + static_cast<size_t>(i) * Elem<DT>::kBytes);
-        if constexpr (MASK) return only_allowed<DT>(q, allowed_from(allow, i, last_byte));
-        return q;
+    RowSpan<DT> span;
+    uint32_t last_byte, j0, j1;
+    // part `part` of shares of `per` vectors
+    __device__ __forceinline__ Share(const unsigned char* row, const uint32_t* mask, const RowSpan<DT>& s, uint32_t V, uint32_t part, uint32_t per)
+        : base(row), allow(mask), span(s), last_byte(((V + 31u) >> 5) * 4u - 1u), j0(min(part * per, s.end)), j1(min(j0 + per, s.end)) {}
+    __device__ __forceinline__ bool any() const { return j1 > max(j0, span.first); }
+    // the vector as it is, and its bits of the mask: what is done with them waits for them
+    __device__ __forceinline__ uint4 load(uint32_t j, uint32_t& bits) const {
+        const uint32_t i = span.index(max(min(j, j1 - 1u), span.first));
+        bits = 0u;
+        if constexpr (MASK) bits = allowed_from(allow, i, last_byte);
+        return load_loose(base + static_cast<size_t>(i) * Elem<DT>::kBytes);
     }
+    __device__ __forceinline__ bool mine(uint32_t j) const { return j < j1 && j >= span.first; }
     // the vector of round jb .. jb + T, for a thread that may have none in it
-    __device__ __forceinline__ uint4 own(const uint4& q, uint32_t jb) const {
+    __device__ __forceinline__ uint4 own(uint4 q, uint32_t bits, uint32_t jb) const {
         constexpr uint32_t none = Elem<DT>::kNone;
-        if (jb + T <= j1) return q;  // (uniform)
-        return jb + threadIdx.x < j1 ? q : make_uint4(none, none, none, none);
+        if constexpr (MASK) q = only_allowed<DT>(q, bits);
+        if (jb + T <= j1 && jb >= span.first) return q;  // (uniform)
+        return mine(jb + threadIdx.x) ? q : make_uint4(none, none, none, none);
     }
 };
 
@@ -370,47 +391,47 @@ __device__ __forceinline__ RowSums block_sums(Running<ENT>& a, const Scale& c, f
     return r;
 }
 
-// ---- the parts of a row: what each leaves for the others, and what they make of it (in the order of the parts, whoever does)
+// ---- the parts of a row: what each leaves for the others, and what they make of it (in the order of the parts, whoever does). The sums in 64 bits:
+// rounded to 32, a log-probability near the middle of two floats comes out as the other one in twenty, which adds up in the ratio of a long answer.
 struct PartSums {
-    float m, s, t, x;  // x: the logit of the row's token, from the part that has it
+    float m, x;  // x: the logit of the row's token, from the part that has it
+    double s, t;
 };
-constexpr uint32_t kPartWords = 4u;  // 64-bit words a part: two, each twice
-__device__ __forceinline__ unsigned long long two_floats(float lo, float hi) { return (static_cast<unsigned long long>(__float_as_uint(hi)) << 32) | __float_as_uint(lo); }
-__device__ __forceinline__ float low_float(unsigned long long v) { return __uint_as_float(static_cast<uint32_t>(v)); }
-__device__ __forceinline__ float high_float(unsigned long long v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
-// part p's words among those of `parts`: m and s, t and x (BOTH: where somebody asks for them)
-template <bool BOTH>
+constexpr uint32_t kPartWords = 6u;  // 64-bit words a part: three, each twice
+// part p's words among those of `parts`: m and x, s, t (ENT)
+template <bool ENT>
 __device__ __forceinline__ void leave_part(unsigned long long* meet, uint32_t parts, uint32_t p, const PartSums& w, unsigned long long tag) {
-    leave_word(meet + p, parts, two_floats(w.m, w.s), tag);
-    if (BOTH) leave_word(meet + 2u * parts + p, parts, two_floats(w.t, w.x), tag);
-}
-template <bool BOTH>
-__device__ __forceinline__ bool find_part(const unsigned long long* meet, uint32_t parts, uint32_t p, unsigned long long tag, PartSums& w) {
-    unsigned long long ms, tx = 0ull;
-    const bool a = find_word(meet + p, parts, tag, ms), b = !BOTH || find_word(meet + 2u * parts + p, parts, tag, tx);
-    w = PartSums{low_float(ms), high_float(ms), low_float(tx), high_float(tx)};
-    return a && b;
-}
-template <bool BOTH>
-__device__ __forceinline__ void break_part(unsigned long long* meet, uint32_t parts, uint32_t p) {
-    break_word(meet + p, parts);
-    if (BOTH) break_word(meet + 2u * parts + p, parts);
+    leave_word(meet + p, parts, (static_cast<unsigned long long>(__float_as_uint(w.x)) << 32) | __float_as_uint(w.m), tag);
+    leave_word(meet + 2u * parts + p, parts, static_cast<unsigned long long>(__double_as_longlong(w.s)), tag);
+    if (ENT) leave_word(meet + 4u * parts + p, parts, static_cast<unsigned long long>(__double_as_longlong(w.t)), tag);
 }
 template <bool ENT>
-__device__ __forceinline__ PartSums part_sums(const RowSums& r, float x) {
-    return PartSums{r.m, static_cast<float>(r.s), ENT ? static_cast<float>(r.t) : 0.f, x};
+__device__ __forceinline__ bool find_part(const unsigned long long* meet, uint32_t parts, uint32_t p, unsigned long long tag, PartSums& w) {
+    unsigned long long mx, s, t = 0ull;
+    bool here = find_word(meet + p, parts, tag, mx);
+    here = find_word(meet + 2u * parts + p, parts, tag, s) && here;
+    if (ENT) here = find_word(meet + 4u * parts + p, parts, tag, t) && here;
+    w = PartSums{__uint_as_float(static_cast<uint32_t>(mx)), __uint_as_float(static_cast<uint32_t>(mx >> 32)), __longlong_as_double(static_cast<long long>(s)),
+                 __longlong_as_double(static_cast<long long>(t))};
+    return here;
+}
+template <bool ENT>
+__device__ __forceinline__ void break_part(unsigned long long* meet, uint32_t parts, uint32_t p) {
+    break_word(meet + p, parts);
+    break_word(meet + 2u * parts + p, parts);
+    if (ENT) break_word(meet + 4u * parts + p, parts);
 }
 // a wave, a lane a part
 template <bool ENT>
 __device__ __forceinline__ RowSums join_parts(bool in, const PartSums& w, const Scale& c) {
     RowSums r{};
     const float m = in ? w.m : -FLT_MAX;
-    const double s = in ? static_cast<double>(w.s) : 0.0;
+    const double s = in ? w.s : 0.0;
     r.m = wave_max(m);
     const float d = c.of(m - r.m);
     const double e = static_cast<double>(exp2_fast(d));
     r.s = wave_sum(s * e);
-    if (ENT) r.t = wave_sum(e * ((in ? static_cast<double>(w.t) : 0.0) + s * static_cast<double>(fmaxf(d, kFarBelow))));
+    if (ENT) r.t = wave_sum(e * ((in ? w.t : 0.0) + s * static_cast<double>(fmaxf(d, kFarBelow))));
     return r;
 }
 
@@ -430,16 +451,19 @@ __global__ void __launch_bounds__(T) score_rows_kernel(ScoreArgs A) {
     constexpr uint32_t kPer = Elem<DT>::kPer, kU = 4u;  // vectors of a thread on their way together
     __shared__ float red_m[T / 64];
     __shared__ double red_s[T / 64], red_t[T / 64];
-    const uint32_t row = grid_row(), part = blockIdx.x, t = threadIdx.x, V = A.R.vocab;
+    uint32_t row = grid_row();
     if (row >= A.R.rows) return;
+    row = A.R.rows - 1u - row;
+    const uint32_t part = blockIdx.x, t = threadIdx.x, V = A.R.vocab;
     const unsigned char* base = A.R.logits + row * A.R.row_bytes;
     const RowSpan<DT> span(base, V);
-    const uint32_t j0 = min(part * A.per, span.vectors), j1 = min(j0 + A.per, span.vectors);
-    const Share<DT, MASK, T> share{base, MASK ? A.R.allow + row * A.R.allow_stride : nullptr, span.head, ((V + 31u) >> 5) * 4u - 1u, j0, j1};
+    const Share<DT, MASK, T> share(base, MASK ? A.R.allow + row * A.R.allow_stride : nullptr, span, V, part, A.per);
+    const uint32_t j0 = share.j0, j1 = share.any() ? share.j1 : share.j0;
     uint4 q[kU];
+    uint32_t bits[kU];
     if (j0 < j1) {
 #pragma unroll
-        for (uint32_t u = 0; u < kU; ++u) q[u] = share.load(j0 + u * T + t);
+        for (uint32_t u = 0; u < kU; ++u) q[u] = share.load(j0 + u * T + t, bits[u]);
     }
     // (the row's own entries come while its logits do)
     const int32_t id = A.R.ids ? A.R.ids[row] : -1;
@@ -451,22 +475,26 @@ __global__ void __launch_bounds__(T) score_rows_kernel(ScoreArgs A) {
     Running<ENT> a;
     for (uint32_t jb = j0; jb < j1; jb += kU * T) {
         uint4 next[kU];
+        uint32_t next_bits[kU];
         const bool more = jb + kU * T < j1;
         if (more) {
 #pragma unroll
-            for (uint32_t u = 0; u < kU; ++u) next[u] = share.load(jb + (kU + u) * T + t);
+            for (uint32_t u = 0; u < kU; ++u) next[u] = share.load(jb + (kU + u) * T + t, next_bits[u]);
         }
 #pragma unroll
         for (uint32_t u = 0; u < kU; ++u) {
             if (jb + u * T < j1) {  // (uniform)
                 float x[kPer];
-                unpack<DT>(share.own(q[u], jb + u * T), x);
+                unpack<DT>(share.own(q[u], bits[u], jb + u * T), x);
                 a.take(x, c);
             }
         }
         if (more) {
 #pragma unroll
-            for (uint32_t u = 0; u < kU; ++u) q[u] = next[u];
+            for (uint32_t u = 0; u < kU; ++u) {
+                q[u] = next[u];
+                bits[u] = next_bits[u];
+            }
         }
     }
     if (part == 0u && t < span.rest) {
@@ -477,7 +505,7 @@ __global__ void __launch_bounds__(T) score_rows_kernel(ScoreArgs A) {
     if (t >= 64u) return;
     if (A.parts > 1u) {  // (at most 64)
         unsigned long long* meet = A.meet + static_cast<size_t>(row) * A.parts * kPartWords;
-        if (t == 0u) leave_part<ENT>(meet, A.parts, part, part_sums<ENT>(r, 0.f), A.tag);
+        if (t == 0u) leave_part<ENT>(meet, A.parts, part, PartSums{r.m, 0.f, r.s, r.t}, A.tag);
         words_arrived();
         const bool in = t < A.parts;
         PartSums w{};
@@ -503,7 +531,7 @@ struct GradArgs {
     const float* d_entropy;
     unsigned char* out;
     uint64_t out_bytes;  // between rows
-    uint32_t chunks;     // workgroups a row
+    uint32_t past_row;   // from this row on the gradient goes past the caches
 };
 
 // what a row's derivatives need: dx = e (a + b d) with e = 2^d, d = (x - m) t log2(e), and g t more at the row's token
@@ -547,12 +575,13 @@ __global__ void __launch_bounds__(T) grad_rows_kernel(GradArgs A) {
     uint32_t row = grid_row();
     if (row >= A.R.rows) return;
     row = A.R.rows - 1u - row;
+    const bool past = row >= A.past_row;
     const uint32_t chunk = blockIdx.x, t = threadIdx.x, V = A.R.vocab;
     const unsigned char* base = A.R.logits + row * A.R.row_bytes;
     unsigned char* out = A.out + row * A.out_bytes;
     const RowSpan<DT> span(out, V);
     const uint32_t* allow = MASK ? A.R.allow + row * A.R.allow_stride : nullptr;
-    const uint32_t last_byte = ((V + 31u) >> 5) * 4u - 1u;
+    const Share<DT, MASK, T> share(base, allow, span, V, 0u, span.end);
     const float inv_t = A.R.inv_t ? A.R.inv_t[row] : 1.f;
     const int32_t id = A.R.ids ? A.R.ids[row] : -1;
     const bool has_id = static_cast<uint32_t>(id) < V;
@@ -560,22 +589,19 @@ __global__ void __launch_bounds__(T) grad_rows_kernel(GradArgs A) {
     const RowSlope r = row_slope<ENT>(A.stats[2 * static_cast<size_t>(row)], A.stats[2 * static_cast<size_t>(row) + 1], inv_t,
                                       has_id && A.d_logprob ? A.d_logprob[row] : 0.f, ENT ? A.d_entropy[row] : 0.f, ENT ? A.entropy[row] : 0.f);
     const uint32_t j0 = chunk * (T * U) + t;
-    auto store = [&](uint32_t j, const uint4& q) { *reinterpret_cast<uint4*>(out + static_cast<size_t>(span.index(j)) * Elem<DT>::kBytes) = q; };
+    auto store = [&](uint32_t j, const uint4& q) { store_vector(out + static_cast<size_t>(span.index(j)) * Elem<DT>::kBytes, q, past); };
     if (r.none) {  // (uniform) not read
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u)
-            if (j0 + u * T < span.vectors) store(j0 + u * T, make_uint4(0u, 0u, 0u, 0u));
+            if (span.has(j0 + u * T)) store(j0 + u * T, make_uint4(0u, 0u, 0u, 0u));
         if (chunk == 0u && t < span.rest) store_logit<DT>(out, span.rest_index(t), 0.f);
         return;
     }
     uint4 q[U];
+    uint32_t bits[U];
+    if (share.any()) {
 #pragma unroll
-    for (uint32_t u = 0; u < U; ++u) {
-        const uint32_t j = j0 + u * T;
-        if (j < span.vectors) {
-            q[u] = load_loose(base + static_cast<size_t>(span.index(j)) * Elem<DT>::kBytes);
-            if constexpr (MASK) q[u] = only_allowed<DT>(q[u], allowed_from(allow, span.index(j), last_byte));
-        }
+        for (uint32_t u = 0; u < U; ++u) q[u] = share.load(j0 + u * T, bits[u]);
     }
     if (chunk == 0u && t < span.rest) {
         const uint32_t i = span.rest_index(t);
@@ -587,7 +613,10 @@ __global__ void __launch_bounds__(T) grad_rows_kernel(GradArgs A) {
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) {
         const uint32_t j = j0 + u * T;
-        if (j < span.vectors) store(j, slope_vector<DT, ENT>(q[u], span.index(j), r, c, static_cast<uint32_t>(id)));
+        if (span.has(j)) {
+            if constexpr (MASK) q[u] = only_allowed<DT>(q[u], bits[u]);
+            store(j, slope_vector<DT, ENT>(q[u], span.index(j), r, c, static_cast<uint32_t>(id)));
+        }
     }
 }
 
@@ -596,9 +625,9 @@ __global__ void __launch_bounds__(T) grad_rows_kernel(GradArgs A) {
 // that all parts run at once: a part that does not find another's words in time works that part's sums out itself, in the
 // same order and so to the same bits. (Where the gradient goes over the logits: a part writes only after its words have arrived. So logits
 // read before a look that still finds no words are the logits, and the token's logit goes with the words, not to be read
-// by a part that comes late.) The words stay until every part has seen them. Few rows' terms meet in this launch, and the parts leave a mark each when they
-// are through: whoever sees all marks of a row breaks its words. Of more rows a second launch adds up the terms and breaks the words: it costs 5 us, and a
-// wave that looks at all rows' words as much from some 500 rows on.
+// by a part that comes late.) The words stay until every part has seen them:
+// the parts leave a mark each when they are through, and whoever sees all marks of a row breaks its words. The rows' terms meet in this launch as well. Of more rows
+// than kMostSlots a second launch adds up the terms and breaks the words (5 us).
 struct RowsArgs {
     LossRows R;
     PolicyIn P;
@@ -606,6 +635,7 @@ struct RowsArgs {
     float* entropy;
     unsigned char* out;
     uint64_t out_bytes;
+    uint32_t past_row;  // as GradArgs
     double* terms;             // [kPolicySums][rows], or:
     unsigned long long* sums_meet;  // [kPolicySums][2][rows], for rows that meet in this launch
     float* sums;
@@ -623,31 +653,40 @@ __global__ void __launch_bounds__(T, WAVES) policy_rows_kernel(RowsArgs A) {
     __shared__ RowSlope shared_slope;
     __shared__ unsigned long long missing;
     __shared__ PartSums found[64];
-    const uint32_t row = grid_row(), part = blockIdx.x, t = threadIdx.x, V = A.R.vocab, per = A.per;
+    uint32_t row = grid_row();
     if (row >= A.R.rows) return;
+    row = A.R.rows - 1u - row;
+    const bool past = row >= A.past_row;
+    const uint32_t part = blockIdx.x, t = threadIdx.x, V = A.R.vocab, per = A.per;
     const unsigned char* base = A.R.logits + row * A.R.row_bytes;
     unsigned char* out = A.out + row * A.out_bytes;
     const RowSpan<DT> span(out, V);
-    const uint32_t j0 = min(part * per, span.vectors), j1 = min(j0 + per, span.vectors);
+    const uint32_t* allow = MASK ? A.R.allow + row * A.R.allow_stride : nullptr;
+    const Share<DT, MASK, T> share(base, allow, span, V, part, per);
+    const uint32_t j0 = share.j0, j1 = share.any() ? share.j1 : share.j0;
     const int32_t id = A.R.ids[row];
     const bool has_id = static_cast<uint32_t>(id) < V;
     const double weight = policy_weight(A.P, row);
     const bool rest = part == 0u && t < span.rest;
     const uint32_t rest_i = rest ? span.rest_index(t) : 0u;
-    auto store = [&](uint32_t j, const uint4& q) { *reinterpret_cast<uint4*>(out + static_cast<size_t>(span.index(j)) * Elem<DT>::kBytes) = q; };
+    auto store = [&](uint32_t j, const uint4& q) { store_vector(out + static_cast<size_t>(span.index(j)) * Elem<DT>::kBytes, q, past); };
     auto nothing = [&]() {
-        for (uint32_t j = j0 + t; j < j1; j += T) store(j, make_uint4(0u, 0u, 0u, 0u));
+        for (uint32_t j = j0 + t; j < j1; j += T)
+            if (j >= span.first) store(j, make_uint4(0u, 0u, 0u, 0u));
         if (rest) store_logit<DT>(out, rest_i, 0.f);
     };
     unsigned long long* meet = A.meet + static_cast<size_t>(row) * A.parts * (A.terms ? kPartWords : kPartWords + 2u);
     double terms[kPolicySums] = {};
     auto leave_terms = [&]() {  // the row's, by the first thread of its first part
-        if (!A.terms) return leave_sums(A.sums_meet, A.R.rows, row, terms, A.tag);
+        if (!A.terms) {
+            if (A.R.rows > 1u) leave_sums(A.sums_meet, A.R.rows, row, terms, A.tag);
+            return;
+        }
 #pragma unroll
         for (uint32_t k = 0; k < kPolicySums; ++k) A.terms[static_cast<size_t>(k) * A.R.rows + row] = terms[k];
     };
     auto finish = [&]() {  // by its first wave, when everything else is done
-        if (A.terms || !gather_sums(A.sums_meet, A.R.rows, terms, A.tag)) return;
+        if (A.terms || (A.R.rows > 1u && !gather_sums(A.sums_meet, A.R.rows, row, terms, A.tag))) return;
 #pragma unroll
         for (uint32_t k = 0; k < kPolicySums; ++k)
             if (t == 0u) A.sums[k] = static_cast<float>(terms[k]);
@@ -665,19 +704,19 @@ __global__ void __launch_bounds__(T, WAVES) policy_rows_kernel(RowsArgs A) {
         }
         return;
     }
-    const uint32_t* allow = MASK ? A.R.allow + row * A.R.allow_stride : nullptr;
-    const Share<DT, MASK, T> share{base, allow, span.head, ((V + 31u) >> 5) * 4u - 1u, j0, j1};
     uint4 q[NV];
+    uint32_t bits[NV];
     if (j0 < j1) {
 #pragma unroll
         for (int k = 0; k < NV; ++k)
-            if (k == 0 || j0 + k * T < j1) q[k] = share.load(j0 + k * T + t);  // (uniform)
+            if (k == 0 || j0 + k * T < j1) q[k] = share.load(j0 + k * T + t, bits[k]);  // (uniform)
     }
     float x_rest = -INFINITY;
     if (rest && (!MASK || allowed(allow, rest_i))) x_rest = load_logit<DT>(base, rest_i);
     const float inv_t = A.R.inv_t ? A.R.inv_t[row] : 1.f;
     // the part that has the row's token, and its logit
-    const uint32_t id_at = static_cast<uint32_t>(id) - span.head, id_part = id_at / kPer < span.vectors ? id_at / kPer / per : 0u;
+    const uint32_t id_at = (static_cast<uint32_t>(id) - span.head) / kPer + span.first;
+    const uint32_t id_part = static_cast<uint32_t>(id) >= span.head && id_at < span.end ? id_at / per : 0u;
     auto token_logit = [&]() { return !MASK || allowed(allow, static_cast<uint32_t>(id)) ? load_logit<DT>(base, static_cast<uint32_t>(id)) : -INFINITY; };
     PolicyRow token{};
     float x_id = 0.f;
@@ -691,7 +730,8 @@ __global__ void __launch_bounds__(T, WAVES) policy_rows_kernel(RowsArgs A) {
     for (int k = 0; k < NV; ++k) {
         if (j0 + k * T < j1) {  // (uniform)
             float x[kPer];
-            unpack<DT>(share.own(q[k], j0 + k * T), x);
+            q[k] = share.own(q[k], bits[k], j0 + k * T);
+            unpack<DT>(q[k], x);
             a.take(x, c);
         }
     }
@@ -699,13 +739,13 @@ __global__ void __launch_bounds__(T, WAVES) policy_rows_kernel(RowsArgs A) {
     RowSums r = block_sums<ENT, T>(a, c, red_m, red_s, red_t);
     if (A.parts > 1u) {
         if (t < 64u) {
-            if (t == 0u) leave_part<true>(meet, A.parts, part, part_sums<ENT>(r, x_id), A.tag);
+            if (t == 0u) leave_part<ENT>(meet, A.parts, part, PartSums{r.m, x_id, r.s, r.t}, A.tag);
             words_arrived();
             const bool in = t < A.parts;
             PartSums w{};
             bool here = !in;
             for (uint32_t look = 0; look < kLooks; ++look) {
-                if (!here) here = find_part<true>(meet, A.parts, t, A.tag, w);
+                if (!here) here = find_part<ENT>(meet, A.parts, t, A.tag, w);
                 if (__ballot(!here) == 0ull) break;
                 __builtin_amdgcn_s_sleep(4);
             }
@@ -715,12 +755,14 @@ __global__ void __launch_bounds__(T, WAVES) policy_rows_kernel(RowsArgs A) {
         }
         __syncthreads();
         for (unsigned long long late = missing; late; late &= late - 1ull) {  // (uniform)
-            const uint32_t p = static_cast<uint32_t>(__ffsll(late) - 1), p0 = min(p * per, span.vectors), p1 = min(p0 + per, span.vectors);
-            const Share<DT, MASK, T> theirs{base, allow, span.head, share.last_byte, p0, p1};
+            const uint32_t p = static_cast<uint32_t>(__ffsll(late) - 1);
+            const Share<DT, MASK, T> theirs(base, allow, span, V, p, per);
             Running<ENT> b;
-            for (uint32_t jb = p0; jb < p1; jb += T) {
+            for (uint32_t jb = theirs.j0; theirs.any() && jb < theirs.j1; jb += T) {
                 float x[kPer];
-                unpack<DT>(theirs.own(theirs.load(jb + t), jb), x);
+                uint32_t bits_late;
+                const uint4 late_q = theirs.load(jb + t, bits_late);
+                unpack<DT>(theirs.own(late_q, bits_late, jb), x);
                 b.take(x, c);
             }
             if (p == 0u && t < span.rest) {
@@ -731,9 +773,9 @@ __global__ void __launch_bounds__(T, WAVES) policy_rows_kernel(RowsArgs A) {
             __syncthreads();
             const RowSums o = block_sums<ENT, T>(b, c, red_m, red_s, red_t);
             if (t == 0u) {  // (everybody's logits have come: the barrier in block_sums)
-                PartSums w = part_sums<ENT>(o, x_late), came{};
+                PartSums w{o.m, x_late, o.s, o.t}, came{};
                 words_arrived();
-                if (find_part<true>(meet, A.parts, p, A.tag, came)) w = came;
+                if (find_part<ENT>(meet, A.parts, p, A.tag, came)) w = came;
                 found[p] = w;
             }
         }
@@ -764,7 +806,7 @@ __global__ void __launch_bounds__(T, WAVES) policy_rows_kernel(RowsArgs A) {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const uint32_t j = j0 + k * T + t;
-            if (j < j1) store(j, slope_vector<DT, SLOPE>(q[k], span.index(j), s, c, static_cast<uint32_t>(id)));
+            if (share.mine(j)) store(j, slope_vector<DT, SLOPE>(q[k], span.index(j), s, c, static_cast<uint32_t>(id)));
         }
         if (rest) {
             float y = slope_at<SLOPE>(x_rest, s, c);
@@ -779,7 +821,7 @@ __global__ void __launch_bounds__(T, WAVES) policy_rows_kernel(RowsArgs A) {
         unsigned long long mark;
         const bool in = t < A.parts, here = !in || find_word(marks + t, A.parts, A.tag, mark);
         if (__ballot(!here) == 0ull && in) {  // everybody is through
-            break_part<true>(meet, A.parts, t);
+            break_part<ENT>(meet, A.parts, t);
             break_word(marks + t, A.parts);
         }
     }
@@ -835,7 +877,7 @@ __global__ void __launch_bounds__(T) policy_kernel(PolicyArgs A) {
     if (groups > 1u) {
         if (t == 0u) leave_sums(A.meet, groups, blockIdx.x, sum, A.tag);
         words_arrived();
-        if (!gather_sums(A.meet, groups, sum, A.tag)) return;
+        if (!gather_sums(A.meet, groups, blockIdx.x, sum, A.tag)) return;
     }
     if (t == 0u) {
 #pragma unroll
@@ -906,7 +948,7 @@ __global__ void __launch_bounds__(T) preference_kernel(PreferenceArgs A) {
     if (groups > 1u) {
         if (t == 0u) leave_sums(A.meet, groups, blockIdx.x, sum, A.tag);
         words_arrived();
-        if (!gather_sums(A.meet, groups, sum, A.tag)) return;
+        if (!gather_sums(A.meet, groups, blockIdx.x, sum, A.tag)) return;
     }
     if (t == 0u) A.loss[0] = static_cast<float>(sum[0]);
 }

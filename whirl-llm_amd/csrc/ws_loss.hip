@@ -5,22 +5,26 @@
 namespace ws {
 
 namespace {
-constexpr uint32_t kScoreThreads = 256u, kGradThreads = 256u, kGradVectors = 4u, kPolicyThreads = 1024u;
+constexpr uint32_t kScoreThreads = 256u, kGradThreads = 256u, kGradVectors = 2u, kPolicyThreads = 1024u;
+// vectors of a workgroup's share: up to the first a wave takes them, up to the second and third 256 threads of policy_rows_kernel
+constexpr uint32_t kLeastShare = 4u * 64u, kSmallShare = 4u * 256u, kMostShare = 12u * 256u;
 
 template <int DT, bool ENT, bool MASK>
 struct Score {
     static void go(hipStream_t s, const ScoreArgs& a) {
-        hipLaunchKernelGGL((score_rows_kernel<DT, ENT, MASK, kScoreThreads>), grid_of(a.parts, a.R.rows), dim3(kScoreThreads), 0, s, a);
+        if (a.per <= kLeastShare) hipLaunchKernelGGL((score_rows_kernel<DT, ENT, MASK, 64>), grid_of(a.parts, a.R.rows), dim3(64), 0, s, a);
+        else hipLaunchKernelGGL((score_rows_kernel<DT, ENT, MASK, kScoreThreads>), grid_of(a.parts, a.R.rows), dim3(kScoreThreads), 0, s, a);
     }
 };
 template <int DT, bool ENT, bool MASK>
 struct Grad {
     static void go(hipStream_t s, const GradArgs& a) {
-        hipLaunchKernelGGL((grad_rows_kernel<DT, ENT, MASK, kGradThreads, kGradVectors>), grid_of(a.chunks, a.R.rows), dim3(kGradThreads), 0, s, a);
+        constexpr uint32_t each = kGradThreads * kGradVectors;
+        const uint32_t chunks = (a.R.vocab / Elem<DT>::kPer + 7u + each - 1u) / each;  // (the vectors of a row: RowSpan)
+        hipLaunchKernelGGL((grad_rows_kernel<DT, ENT, MASK, kGradThreads, kGradVectors>), grid_of(chunks, a.R.rows), dim3(kGradThreads), 0, s, a);
     }
 };
 // the builds of policy_rows_kernel: threads, vectors a thread
-constexpr uint32_t kSmallShare = 4u * 256u, kMostShare = 12u * 256u;
 template <int DT, bool ENT, bool SLOPE, bool MASK, int T, int NV, int WAVES>
 void rows(hipStream_t s, const RowsArgs& a) {
     hipLaunchKernelGGL((policy_rows_kernel<DT, ENT, SLOPE, MASK, T, NV, WAVES>), grid_of(a.parts, a.R.rows), dim3(T), 0, s, a);
@@ -30,7 +34,8 @@ struct Rows {
     template <bool SLOPE>
     static void of_size(hipStream_t s, const RowsArgs& a) {
         const uint32_t share = a.per;
-        if (share <= kSmallShare) rows<DT, ENT, SLOPE, MASK, 256, 4, 6>(s, a);
+        if (share <= kLeastShare && a.parts == 1u) rows<DT, ENT, SLOPE, MASK, 64, 4, 6>(s, a);
+        else if (share <= kSmallShare) rows<DT, ENT, SLOPE, MASK, 256, 4, 6>(s, a);
         else rows<DT, ENT, SLOPE, MASK, 256, 12, 5>(s, a);
     }
     static void go(hipStream_t s, const RowsArgs& a, bool slope) {
@@ -52,11 +57,6 @@ void by_kind(int dtype, bool ent, bool mask, A&&... a) {
 }
 }  // namespace
 
-uint32_t loss_grad_chunks(int dtype, uint32_t vocab) {
-    const uint32_t vectors = vocab / (dtype == 0 ? 4u : 8u), each = kGradThreads * kGradVectors;
-    return vectors ? (vectors + each - 1u) / each : 1u;
-}
-uint32_t loss_threads() { return kScoreThreads; }
 uint32_t loss_most_share() { return kMostShare; }
 
 int launch_score(hipStream_t stream, int dtype, const ScoreArgs& a) {
