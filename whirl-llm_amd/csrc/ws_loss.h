@@ -184,11 +184,12 @@ __device__ __forceinline__ uint4 load_loose(const unsigned char* at) {
     const LooseVec v = *reinterpret_cast<const LooseVec*>(at);
     return make_uint4(v.x, v.y, v.z, v.w);
 }
-// a gradient's vector, `past` the caches or through them. (The first written out: the compiler makes one store of the two, the second.)
+// a gradient's vector, `past` the caches or through them. (The first written out: the compiler makes one store of the two, the second. The pause is what the store's data registers
+// need before they are written again, which the compiler sees to for its own stores.)
 __device__ __forceinline__ void store_vector(unsigned char* at, const uint4& q, bool past) {
     typedef uint32_t four __attribute__((ext_vector_type(4)));
     const four v{q.x, q.y, q.z, q.w};
-    if (past) asm volatile("global_store_dwordx4 %0, %1, off nt" ::"v"(at), "v"(v) : "memory");
+    if (past) asm volatile("global_store_dwordx4 %0, %1, off nt\n\ts_nop 1" ::"v"(at), "v"(v) : "memory");
     else *reinterpret_cast<four*>(at) = v;
 }
 template <int DT>
@@ -550,9 +551,10 @@ __device__ __forceinline__ RowSlope row_slope(float m, float S, float inv_t, flo
     r.at_id = g * inv_t;
     return r;
 }
-template <bool ENT>
+// (bf16 results: the exponent with the factor's first float alone is 2^-23 |d| off relative to its power at most, a thousandth of their rounding)
+template <int DT, bool ENT>
 __device__ __forceinline__ float slope_at(float x, const RowSlope& r, const Scale& c) {
-    const float d = c.of(x - r.m), e = exp2_fast(d);
+    const float d = DT == 0 ? c.of(x - r.m) : __fmul_rn(x - r.m, c.hi), e = exp2_fast(d);
     return e * (ENT ? fmaf(r.b, fmaxf(d, kFarBelow), r.a) : r.a);
 }
 template <int DT, bool ENT>
@@ -561,7 +563,7 @@ __device__ __forceinline__ uint4 slope_vector(const uint4& q, uint32_t first, co
     float x[kPer], y[kPer];
     unpack<DT>(q, x);
 #pragma unroll
-    for (uint32_t k = 0; k < kPer; ++k) y[k] = slope_at<ENT>(x[k], r, c);
+    for (uint32_t k = 0; k < kPer; ++k) y[k] = slope_at<DT, ENT>(x[k], r, c);
     if (id - first < kPer) {
 #pragma unroll
         for (uint32_t k = 0; k < kPer; ++k)
@@ -606,7 +608,7 @@ __global__ void __launch_bounds__(T) grad_rows_kernel(GradArgs A) {
     if (chunk == 0u && t < span.rest) {
         const uint32_t i = span.rest_index(t);
         const float x = !MASK || allowed(allow, i) ? load_logit<DT>(base, i) : -INFINITY;
-        float y = slope_at<ENT>(x, r, c);
+        float y = slope_at<DT, ENT>(x, r, c);
         if (i == static_cast<uint32_t>(id) && x != -INFINITY) y += r.at_id;
         store_logit<DT>(out, i, y);
     }
@@ -809,7 +811,7 @@ __global__ void __launch_bounds__(T, WAVES) policy_rows_kernel(RowsArgs A) {
             if (share.mine(j)) store(j, slope_vector<DT, SLOPE>(q[k], span.index(j), s, c, static_cast<uint32_t>(id)));
         }
         if (rest) {
-            float y = slope_at<SLOPE>(x_rest, s, c);
+            float y = slope_at<DT, SLOPE>(x_rest, s, c);
             if (rest_i == static_cast<uint32_t>(id) && x_rest != -INFINITY) y += s.at_id;
             store_logit<DT>(out, rest_i, y);
         }
