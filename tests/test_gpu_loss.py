@@ -417,3 +417,120 @@ def test_captured_steps_replayed():
                 assert torch.equal(a, b), (k, i)
                 assert torch.equal(e, b), (k, i)
     torch.cuda.current_stream().wait_stream(side)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_parts_that_do_not_wait_for_each_other_give_the_same_bits(dtype):
+    """ws_policy.spins = 1: a part looks once and then works the missing parts' sums out itself, while their gradient may already be going over the logits. To the bit what
+    waiting gives, in place or not, and the sums' and parts' words are left as the next call needs them (replays of a captured graph). In place has bits of its own: which
+    thread adds up which logits goes by the boundaries of the memory that the gradient is written to."""
+    m = gc.pkg()
+    for rows, V, masked in ((1, 151936, False), (6, 100003, True), (40, 65537, False), (200, 50257, False)):
+        c = make(rows, V, dtype, 61 + rows, masked, 3, 1)
+        old, adv = torch.full((rows,), -7.0, device=DEV), torch.linspace(-1, 1, rows, device=DEV)
+        args = dict(ref_logprob=old, inv_t=c["dinv"], allow=c["dallow"], kl_coef=0.1, entropy_coef=0.02)
+        want = m.policy_loss_rows(c["dx"], c["dids"], old, adv, **args)
+        start = c["dx"].clone()
+        own = [t.clone() for t in m.policy_loss_rows(c["dx"], c["dids"], old, adv, out=c["dx"], **args)]
+        for _ in range(4):
+            c["dx"].copy_(start)
+            got = m.policy_loss_rows(c["dx"], c["dids"], old, adv, spins=1, **args)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+            got = m.policy_loss_rows(c["dx"], c["dids"], old, adv, spins=1, out=c["dx"], **args)
+            assert all(torch.equal(a, b) for a, b in zip(got, own))
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            c["dx"].copy_(start)
+            side.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            graph.capture_begin()
+            held = m.policy_loss_rows(c["dx"], c["dids"], old, adv, spins=1, out=c["dx"], **args)
+            graph.capture_end()
+            for _ in range(3):
+                c["dx"].copy_(start)
+                graph.replay()
+                side.synchronize()
+                assert all(torch.equal(a, b) for a, b in zip(held, own))
+        torch.cuda.current_stream().wait_stream(side)
+
+
+def test_rows_far_apart():
+    """Offsets beyond 32 bits: three rows 1.5e9 elements apart, of logits and of their gradient."""
+    m = gc.pkg()
+    V, stride = 5003, 1500000001
+    c = make(3, V, BF16, 71)
+    mem, out = torch.empty(3 * stride, dtype=BF16, device=DEV), torch.empty(3 * stride, dtype=BF16, device=DEV)
+    far, far_out = mem.view(3, stride)[:, :V], out.view(3, stride)[:, :V]
+    far.copy_(c["x"])
+    old, adv = torch.full((3,), -7.0, device=DEV), torch.ones(3, device=DEV)
+    near_by = m.policy_loss_rows(c["dx"], c["dids"], old, adv, entropy_coef=0.1)
+    away = m.policy_loss_rows(far, c["dids"], old, adv, entropy_coef=0.1, out=far_out)
+    # (rows begin elsewhere against the 16-byte boundaries, so a thread has other logits: sums differ in their last bits, within twice what either may be off)
+    assert float((near_by[1] - away[1]).abs().max()) <= 2 * float(lr.lp_tol(lr.score(c["x"], c["ids"]), V).max())
+    assert float((near_by[3].float() - away[3].float()).abs().max()) <= 2 ** -8 * float(near_by[3].float().abs().max())
+    lp, stats, H = m.token_logprobs(far, c["dids"], want_entropy=True)
+    r = lr.score(c["x"], c["ids"])
+    near(lp, r["lp"], lr.lp_tol(r, V), "logprob")
+    near(H, r["H"], lr.H_tol(r, V), "entropy")
+    g = m.token_logprobs_grad(far, c["dids"], stats, d_logprob=adv, out=far_out)
+    want, size = lr.grad(r, torch.ones(3, dtype=torch.float64), torch.zeros(3, dtype=torch.float64))
+    near(g, want, lr.grad_tol(r, size, want, V, BF16), "gradient")
+
+
+def test_scores_without_a_workspace():
+    """Through the C entry point: every row is one workgroup's then."""
+    import ctypes as C
+    m = gc.pkg()
+    for rows, V in ((2, 151936), (1, 40000)):
+        c = make(rows, V, F32, 81)
+        r = lr.score(c["x"], c["ids"], c["inv_t"])
+        d = m.LossRows(c["dx"].data_ptr(), m.DTYPE_F32, rows, V, V, c["dids"].data_ptr(), c["dinv"].data_ptr())
+        assert m.lib().ws_token_logprobs_workspace(C.byref(d)) > 0
+        lp, stats, H = torch.empty(rows, device=DEV), torch.empty((rows, 2), device=DEV), torch.empty(rows, device=DEV)
+        m.check(m.lib().ws_token_logprobs(torch.cuda.current_stream().cuda_stream, C.byref(d), lp.data_ptr(), stats.data_ptr(), H.data_ptr(), None, 0), "ws_token_logprobs")
+        # (a thread adds V / 256 terms here, as everywhere the tolerance says)
+        near(lp, r["lp"], lr.lp_tol(r, V), "logprob")
+        near(H, r["H"], lr.H_tol(r, V), "entropy")
+        assert torch.equal(stats[:, 0].cpu().double(), r["m"])
+
+
+def test_calls_on_two_streams_at_once():
+    m = gc.pkg()
+    cases = [make(8, 90000, BF16, 91 + i) for i in range(2)]
+    old = torch.full((8,), -7.0, device=DEV)
+    adv = torch.linspace(-1, 1, 8, device=DEV)
+    call = lambda c: m.policy_loss_rows(c["dx"], c["dids"], old, adv, inv_t=c["dinv"], entropy_coef=0.02)  # noqa: E731
+    want = [call(c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, (s, c) in enumerate(zip(streams, cases)):
+            with torch.cuda.stream(s):
+                got[i].append(call(c))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(g, want[i]))
+
+
+def test_arguments_that_are_refused():
+    m = gc.pkg()
+    x, ids, v = torch.zeros((4, 100), device=DEV), torch.zeros(4, dtype=torch.int32, device=DEV), torch.zeros(4, device=DEV)
+    st = torch.ones((4, 2), device=DEV)
+    words = torch.zeros((4, 4), dtype=torch.int32, device=DEV)
+    bad = [lambda: m.token_logprobs(x.half(), ids), lambda: m.token_logprobs(x[:, ::2], ids), lambda: m.token_logprobs(x[0], ids), lambda: m.token_logprobs(x, ids.long()),
+           lambda: m.token_logprobs(x, ids[:3]), lambda: m.token_logprobs(x, ids.cpu()), lambda: m.token_logprobs(x, ids, inv_t=v.double()),
+           lambda: m.token_logprobs(x, ids, allow=words[:, :3]), lambda: m.token_logprobs(x, ids, allow=words[:3]), lambda: m.token_logprobs(x[:1].expand(4, 100), ids),
+           lambda: m.token_logprobs_grad(x, ids, None, d_logprob=v), lambda: m.token_logprobs_grad(x, ids, st[:3], d_logprob=v), lambda: m.token_logprobs_grad(x, ids, st, d_entropy=v),
+           lambda: m.token_logprobs_grad(x, ids, st, d_logprob=v, out=x.bfloat16()), lambda: m.token_logprobs_grad(x, ids, st, d_logprob=v, out=x[:3]),
+           lambda: m.token_logprobs_grad(x.view(-1)[:396].view(4, 99), ids, st, d_logprob=v, out=x.view(-1)[4:].view(4, 99)),
+           lambda: m.policy_loss_rows(x, None, v, v), lambda: m.policy_loss_rows(x, ids, None, v), lambda: m.policy_loss_rows(x, ids, v, v, kl_coef=0.1),
+           lambda: m.policy_loss_rows(x, ids, v, v, dual_clip=0.5), lambda: m.policy_loss(v, v, v, entropy_coef=0.1), lambda: m.policy_loss(v, v[:3], v),
+           lambda: m.policy_loss(v, v, v, clip_low=2.0), lambda: m.preference_loss(v, ids[:1]), lambda: m.preference_loss(v, ids), lambda: m.preference_loss(v, ids[:3], label_smoothing=2.0),
+           lambda: m.preference_loss(v, ids[:3], ref_logprob=v[:2])]
+    for i, call in enumerate(bad):
+        with pytest.raises(m.WsError):
+            call()
+            raise AssertionError(i)

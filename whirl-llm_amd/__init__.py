@@ -118,7 +118,7 @@ class Policy(C.Structure):
     """ws_policy of include/whirl_sampling_abi.h."""
     _fields_ = [("old_logprob", C.c_void_p), ("ref_logprob", C.c_void_p), ("advantage", C.c_void_p), ("weight", C.c_void_p),
                 ("clip_low", C.c_double), ("clip_high", C.c_double), ("dual_clip", C.c_double), ("kl_coef", C.c_double),
-                ("entropy_coef", C.c_double)]
+                ("entropy_coef", C.c_double), ("spins", C.c_uint32)]
 
 
 class Preference(C.Structure):
@@ -687,12 +687,13 @@ def policy_loss(logprob, old_logprob, advantage, ref_logprob=None, entropy=None,
 
 
 def policy_loss_rows(logits, ids, old_logprob, advantage, ref_logprob=None, weight=None, inv_t=None, allow=None, clip_low=0.2, clip_high=0.2,
-                     dual_clip=0.0, kl_coef=0.0, entropy_coef=0.0, want_entropy=False, out=None):
+                     dual_clip=0.0, kl_coef=0.0, entropy_coef=0.0, want_entropy=False, out=None, spins=0):
     """The clipped policy loss from the logits and its gradient by them (ws_policy_loss_rows): token_logprobs, policy_loss and token_logprobs_grad in
     one. Rows without a token and rows of weight 0 count for nothing and are not read. out: where to write the gradient; it may be
-    `logits`. Returns (sums float32 [5], logprob float32 [rows], entropy float32 [rows] or None, d_logits)."""
+    `logits`. spins: ws_policy.spins. Returns (sums float32 [5], logprob float32 [rows], entropy float32 [rows] or None, d_logits)."""
     r, rows, vocab, at = _loss_rows(logits, _given("ids", ids), inv_t, allow)
     p = _policy(old_logprob, advantage, ref_logprob, weight, rows, at, clip_low, clip_high, dual_clip, kl_coef, entropy_coef)
+    p.spins = spins
     out, stride = _gradient_for(logits, out, vocab)
     dev, call, ref = logits.device, lib(), C.byref(r)
     need = call.ws_policy_loss_rows_workspace(ref)

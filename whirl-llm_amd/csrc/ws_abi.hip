@@ -1256,6 +1256,7 @@ int ws_policy_loss_rows(void* stream, const ws_loss_rows* r, const ws_policy* p,
         a.per = share_of(row_vectors(r), n.parts);
         a.meet = reinterpret_cast<unsigned long long*>(work + n.meet);
         a.tag = launch_tag();
+        a.looks = p->spins ? p->spins : 256u;
         if (const int e = ws::launch_policy_rows(S(stream), r->dtype, a, p->entropy_coef != 0.0); e != 0) return e;
         if (n.one) return WS_OK;
         sum.words = a.meet;

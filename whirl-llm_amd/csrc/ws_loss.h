@@ -644,8 +644,8 @@ struct RowsArgs {
     uint32_t parts, per;       // workgroups a row, vectors each
     unsigned long long* meet;  // parts > 1: [rows][kPartWords][parts]; of rows that meet in this launch [rows][kPartWords + 2][parts], the last two the parts' marks
     unsigned long long tag;
+    uint32_t looks;  // for the other parts' words, a microsecond each
 };
-constexpr uint32_t kLooks = 256u;  // some 0.3 ms; the others usually come within microseconds
 
 template <int DT, bool ENT, bool SLOPE, bool MASK, int T, int NV, int WAVES>  // WAVES: a SIMD's at least
 __global__ void __launch_bounds__(T, WAVES) policy_rows_kernel(RowsArgs A) {
@@ -746,7 +746,7 @@ __global__ void __launch_bounds__(T, WAVES) policy_rows_kernel(RowsArgs A) {
             const bool in = t < A.parts;
             PartSums w{};
             bool here = !in;
-            for (uint32_t look = 0; look < kLooks; ++look) {
+            for (uint32_t look = 0; look < A.looks; ++look) {
                 if (!here) here = find_part<ENT>(meet, A.parts, t, A.tag, w);
                 if (__ballot(!here) == 0ull) break;
                 __builtin_amdgcn_s_sleep(4);
