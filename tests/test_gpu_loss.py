@@ -231,12 +231,12 @@ def test_policy_loss_of_no_tokens():
     assert m.token_logprobs_grad(logits, torch.empty(0, dtype=torch.int32, device=DEV), stats).shape == (0, 100)
 
 
-# rows of one workgroup and of several, of all builds (shares of up to 256, 1024 and 3072 vectors); sums over up to 64, 1024 and 4096 rows, and over more in a second launch
+# rows of one workgroup and of several, of all builds (shares of up to 256, 1024 and 3072 vectors); sums over up to 64 and 1024 rows, of rows of three parts up to 4096, over more in a second launch
 ROWS = [(600, 777), (520, 12400), (513, 25001), (1030, 1100), (4096, 261), (4097, 300), (1, 1), (1, 129), (7, 1000), (16, 50257), (3, 151936), (5, 262144), (130, 3), (140, 1001), (130, 20480), (129, 20485), (128, 40961), (130, 50257), (128, 81921), (128, 151936),
         (128, 160007)]
 
 
-POLICY_CASES = [(rows, V, dtype, kind) for rows, V in ROWS for dtype in (F32, BF16) for kind in ("plain", "entropy", "bonus", "masked")] + [(4100, 12500, F32, "bonus")]
+POLICY_CASES = [(rows, V, dtype, kind) for rows, V in ROWS for dtype in (F32, BF16) for kind in ("plain", "entropy", "bonus", "masked")] + [(4100, 12500, F32, "bonus"), (1027, 24700, F32, "masked")]
 
 
 @pytest.mark.parametrize("rows,V,dtype,kind", POLICY_CASES)

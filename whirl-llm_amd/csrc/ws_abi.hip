@@ -1154,7 +1154,9 @@ RowsPlan rows_plan(const ws_loss_rows* r) {
     if (parts > 64u) parts = 64u;
     if (parts < least) parts = least;
     n.parts = parts < 1u ? 1u : parts;
-    n.one = r->rows != 0u && r->rows <= ws::kMostSlots;
+    // (Whose first part's workgroups look at the sums before they end: beyond 1024 rows worth it where they are one in three or fewer. In one launch / in two, us: 700 x 50257 bf16 40.0 / 42.0,
+    // 1024 x 151936 124.5 / 129.4, 2048 x 65536 109.7 / 111.1; with two parts a row 1500 x 32000 53.6 / 50.5, 3000 x 32000 94 / 82, with one 4000 x 8000 38.0 / 35.4.)
+    n.one = r->rows != 0u && r->rows <= (n.parts > 2u ? ws::kMostSlots : 1024u);
     n.words = meet_bytes(r->rows, n.parts, ws::kPartWords + (n.one ? 2u : 0u));
     n.groups = r->rows < 64u * 1024u ? r->rows / 1024u + 1u : 64u;  // (of the second launch)
     n.meet = ws::sums_bytes(n.one ? r->rows : n.groups, ws::kPolicySums);
