@@ -552,7 +552,8 @@ int ws_spec_verify_classic(void* stream, const ws_spec_verify* v);
  * Logits that are not allowed count as -inf, whatever they hold. A row where nothing is left (every allowed logit -inf, or none
  * allowed) has stats {-inf, 0}, entropy 0 and, if it has a token, logprob -inf, and its derivatives are 0. A token that is not allowed
  * has logprob -inf and its row the derivatives of the others. An allowed logit of +inf or NaN, or an inv_t that is
- * not a positive finite number, makes everything of its row NaN. Results are the same bits on every run.
+ * not a positive finite number, makes everything of its row NaN. Results are the same bits on every run over the same memory (which thread
+ * adds up which logits goes by where a row - of ws_policy_loss_rows its gradient - lies against the 128-byte lines).
  * rows and vocab: at most 1048575 each. */
 typedef struct ws_loss_rows {
     const void* logits; /* device, [rows][row_stride] of dtype, aligned to its elements */
@@ -562,7 +563,7 @@ typedef struct ws_loss_rows {
     uint64_t row_stride;    /* elements between rows (>= vocab) */
     const int32_t* ids;     /* device [rows] (NULL: no row has a token) */
     const float* inv_t;     /* device [rows], 1 / temperature (NULL: 1) */
-    const uint32_t* allow;  /* bitmap as in ws_batch (NULL: all) */
+    const uint32_t* allow;  /* bitmap as in ws_batch, 4-byte aligned (NULL: all) */
     uint64_t allow_stride;  /* 32-bit words between rows (>= (vocab + 31) / 32) */
 } ws_loss_rows;
 

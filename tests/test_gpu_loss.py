@@ -231,7 +231,7 @@ def test_policy_loss_of_no_tokens():
     assert m.token_logprobs_grad(logits, torch.empty(0, dtype=torch.int32, device=DEV), stats).shape == (0, 100)
 
 
-# rows of one workgroup and of several, of all builds (shares of up to 256, 1024 and 3072 vectors); sums over up to 64 and 1024 rows, of rows of three parts up to 4096, over more in a second launch
+# rows of one workgroup and of several, of all builds (shares of up to 256 vectors, of 4 and of 12 times as many); sums over up to 64 and 1024 rows, of rows of three parts up to 4096, over more in a second launch
 ROWS = [(600, 777), (520, 12400), (513, 25001), (1030, 1100), (4096, 261), (4097, 300), (1, 1), (1, 129), (7, 1000), (16, 50257), (3, 151936), (5, 262144), (130, 3), (140, 1001), (130, 20480), (129, 20485), (128, 40961), (130, 50257), (128, 81921), (128, 151936),
         (128, 160007)]
 
@@ -534,3 +534,38 @@ def test_arguments_that_are_refused():
         with pytest.raises(m.WsError):
             call()
             raise AssertionError(i)
+
+
+FIRST_CALL = """
+import sys, torch
+sys.path[:0] = [{root!r}]
+from __graft_entry__ import load_package
+m = load_package()
+x = torch.randn(3, 70001, device="cuda:0")
+ids = torch.zeros(3, dtype=torch.int32, device="cuda:0")
+v = torch.zeros(3, device="cuda:0")
+side = torch.cuda.Stream()
+torch.cuda.synchronize()
+assert m.lib().ws_probe() == 0
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.stream(side):
+    graph.capture_begin()
+    lp, stats, _ = m.token_logprobs(x, ids)
+    sums, lp2, H, d = m.policy_loss_rows(x, ids, v, v + 1.0, entropy_coef=0.1)
+    graph.capture_end()
+    for k in range(3):
+        x.add_(0.25)
+        graph.replay()
+        want = m.token_logprobs(x, ids), m.policy_loss_rows(x, ids, v, v + 1.0, entropy_coef=0.1)
+        side.synchronize()
+        assert torch.equal(lp, want[0][0]) and torch.equal(d, want[1][3]) and torch.equal(sums, want[1][0])
+print("captured first")
+"""
+
+
+def test_first_calls_of_a_process_under_capture():
+    """ws_probe loads the kernels, so a captured call may be the first that needs them."""
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL.format(root=gc.ROOT)], capture_output=True, text=True, timeout=110)
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stderr[-2000:]

@@ -24,7 +24,7 @@ def policy_of(m, **change):
 
 
 BAD_ROWS = [dict(logits=None), dict(logits=AT + 2), dict(dtype=2), dict(dtype=-1), dict(vocab=0), dict(vocab=1 << 20), dict(rows=1 << 20), dict(row_stride=99),
-            dict(allow=AT, allow_stride=3), dict(dtype=1, logits=AT + 1)]
+            dict(allow=AT, allow_stride=3), dict(allow=AT + 2, allow_stride=4), dict(dtype=1, logits=AT + 1)]
 
 
 @pytest.mark.parametrize("change", BAD_ROWS)

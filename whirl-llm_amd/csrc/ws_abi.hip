@@ -66,6 +66,7 @@ int launch_grad(hipStream_t stream, int dtype, const GradArgs& a);
 int launch_policy_rows(hipStream_t stream, int dtype, const RowsArgs& a, bool slope);
 int launch_policy(hipStream_t stream, const PolicyArgs& a, unsigned groups);
 int launch_preference(hipStream_t stream, const PreferenceArgs& a, unsigned groups);
+int prepare_loss();
 uint32_t loss_most_share();  // vectors of a row that a workgroup of policy_rows_kernel holds
 }  // namespace ws
 
@@ -522,6 +523,7 @@ int prepare_all() {
     if (const int e = ws::prepare_twin(kMaxLds - kStaticTwin); e != 0) return e;
     if (const int e = ws::prepare_few(kMaxLds - kStaticFew); e != 0) return e;
     if (const int e = ws::prepare_top(); e != 0) return e;
+    if (const int e = ws::prepare_loss(); e != 0) return e;
     return ws::prepare_short(kMaxLds - kStaticShort);
 }
 
@@ -1088,7 +1090,7 @@ bool aligned(const void* p, uint64_t to) { return reinterpret_cast<uintptr_t>(p)
 bool loss_rows_ok(const ws_loss_rows* r) {
     if (!r || (r->dtype != WS_DTYPE_F32 && r->dtype != WS_DTYPE_BF16) || r->vocab == 0 || r->vocab > 1048575u || r->rows > kMostLossRows) return false;
     if (r->rows && (!r->logits || !aligned(r->logits, elem_bytes(r->dtype)))) return false;
-    if (r->row_stride < r->vocab || (r->allow && r->allow_stride < (r->vocab + 31u) / 32u)) return false;
+    if (r->row_stride < r->vocab || (r->allow && (r->allow_stride < (r->vocab + 31u) / 32u || !aligned(r->allow, 4u)))) return false;
     return true;
 }
 // bytes from a matrix's first element to behind its last

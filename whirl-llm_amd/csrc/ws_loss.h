@@ -436,14 +436,15 @@ __device__ __forceinline__ RowSums join_parts(bool in, const PartSums& w, const 
     return r;
 }
 
-// ---- log-probabilities: a workgroup a row, or `parts` of them
+// ---- log-probabilities: a workgroup a row, or `parts` of them. The next four vectors of a thread are on their way while it works on four. What bounds it: memory, and of bf16 rows the vector units as
+// much (7.8 instructions a logit, and some 200 a wave for its sums): 2048 x 151936 bf16 111 us = 5.6 TB/s, fp32 209 us = 5.95 TB/s.
 struct ScoreArgs {
     LossRows R;
     float* logprob;
     float* stats;
     float* entropy;
     uint32_t parts, per;       // workgroups a row, vectors each
-    unsigned long long* meet;  // parts > 1: [rows][parts][kPartWords], broken again by whoever joins them
+    unsigned long long* meet;  // parts > 1: [rows][kPartWords][parts], broken again by whoever joins them
     unsigned long long tag;
 };
 
@@ -523,7 +524,8 @@ __global__ void __launch_bounds__(T) score_rows_kernel(ScoreArgs A) {
     if (ENT) A.entropy[row] = static_cast<float>(v.H);
 }
 
-// ---- the gradient
+// ---- the gradient: two vectors a thread and no more, so that many workgroups are at different stages (four: 1024 x 151936 bf16, a quarter of the rows without derivatives, 101 us, two: 90; one: 106, three: 93;
+// all past the caches). Memory bounds it: 5.8 TB/s there.
 struct GradArgs {
     LossRows R;
     const float* stats;
@@ -627,9 +629,11 @@ __global__ void __launch_bounds__(T) grad_rows_kernel(GradArgs A) {
 // that all parts run at once: a part that does not find another's words in time works that part's sums out itself, in the
 // same order and so to the same bits. (Where the gradient goes over the logits: a part writes only after its words have arrived. So logits
 // read before a look that still finds no words are the logits, and the token's logit goes with the words, not to be read
-// by a part that comes late.) The words stay until every part has seen them:
-// the parts leave a mark each when they are through, and whoever sees all marks of a row breaks its words. The rows' terms meet in this launch as well. Of more rows
-// than kMostSlots a second launch adds up the terms and breaks the words (5 us).
+// by a part that comes late.) The words stay until every part has seen them: where the rows' terms meet in this launch too (`terms` is NULL), the parts leave a mark each when they are
+// through, and whoever sees all marks of a row breaks its words; else a second launch adds up the terms and breaks the words.
+// What bounds it: memory, and the vector units at 80 % (16.6 instructions a logit, 19.6 with entropy). 2048 x 151936 bf16 with entropy, a fifth of the rows not counting, 214 us = 5.2 TB/s; 4096 x
+// 262144 741 us = 5.8 TB/s; a row in one workgroup of 1024 threads, what its registers do not hold read twice, 282 and 988. Shares of 11, 14, 16 or 19 vectors a thread are up to 8 % slower, workgroups of 512
+// threads 10 to 20 %: a unit then holds fewer of them, and fewer are at another stage than their neighbours.
 struct RowsArgs {
     LossRows R;
     PolicyIn P;
@@ -639,7 +643,7 @@ struct RowsArgs {
     uint64_t out_bytes;
     uint32_t past_row;  // as GradArgs
     double* terms;             // [kPolicySums][rows], or:
-    unsigned long long* sums_meet;  // [kPolicySums][2][rows], for rows that meet in this launch
+    unsigned long long* sums_meet;  // [kPolicySums][2][rows] and, of more than 64, [kPolicySums][2][64]: for rows that meet in this launch
     float* sums;
     uint32_t parts, per;       // workgroups a row, vectors each
     unsigned long long* meet;  // parts > 1: [rows][kPartWords][parts]; of rows that meet in this launch [rows][kPartWords + 2][parts], the last two the parts' marks
@@ -840,7 +844,7 @@ struct PolicyArgs {
     float* d_logprob;
     float* d_entropy;
     float* sums;
-    unsigned long long* meet;  // [kPolicySums][2][workgroups]
+    unsigned long long* meet;  // [kPolicySums][2][workgroups] and, of more than 64, [kPolicySums][2][64]
     unsigned long long tag;
     unsigned long long* words;  // the rows' parts' words, to be broken
     uint64_t n_words;

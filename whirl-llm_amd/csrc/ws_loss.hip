@@ -57,6 +57,12 @@ void by_kind(int dtype, bool ent, bool mask, A&&... a) {
 }
 }  // namespace
 
+// loads this file's kernels on the current device (the first launch would; under capture there is nothing left to do then)
+int prepare_loss() {
+    hipFuncAttributes fa;
+    return static_cast<int>(hipFuncGetAttributes(&fa, reinterpret_cast<const void*>(&policy_kernel<kPolicyThreads>)));
+}
+
 uint32_t loss_most_share() { return kMostShare; }
 
 int launch_score(hipStream_t stream, int dtype, const ScoreArgs& a) {
