@@ -15,7 +15,7 @@ from test_lds_budget import READELF
 from test_meeting_order import LIB, code_objects
 
 KERNELS = r"score_rows_kernel|grad_rows_kernel|policy_rows_kernel|policy_kernel|preference_kernel"
-N_KERNELS = 16 + 8 + 36 + 2  # scores, gradients, policy rows of three builds, the two losses over log-probabilities
+N_KERNELS = 16 + 8 + 36 + 6 + 2  # scores, gradients, policy rows of three builds and of a fourth for fp32, the two losses over log-probabilities
 VECTOR = re.compile(r"v_(?!writelane|readlane|readfirstlane)|scratch_|global_|ds_|flat_|buffer_")
 ENDS = re.compile(r"s_cbranch|s_branch|s_and_saveexec|s_mov_b64 exec|s_and_b64 exec|s_xor_b64 exec|s_andn2_b64 exec")
 

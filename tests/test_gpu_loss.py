@@ -44,7 +44,7 @@ def near(got, want, tol, what):
         raise AssertionError((what, i, float(got[tuple(i)]), float(want[tuple(i)]), float(tol[tuple(i)]), int(bad.sum()), bad.numel()))
 
 
-SHAPES = [(1, 1), (3, 2), (2, 7), (5, 31), (4, 33), (6, 129), (9, 1000), (3, 4099), (300, 777), (2, 20481), (3, 50257), (260, 8200), (1, 151936), (2, 262144), (2, 65543)]
+SHAPES = [(1, 1), (3, 2), (2, 7), (5, 31), (4, 33), (6, 129), (9, 1000), (3, 4099), (300, 777), (2, 20481), (3, 50257), (260, 8200), (1, 151936), (2, 262144), (2, 65543), (2, 1048575)]
 
 
 @pytest.mark.parametrize("rows,V", SHAPES)
@@ -236,7 +236,8 @@ ROWS = [(600, 777), (520, 12400), (513, 25001), (1030, 1100), (4096, 261), (4097
         (128, 160007)]
 
 
-POLICY_CASES = [(rows, V, dtype, kind) for rows, V in ROWS for dtype in (F32, BF16) for kind in ("plain", "entropy", "bonus", "masked")] + [(4100, 12500, F32, "bonus"), (1027, 24700, F32, "masked")]
+POLICY_CASES = [(rows, V, dtype, kind) for rows, V in ROWS for dtype in (F32, BF16) for kind in ("plain", "entropy", "bonus", "masked")] + [(4100, 12500, F32, "bonus"), (1027, 24700, F32, "masked")] \
+    + [(5, 1048575, dtype, kind) for dtype in (F32, BF16) for kind in ("plain", "entropy", "bonus", "masked")] + [(2, V, F32, "masked") for V in (786407, 786409)]  # the longest, and 64 full shares
 
 
 @pytest.mark.parametrize("rows,V,dtype,kind", POLICY_CASES)
@@ -425,7 +426,7 @@ def test_parts_that_do_not_wait_for_each_other_give_the_same_bits(dtype):
     waiting gives, in place or not, and the sums' and parts' words are left as the next call needs them (replays of a captured graph). In place has bits of its own: which
     thread adds up which logits goes by the boundaries of the memory that the gradient is written to."""
     m = gc.pkg()
-    for rows, V, masked in ((1, 151936, False), (6, 100003, True), (40, 65537, False), (200, 50257, False)):
+    for rows, V, masked in ((1, 151936, False), (6, 100003, True), (40, 65537, False), (200, 50257, False), (2, 1048575, True)):
         c = make(rows, V, dtype, 61 + rows, masked, 3, 1)
         old, adv = torch.full((rows,), -7.0, device=DEV), torch.linspace(-1, 1, rows, device=DEV)
         args = dict(ref_logprob=old, inv_t=c["dinv"], allow=c["dallow"], kl_coef=0.1, entropy_coef=0.02)
@@ -482,7 +483,7 @@ def test_scores_without_a_workspace():
     """Through the C entry point: every row is one workgroup's then."""
     import ctypes as C
     m = gc.pkg()
-    for rows, V in ((2, 151936), (1, 40000)):
+    for rows, V in ((2, 151936), (1, 40000), (1, 1048575)):
         c = make(rows, V, F32, 81)
         r = lr.score(c["x"], c["ids"], c["inv_t"])
         d = m.LossRows(c["dx"].data_ptr(), m.DTYPE_F32, rows, V, V, c["dids"].data_ptr(), c["dinv"].data_ptr())

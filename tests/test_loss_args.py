@@ -86,6 +86,18 @@ def test_policy_outputs_and_workspaces_that_are_refused():
     assert lib.ws_policy_loss(None, 1 << 31, C.byref(p), AT, None, AT, AT, None, AT, 1 << 20) == m.E_INVALID
 
 
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("rows,words", [(1, 8), (2000, 8), (4096, 8), (5000, 6)])
+def test_the_longest_rows_have_no_more_parts_than_can_meet(dtype, rows, words):
+    """A wave looks at a row's parts, one a lane: 64 at most, each with six words and, where the rows' sums meet in the same launch, two for its mark."""
+    m = gc.pkg()
+    r = rows_of(m, dtype=dtype, rows=rows, vocab=1048575, row_stride=1048575)
+    slots, second = (0 if rows == 1 else rows + (64 if rows > 64 else 0), 0) if words == 8 else (rows // 1024 + 1, rows * 5 * 8)
+    sums = slots * 5 * 16
+    parts = (m.lib().ws_policy_loss_rows_workspace(C.byref(r)) - sums - second) / (rows * words * 8)
+    assert parts == int(parts) and 2 <= parts <= 64
+
+
 @pytest.mark.parametrize("change", [dict(pairs=0), dict(pairs=1 << 31), dict(rows=1 << 31), dict(seq_off=None), dict(logprob=None), dict(loss=None), dict(pair_loss=None),
                                     dict(reward=None), dict(d_logprob=None), dict(beta=float("nan")), dict(label_smoothing=-0.1), dict(label_smoothing=1.5),
                                     dict(label_smoothing=float("nan"))])

@@ -1155,8 +1155,8 @@ RowsPlan rows_plan(const ws_loss_rows* r) {
     const uint32_t vectors = row_vectors(r), least = (vectors + ws::loss_most_share() - 1u) / ws::loss_most_share();
     uint32_t parts = r->rows ? 2u * static_cast<uint32_t>(compute_units()) / r->rows : 1u;
     if (parts > vectors / 256u) parts = vectors / 256u;
-    if (parts > 64u) parts = 64u;
     if (parts < least) parts = least;
+    if (parts > 64u) parts = 64u;  // (what a wave looks at; fp32 rows of more than 786 000 tokens then have shares of workgroups of 512)
     n.parts = parts < 1u ? 1u : parts;
     // (Whose first part's workgroups look at the sums before they end: beyond 1024 rows worth it where they are one in three or fewer. In one launch / in two, us: 700 x 50257 bf16 40.0 / 42.0,
     // 1024 x 151936 124.5 / 129.4, 2048 x 65536 109.7 / 111.1; with two parts a row 1500 x 32000 53.6 / 50.5, 3000 x 32000 94 / 82, with one 4000 x 8000 38.0 / 35.4.)

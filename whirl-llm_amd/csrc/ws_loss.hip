@@ -6,8 +6,10 @@ namespace ws {
 
 namespace {
 constexpr uint32_t kScoreThreads = 256u, kGradThreads = 256u, kGradVectors = 2u, kPolicyThreads = 1024u;
-// vectors of a workgroup's share: up to the first a wave takes them, up to the second and third 256 threads of policy_rows_kernel
-constexpr uint32_t kLeastShare = 4u * 64u, kSmallShare = 4u * 256u, kMostShare = 12u * 256u;
+// vectors of a workgroup's share: up to the first a wave takes them, up to the second and third 256 threads of policy_rows_kernel, beyond it 512 (fp32 rows that 64 parts of the third do not hold)
+constexpr uint32_t kLeastShare = 4u * 64u, kSmallShare = 4u * 256u, kMostShare = 12u * 256u, kWideShare = 12u * 512u;
+// (the longest rows that the entry points take, in vectors, and the 64 parts that can meet)
+static_assert((1048575u / Elem<0>::kPer + 7u + 63u) / 64u + 7u <= kWideShare && (1048575u / Elem<1>::kPer + 7u + 63u) / 64u + 7u <= kMostShare);
 
 template <int DT, bool ENT, bool MASK>
 struct Score {
@@ -36,7 +38,8 @@ struct Rows {
         const uint32_t share = a.per;
         if (share <= kLeastShare && a.parts == 1u) rows<DT, ENT, SLOPE, MASK, 64, 4, 6>(s, a);
         else if (share <= kSmallShare) rows<DT, ENT, SLOPE, MASK, 256, 4, 6>(s, a);
-        else rows<DT, ENT, SLOPE, MASK, 256, 12, 5>(s, a);
+        else if (DT != 0 || share <= kMostShare) rows<DT, ENT, SLOPE, MASK, 256, 12, 5>(s, a);
+        else if constexpr (DT == 0) rows<DT, ENT, SLOPE, MASK, 512, 12, 4>(s, a);
     }
     static void go(hipStream_t s, const RowsArgs& a, bool slope) {
         if constexpr (ENT) {
