@@ -122,9 +122,12 @@ def H_tol(r, V):
     return sum_tol(r, V) * (1.0 + 2.0 * mean) + EPS * (2.0 * square + r["H"].abs() + 4.0 * mean)
 
 
-def grad_tol(r, size, want, V, dtype, extra=0.0):
+def grad_tol(r, size, want, V, dtype, extra=0.0, h=None):
     """Each entry: p as above (its own exponent, S), six roundings of factors and sums (extra: relative error of g and h), and the rounding to the
-    logits' type."""
+    logits' type. h, the derivative by the entropy: ln p = d - ln S comes from the S of the stats, a float32. S (1 + e) with |e| <= EPS has ln S + ln(1 + e),
+    so ln p is off by up to EPS / (1 - EPS) whatever its size - where one token has nearly all of the row, ln p is 5e-4 and that is more than any rounding
+    relative to it - and the entry by t |h| p times that."""
     step = torch.finfo(dtype).eps / 2
     rel = EPS * (2.0 * r["a"].abs() + 12.0) + sum_tol(r, V)[:, None] + extra
-    return size * rel + want.abs() * step + 2.0 ** -126
+    tol = size * rel + want.abs() * step + 2.0 ** -126
+    return tol if h is None else tol + (r["t"] * h.double().abs())[:, None] * r["p"] * (EPS / (1.0 - EPS))

@@ -44,7 +44,7 @@ def near(got, want, tol, what):
         raise AssertionError((what, i, float(got[tuple(i)]), float(want[tuple(i)]), float(tol[tuple(i)]), int(bad.sum()), bad.numel()))
 
 
-SHAPES = [(1, 1), (3, 2), (2, 7), (5, 31), (4, 33), (6, 129), (9, 1000), (3, 4099), (300, 777), (2, 20481), (3, 50257), (260, 8200), (1, 151936), (2, 262144), (2, 65543), (2, 1048575)]
+SHAPES = [(1, 1), (3, 2), (2, 7), (5, 31), (4, 33), (6, 129), (9, 1000), (3, 4099), (300, 777), (2, 20481), (3, 50257), (260, 8200), (1, 151936), (2, 262144), (2, 65543), (2, 1048575), (70001, 9)]  # (more rows than a grid has in its second dimension)
 
 
 @pytest.mark.parametrize("rows,V", SHAPES)
@@ -81,11 +81,11 @@ def test_gradient(rows, V, dtype, masked):
             mem = torch.full((rows, V + 5), 77.0, dtype=dtype, device=DEV)
             out = m.token_logprobs_grad(c["dx"], c["dids"], stats, d_logprob=g.to(DEV), entropy=H if with_h else None, d_entropy=h.to(DEV) if with_h else None,
                                         inv_t=c["dinv"], allow=c["dallow"], out=mem[:, :V])
-            near(out, want, lr.grad_tol(r, size, want, V, dtype), "gradient")
+            near(out, want, lr.grad_tol(r, size, want, V, dtype, h=h if with_h else None), "gradient")
             assert bool((mem[:, V:] == 77.0).all()), "written beyond the row"
         own = m.token_logprobs_grad(c["dx"], c["dids"], stats, d_logprob=g.to(DEV), entropy=H, d_entropy=h.to(DEV), inv_t=c["dinv"], allow=c["dallow"], out=c["dx"])
         assert own.data_ptr() == c["dx"].data_ptr()  # (in place)
-        near(own, want, lr.grad_tol(r, size, want, V, dtype), "gradient in place")
+        near(own, want, lr.grad_tol(r, size, want, V, dtype, h=h), "gradient in place")
 
 
 SPECIAL = ["none_allowed", "all_minus_inf", "lowest", "some_lowest", "id_masked", "no_id", "id_past_the_row", "nan_masked", "inf_masked", "nan", "inf", "cold", "hot", "t_zero",
@@ -237,7 +237,8 @@ ROWS = [(600, 777), (520, 12400), (513, 25001), (1030, 1100), (4096, 261), (4097
 
 
 POLICY_CASES = [(rows, V, dtype, kind) for rows, V in ROWS for dtype in (F32, BF16) for kind in ("plain", "entropy", "bonus", "masked")] + [(4100, 12500, F32, "bonus"), (1027, 24700, F32, "masked")] \
-    + [(5, 1048575, dtype, kind) for dtype in (F32, BF16) for kind in ("plain", "entropy", "bonus", "masked")] + [(2, V, F32, "masked") for V in (786407, 786409)]  # the longest, and 64 full shares
+    + [(5, 1048575, dtype, kind) for dtype in (F32, BF16) for kind in ("plain", "entropy", "bonus", "masked")] + [(2, V, F32, "masked") for V in (786407, 786409)] \
+    + [(32772, 9, F32, "bonus"), (32769, 17, BF16, "masked")]  # the longest, 64 full shares, more rows than a grid has in its second dimension
 
 
 @pytest.mark.parametrize("rows,V,dtype,kind", POLICY_CASES)
@@ -453,6 +454,39 @@ def test_parts_that_do_not_wait_for_each_other_give_the_same_bits(dtype):
                 graph.replay()
                 side.synchronize()
                 assert all(torch.equal(a, b) for a, b in zip(held, own))
+        torch.cuda.current_stream().wait_stream(side)
+
+
+def test_sums_of_a_second_launch_replayed():
+    """Rows of one and of two parts, more than meet in one launch: the second launch adds up and breaks the parts' words. Captured, replayed on changed logits, eager calls between."""
+    m = gc.pkg()
+    assert m.lib().ws_probe() == 0
+    for rows, V in ((1030, 5000), (1030, 40000)):
+        c = make(rows, V, BF16, 57)
+        old, adv = torch.full((rows,), -8.0, device=DEV), torch.linspace(-1, 1, rows, device=DEV)
+        start = c["dx"].clone()
+
+        def step():
+            return m.policy_loss_rows(c["dx"], c["dids"], old, adv, ref_logprob=old, inv_t=c["dinv"], kl_coef=0.1, entropy_coef=0.01)
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            eager = []
+            for k in range(3):
+                c["dx"].copy_(torch.roll(start, 5 * k, 1))
+                eager.append([t.clone() for t in step()])
+            side.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            graph.capture_begin()
+            held = step()
+            graph.capture_end()
+            for k in range(3):
+                c["dx"].copy_(torch.roll(start, 5 * k, 1))
+                graph.replay()
+                between = step()
+                side.synchronize()
+                assert all(torch.equal(a, b) and torch.equal(e, b) for a, b, e in zip(held, eager[k], between)), (rows, V, k)
         torch.cuda.current_stream().wait_stream(side)
 
 

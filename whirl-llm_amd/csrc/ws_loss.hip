@@ -6,7 +6,8 @@ namespace ws {
 
 namespace {
 constexpr uint32_t kScoreThreads = 256u, kGradThreads = 256u, kGradVectors = 2u, kPolicyThreads = 1024u;
-// vectors of a workgroup's share: up to the first a wave takes them, up to the second and third 256 threads of policy_rows_kernel, beyond it 512 (fp32 rows that 64 parts of the third do not hold)
+// vectors of a workgroup's share: up to the first a wave takes them, up to the second and third 256 threads of policy_rows_kernel, beyond it 512 (fp32 rows that 64 parts of the third
+// do not hold: 400 x 786 400 on one side of the border 589 us, x 786 416 on the other 707)
 constexpr uint32_t kLeastShare = 4u * 64u, kSmallShare = 4u * 256u, kMostShare = 12u * 256u, kWideShare = 12u * 512u;
 // (the longest rows that the entry points take, in vectors, and the 64 parts that can meet)
 static_assert((1048575u / Elem<0>::kPer + 7u + 63u) / 64u + 7u <= kWideShare && (1048575u / Elem<1>::kPer + 7u + 63u) / 64u + 7u <= kMostShare);
