@@ -600,7 +600,7 @@ typedef struct ws_policy {
     double kl_coef;
     double entropy_coef;
     uint32_t spins;           /* ws_policy_loss_rows: how often a workgroup that shares a row looks for the others' sums (a look takes about a microsecond) before it
-                                 works them out itself - slower, the same result: nothing says that they all run at once; 0 = 256 looks */
+                                 works them out itself - slower, the same result: nothing says that they all run at once; 0 = 256 looks, at most 65536 */
 } ws_policy;
 /* sums: loss, sum of weight * -gain, of weight * kl, of weight * entropy, and the weight of the tokens whose gain a clip holds */
 enum { WS_POLICY_LOSS = 0, WS_POLICY_SURROGATE = 1, WS_POLICY_KL = 2, WS_POLICY_ENTROPY = 3, WS_POLICY_CLIPPED = 4, WS_POLICY_SUMS = 5 };

@@ -51,7 +51,7 @@ def test_outputs_and_gradients_that_are_refused():
 
 
 BAD_POLICIES = [dict(old_logprob=None), dict(advantage=None), dict(clip_low=-0.1), dict(clip_low=1.1), dict(clip_low=float("nan")), dict(clip_high=-1e-9), dict(clip_high=float("nan")),
-                dict(dual_clip=1.0), dict(dual_clip=-2.0), dict(dual_clip=float("nan")), dict(kl_coef=float("nan")), dict(entropy_coef=float("nan")), dict(ref_logprob=None),
+                dict(dual_clip=1.0), dict(spins=65537), dict(dual_clip=-2.0), dict(dual_clip=float("nan")), dict(kl_coef=float("nan")), dict(entropy_coef=float("nan")), dict(ref_logprob=None),
                 dict(entropy_coef=0.01)]
 
 

@@ -1132,9 +1132,11 @@ uint32_t past_row(const ws_loss_rows* r) {
 }
 bool workspace_ok(const void* w, uint64_t bytes, uint64_t need) { return need == 0 || (w && bytes >= need && aligned(w, 8u)); }
 
+constexpr uint32_t kMostLooks = 65536u;  // (a wait ends: some 65 ms)
 bool policy_ok(const ws_policy* p, uint32_t rows, bool entropy) {
     if (!p || (rows && (!p->old_logprob || !p->advantage))) return false;
     if (!(p->clip_low >= 0.0 && p->clip_low <= 1.0) || !(p->clip_high >= 0.0) || !(p->dual_clip == 0.0 || p->dual_clip > 1.0)) return false;
+    if (p->spins > kMostLooks) return false;
     return p->kl_coef == p->kl_coef && p->entropy_coef == p->entropy_coef && (p->ref_logprob || p->kl_coef == 0.0) && (entropy || p->entropy_coef == 0.0);
 }
 ws::PolicyIn policy_in(const ws_policy* p, uint32_t rows) {
