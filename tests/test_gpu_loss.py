@@ -490,6 +490,19 @@ def test_sums_of_a_second_launch_replayed():
         torch.cuda.current_stream().wait_stream(side)
 
 
+@pytest.mark.parametrize("rows,V,stride", [(5, 40, 40), (5, 40, 48), (1, 40, 100), (5, 1, 1), (5, 1, 3), (1, 1, 1)])
+def test_gradients_of_rows_apart_are_contiguous(rows, V, stride):
+    m = gc.pkg()
+    x = torch.randn(rows, stride, device=DEV)[:, :V]
+    ids, v = torch.zeros(rows, dtype=torch.int32, device=DEV), torch.ones(rows, device=DEV)
+    lp, stats, _ = m.token_logprobs(x, ids)
+    for d in (m.token_logprobs_grad(x, ids, stats, d_logprob=v), m.policy_loss_rows(x, ids, lp, -rows * v)[3]):
+        assert d.shape == (rows, V) and d.is_contiguous()
+        want = -torch.softmax(x.double(), 1)
+        want[:, 0] += 1.0
+        assert float((d.double() - want).abs().max()) <= 60 * lr.EPS  # (sums and powers as in loss_ref.sum_tol: 42 half steps and the exponents' 16)
+
+
 def test_rows_far_apart():
     """Offsets beyond 32 bits: three rows 1.5e9 elements apart, of logits and of their gradient."""
     m = gc.pkg()

