@@ -623,7 +623,9 @@ int ws_policy_loss_rows(void* stream, const ws_loss_rows* r, const ws_policy* p,
 /* The loss of paired log ratios: answers 2 p (preferred) and 2 p + 1 of pair p are the rows seq_off[2 p] .. seq_off[2 p + 1] and
  * seq_off[2 p + 1] .. seq_off[2 p + 2]; with s their sums of logprob - ref_logprob and h = beta * (s_preferred - s_other)
  *   pair_loss = (1 - label_smoothing) * ln(1 + exp(-h)) + label_smoothing * ln(1 + exp(h)),    loss = sum of weight * pair_loss,
- * reward[p] = beta * s of the two. Answers may be empty. seq_off ascends; offsets beyond `rows` end there. d_logprob is written for all rows, 0 for those
+ * reward[p] = beta * s of the two. A term whose factor is 0 is left out. A token whose logprob and ref_logprob are both -inf (neither model can give it: a mask leaves it out)
+ * counts for nothing: it adds nothing, its derivative is 0. An answer with another token of logprob -inf has s = -inf, and its pair the limits: the loss 0 or +inf, the
+ * derivatives those of h = +-inf. Where both of a pair's s are -inf h has no value, and loss and derivatives are NaN unless the pair weighs 0. Answers may be empty. seq_off ascends; offsets beyond `rows` end there. d_logprob is written for all rows, 0 for those
  * of no answer. A pair of weight 0 counts for nothing. workspace as above, of ws_preference_loss_workspace() bytes; required where that is
  * not 0. */
 typedef struct ws_preference {

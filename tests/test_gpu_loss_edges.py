@@ -1,0 +1,93 @@
+"""GPU: the operators over log-probabilities where their formulas meet infinities, empty rows and the ends of their types, and what their calls leave behind.
+Expected values come from the formulas in 64 bits, with the limits that the header states written out; tolerances as in loss_ref.py, where they are derived."""
+import math
+
+import pytest
+import torch
+
+import gpu_cases as gc
+import loss_ref as lr
+from test_gpu_loss import DEV, F32, near
+
+pytestmark = pytest.mark.gpu
+INF = math.inf
+f32 = lambda *v: torch.tensor(v, dtype=F32)  # noqa: E731
+
+
+def preference_by_limits(lp, ref, off, w, beta, smoothing):
+    """The loss of each pair with a term of factor 0 left out and tokens that neither model can give skipped: (loss, pair losses, rewards, derivatives)."""
+    P = (len(off) - 1) // 2
+    total, each, reward, d = 0.0, [], [], [0.0] * len(lp)
+    for p in range(P):
+        s, live = [], []
+        for a, b in ((off[2 * p], off[2 * p + 1]), (off[2 * p + 1], off[2 * p + 2])):
+            rows = [i for i in range(a, b) if not (lp[i] == -INF and ref[i] == -INF)]
+            s.append(math.fsum(lp[i] - ref[i] for i in rows) if all(math.isfinite(lp[i]) and math.isfinite(ref[i]) for i in rows) else sum(lp[i] - ref[i] for i in rows))
+            live.append(rows)
+        h = beta * (s[0] - s[1])
+        soft = lambda v: INF if v == INF else (0.0 if v == -INF else max(v, 0.0) + math.log1p(math.exp(-abs(v))))  # noqa: E731
+        loss = 0.0 if smoothing == 1.0 else (1.0 - smoothing) * soft(-h)
+        loss += 0.0 if smoothing == 0.0 else smoothing * soft(h)
+        sigma = 0.0 if h == INF else (1.0 if h == -INF else 1.0 / (1.0 + math.exp(h)))
+        each.append(loss)
+        reward.append([beta * s[0], beta * s[1]])
+        if w[p] != 0.0:
+            total += w[p] * loss
+            for k, sign in ((0, 1.0), (1, -1.0)):
+                for i in live[k]:
+                    d[i] = sign * w[p] * beta * (smoothing - sigma)
+    return [torch.tensor(v, dtype=torch.float64) for v in ([total], each, reward, d)]
+
+
+@pytest.mark.parametrize("smoothing", [0.0, 0.25, 1.0])
+@pytest.mark.parametrize("where", ["chosen", "rejected", "both weigh nothing", "neither model", "reference"])
+@pytest.mark.parametrize("lengths", [[3, 2, 4, 5, 1, 1], [700, 513, 30, 1030, 2, 9]])
+def test_preference_of_tokens_that_a_mask_leaves_out(lengths, where, smoothing):
+    """A token of log-probability -inf in one pair of three: that pair's loss goes to its limit, the others' and all gradients stay. Sums in 64 bits, outputs rounded once: 1e-10 as in
+    test_gpu_loss.py."""
+    m = gc.pkg()
+    g = torch.Generator().manual_seed(7)
+    off = [0]
+    for n in lengths:
+        off.append(off[-1] + n)
+    n = off[-1] + 2
+    lp, ref = -5.0 * torch.rand(n, generator=g), -5.0 * torch.rand(n, generator=g)
+    w = f32(0.5, 0.25, 1.0)
+    last = off[4] - 1 if where == "rejected" else off[3] - 1  # of the middle pair's second or first answer
+    if where == "neither model":
+        lp[last] = ref[last] = lp[off[4] - 1] = ref[off[4] - 1] = -INF
+    elif where == "reference":
+        ref[last] = -INF
+    else:
+        lp[last] = -INF
+    if where == "both weigh nothing":
+        lp[off[4] - 1] = -INF
+        w[1] = 0.0
+    beta = 0.1
+    got = m.preference_loss(lp.to(DEV), torch.tensor(off, dtype=torch.int32, device=DEV), ref_logprob=ref.to(DEV), weight=w.to(DEV), beta=beta, label_smoothing=smoothing)
+    want = preference_by_limits(lp.double().tolist(), ref.double().tolist(), off, w.double().tolist(), beta, smoothing) if where != "both weigh nothing" else None
+    if want is None:  # (the difference of the two has no value: the pair's loss is NaN, and counts for nothing)
+        assert math.isnan(got[1][1].item()) and not got[3][off[2]:off[4]].any() and got[2][1].tolist() == [-INF, -INF]
+        lp[off[2]:off[4]] = 0.0
+        want = preference_by_limits(lp.double().tolist(), ref.double().tolist(), off, w.double().tolist(), beta, smoothing)
+        got = [got[0], got[1].clone(), got[2].clone(), got[3]]
+        got[1][1], got[2][1] = want[1][1], want[2][1]
+    tol = lambda v: torch.nan_to_num((lr.EPS * 1.001 + 1e-10) * v.abs(), posinf=0.0) + 1e-10  # noqa: E731
+    for a, b, what in zip(got[:3], want[:3], ("loss", "pair_loss", "reward")):
+        near(a, b, tol(b), what)
+    near(got[3], want[3], (lr.EPS * 1.001 + 1e-10) * want[3].abs() + 2.0 ** -149, "d_logprob")
+    if where == "rejected" and smoothing == 0.0:
+        assert got[1][1].item() == 0.0 and math.isfinite(got[0].item())
+    if where == "chosen" and smoothing == 1.0:
+        assert got[1][1].item() == 0.0 and math.isfinite(got[0].item())
+    if where == "neither model":
+        assert bool(torch.isfinite(got[0]).all()) and got[3][last].item() == 0.0 and got[3][off[2]].item() != 0.0
+
+
+def test_preference_without_a_reference_and_a_token_that_a_mask_leaves_out():
+    m = gc.pkg()
+    lp = f32(-1.0, -2.0, -INF, -1.5, -0.5)
+    loss, each, reward, d = m.preference_loss(lp.to(DEV), torch.tensor([0, 2, 3, 4, 5], dtype=torch.int32, device=DEV), beta=0.5)
+    other = math.log1p(math.exp(0.5))  # (h = -0.5 of the second pair: -1.5 against -0.5, halved)
+    assert each[0].item() == 0.0 and abs(each[1].item() - other) <= 2 * lr.EPS * other and abs(loss.item() - other / 2) <= 2 * lr.EPS * other
+    assert reward[0].tolist() == [-1.5, -INF] and d[:3].tolist() == [0.0, 0.0, 0.0] and d[3].item() < 0.0 < d[4].item()
