@@ -91,3 +91,55 @@ def test_preference_without_a_reference_and_a_token_that_a_mask_leaves_out():
     other = math.log1p(math.exp(0.5))  # (h = -0.5 of the second pair: -1.5 against -0.5, halved)
     assert each[0].item() == 0.0 and abs(each[1].item() - other) <= 2 * lr.EPS * other and abs(loss.item() - other / 2) <= 2 * lr.EPS * other
     assert reward[0].tolist() == [-1.5, -INF] and d[:3].tolist() == [0.0, 0.0, 0.0] and d[3].item() < 0.0 < d[4].item()
+
+
+# (logprob, old, advantage, ref): tokens where a difference of infinities or 0 * inf stands in the formulas
+AT_THE_ENDS = [(-INF, -2.0, 1.0, -1.0), (-INF, -2.0, -1.0, -1.0), (-INF, -2.0, 1.0, -INF), (-INF, -2.0, -1.0, -INF), (-1.0, -2.0, 1.0, -INF), (-INF, -2.0, 0.0, -1.0), (-1.25, -1.0, 0.5, -0.75),
+               (-1.0, -1.25, 0.5, -1.0)]
+
+
+def policy_by_limits(lp, old, A, ref, w, H, clip_low, clip_high, dual_clip, kl_coef, entropy_coef):
+    """One token: ([loss, surrogate, kl, entropy, clipped], derivative by the log-probability, by the entropy)."""
+    lp = -INF if lp < -3.4028236e38 else lp  # (a float's)
+    if w == 0.0 or (lp == -INF and old == -INF):
+        return [0.0] * 5, 0.0, 0.0
+    ratio = 0.0 if lp == -INF else (INF if lp - old > 709.0 else math.exp(lp - old))
+    times = lambda a, b: 0.0 if b == 0.0 else a * b  # noqa: E731
+    free, held = times(ratio, A), times(min(max(ratio, 1.0 - clip_low), 1.0 + clip_high), A)
+    gain, clipped = (held, True) if held < free else (free, False)
+    if dual_clip and A < 0.0 and gain < dual_clip * A:
+        gain, clipped = dual_clip * A, True
+    kl, back = 0.0, 0.0
+    if ref is not None and not (lp == -INF and ref == -INF):
+        b = ref - lp
+        kl, back = (INF, INF) if b > 709.0 else ((INF, -1.0) if b == -INF else (math.expm1(b) - b, math.expm1(b)))
+    loss = -gain + (kl_coef * kl if kl_coef else 0.0) - entropy_coef * H
+    return [w * loss, -w * gain, w * kl, w * H, w * clipped], w * ((0.0 if clipped else -free) - (kl_coef * back if kl_coef else 0.0)), -entropy_coef * w
+
+
+@pytest.mark.parametrize("dual_clip", [0.0, 3.0])
+@pytest.mark.parametrize("kl_coef", [0.0, 0.05])
+@pytest.mark.parametrize("with_ref", [False, True])
+def test_policy_loss_at_the_ends(with_ref, kl_coef, dual_clip):
+    """Each token by itself, then all that stay finite together. 64 bits, rounded once: half a step."""
+    m = gc.pkg()
+    if kl_coef and not with_ref:
+        pytest.skip("a KL term needs a reference")
+    o = dict(clip_low=0.2, clip_high=0.28, dual_clip=dual_clip, kl_coef=kl_coef, entropy_coef=0.01)
+    finite = []
+    for lp, old, A, ref in AT_THE_ENDS:
+        want = policy_by_limits(lp, old, A, ref if with_ref else None, 1.0, 2.0, **o)
+        d = dict(ref_logprob=f32(ref).to(DEV) if with_ref else None, entropy=f32(2.0).to(DEV), **o)
+        sums, g, h = m.policy_loss(f32(lp).to(DEV), f32(old).to(DEV), f32(A).to(DEV), **d)
+        sums_w = torch.tensor(want[0], dtype=torch.float64)
+        near(sums, sums_w, torch.nan_to_num(sums_w.abs(), posinf=0.0) * lr.EPS * 1.001 + 1e-12, ("sums", lp, old, A, ref))
+        near(g, torch.tensor([want[1]], dtype=torch.float64), (0.0 if math.isinf(want[1]) else abs(want[1])) * lr.EPS * 1.001, ("d_logprob", lp, old, A, ref))
+        near(h, torch.tensor([want[2]], dtype=torch.float64), abs(want[2]) * lr.EPS * 1.001, ("d_entropy", lp, old, A, ref))
+        if all(math.isfinite(v) for v in want[0]):
+            finite.append((lp, old, A, ref, want))
+    assert len(finite) >= 4
+    n = len(finite)
+    col = lambda k: torch.tensor([f[k] for f in finite], dtype=F32, device=DEV)  # noqa: E731
+    sums, g, h = m.policy_loss(col(0), col(1), col(2), ref_logprob=col(3) if with_ref else None, entropy=torch.full((n,), 2.0, device=DEV), weight=torch.ones(n, device=DEV), **o)
+    want = torch.tensor([f[4][0] for f in finite], dtype=torch.float64)
+    near(sums, want.sum(0), want.abs().sum(0) * lr.EPS * 1.001, "sums together")

@@ -54,6 +54,7 @@ __device__ __forceinline__ PolicyRow policy_row(const PolicyIn& P, uint32_t row)
 // derivative, so the comparison is made in 64 bits: rounded to 32, one token in some million would fall on the other side.
 __device__ __forceinline__ PolicyToken policy_token(const PolicyIn& P, const PolicyRow& T, double lp, double H) {
     PolicyToken o;
+    if (static_cast<float>(lp) == -INFINITY) lp = -static_cast<double>(INFINITY);  // (as the caller sees it, and compares it with the others')
     const double w = T.weight, A = static_cast<double>(T.advantage), r = exp(lp - static_cast<double>(T.old_logprob));
     const double free = r * A, held = fmin(fmax(r, 1.0 - P.clip_low), 1.0 + P.clip_high) * A;
     double gain = held < free ? held : free;
@@ -63,10 +64,10 @@ __device__ __forceinline__ PolicyToken policy_token(const PolicyIn& P, const Pol
         clipped = true;
     }
     double kl = 0.0, back = 0.0;
-    if (P.ref_logprob) {  // exp(b) - b - 1 with b = ref - lp, never negative
-        const double b = static_cast<double>(T.ref_logprob) - lp;
+    if (P.ref_logprob) {  // exp(b) - b - 1 with b = ref - lp, never negative; +inf where b is (not inf - inf); 0 where both are -inf: no token of either's
+        const double ref = static_cast<double>(T.ref_logprob), b = ref == lp ? 0.0 : ref - lp;
         back = expm1(b);
-        kl = back - b;
+        kl = b == static_cast<double>(INFINITY) ? b : back - b;
     }
     o.g = w * ((clipped ? 0.0 : -free) - (P.kl_coef != 0.0 ? P.kl_coef * back : 0.0));
     o.h = -P.entropy_coef * w;
