@@ -95,7 +95,8 @@ def test_preference_without_a_reference_and_a_token_that_a_mask_leaves_out():
 
 # (logprob, old, advantage, ref): tokens where a difference of infinities or 0 * inf stands in the formulas
 AT_THE_ENDS = [(-INF, -2.0, 1.0, -1.0), (-INF, -2.0, -1.0, -1.0), (-INF, -2.0, 1.0, -INF), (-INF, -2.0, -1.0, -INF), (-1.0, -2.0, 1.0, -INF), (-INF, -2.0, 0.0, -1.0), (-1.25, -1.0, 0.5, -0.75),
-               (-1.0, -1.25, 0.5, -1.0)]
+               (-1.0, -1.25, 0.5, -1.0), (-1.0, -900.0, 0.0, -1.0), (-1.0, -INF, 0.0, -1.0), (-1.0, -INF, 1.0, -1.0), (-1.0, -INF, -1.0, -1.0), (-1.0, -900.0, -2.0, -1.5),
+               (-900.0, -1.0, 0.0, -900.0)]
 
 
 def policy_by_limits(lp, old, A, ref, w, H, clip_low, clip_high, dual_clip, kl_coef, entropy_coef):

@@ -55,7 +55,7 @@ __device__ __forceinline__ PolicyRow policy_row(const PolicyIn& P, uint32_t row)
 __device__ __forceinline__ PolicyToken policy_token(const PolicyIn& P, const PolicyRow& T, double lp, double H) {
     PolicyToken o;
     if (static_cast<float>(lp) == -INFINITY) lp = -static_cast<double>(INFINITY);  // (as the caller sees it, and compares it with the others')
-    const double w = T.weight, A = static_cast<double>(T.advantage), r = exp(lp - static_cast<double>(T.old_logprob));
+    const double w = T.weight, A = static_cast<double>(T.advantage), e = exp(lp - static_cast<double>(T.old_logprob)), r = e > DBL_MAX ? DBL_MAX : e;  // (+inf times an advantage of 0: NaN)
     const double free = r * A, held = fmin(fmax(r, 1.0 - P.clip_low), 1.0 + P.clip_high) * A;
     double gain = held < free ? held : free;
     bool clipped = held < free;
