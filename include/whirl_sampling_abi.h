@@ -589,7 +589,7 @@ int ws_token_logprobs_grad(void* stream, const ws_loss_rows* r, const float* sta
  *   kl   = exp(ref - logprob) - (ref - logprob) - 1;
  *   loss = sum of weight * (-gain + kl_coef * kl - entropy_coef * entropy).
  * A token of weight 0 counts for nothing, whatever its other entries hold. Where the clip holds the gain, it has no derivative.
- * A token of logprob -inf has the ratio 0 and, where ref is not -inf too, kl = +inf (ref = -inf alone: +inf as well; both: 0). An advantage of 0 has the gain 0,
+ * A token whose logprob and old_logprob are both -inf (a mask leaves it out, or its row empty, for either model) counts for nothing too. Another of logprob -inf has the ratio 0 and, where ref is not -inf too, kl = +inf (ref = -inf alone: +inf as well; both: 0). An advantage of 0 has the gain 0,
  * whatever the ratio. */
 typedef struct ws_policy {
     const float* old_logprob; /* device [rows]: of the model that drew the tokens */

@@ -7,7 +7,7 @@ import torch
 
 import gpu_cases as gc
 import loss_ref as lr
-from test_gpu_loss import DEV, F32, near
+from test_gpu_loss import BF16, DEV, F32, SPECIAL, make, near
 
 pytestmark = pytest.mark.gpu
 INF = math.inf
@@ -96,7 +96,7 @@ def test_preference_without_a_reference_and_a_token_that_a_mask_leaves_out():
 # (logprob, old, advantage, ref): tokens where a difference of infinities or 0 * inf stands in the formulas
 AT_THE_ENDS = [(-INF, -2.0, 1.0, -1.0), (-INF, -2.0, -1.0, -1.0), (-INF, -2.0, 1.0, -INF), (-INF, -2.0, -1.0, -INF), (-1.0, -2.0, 1.0, -INF), (-INF, -2.0, 0.0, -1.0), (-1.25, -1.0, 0.5, -0.75),
                (-1.0, -1.25, 0.5, -1.0), (-1.0, -900.0, 0.0, -1.0), (-1.0, -INF, 0.0, -1.0), (-1.0, -INF, 1.0, -1.0), (-1.0, -INF, -1.0, -1.0), (-1.0, -900.0, -2.0, -1.5),
-               (-900.0, -1.0, 0.0, -900.0)]
+               (-900.0, -1.0, 0.0, -900.0), (-INF, -INF, 1.0, -1.0), (-INF, -INF, -1.0, -INF), (-INF, -INF, 0.0, -2.0)]
 
 
 def policy_by_limits(lp, old, A, ref, w, H, clip_low, clip_high, dual_clip, kl_coef, entropy_coef):
@@ -144,3 +144,104 @@ def test_policy_loss_at_the_ends(with_ref, kl_coef, dual_clip):
     sums, g, h = m.policy_loss(col(0), col(1), col(2), ref_logprob=col(3) if with_ref else None, entropy=torch.full((n,), 2.0, device=DEV), weight=torch.ones(n, device=DEV), **o)
     want = torch.tensor([f[4][0] for f in finite], dtype=torch.float64)
     near(sums, want.sum(0), want.abs().sum(0) * lr.EPS * 1.001, "sums together")
+
+
+def special_case(dtype, V, seed=5):
+    """The rows of test_special_rows, for the policy step: (case, score in 64 bits, names)."""
+    rows = len(SPECIAL)
+    c = make(rows, V, dtype, seed, masked=True)
+    x, ids, inv_t, allow = c["x"], c["ids"], c["inv_t"], c["allow"]
+    at = {n: i for i, n in enumerate(SPECIAL)}
+    allow[:, 0] = True
+    ids[ids == 1] = 0
+    allow[:, 1] = False
+    allow[at["none_allowed"]] = False
+    x[at["all_minus_inf"]] = -INF
+    x[at["lowest"]] = torch.finfo(dtype).min
+    x[at["some_lowest"], ::2] = torch.finfo(dtype).min
+    ids[at["id_masked"]] = 1
+    ids[at["no_id"]] = -1
+    ids[at["id_past_the_row"]] = V
+    x[at["nan_masked"], 1] = math.nan
+    x[at["inf_masked"], 1] = INF
+    x[at["nan"], 0] = math.nan
+    x[at["inf"], 0] = INF
+    inv_t[at["cold"]] = 1000.0
+    inv_t[at["hot"]] = 1e-3
+    for n, v in (("t_zero", 0.0), ("t_nan", math.nan), ("t_inf", INF), ("t_negative", -1.0)):
+        inv_t[at[n]] = v
+    x[at["huge"], 0] = x[at["huge"], 2] = 1e9
+    allow[at["huge"], 2] = True
+    allow[at["one_allowed"]] = False
+    allow[at["one_allowed"], 0] = True
+    ids[at["one_allowed"]] = 0
+    x[at["id_minus_inf"], ids[at["id_minus_inf"]].long()] = -INF
+    ids[at["lowest"]] = ids[at["huge"]] = 0
+    if V < 6:  # the lowest number against another: -5e38, which is no float
+        ids[at["some_lowest"]] = 0
+        inv_t[at["some_lowest"]] = 1.5
+        allow[at["some_lowest"], 3] = True
+    else:
+        ids[at["some_lowest"]] = int(allow[at["some_lowest"], 3::2].nonzero()[0]) * 2 + 3
+    r = lr.score(x, ids, inv_t, allow)
+    r["lp"] = torch.where(torch.isneginf(r["lp"].float()), torch.full_like(r["lp"], -INF), r["lp"])
+    return c, r, at
+
+
+BAD = ("nan", "inf", "t_zero", "t_nan", "t_inf", "t_negative")  # rows that are NaN
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V,spins", [(5, 0), (1000, 0), (40001, 0), (40001, 1)])
+@pytest.mark.parametrize("old_kind", ["all -inf", "finite"])
+@pytest.mark.parametrize("with_ref", [False, True])
+def test_policy_loss_rows_of_special_rows(dtype, V, spins, old_kind, with_ref):
+    """The policy step over them, from one part a row and from several, waiting or not: the sums of all rows that are not NaN, and every row's outputs. `finite`: the dead tokens' old
+    log-probability is -2, they have the ratio 0 (and an infinite KL term where there is a reference: a call of their own)."""
+    m = gc.pkg()
+    c, r, at = special_case(dtype, V)
+    g = c["g"]
+    dead = torch.isneginf(r["lp"]).nonzero()[:, 0].tolist()
+    assert set(dead) >= {at[n] for n in ("none_allowed", "all_minus_inf", "id_masked", "id_minus_inf")}
+    live = [i for n, i in at.items() if n not in BAD]
+    noise = lambda: 0.1 * torch.randn(len(SPECIAL), generator=g)  # noqa: E731
+    old = torch.nan_to_num((r["lp"] + noise()).float(), nan=-3.0, neginf=-INF)
+    ref = torch.nan_to_num((r["lp"] + noise()).float(), nan=-3.0, neginf=-INF)
+    adv = torch.randn(len(SPECIAL), generator=g)
+    w = torch.rand(len(SPECIAL), generator=g) + 0.5
+    if old_kind == "finite":
+        old[dead] = -2.0
+    o = dict(clip_low=0.2, clip_high=0.28, dual_clip=3.0, kl_coef=0.05 if with_ref else 0.0, entropy_coef=0.01)
+    ratio = (r["lp"] - old.double()).exp()
+    assert all(bool(((ratio - b).abs()[live].nan_to_num(1.0) > 1e-4).all()) for b in (0.8, 1.28, 3.0))
+    for rows in (live, list(range(len(SPECIAL)))):
+        pick = lambda t: t[rows].to(DEV).contiguous()  # noqa: E731
+        x = pick(c["x"].to(dtype))
+        out = m.policy_loss_rows(x, pick(c["ids"]), pick(old), pick(adv), ref_logprob=pick(ref) if with_ref else None, weight=pick(w), inv_t=pick(c["inv_t"]),
+                                 allow=lr.pack_allow(c["allow"][rows]).to(DEV), want_entropy=True, spins=spins, **o)
+        own = m.policy_loss_rows(x, pick(c["ids"]), pick(old), pick(adv), ref_logprob=pick(ref) if with_ref else None, weight=pick(w), inv_t=pick(c["inv_t"]),
+                                 allow=lr.pack_allow(c["allow"][rows]).to(DEV), want_entropy=True, spins=spins, out=x, **o)
+        for a, b in zip(out, own):  # (the new gradient and the logits both begin on a boundary)
+            assert torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(a.float().nan_to_num(7.0), b.float().nan_to_num(7.0))
+        want, dg, dh = zip(*[policy_by_limits(float(r["lp"][i]), float(old[i]), float(adv[i]), float(ref[i]) if with_ref else None, float(w[i]) if bool(r["has"][i]) else 0.0, float(r["H"][i]), **o)
+                             if SPECIAL[i] not in BAD else ([math.nan, math.nan, math.nan if with_ref else 0.0, math.nan, 0.0], 0.0, 0.0) for i in rows])
+        want = torch.tensor(want, dtype=torch.float64)
+        sums = want.sum(0)
+        off, Hoff = lr.lp_tol(r, V)[rows].nan_to_num(0.0), lr.H_tol(r, V)[rows].nan_to_num(0.0)
+        size = (ratio * adv.double().abs())[rows].nan_to_num(0.0, posinf=0.0).clamp(max=10.0) + 2.0  # (ratios and KL terms are below e^0.5 here)
+        near(out[0], sums, (w[rows].double() * (size * off + Hoff)).sum() + lr.EPS * sums.abs().nan_to_num(0.0, posinf=0.0) + 1e-12 * want.abs().sum().nan_to_num(0.0, posinf=0.0), ("sums", len(rows)))
+        has = r["has"][rows]
+        near(out[1], torch.where(has, r["lp"][rows], torch.zeros_like(r["lp"][rows])), off, "logprob")
+        near(out[2], torch.where(has, r["H"][rows], torch.zeros_like(r["H"][rows])), Hoff, "entropy")
+        dg, dh = torch.tensor(dg, dtype=torch.float64), torch.tensor(dh, dtype=torch.float64)
+        part = {k: v[rows] for k, v in r.items()}
+        d, gsize = lr.grad(part, dg, dh)
+        tol = lr.grad_tol(part, gsize, d, V, dtype, h=dh) + part["t"][:, None] * (w[rows].double() * size * (1.01 * off + 4 * lr.EPS))[:, None] * (part["p"] + 1.0 * (torch.arange(V)[None] == part["at"][:, None])) \
+            + dh.abs()[:, None] * part["p"] * part["t"][:, None] * Hoff[:, None]
+        k = [i for i, row in enumerate(rows) if SPECIAL[row] not in BAD]
+        near(out[3][k], d[k], tol[k], "gradient")
+        for i, row in enumerate(rows):
+            if SPECIAL[row] in BAD:
+                assert math.isnan(out[1][i].item()) and bool(torch.isnan(out[3][i].float()).all()), SPECIAL[row]
+            if SPECIAL[row] in ("none_allowed", "all_minus_inf", "no_id", "id_past_the_row") or (row in dead and old_kind == "all -inf"):
+                assert not out[3][i].any(), SPECIAL[row]

@@ -53,8 +53,11 @@ __device__ __forceinline__ PolicyRow policy_row(const PolicyIn& P, uint32_t row)
 // gain = min(r A, clip(r) A) with r = exp(lp - old); for A < 0 not below dual_clip * A. Where the clip holds it there is no
 // derivative, so the comparison is made in 64 bits: rounded to 32, one token in some million would fall on the other side.
 __device__ __forceinline__ PolicyToken policy_token(const PolicyIn& P, const PolicyRow& T, double lp, double H) {
-    PolicyToken o;
-    if (static_cast<float>(lp) == -INFINITY) lp = -static_cast<double>(INFINITY);  // (as the caller sees it, and compares it with the others')
+    PolicyToken o{};
+    if (static_cast<float>(lp) == -INFINITY) {
+        lp = -static_cast<double>(INFINITY);  // (as the caller sees it, and compares it with the others')
+        if (T.old_logprob == -INFINITY) return o;  // neither model can give it, and the ratio has no value: it counts for nothing
+    }
     const double w = T.weight, A = static_cast<double>(T.advantage), e = exp(lp - static_cast<double>(T.old_logprob)), r = e > DBL_MAX ? DBL_MAX : e;  // (+inf times an advantage of 0: NaN)
     const double free = r * A, held = fmin(fmax(r, 1.0 - P.clip_low), 1.0 + P.clip_high) * A;
     double gain = held < free ? held : free;
