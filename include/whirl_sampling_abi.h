@@ -578,7 +578,8 @@ int ws_token_logprobs(void* stream, const ws_loss_rows* r, float* logprob, float
 
 /* Their gradient: with g = d_logprob[row] (NULL: 0; a row without a token: 0) and h = d_entropy[row] (NULL: 0) the derivatives of some loss by
  * the row's logprob and entropy, d_logits[row][v] = inv_t * (g * (1[v = y] - p_v) - h * p_v * (ln p_v + entropy[row])), in the
- * logits' dtype. stats, entropy: what ws_token_logprobs wrote (entropy only with d_entropy). A row with g = h = 0 is not read and
+ * logits' dtype. Where g or h is infinite, or so large that these factors pass what a float holds, tokens that are not allowed have 0 all the same and the others a large number, not NaN.
+ * stats, entropy: what ws_token_logprobs wrote (entropy only with d_entropy). A row with g = h = 0 is not read and
  * gets zeros. d_logits: [rows][d_stride], the first vocab of a row are written; it may be the logits themselves (same address and stride), but not
  * overlap them otherwise. */
 int ws_token_logprobs_grad(void* stream, const ws_loss_rows* r, const float* stats, const float* d_logprob, const float* entropy,

@@ -245,3 +245,38 @@ def test_policy_loss_rows_of_special_rows(dtype, V, spins, old_kind, with_ref):
                 assert math.isnan(out[1][i].item()) and bool(torch.isnan(out[3][i].float()).all()), SPECIAL[row]
             if SPECIAL[row] in ("none_allowed", "all_minus_inf", "no_id", "id_past_the_row") or (row in dead and old_kind == "all -inf"):
                 assert not out[3][i].any(), SPECIAL[row]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [9, 40001])
+def test_infinite_derivatives_leave_masked_places_at_zero(dtype, V):
+    """g or h infinite, or so large that t g / S passes the largest float: what is not allowed has the derivative 0 all the same, and nothing is NaN."""
+    m = gc.pkg()
+    c = make(4, V, dtype, 11, masked=True)
+    c["x"][:, 0] = INF  # (in a masked place)
+    c["allow"][:, 0] = False
+    c["ids"][c["ids"] == 0] = 1
+    c["allow"][:, 1] = True
+    inv_t = torch.full((4,), 4.0)
+    x, ids, allow, inv = c["x"].to(DEV), c["ids"].to(DEV), lr.pack_allow(c["allow"]).to(DEV), inv_t.to(DEV)
+    lp, stats, H = m.token_logprobs(x, ids, inv_t=inv, allow=allow, want_entropy=True)
+    g = f32(-INF, INF, 3e38, -3e38).to(DEV)
+    masked = ~c["allow"]
+    for d_entropy in (None, torch.zeros(4, device=DEV)):
+        d = m.token_logprobs_grad(x, ids, stats, d_logprob=g, entropy=H, d_entropy=d_entropy, inv_t=inv, allow=allow).cpu().float()
+        assert not torch.isnan(d).any() and not d[masked].any()
+        own = torch.zeros_like(masked).scatter(1, c["ids"].long()[:, None], True)
+        sign = torch.sign(g.cpu())[:, None].expand_as(d)
+        assert bool((d * sign <= 0.0)[~own].all()) and bool((d * sign)[own].gt(0.0).all())
+    for h in (f32(INF, -INF, 3e38, -3e38), f32(-3e38, INF, 1.0, INF)):
+        for by_lp in (None, g):
+            d = m.token_logprobs_grad(x, ids, stats, d_logprob=by_lp, entropy=H, d_entropy=h.to(DEV), inv_t=inv, allow=allow).cpu().float()
+            assert not torch.isnan(d).any() and not d[masked].any() and bool((d.abs().amax(1) > 0.0).all())
+    # a KL term that is infinite: the row's token is masked out, the reference could give it
+    ids[0] = 0
+    old, ref = torch.full((4,), -2.0, device=DEV), f32(-1.0, 0.0, 0.0, 0.0).to(DEV)
+    ref[1:] = lp[1:]
+    sums, lp, _, d = m.policy_loss_rows(x, ids, old, torch.ones(4, device=DEV), ref_logprob=ref, inv_t=inv, allow=allow, kl_coef=0.1)
+    assert lp[0].item() == -INF and sums[0].item() == INF and sums[2].item() == INF and math.isfinite(sums[1].item())
+    d = d.cpu().float()
+    assert not torch.isnan(d).any() and not d[masked].any() and bool((d[0][c["allow"][0]] >= 0.0).all()) and bool((d[0] > 1e30).any())

@@ -552,8 +552,11 @@ __device__ __forceinline__ RowSlope row_slope(float m, float S, float inv_t, flo
     r.m = m;
     r.none = (g == 0.f && (!ENT || h == 0.f)) || S == 0.f;
     const float f = -inv_t / S;
-    r.a = f * (ENT ? fmaf(h, H - __logf(S), g) : g);
-    r.b = ENT ? f * h * 0.69314718f : 0.f;
+    // held so that a + b d, |d| <= 1000 where it counts, is finite: an infinity times a power of 0 would be NaN, in every masked place
+    auto held = [](float v, float most) { return fabsf(v) > most ? copysignf(most, v) : v; };
+    const float h_held = held(h, 0x1p100f);
+    r.a = held(f * (ENT ? fmaf(h_held, H - __logf(S), held(g, FLT_MAX)) : g), 0x1p126f);
+    r.b = ENT ? held(f * h_held * 0.69314718f, 0x1p112f) : 0.f;
     r.at_id = g * inv_t;
     return r;
 }
