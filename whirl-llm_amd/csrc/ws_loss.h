@@ -913,61 +913,62 @@ struct PreferenceArgs {
     unsigned long long* meet;  // [2][workgroups]
     unsigned long long tag;
 };
-__device__ __forceinline__ double softplus(double v) { return fmax(v, 0.0) + log1p(exp(-fabs(v))); }
 
 template <int T>
 __global__ void __launch_bounds__(T) preference_kernel(PreferenceArgs A) {
     __shared__ double red[2][T / 64];
-    __shared__ uint32_t red_skip[T / 64];
     __shared__ float slope;
-    __shared__ bool skips;  // of the pair's tokens some count for nothing
+    __shared__ bool again;
     const uint32_t t = threadIdx.x, groups = gridDim.x;
     double mine = 0.0;
-    // (that neither model can give: what a mask leaves out of both)
-    auto neither = [&](uint32_t row) { return A.ref_logprob && A.logprob[row] == -INFINITY && A.ref_logprob[row] == -INFINITY; };
     for (uint32_t p = blockIdx.x; p < A.pairs; p += groups) {
         uint32_t at[3];  // the chosen answer is [at0, at1), the other [at1, at2); offsets past the rows end there
 #pragma unroll
         for (uint32_t k = 0; k < 3u; ++k) at[k] = min(A.seq_off[2u * p + k], A.rows);
-        double s[2] = {0.0, 0.0};
+        // A token that neither model can give counts for nothing. It makes its answer's sum NaN (-inf - -inf), and only where one is
+        // are such tokens looked for, in a second pass. (Looked for in the first: 64 pairs of answers of up to 2048 tokens 7.3 us, and 7.1.)
+        auto neither = [&](uint32_t row) { return A.logprob[row] == -INFINITY && A.ref_logprob && A.ref_logprob[row] == -INFINITY; };
         bool skip = false;
+        while (true) {  // (twice at most)
+            double s[2] = {0.0, 0.0};
+            if (!skip) {
 #pragma unroll
-        for (uint32_t k = 0; k < 2u; ++k) {
-            for (uint32_t row = at[k] + t; row < at[k + 1u]; row += T) {
-                const float lp = A.logprob[row], ref = A.ref_logprob ? A.ref_logprob[row] : 0.f;
-                const bool none = lp == -INFINITY && ref == -INFINITY;
-                s[k] += none ? 0.0 : static_cast<double>(lp) - static_cast<double>(ref);
-                skip = skip || none;
+                for (uint32_t k = 0; k < 2u; ++k)
+                    for (uint32_t row = at[k] + t; row < at[k + 1u]; row += T) s[k] += static_cast<double>(A.logprob[row]) - (A.ref_logprob ? static_cast<double>(A.ref_logprob[row]) : 0.0);
+            } else {
+#pragma unroll
+                for (uint32_t k = 0; k < 2u; ++k)
+                    for (uint32_t row = at[k] + t; row < at[k + 1u]; row += T) s[k] += neither(row) ? 0.0 : static_cast<double>(A.logprob[row]) - static_cast<double>(A.ref_logprob[row]);
             }
-        }
-        const bool wave_skips = __ballot(skip) != 0ull;
-        if (lane_id() == 0) red_skip[wave_id()] = wave_skips;
 #pragma unroll
-        for (uint32_t k = 0; k < 2u; ++k) {
-            s[k] = wave_sum(s[k]);
-            if (lane_id() == 0) red[k][wave_id()] = s[k];
-        }
-        __syncthreads();
-        if (t < 64u) {
-#pragma unroll
-            for (uint32_t k = 0; k < 2u; ++k) s[k] = wave_sum(t < T / 64u ? red[k][t] : 0.0);
-            const bool any_skips = __ballot(t < T / 64u && red_skip[t < T / 64u ? t : 0u] != 0u) != 0ull;
-            const double w = A.weight ? static_cast<double>(A.weight[p]) : A.weight_all, h = A.beta * (s[0] - s[1]);
-            // a term of factor 0 is left out: the other answer's sum may be -inf, and 0 times the term's infinity NaN
-            const double loss = (A.smoothing != 1.0 ? (1.0 - A.smoothing) * softplus(-h) : 0.0) + (A.smoothing != 0.0 ? A.smoothing * softplus(h) : 0.0);
-            if (w != 0.0) mine += w * loss;
-            if (t == 0u) {
-                A.pair_loss[p] = static_cast<float>(loss);
-                A.reward[2u * static_cast<size_t>(p)] = static_cast<float>(A.beta * s[0]);
-                A.reward[2u * static_cast<size_t>(p) + 1u] = static_cast<float>(A.beta * s[1]);
-                slope = w != 0.0 ? static_cast<float>(w * A.beta * (A.smoothing - 1.0 / (1.0 + exp(h)))) : 0.f;
-                skips = any_skips;
+            for (uint32_t k = 0; k < 2u; ++k) {
+                s[k] = wave_sum(s[k]);
+                if (lane_id() == 0) red[k][wave_id()] = s[k];
             }
+            __syncthreads();
+            if (t < 64u) {
+#pragma unroll
+                for (uint32_t k = 0; k < 2u; ++k) s[k] = wave_sum(t < T / 64u ? red[k][t] : 0.0);
+                const bool look = !skip && A.ref_logprob && (s[0] != s[0] || s[1] != s[1]);
+                const double w = A.weight ? static_cast<double>(A.weight[p]) : A.weight_all, h = A.beta * (s[0] - s[1]);
+                const double tail = log1p(exp(-fabs(h)));  // of both ln(1 + exp(+-h)) what the larger of +-h and 0 leaves
+                // a term of factor 0 is left out: the other answer's sum may be -inf, and 0 times the term's infinity NaN
+                const double loss = (A.smoothing != 1.0 ? (1.0 - A.smoothing) * (fmax(-h, 0.0) + tail) : 0.0) + (A.smoothing != 0.0 ? A.smoothing * (fmax(h, 0.0) + tail) : 0.0);
+                if (w != 0.0 && !look) mine += w * loss;
+                if (t == 0u) {
+                    A.pair_loss[p] = static_cast<float>(loss);
+                    A.reward[2u * static_cast<size_t>(p)] = static_cast<float>(A.beta * s[0]);
+                    A.reward[2u * static_cast<size_t>(p) + 1u] = static_cast<float>(A.beta * s[1]);
+                    slope = w != 0.0 ? static_cast<float>(w * A.beta * (A.smoothing - 1.0 / (1.0 + exp(h)))) : 0.f;
+                    again = look;
+                }
+            }
+            __syncthreads();
+            if (!again) break;
+            skip = true;
         }
-        __syncthreads();
         const float c = slope;
-        const bool look = skips;
-        for (uint32_t row = at[0] + t; row < at[2]; row += T) A.d_logprob[row] = look && neither(row) ? 0.f : (row < at[1] ? c : -c);
+        for (uint32_t row = at[0] + t; row < at[2]; row += T) A.d_logprob[row] = skip && neither(row) ? 0.f : (row < at[1] ? c : -c);
     }
     // rows of no answer: before the first, behind the last
     const uint32_t first = min(A.seq_off[0], A.rows), behind = min(A.seq_off[2u * A.pairs], A.rows);
