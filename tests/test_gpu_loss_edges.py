@@ -1,5 +1,6 @@
 """GPU: the operators over log-probabilities where their formulas meet infinities, empty rows and the ends of their types, and what their calls leave behind.
 Expected values come from the formulas in 64 bits, with the limits that the header states written out; tolerances as in loss_ref.py, where they are derived."""
+import ctypes as C
 import math
 
 import pytest
@@ -280,3 +281,21 @@ def test_infinite_derivatives_leave_masked_places_at_zero(dtype, V):
     assert lp[0].item() == -INF and sums[0].item() == INF and sums[2].item() == INF and math.isfinite(sums[1].item())
     d = d.cpu().float()
     assert not torch.isnan(d).any() and not d[masked].any() and bool((d[0][c["allow"][0]] >= 0.0).all()) and bool((d[0] > 1e30).any())
+
+
+def test_results_do_not_keep_their_workspace():
+    """A result's memory is its own entries', and behind them a workspace of 4 KiB at most: a larger one, of megabytes with many rows, goes when the call is made."""
+    m = gc.pkg()
+    c = make(600, 65537, BF16, 3)
+    v = torch.zeros(600, device=DEV)
+    off = torch.arange(0, 601, dtype=torch.int32, device=DEV)
+    r = m.LossRows(c["dx"].data_ptr(), m.DTYPE_BF16, 600, 65537, 65537)
+    assert m.lib().ws_policy_loss_rows_workspace(C.byref(r)) > 100000 and m.lib().ws_token_logprobs_workspace(C.byref(r)) > 10000
+    lp, stats, H = m.token_logprobs(c["dx"], c["dids"], want_entropy=True)
+    many = torch.zeros(300000, device=DEV)
+    results = [lp, stats, H, *m.policy_loss_rows(c["dx"], c["dids"], v, v, want_entropy=True), *m.preference_loss(lp, off), *m.policy_loss(many, many, many)]
+    one = m.token_logprobs(c["dx"][:1], c["dids"][:1])
+    for t in [*results, *one]:
+        if t is not None:
+            own = t.numel() * t.element_size()
+            assert own <= t.untyped_storage().nbytes() <= own + 4096 + 8 and t.storage_offset() == 0, t.shape

@@ -629,11 +629,16 @@ def _gradient_for(logits, out, vocab):
 
 
 def _with_work(words, need, dev):
-    """A float32 result of `words` entries with the call's workspace behind it, and where that is: memory of any contents, asked for with every call as the
-    greedy picks' is, so that every stream, thread and captured graph has its own. The result is cut to its size when the call is made."""
+    """(a float32 result of `words` entries, where the call's workspace is, what holds that until the call is made). The workspace is memory of any contents, asked for with every call as
+    the greedy picks' is, so that every stream, thread and captured graph has its own. As theirs, one of up to 4 KiB lies behind the result, which is cut to its size when
+    the call is made (an allocation less: 1 us of a lone row's 10); a larger one, megabytes with many rows, would stay as long as the result does and goes
+    when the call is made: the next to get its memory is behind the launch on the stream."""
+    if need > _PICK_BYTES:
+        work = torch.empty(need, dtype=torch.uint8, device=dev)
+        return torch.empty(words, dtype=_F32, device=dev), work.data_ptr(), work
     first = (words + 1) & ~1
     t = torch.empty(first + (need + 3) // 4, dtype=_F32, device=dev)
-    return t, t.data_ptr() + 4 * first
+    return t, t.data_ptr() + 4 * first, None
 
 
 def token_logprobs(logits, ids, inv_t=None, allow=None, want_entropy=False):
@@ -644,7 +649,7 @@ def token_logprobs(logits, ids, inv_t=None, allow=None, want_entropy=False):
     r, rows, vocab, at = _loss_rows(logits, ids, inv_t, allow)
     dev, call, ref = logits.device, lib(), C.byref(r)
     need = call.ws_token_logprobs_workspace(ref)
-    stats, work = _with_work(2 * rows, need, dev)
+    stats, work, held = _with_work(2 * rows, need, dev)
     logprob = torch.empty(rows, dtype=_F32, device=dev)
     entropy = torch.empty(rows, dtype=_F32, device=dev) if want_entropy else None
     check(call.ws_token_logprobs(_stream(), ref, logprob.data_ptr(), stats.data_ptr(), _p(entropy), work, need), "ws_token_logprobs")
@@ -678,12 +683,12 @@ def policy_loss(logprob, old_logprob, advantage, ref_logprob=None, entropy=None,
     p = _policy(old_logprob, advantage, ref_logprob, weight, rows, at, clip_low, clip_high, dual_clip, kl_coef, entropy_coef)
     call = lib()
     need = call.ws_policy_loss_workspace(rows)
-    sums, work = _with_work(5, need, dev)
+    sums, work, held = _with_work(5, need, dev)
     d_logprob = torch.empty(rows, dtype=_F32, device=dev)
     d_entropy = torch.empty(rows, dtype=_F32, device=dev) if entropy is not None else None
     check(call.ws_policy_loss(_stream(), rows, C.byref(p), _vector("logprob", logprob, _F32, rows, at), _vector("entropy", entropy, _F32, rows, at), sums.data_ptr(),
                               d_logprob.data_ptr(), _p(d_entropy), work, need), "ws_policy_loss")
-    return sums.resize_(5), d_logprob, d_entropy
+    return sums if held is not None else sums.resize_(5), d_logprob, d_entropy
 
 
 def policy_loss_rows(logits, ids, old_logprob, advantage, ref_logprob=None, weight=None, inv_t=None, allow=None, clip_low=0.2, clip_high=0.2,
@@ -697,11 +702,11 @@ def policy_loss_rows(logits, ids, old_logprob, advantage, ref_logprob=None, weig
     out, stride = _gradient_for(logits, out, vocab)
     dev, call, ref = logits.device, lib(), C.byref(r)
     need = call.ws_policy_loss_rows_workspace(ref)
-    sums, work = _with_work(5, need, dev)
+    sums, work, held = _with_work(5, need, dev)
     logprob = torch.empty(rows, dtype=_F32, device=dev)
     entropy = torch.empty(rows, dtype=_F32, device=dev) if want_entropy or entropy_coef != 0.0 else None
     check(call.ws_policy_loss_rows(_stream(), ref, C.byref(p), sums.data_ptr(), logprob.data_ptr(), _p(entropy), out.data_ptr(), stride, work, need), "ws_policy_loss_rows")
-    return sums.resize_(5), logprob, entropy, out
+    return sums if held is not None else sums.resize_(5), logprob, entropy, out
 
 
 def preference_loss(logprob, seq_off, ref_logprob=None, weight=None, beta=0.1, label_smoothing=0.0):
@@ -714,7 +719,7 @@ def preference_loss(logprob, seq_off, ref_logprob=None, weight=None, beta=0.1, l
         raise WsError("seq_off: 2 * pairs + 1 offsets of one pair at least")
     call = lib()
     need = call.ws_preference_loss_workspace(pairs)
-    loss, work = _with_work(1, need, dev)
+    loss, work, held = _with_work(1, need, dev)
     pair_loss = torch.empty(pairs, dtype=_F32, device=dev)
     reward = torch.empty((pairs, 2), dtype=_F32, device=dev)
     d_logprob = torch.empty(rows, dtype=_F32, device=dev)
@@ -722,7 +727,7 @@ def preference_loss(logprob, seq_off, ref_logprob=None, weight=None, beta=0.1, l
                    _vector("ref_logprob", ref_logprob, _F32, rows, at), _vector("weight", weight, _F32, pairs, at), beta, label_smoothing, loss.data_ptr(),
                    pair_loss.data_ptr(), reward.data_ptr(), d_logprob.data_ptr())
     check(call.ws_preference_loss(_stream(), C.byref(a), work, need), "ws_preference_loss")
-    return loss.resize_(1), pair_loss, reward, d_logprob
+    return loss if held is not None else loss.resize_(1), pair_loss, reward, d_logprob
 
 
 # ---------------------------------------------------------------------------------------------------------------------
