@@ -571,7 +571,8 @@ typedef struct ws_loss_rows {
 /* Log-probabilities and entropies. stats[row] = {m, S}, the layout of ws_batch.stats: what ws_token_logprobs_grad needs of the forward
  * pass. workspace: device memory of ws_token_logprobs_workspace() bytes (0: none is needed), 8-byte aligned, of any
  * contents, nobody else's until the launch is done (few rows are shared by up to 64 workgroups each, which meet there; a captured
- * launch may be replayed). Without it every row is one workgroup's: slower, the sums in another order. */
+ * launch may be replayed). Without it (NULL) every row is one workgroup's: slower, the sums in another order.
+ * One that is too small or misaligned is refused. */
 uint64_t ws_token_logprobs_workspace(const ws_loss_rows* r);
 int ws_token_logprobs(void* stream, const ws_loss_rows* r, float* logprob, float* stats, float* entropy /* may be NULL */, void* workspace,
                       uint64_t workspace_bytes);

@@ -1190,6 +1190,7 @@ int ws_token_logprobs(void* stream, const ws_loss_rows* r, float* logprob, float
     if (!loss_rows_ok(r)) return WS_E_INVALID;
     if (r->rows == 0) return WS_OK;
     if (!logprob || !stats) return WS_E_INVALID;
+    if (workspace && !workspace_ok(workspace, workspace_bytes, ws_token_logprobs_workspace(r))) return WS_E_WORKSPACE;
     ws::ScoreArgs a{};
     a.R = loss_rows(r);
     a.logprob = logprob;
@@ -1197,7 +1198,7 @@ int ws_token_logprobs(void* stream, const ws_loss_rows* r, float* logprob, float
     a.entropy = entropy;
     a.parts = score_parts(r, entropy != nullptr);
     if (a.parts > 1u) {
-        if (workspace && workspace_ok(workspace, workspace_bytes, meet_bytes(r->rows, a.parts, ws::kPartWords))) {
+        if (workspace) {  // (the call without entropy shares a row between as many workgroups or more)
             a.meet = static_cast<unsigned long long*>(workspace);
             a.tag = launch_tag();
         } else {
