@@ -582,7 +582,7 @@ int ws_token_logprobs(void* stream, const ws_loss_rows* r, float* logprob, float
  * logits' dtype. Where g or h is infinite, or so large that these factors pass what a float holds, tokens that are not allowed have 0 all the same and the others a large number, not NaN.
  * stats, entropy: what ws_token_logprobs wrote (entropy only with d_entropy). A row with g = h = 0 is not read and
  * gets zeros. d_logits: [rows][d_stride], the first vocab of a row are written; it may be the logits themselves (same address and stride), but not
- * overlap them otherwise. */
+ * overlap them otherwise. Where the strides are the same its rows may lie between the logits' (the halves of one matrix's rows); else one lies behind the other. */
 int ws_token_logprobs_grad(void* stream, const ws_loss_rows* r, const float* stats, const float* d_logprob, const float* entropy,
                            const float* d_entropy, void* d_logits, uint64_t d_stride);
 

@@ -299,3 +299,32 @@ def test_results_do_not_keep_their_workspace():
         if t is not None:
             own = t.numel() * t.element_size()
             assert own <= t.untyped_storage().nbytes() <= own + 4096 + 8 and t.storage_offset() == 0, t.shape
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gradient_between_the_logits_rows(dtype):
+    """Logits and gradient in the two halves of one matrix's rows, in either order: they do not overlap. And one row, whose stride is nobody's."""
+    m = gc.pkg()
+    rows, V = 5, 1003
+    for at, to in ((0, V + 3), (V + 3, 0), (0, V)):
+        c = make(rows, V, dtype, 17)
+        both = torch.full((rows, 2 * V + 6), 5.0, dtype=dtype, device=DEV)
+        x, d = both[:, at:at + V], both[:, to:to + V]
+        x.copy_(c["x"])
+        g = torch.randn(rows, generator=c["g"]).to(DEV)
+        lp, stats, _ = m.token_logprobs(x, c["dids"])
+        want = m.token_logprobs_grad(x.clone(), c["dids"], stats, d_logprob=g)
+        got = m.token_logprobs_grad(x, c["dids"], stats, d_logprob=g, out=d)
+        assert got.data_ptr() == d.data_ptr() and torch.equal(got, want) and torch.equal(x.cpu(), c["x"])
+        rest = torch.ones(2 * V + 6, dtype=torch.bool)
+        rest[at:at + V] = rest[to:to + V] = False
+        assert bool((both.cpu()[:, rest] == 5.0).all())
+        one = m.policy_loss_rows(x, c["dids"], lp, g, out=d)
+        r = lr.score(c["x"], c["ids"])
+        want, size = lr.grad(r, -g.cpu().double() / rows, torch.zeros(rows, dtype=torch.float64))
+        near(one[3], want, lr.grad_tol(r, size, want, V, dtype, extra=2 * float(lr.lp_tol(r, V).max())), "policy gradient")
+    x = c["x"][:1].to(DEV)
+    d = m.LossRows(x.data_ptr(), m.DTYPE_F32 if dtype is F32 else m.DTYPE_BF16, 1, V, V, c["dids"].data_ptr())
+    want = m.token_logprobs_grad(x, c["dids"][:1], stats[:1], d_logprob=g[:1])
+    m.check(m.lib().ws_token_logprobs_grad(torch.cuda.current_stream().cuda_stream, C.byref(d), stats.data_ptr(), g.data_ptr(), None, None, x.data_ptr(), V + 9), "ws_token_logprobs_grad")
+    assert torch.equal(x, want)

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import gpu_cases as gc
-from test_loss_args import AT, rows_of
+from test_loss_args import AT, policy_of, rows_of
 
 
 @pytest.fixture(autouse=True)
@@ -24,3 +24,23 @@ def test_scores_refuse_a_workspace_that_is_too_small_or_misaligned(entropy):
     call = lambda work, size: lib.ws_token_logprobs(None, C.byref(r), AT, AT, entropy, work, size)  # noqa: E731
     assert call(AT, need - 1) == call(AT, 0) == call(AT + 4, need) == m.E_WORKSPACE
     assert call(None, 0) not in (m.E_WORKSPACE, m.E_INVALID) and call(AT, need) not in (m.E_WORKSPACE, m.E_INVALID) and call(None, need) not in (m.E_WORKSPACE, m.E_INVALID)
+
+
+# (gradient's place behind the logits in elements, stride of the logits, of the gradient, rows): vocab 100
+APART = [(100, 200, 200, 4), (150, 300, 300, 4), (-100, 200, 200, 4), (-200, 300, 300, 4), (100 + 200, 200, 200, 4), (0, 100, 500, 1), (0, 500, 100, 1), (400, 100, 100, 4), (100, 100, 100, 1)]
+OVER = [(99, 200, 200, 4), (101, 200, 200, 4), (-99, 200, 200, 4), (-101, 200, 200, 4), (100, 199, 199, 4), (299, 200, 200, 4), (100, 200, 201, 4), (0, 200, 201, 4), (99, 500, 500, 1), (-99, 100, 100, 1),
+        (0, 1 << 63, 100, 3), (-400, 100, 1 << 62, 4), (400, 1 << 62, 100, 5)]
+
+
+@pytest.mark.parametrize("dtype,each", [(0, 4), (1, 2)])
+def test_gradients_between_the_rows_of_the_logits(dtype, each):
+    """Memory that does not overlap the logits is taken, also between their rows; what overlaps them is refused, also where a matrix's size passes 64 bits."""
+    m = gc.pkg()
+    lib, p, at = m.lib(), policy_of(m), AT << 8
+    for taken, places in ((True, APART), (False, OVER)):
+        for off, stride, d_stride, rows in places:
+            r = rows_of(m, logits=at, dtype=dtype, rows=rows, row_stride=stride)
+            d = at + off * each
+            codes = (lib.ws_token_logprobs_grad(None, C.byref(r), AT, AT, None, None, d, d_stride),
+                     lib.ws_policy_loss_rows(None, C.byref(r), C.byref(p), AT, AT, None, d, d_stride, AT, 1 << 20))
+            assert all((c != m.E_INVALID) == taken for c in codes), (off, stride, d_stride, rows, codes)

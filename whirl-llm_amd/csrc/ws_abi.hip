@@ -1093,16 +1093,22 @@ bool loss_rows_ok(const ws_loss_rows* r) {
     if (r->row_stride < r->vocab || (r->allow && (r->allow_stride < (r->vocab + 31u) / 32u || !aligned(r->allow, 4u)))) return false;
     return true;
 }
-// bytes from a matrix's first element to behind its last
-uint64_t extent(uint32_t rows, uint32_t vocab, uint64_t stride, uint64_t each) { return rows ? ((rows - 1u) * stride + vocab) * each : 0u; }
-// d_logits: the logits themselves, or memory of its own
+// bytes from a matrix's first element to behind its last (128 bits: a stride may be any number)
+unsigned __int128 extent(uint32_t rows, uint32_t vocab, uint64_t stride, uint64_t each) { return rows ? (static_cast<unsigned __int128>(rows - 1u) * stride + vocab) * each : 0u; }
+// d_logits: the logits themselves, or memory of its own, which may lie between their rows
 bool gradient_ok(const ws_loss_rows* r, const void* d, uint64_t stride) {
     if (!r->rows) return true;
     const uint64_t e = elem_bytes(r->dtype);
     if (!d || !aligned(d, e) || stride < r->vocab) return false;
-    if (d == r->logits && stride == r->row_stride) return true;
-    const uintptr_t a = reinterpret_cast<uintptr_t>(r->logits), b = reinterpret_cast<uintptr_t>(d);
-    return a + extent(r->rows, r->vocab, r->row_stride, e) <= b || b + extent(r->rows, r->vocab, stride, e) <= a;
+    const bool same_stride = stride == r->row_stride || r->rows == 1u;
+    if (d == r->logits && same_stride) return true;
+    const uint64_t a = reinterpret_cast<uintptr_t>(r->logits), b = reinterpret_cast<uintptr_t>(d);
+    if (a + extent(r->rows, r->vocab, r->row_stride, e) <= b || b + extent(r->rows, r->vocab, stride, e) <= a) return true;
+    if (!same_stride || r->rows == 1u) return false;
+    // (rows of one stride: from a row of the one to the next of the other, in both directions. Beyond the address space a stride has no second row.)
+    const unsigned __int128 row = static_cast<unsigned __int128>(r->vocab) * e, step = static_cast<unsigned __int128>(stride) * e;
+    const unsigned __int128 behind = a < b ? (b - a) % step : step - 1u - (a - b - 1u) % step;
+    return behind >= row && behind + row <= step;
 }
 ws::LossRows loss_rows(const ws_loss_rows* r) {
     return ws::LossRows{static_cast<const unsigned char*>(r->logits), r->row_stride * elem_bytes(r->dtype), r->rows, r->vocab, r->ids, r->inv_t, r->allow, r->allow_stride};
