@@ -328,3 +328,13 @@ def test_gradient_between_the_logits_rows(dtype):
     want = m.token_logprobs_grad(x, c["dids"][:1], stats[:1], d_logprob=g[:1])
     m.check(m.lib().ws_token_logprobs_grad(torch.cuda.current_stream().cuda_stream, C.byref(d), stats.data_ptr(), g.data_ptr(), None, None, x.data_ptr(), V + 9), "ws_token_logprobs_grad")
     assert torch.equal(x, want)
+
+
+def test_pairs_and_looks_past_32_bits_are_refused():
+    m = gc.pkg()
+    x, ids, v = torch.zeros((2, 9), device=DEV), torch.zeros(2, dtype=torch.int32, device=DEV), torch.zeros(2, device=DEV)
+    for spins in (-1, 65537, 1 << 32, (1 << 32) + 1):
+        with pytest.raises(m.WsError):
+            m.policy_loss_rows(x, ids, v, v, spins=spins)
+    with pytest.raises(m.WsError, match="at most"):
+        m.preference_loss(v, torch.empty((1 << 33) + 1, dtype=torch.int8, device="meta"))

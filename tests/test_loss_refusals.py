@@ -44,3 +44,20 @@ def test_gradients_between_the_rows_of_the_logits(dtype, each):
             codes = (lib.ws_token_logprobs_grad(None, C.byref(r), AT, AT, None, None, d, d_stride),
                      lib.ws_policy_loss_rows(None, C.byref(r), C.byref(p), AT, AT, None, d, d_stride, AT, 1 << 20))
             assert all((c != m.E_INVALID) == taken for c in codes), (off, stride, d_stride, rows, codes)
+
+
+def test_sizes_past_32_bits_are_refused():
+    """A C structure's entry keeps the lower 32 bits of a number: 2^32 + 3 rows would be three. (Tensors without memory: what is looked at first is the size.)"""
+    m = gc.pkg()
+    many = (1 << 32) + 3
+    empty = lambda *shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device="meta")  # noqa: E731
+    ids, v, long = empty(3, dtype=torch.int32), empty(3), empty(many)
+    calls = []
+    for x in (empty(many, 1), empty(1, many), empty(1 << 20, 3), empty(3, 1 << 20)):
+        calls += [lambda x=x: m.token_logprobs(x, ids), lambda x=x: m.token_logprobs_grad(x, ids, v), lambda x=x: m.policy_loss_rows(x, ids, v, v)]
+    for x in (long, empty((1 << 30) + 1)):
+        calls += [lambda x=x: m.policy_loss(x, x, x), lambda x=x: m.preference_loss(x, ids)]
+    for i, call in enumerate(calls):
+        with pytest.raises(m.WsError, match="at most"):
+            call()
+            raise AssertionError(i)

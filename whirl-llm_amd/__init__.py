@@ -571,6 +571,7 @@ def spec_verify_classic(p, q, draft, seed, step0, rng=RNG_PHILOX, tol=0.0, works
 
 _LOSS_DTYPES = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}
 _F32, _I32 = torch.float32, torch.int32
+_MOST_ROWS, _MOST_TOKENS, _MOST_SPINS = 1048575, 1 << 30, 65536  # of logits, of log-probabilities, ws_policy.spins
 
 
 def _vector(name, t, dtype, n, at):
@@ -596,11 +597,21 @@ def _device_of(name, t):
     return at
 
 
+def _tokens_of(name, t):
+    """The number of a vector's entries, one of those that the calls over log-probabilities take."""
+    n = t.numel()
+    if n > _MOST_TOKENS:
+        raise WsError(f"{name}: {n} entries, at most {_MOST_TOKENS}")
+    return n
+
+
 def _rows_stride(name, t):
     """(rows, vocab, elements between rows) of a matrix."""
     if t.dim() != 2 or t.dtype not in _LOSS_DTYPES:
         raise WsError(f"{name}: [rows, vocab] float32 / bfloat16 device tensor")
     (rows, vocab), (stride, inner) = t.shape, t.stride()
+    if rows > _MOST_ROWS or vocab > _MOST_ROWS:  # (here, since a C structure's entry would keep the lower 32 bits)
+        raise WsError(f"{name}: {rows} x {vocab}, at most {_MOST_ROWS} rows and tokens")
     if rows < 2:
         stride = vocab
     if (inner != 1 and vocab > 1) or stride < vocab:
@@ -679,7 +690,7 @@ def policy_loss(logprob, old_logprob, advantage, ref_logprob=None, entropy=None,
     """The clipped policy loss over float32 [rows] log-probabilities (ws_policy_loss). weight: float32 [rows], 0 = the token counts for nothing (None:
     1 / rows each). Returns (sums float32 [5] = loss, surrogate, KL, entropy, clipped weight; d_logprob float32 [rows]; d_entropy float32
     [rows], or None without entropy)."""
-    rows, at, dev = logprob.numel(), _device_of("logprob", logprob), logprob.device
+    rows, at, dev = _tokens_of("logprob", logprob), _device_of("logprob", logprob), logprob.device
     p = _policy(old_logprob, advantage, ref_logprob, weight, rows, at, clip_low, clip_high, dual_clip, kl_coef, entropy_coef)
     call = lib()
     need = call.ws_policy_loss_workspace(rows)
@@ -697,6 +708,8 @@ def policy_loss_rows(logits, ids, old_logprob, advantage, ref_logprob=None, weig
     one. Rows without a token and rows of weight 0 count for nothing and are not read. out: where to write the gradient; it may be
     `logits`. spins: ws_policy.spins. Returns (sums float32 [5], logprob float32 [rows], entropy float32 [rows] or None, d_logits)."""
     r, rows, vocab, at = _loss_rows(logits, _given("ids", ids), inv_t, allow)
+    if not 0 <= spins <= _MOST_SPINS:
+        raise WsError(f"spins: {spins}, at most {_MOST_SPINS}")
     p = _policy(old_logprob, advantage, ref_logprob, weight, rows, at, clip_low, clip_high, dual_clip, kl_coef, entropy_coef)
     p.spins = spins
     out, stride = _gradient_for(logits, out, vocab)
@@ -713,10 +726,10 @@ def preference_loss(logprob, seq_off, ref_logprob=None, weight=None, beta=0.1, l
     """The loss of paired log ratios over float32 [rows] log-probabilities (ws_preference_loss). seq_off: int32 [2 * pairs + 1], ascending: rows
     seq_off[2 p] .. seq_off[2 p + 1] are the preferred answer of pair p, the next ones the other. weight: float32 [pairs] (None: 1 / pairs
     each). Returns (loss float32 [1], pair_loss float32 [pairs], reward float32 [pairs, 2], d_logprob float32 [rows])."""
-    rows, at, dev = logprob.numel(), _device_of("logprob", logprob), logprob.device
+    rows, at, dev = _tokens_of("logprob", logprob), _device_of("logprob", logprob), logprob.device
     pairs = (seq_off.numel() - 1) // 2
-    if pairs < 1:
-        raise WsError("seq_off: 2 * pairs + 1 offsets of one pair at least")
+    if pairs < 1 or pairs > _MOST_TOKENS:
+        raise WsError(f"seq_off: 2 * pairs + 1 offsets, of one pair at least and {_MOST_TOKENS} at most")
     call = lib()
     need = call.ws_preference_loss_workspace(pairs)
     loss, work, held = _with_work(1, need, dev)
