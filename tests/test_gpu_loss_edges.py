@@ -338,3 +338,32 @@ def test_pairs_and_looks_past_32_bits_are_refused():
             m.policy_loss_rows(x, ids, v, v, spins=spins)
     with pytest.raises(m.WsError, match="at most"):
         m.preference_loss(v, torch.empty((1 << 33) + 1, dtype=torch.int8, device="meta"))
+
+
+def test_a_gradient_written_over_a_tensor_is_seen_by_autograd():
+    """`out` is overwritten: what autograd keeps of it is no longer what it was, and a backward pass that needs it has to say so. The gradient itself is carried on with logits.backward."""
+    m = gc.pkg()
+    c = make(4, 300, F32, 29)
+    v = torch.zeros(4, device=DEV)
+    lp, stats, _ = m.token_logprobs(c["dx"], c["dids"])
+    calls = (lambda x, out: m.token_logprobs_grad(x, c["dids"], stats, d_logprob=v + 1.0, out=out), lambda x, out: m.policy_loss_rows(x, c["dids"], lp, v + 1.0, out=out)[3])
+    for call in calls:
+        hidden = c["dx"].clone().requires_grad_()
+        logits = 30.0 * torch.tanh(hidden / 30.0)
+        d = call(logits, None)
+        assert not d.requires_grad
+        (want,) = torch.autograd.grad(logits, hidden, d)
+        assert bool(want.any())
+        logits = 30.0 * torch.tanh(hidden / 30.0)  # (keeps the tangent, which is another tensor: over these logits it can be written)
+        d = call(logits, logits)
+        (got,) = torch.autograd.grad(logits, hidden, d.clone())
+        assert torch.equal(got, want)
+        logits = torch.tanh(hidden)  # (keeps these)
+        version = logits._version
+        d = call(logits, logits)
+        assert logits._version > version
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(logits, hidden, d.clone())
+        with torch.inference_mode():
+            x = c["dx"].clone()
+            call(x, x)

@@ -636,7 +636,9 @@ def _gradient_for(logits, out, vocab):
         return torch.empty_like(logits), vocab  # (contiguous, of rows that lie apart too; 1.2 us of the host, new_empty 1.8)
     if out.shape != logits.shape or out.dtype is not logits.dtype or out.get_device() != logits.get_device():
         raise WsError("out: of the logits' shape and dtype, on their device")
-    return out, _rows_stride("out", out)[2]
+    stride = _rows_stride("out", out)[2]
+    torch.autograd.graph.increment_version(out)  # (a backward pass that has kept it has to see that it is overwritten)
+    return out, stride
 
 
 def _with_work(words, need, dev):
@@ -670,7 +672,8 @@ def token_logprobs(logits, ids, inv_t=None, allow=None, want_entropy=False):
 def token_logprobs_grad(logits, ids, stats, d_logprob=None, entropy=None, d_entropy=None, inv_t=None, allow=None, out=None):
     """Gradient with respect to the logits of a loss whose derivatives by token_logprobs' logprob and entropy are d_logprob and d_entropy (float32
     [rows], None: 0), in the logits' dtype (ws_token_logprobs_grad). stats, entropy: what token_logprobs returned for the same logits,
-    ids, inv_t and allow. out: where to write it; it may be `logits`. A row whose derivatives are 0 is not read."""
+    ids, inv_t and allow. out: where to write it; it may be `logits`. A row whose derivatives are 0 is not read. Nothing here is recorded by autograd: the gradient goes on
+    with logits.backward(gradient), over the logits too where what made them does not keep them."""
     r, rows, vocab, at = _loss_rows(logits, ids, inv_t, allow)
     out, stride = _gradient_for(logits, out, vocab)
     check(lib().ws_token_logprobs_grad(_stream(), C.byref(r), _vector("stats", _given("stats", stats), _F32, 2 * rows, at), _vector("d_logprob", d_logprob, _F32, rows, at),
@@ -706,7 +709,7 @@ def policy_loss_rows(logits, ids, old_logprob, advantage, ref_logprob=None, weig
                      dual_clip=0.0, kl_coef=0.0, entropy_coef=0.0, want_entropy=False, out=None, spins=0):
     """The clipped policy loss from the logits and its gradient by them (ws_policy_loss_rows): token_logprobs, policy_loss and token_logprobs_grad in
     one. Rows without a token and rows of weight 0 count for nothing and are not read. out: where to write the gradient; it may be
-    `logits`. spins: ws_policy.spins. Returns (sums float32 [5], logprob float32 [rows], entropy float32 [rows] or None, d_logits)."""
+    `logits`. spins: ws_policy.spins. Nothing here is recorded by autograd (token_logprobs_grad). Returns (sums float32 [5], logprob float32 [rows], entropy float32 [rows] or None, d_logits)."""
     r, rows, vocab, at = _loss_rows(logits, _given("ids", ids), inv_t, allow)
     if not 0 <= spins <= _MOST_SPINS:
         raise WsError(f"spins: {spins}, at most {_MOST_SPINS}")
