@@ -367,3 +367,21 @@ def test_a_gradient_written_over_a_tensor_is_seen_by_autograd():
         with torch.inference_mode():
             x = c["dx"].clone()
             call(x, x)
+
+
+@pytest.mark.parametrize("rows,V", [(3, 50257), (300, 50257), (5, 777), (2, 151936)])
+def test_entropy_gradient_of_nearly_even_rows(rows, V):
+    """Where a row is nearly even ln p + H is small beside ln p and H: H - ln S is taken before either is rounded. An entry is h t p (d - mean d) with exponents d of a thousandth: the difference
+    x - m, the product with the split factor and the power round by EPS |d| and one step, the mean's sums by sum_tol's steps; one more rounding each of factors and result."""
+    m = gc.pkg()
+    g = torch.Generator().manual_seed(V)
+    ids, none, h = torch.zeros(rows, dtype=torch.int32, device=DEV), torch.zeros(rows, device=DEV), -1.0
+    for sigma in (0.0, 1e-3):
+        x = 3.0 + sigma * torch.randn((rows, V), generator=g)
+        r = lr.score(x, ids.cpu())
+        _, _, _, d = m.policy_loss_rows(x.to(DEV), ids, none, none, weight=none + 1.0, entropy_coef=1.0)
+        want, _ = lr.grad(r, torch.zeros(rows, dtype=torch.float64), torch.full((rows,), h, dtype=torch.float64))
+        mean = (r["p"] * r["a"].abs()).sum(1, keepdim=True)
+        near(d, want, r["p"] * (r["a"].abs() + mean) * lr.EPS * (2.0 * 42.0) + 2.0 ** -126, ("gradient", sigma))
+        if sigma == 0.0:
+            assert not d.any()

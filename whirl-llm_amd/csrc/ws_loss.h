@@ -355,19 +355,21 @@ struct RowSums {
 };
 struct RowValue {
     double lp, H;
-    bool any;  // some token is allowed
+    double rise;  // H - ln S
+    bool any;     // some token is allowed
 };
 __device__ __forceinline__ RowValue row_value(const RowSums& r, float inv_t, bool has_id, float x_id) {
     RowValue v;
     v.any = !(r.s == 0.0);
     if (!v.any) {  // nothing is allowed: no token has a probability
         v.lp = has_id ? -static_cast<double>(INFINITY) : 0.0;
-        v.H = 0.0;
+        v.H = v.rise = 0.0;
         return v;
     }
     const double lnS = log(r.s);
     v.lp = has_id ? (static_cast<double>(x_id) - static_cast<double>(r.m)) * static_cast<double>(inv_t) - lnS : 0.0;
-    v.H = lnS - 0.69314718055994530942 * (r.t / r.s);
+    v.rise = -0.69314718055994530942 * (r.t / r.s);
+    v.H = lnS + v.rise;
     return v;
 }
 
@@ -547,7 +549,7 @@ struct RowSlope {
     bool none;
 };
 template <bool ENT>
-__device__ __forceinline__ RowSlope row_slope(float m, float S, float inv_t, float g, float h, float H) {
+__device__ __forceinline__ RowSlope row_slope(float m, float S, float inv_t, float g, float h, float rise) {  // rise: H - ln S
     RowSlope r;
     r.m = m;
     r.none = (g == 0.f && (!ENT || h == 0.f)) || S == 0.f;
@@ -555,7 +557,7 @@ __device__ __forceinline__ RowSlope row_slope(float m, float S, float inv_t, flo
     // held so that a + b d, |d| <= 1000 where it counts, is finite: an infinity times a power of 0 would be NaN, in every masked place
     auto held = [](float v, float most) { return fabsf(v) > most ? copysignf(most, v) : v; };
     const float h_held = held(h, 0x1p100f);
-    r.a = held(f * (ENT ? fmaf(h_held, H - __logf(S), held(g, FLT_MAX)) : g), 0x1p126f);
+    r.a = held(f * (ENT ? fmaf(h_held, rise, held(g, FLT_MAX)) : g), 0x1p126f);
     r.b = ENT ? held(f * h_held * 0.69314718f, 0x1p112f) : 0.f;
     r.at_id = g * inv_t;
     return r;
@@ -597,8 +599,9 @@ __global__ void __launch_bounds__(T) grad_rows_kernel(GradArgs A) {
     const int32_t id = A.R.ids ? A.R.ids[row] : -1;
     const bool has_id = static_cast<uint32_t>(id) < V;
     const Scale c(inv_t);
-    const RowSlope r = row_slope<ENT>(A.stats[2 * static_cast<size_t>(row)], A.stats[2 * static_cast<size_t>(row) + 1], inv_t,
-                                      has_id && A.d_logprob ? A.d_logprob[row] : 0.f, ENT ? A.d_entropy[row] : 0.f, ENT ? A.entropy[row] : 0.f);
+    const float S = A.stats[2 * static_cast<size_t>(row) + 1];
+    const RowSlope r = row_slope<ENT>(A.stats[2 * static_cast<size_t>(row)], S, inv_t, has_id && A.d_logprob ? A.d_logprob[row] : 0.f, ENT ? A.d_entropy[row] : 0.f,
+                                      ENT ? A.entropy[row] - __logf(S) : 0.f);
     const uint32_t j0 = chunk * (T * U) + t;
     auto store = [&](uint32_t j, const uint4& q) { store_vector(out + static_cast<size_t>(span.index(j)) * Elem<DT>::kBytes, q, past); };
     if (r.none) {  // (uniform) not read
@@ -802,7 +805,8 @@ __global__ void __launch_bounds__(T, WAVES) policy_rows_kernel(RowsArgs A) {
     if (t == 0u) {
         const RowValue v = row_value(r, inv_t, true, x_id);
         const PolicyToken o = policy_token(A.P, token, v.lp, ENT ? v.H : 0.0);
-        shared_slope = row_slope<SLOPE>(r.m, static_cast<float>(r.s), inv_t, static_cast<float>(o.g), static_cast<float>(o.h), static_cast<float>(v.H));
+        shared_slope = row_slope<SLOPE>(r.m, static_cast<float>(r.s), inv_t, static_cast<float>(o.g), static_cast<float>(o.h),
+                                        static_cast<float>(v.rise));  // (the difference of H and ln S as floats: 1e-6 off where an even row has 0)
         if (part == 0u) {
             A.logprob[row] = static_cast<float>(v.lp);
             if (ENT) A.entropy[row] = static_cast<float>(v.H);
