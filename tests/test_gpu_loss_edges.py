@@ -385,3 +385,18 @@ def test_entropy_gradient_of_nearly_even_rows(rows, V):
         near(d, want, r["p"] * (r["a"].abs() + mean) * lr.EPS * (2.0 * 42.0) + 2.0 ** -126, ("gradient", sigma))
         if sigma == 0.0:
             assert not d.any()
+
+
+@pytest.mark.parametrize("V", [5, 1000, 40001])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_everything_of_a_row_that_is_nan(dtype, V):
+    """Its maximum in `stats` too; a row without a token keeps its logprob of 0."""
+    m = gc.pkg()
+    c, r, at = special_case(dtype, V)
+    c["ids"][at["t_nan"]] = -1
+    lp, stats, H = m.token_logprobs(c["x"].to(DEV), c["ids"].to(DEV), inv_t=c["inv_t"].to(DEV), allow=lr.pack_allow(c["allow"]).to(DEV), want_entropy=True)
+    for n in BAD:
+        assert bool(torch.isnan(stats[at[n]]).all()) and math.isnan(H[at[n]].item()), n
+        assert lp[at[n]].item() == 0.0 if n == "t_nan" else math.isnan(lp[at[n]].item()), n
+    ok = [i for n, i in at.items() if n not in BAD]
+    assert torch.equal(stats[ok, 0].cpu().double(), r["m"][ok])

@@ -524,7 +524,7 @@ __global__ void __launch_bounds__(T) score_rows_kernel(ScoreArgs A) {
     }
     if (t != 0u) return;
     const RowValue v = row_value(r, inv_t, has_id, x_id);
-    A.stats[2 * static_cast<size_t>(row)] = v.any ? r.m : -INFINITY;
+    A.stats[2 * static_cast<size_t>(row)] = !v.any ? -INFINITY : (r.s == r.s ? r.m : static_cast<float>(r.s));  // (NaN is not the largest of anything)
     A.stats[2 * static_cast<size_t>(row) + 1] = static_cast<float>(r.s);
     A.logprob[row] = static_cast<float>(v.lp);
     if (ENT) A.entropy[row] = static_cast<float>(v.H);
