@@ -609,14 +609,15 @@ typedef struct ws_policy {
 /* sums: loss, sum of weight * -gain, of weight * kl, of weight * entropy, and the weight of the tokens whose gain a clip holds */
 enum { WS_POLICY_LOSS = 0, WS_POLICY_SURROGATE = 1, WS_POLICY_KL = 2, WS_POLICY_ENTROPY = 3, WS_POLICY_CLIPPED = 4, WS_POLICY_SUMS = 5 };
 
-/* The loss over log-probabilities the caller has, and its derivatives by them. entropy: device [rows] (NULL: none, entropy_coef must be 0);
+/* The loss over log-probabilities the caller has, and its derivatives by them. Every entry is a token here: the 0 that ws_token_logprobs writes for a row without one counts
+ * unless its weight is 0. entropy: device [rows] (NULL: none, entropy_coef must be 0);
  * d_entropy may be NULL. workspace as above, of ws_policy_loss_workspace() bytes; required where that is not 0. */
 uint64_t ws_policy_loss_workspace(uint32_t rows);
 int ws_policy_loss(void* stream, uint32_t rows, const ws_policy* p, const float* logprob, const float* entropy, float* sums, float* d_logprob,
                    float* d_entropy, void* workspace, uint64_t workspace_bytes);
 
-/* The loss from the logits, and its gradient by them: what ws_token_logprobs, ws_policy_loss and ws_token_logprobs_grad do together,
- * with a row read once where the registers hold it. Rows without a token and rows of weight 0 count for nothing: they are not read, their
+/* The loss from the logits, and its gradient by them: what ws_token_logprobs, ws_policy_loss (with weight 0 for rows without a token) and ws_token_logprobs_grad do
+ * together, with a row read once where the registers hold it. Rows without a token and rows of weight 0 count for nothing: they are not read, their
  * logprob and entropy are 0, their gradient is zero. Without `weight` every row weighs 1 / rows, those without a token too. entropy: out (may be
  * NULL, entropy_coef must be 0 then). d_logits as in ws_token_logprobs_grad. workspace as above, of
  * ws_policy_loss_rows_workspace() bytes; required. */

@@ -400,3 +400,66 @@ def test_everything_of_a_row_that_is_nan(dtype, V):
         assert lp[at[n]].item() == 0.0 if n == "t_nan" else math.isnan(lp[at[n]].item()), n
     ok = [i for n, i in at.items() if n not in BAD]
     assert torch.equal(stats[ok, 0].cpu().double(), r["m"][ok])
+
+
+@pytest.mark.parametrize("rows,V", [(1, 1048575), (2, 1048573), (3, 786409), (2, 262144), (40, 151937), (700, 20485), (3, 4099), (9, 33), (2100, 261)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("masked", [False, True])
+def test_even_rows_count_every_logit_once(rows, V, dtype, masked):
+    """Every power is 1 and every partial sum a whole number: S is the number of allowed tokens, to the bit, and a logit lost or taken twice shows whatever the row's length. ln S in 64 bits, rounded
+    once. The gradient's entries are all the same: -g / S, two roundings of factors and, of bf16, the result's."""
+    m = gc.pkg()
+    g = torch.Generator().manual_seed(rows + V)
+    stride, shift = 3, 1
+    mem = torch.full((rows * (V + stride) + shift,), 50.0, dtype=dtype, device=DEV)
+    x = mem[shift:].view(rows, V + stride)[:, :V]
+    x.fill_(-1.5)
+    ids = torch.randint(V, (rows,), generator=g, dtype=torch.int32)
+    allow = torch.rand((rows, V), generator=g) < 0.4 if masked else torch.ones((rows, V), dtype=torch.bool)
+    allow[torch.arange(rows), ids.long()] = True
+    S = allow.sum(1).double()
+    words = lr.pack_allow(allow).to(DEV) if masked else None
+    dids, inv_t = ids.to(DEV), torch.full((rows,), 0.7, device=DEV)
+    adv = torch.ones(rows, device=DEV)
+    for entropy in (False, True):
+        lp, stats, H = m.token_logprobs(x, dids, inv_t=inv_t, allow=words, want_entropy=entropy)
+        assert torch.equal(stats[:, 1].cpu().double(), S) and bool((stats[:, 0] == -1.5).all())
+        tol = lr.EPS * 1.001 * S.log() + 1e-12
+        near(lp, -S.log(), tol, "logprob")
+        if entropy:
+            near(H, S.log(), tol, "entropy")
+        for spins in (0, 1):
+            _, lp, H, d = m.policy_loss_rows(x, dids, (-S.log()).float().to(DEV), adv, weight=adv, inv_t=inv_t, allow=words, want_entropy=entropy, spins=spins)
+            near(lp, -S.log(), tol, "logprob of the step")
+            if entropy:
+                near(H, S.log(), tol, "entropy of the step")
+            # (the ratio is e^(rounding of the old log-probability): 1 within EPS ln S)
+            want = torch.where(allow, (0.7 / S)[:, None], torch.zeros(1, dtype=torch.float64))
+            want[torch.arange(rows), ids.long()] -= 0.7
+            rel = lr.EPS * (S.log()[:, None] + 6.0) + torch.finfo(dtype).eps / 2
+            near(d, want, 1.001 * rel * (want.abs() + (0.7 / S)[:, None] * allow) + 2.0 ** -126, "gradient")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [5, 1000, 40001])
+def test_the_three_calls_of_a_policy_step_on_special_rows(dtype, V):
+    """Scores, loss and gradient one after the other, rows without a token weighing 0 in the loss: what the policy step does at once (ws_policy_loss sees a log-probability of 0 there, and would count it)."""
+    m = gc.pkg()
+    c, r, at = special_case(dtype, V)
+    rows = [i for n, i in at.items() if n not in BAD]
+    pick = lambda t: t[rows].to(DEV).contiguous()  # noqa: E731
+    x, ids, inv_t, allow = pick(c["x"]), pick(c["ids"]), pick(c["inv_t"]), lr.pack_allow(c["allow"][rows]).to(DEV)
+    old = torch.nan_to_num((r["lp"] + 0.1).float(), neginf=-INF)[rows].to(DEV)
+    adv, w = torch.linspace(-1, 1, len(rows), device=DEV), torch.ones(len(rows), device=DEV)
+    o = dict(kl_coef=0.05, entropy_coef=0.01)
+    want = m.policy_loss_rows(x, ids, old, adv, ref_logprob=old, weight=w, inv_t=inv_t, allow=allow, **o)
+    lp, stats, H = m.token_logprobs(x, ids, inv_t=inv_t, allow=allow, want_entropy=True)
+    has = (ids >= 0) & (ids < V)
+    sums, g, h = m.policy_loss(lp, old, adv, ref_logprob=old, entropy=H, weight=torch.where(has, w, 0.0 * w), **o)
+    d = m.token_logprobs_grad(x, ids, stats, d_logprob=g, entropy=H, d_entropy=h, inv_t=inv_t, allow=allow)
+    # log-probabilities and entropies are rounded between the calls: EPS of their size, and of ratios as much; both sides are off by lp_tol and H_tol
+    off = (2 * lr.lp_tol(r, V) + 2 * lr.H_tol(r, V))[rows].nan_to_num(0.0)
+    near(sums, want[0].cpu(), 3.0 * off.sum() + 4 * lr.EPS * float(want[0].abs().sum()), "sums")
+    assert torch.equal(torch.isneginf(lp), torch.isneginf(want[1])) and not torch.isnan(d).any() and bool(torch.isfinite(sums).all())
+    near(torch.where(has, lp, 0.0 * lp).nan_to_num(neginf=-1e30), want[1].cpu().nan_to_num(neginf=-1e30), off, "logprob")
+    near(d, want[3].cpu().float(), (3.0 * off + 40 * lr.EPS)[:, None] * r["t"][rows][:, None] + 2.0 * torch.finfo(dtype).eps * want[3].cpu().double().abs(), "gradient")

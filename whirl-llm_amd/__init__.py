@@ -690,8 +690,8 @@ def _policy(old_logprob, advantage, ref_logprob, weight, rows, at, clip_low, cli
 
 def policy_loss(logprob, old_logprob, advantage, ref_logprob=None, entropy=None, weight=None, clip_low=0.2, clip_high=0.2, dual_clip=0.0, kl_coef=0.0,
                 entropy_coef=0.0):
-    """The clipped policy loss over float32 [rows] log-probabilities (ws_policy_loss). weight: float32 [rows], 0 = the token counts for nothing (None:
-    1 / rows each). Returns (sums float32 [5] = loss, surrogate, KL, entropy, clipped weight; d_logprob float32 [rows]; d_entropy float32
+    """The clipped policy loss over float32 [rows] log-probabilities (ws_policy_loss). weight: float32 [rows], 0 = the token counts for nothing, which a row without a token needs
+    here, where its log-probability of 0 is one as good as any (None: 1 / rows each). Returns (sums float32 [5] = loss, surrogate, KL, entropy, clipped weight; d_logprob float32 [rows]; d_entropy float32
     [rows], or None without entropy)."""
     rows, at, dev = _tokens_of("logprob", logprob), _device_of("logprob", logprob), logprob.device
     p = _policy(old_logprob, advantage, ref_logprob, weight, rows, at, clip_low, clip_high, dual_clip, kl_coef, entropy_coef)
