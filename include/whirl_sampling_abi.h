@@ -552,7 +552,8 @@ int ws_spec_verify_classic(void* stream, const ws_spec_verify* v);
  * Logits that are not allowed count as -inf, whatever they hold. A row where nothing is left (every allowed logit -inf, or none
  * allowed) has stats {-inf, 0}, entropy 0 and, if it has a token, logprob -inf, and its derivatives are 0. A token that is not allowed
  * has logprob -inf and its row the derivatives of the others. An allowed logit of +inf or NaN, or an inv_t that is
- * not a positive finite number, makes everything of its row NaN (but the logprob of a row without a token). Results are the same bits on every run over the same memory (which thread
+ * not a positive finite number, makes everything of its row NaN (but the logprob of a row without a token). Differences
+ * x_v - m below what a float holds count as -inf. Results are the same bits on every run over the same memory (which thread
  * adds up which logits goes by where a row - of ws_policy_loss_rows its gradient - lies against the 128-byte lines).
  * What these calls write overlaps nothing else that they read or write, but a gradient the logits where its call says so.
  * rows and vocab: at most 1048575 each. */

@@ -463,3 +463,30 @@ def test_the_three_calls_of_a_policy_step_on_special_rows(dtype, V):
     assert torch.equal(torch.isneginf(lp), torch.isneginf(want[1])) and not torch.isnan(d).any() and bool(torch.isfinite(sums).all())
     near(torch.where(has, lp, 0.0 * lp).nan_to_num(neginf=-1e30), want[1].cpu().nan_to_num(neginf=-1e30), off, "logprob")
     near(d, want[3].cpu().float(), (3.0 * off + 40 * lr.EPS)[:, None] * r["t"][rows][:, None] + 2.0 * torch.finfo(dtype).eps * want[3].cpu().double().abs(), "gradient")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("masked", [False, True])
+def test_very_small_inverse_temperatures(dtype, masked):
+    """1 / temperature down to the smallest float, with logits as large as it takes to matter (differences that a float holds): the second float of the factor may not be larger than it is. Below
+    2^-126 floats lie 2^-149 apart: a factor c is off by 2^-149 / c then, and exponents by that much of their size."""
+    m = gc.pkg()
+    rows, V = 6, 3001
+    c = make(rows, V, dtype, 83, masked)
+    inv_t = f32(1e-30, 1e-34, 1e-36, 1e-37, 1.2e-38, 3e-40)
+    x = (torch.rand((rows, V), generator=c["g"]) * 4.0 / inv_t.double()[:, None].clamp(min=2.5e-38)).to(dtype)
+    if masked:
+        x[:, 7] = -INF
+    r = lr.score(x, c["ids"], inv_t, c["allow"])
+    assert float((r["a"].abs().amax(1)).min()) > 0.01
+    dx, ids, inv, allow = x.to(DEV), c["dids"], inv_t.to(DEV), c["dallow"]
+    lp, stats, H = m.token_logprobs(dx, ids, inv_t=inv, allow=allow, want_entropy=True)
+    extra = (2.0 ** -149 / inv_t.double()) * (r["p"] * r["a"].abs()).sum(1) * 2.0
+    near(stats[:, 1], r["S"], r["S"] * (lr.sum_tol(r, V) + extra), "sum")
+    near(lp, r["lp"], lr.lp_tol(r, V) + extra, "logprob")
+    near(H, r["H"], lr.H_tol(r, V) + 4.0 * extra, "entropy")
+    # (times t the gradient would leave the floats: g makes up for it)
+    g = (1.0 / inv_t.double()).clamp(max=1e37).float()
+    for d in (m.token_logprobs_grad(dx, ids, stats, d_logprob=g.to(DEV), inv_t=inv, allow=allow), ):
+        want, size = lr.grad(r, g.double(), torch.zeros(rows, dtype=torch.float64))
+        near(d, want, lr.grad_tol(r, size, want, V, dtype) + size * (2.0 ** -148 / inv_t.double())[:, None] * (1.0 + r["a"].abs()), "gradient")

@@ -297,7 +297,7 @@ struct Scale {
         float h = static_cast<float>(c);
         if (static_cast<double>(h) >= c) h = __uint_as_float(__float_as_uint(h) - 1u);
         hi = inv_t > 0.f && inv_t < INFINITY ? h : __builtin_nanf("");  // (a temperature that is none makes the row NaN)
-        lo = fmaxf(static_cast<float>(c - static_cast<double>(h)), FLT_MIN);
+        lo = fmaxf(static_cast<float>(c - static_cast<double>(h)), 0x1p-149f);  // (the smallest there is: factors below 2^-102 have a second float as small)
     }
     __device__ __forceinline__ float of(float d) const { return fmaf(d, hi, __fmul_rn(d, lo)); }
 };
@@ -553,12 +553,14 @@ __device__ __forceinline__ RowSlope row_slope(float m, float S, float inv_t, flo
     RowSlope r;
     r.m = m;
     r.none = (g == 0.f && (!ENT || h == 0.f)) || S == 0.f;
-    const float f = -inv_t / S;
+    // v t / S, the factor below 1 last: one that leaves the floats' range on the way would lose bits there
+    const float share = -1.f / S;
+    auto factor = [&](float v) { return inv_t < 1.f ? v * share * inv_t : inv_t * share * v; };
     // held so that a + b d, |d| <= 1000 where it counts, is finite: an infinity times a power of 0 would be NaN, in every masked place
     auto held = [](float v, float most) { return fabsf(v) > most ? copysignf(most, v) : v; };
     const float h_held = held(h, 0x1p100f);
-    r.a = held(f * (ENT ? fmaf(h_held, rise, held(g, FLT_MAX)) : g), 0x1p126f);
-    r.b = ENT ? held(f * h_held * 0.69314718f, 0x1p112f) : 0.f;
+    r.a = held(factor(ENT ? fmaf(h_held, rise, held(g, FLT_MAX)) : g), 0x1p126f);
+    r.b = ENT ? held(factor(h_held) * 0.69314718f, 0x1p112f) : 0.f;
     r.at_id = g * inv_t;
     return r;
 }
