@@ -580,10 +580,11 @@ int ws_token_logprobs(void* stream, const ws_loss_rows* r, float* logprob, float
 
 /* Their gradient: with g = d_logprob[row] (NULL: 0; a row without a token: 0) and h = d_entropy[row] (NULL: 0) the derivatives of some loss by
  * the row's logprob and entropy, d_logits[row][v] = inv_t * (g * (1[v = y] - p_v) - h * p_v * (ln p_v + entropy[row])), in the
- * logits' dtype. Where g or h is infinite, or so large that these factors pass what a float holds, tokens that are not allowed have 0 all the same and the others a large number, not NaN.
- * stats, entropy: what ws_token_logprobs wrote (entropy only with d_entropy). A row with g = h = 0 is not read and
- * gets zeros. d_logits: [rows][d_stride], the first vocab of a row are written; it may be the logits themselves (same address and stride), but not
- * overlap them otherwise. Where the strides are the same its rows may lie between the logits' (the halves of one matrix's rows); else one lies behind the other. */
+ * logits' dtype. Where g or h is infinite, or so large that these factors pass what a float holds, tokens that are not allowed have 0 all
+ * the same and the others a large number, not NaN. stats, entropy: what ws_token_logprobs wrote (entropy only with d_entropy). A row with g
+ * = h = 0 is not read and gets zeros. d_logits: [rows][d_stride], the first vocab of a row are written; it may be the logits themselves
+ * (same address and stride), but not overlap them otherwise. Where the strides are the same its rows may lie between the logits' (the
+ * halves of one matrix's rows); else one lies behind the other. */
 int ws_token_logprobs_grad(void* stream, const ws_loss_rows* r, const float* stats, const float* d_logprob, const float* entropy,
                            const float* d_entropy, void* d_logits, uint64_t d_stride);
 
@@ -592,8 +593,9 @@ int ws_token_logprobs_grad(void* stream, const ws_loss_rows* r, const float* sta
  *   kl   = exp(ref - logprob) - (ref - logprob) - 1;
  *   loss = sum of weight * (-gain + kl_coef * kl - entropy_coef * entropy).
  * A token of weight 0 counts for nothing, whatever its other entries hold. Where the clip holds the gain, it has no derivative.
- * A token whose logprob and old_logprob are both -inf (a mask leaves it out, or its row empty, for either model) counts for nothing too. Another of logprob -inf has the ratio 0 and, where ref is not -inf too, kl = +inf (ref = -inf alone: +inf as well; both: 0). An advantage of 0 has the gain 0,
- * whatever the ratio. */
+ * A token whose logprob and old_logprob are both -inf (a mask leaves it out, or its row empty, for either model) counts for nothing too.
+ * Another of logprob -inf has the ratio 0 and, where ref is not -inf too, kl = +inf (ref = -inf alone: +inf as well; both: 0). An advantage
+ * of 0 has the gain 0, whatever the ratio. */
 typedef struct ws_policy {
     const float* old_logprob; /* device [rows]: of the model that drew the tokens */
     const float* ref_logprob; /* device [rows] (NULL: no KL term, kl_coef must be 0) */
@@ -610,18 +612,18 @@ typedef struct ws_policy {
 /* sums: loss, sum of weight * -gain, of weight * kl, of weight * entropy, and the weight of the tokens whose gain a clip holds */
 enum { WS_POLICY_LOSS = 0, WS_POLICY_SURROGATE = 1, WS_POLICY_KL = 2, WS_POLICY_ENTROPY = 3, WS_POLICY_CLIPPED = 4, WS_POLICY_SUMS = 5 };
 
-/* The loss over log-probabilities the caller has, and its derivatives by them. Every entry is a token here: the 0 that ws_token_logprobs writes for a row without one counts
- * unless its weight is 0. entropy: device [rows] (NULL: none, entropy_coef must be 0);
- * d_entropy may be NULL. workspace as above, of ws_policy_loss_workspace() bytes; required where that is not 0. */
+/* The loss over log-probabilities the caller has, and its derivatives by them. Every entry is a token here: the 0 that ws_token_logprobs
+ * writes for a row without one counts unless its weight is 0. entropy: device [rows] (NULL: none, entropy_coef must be 0); d_entropy may be
+ * NULL. workspace as above, of ws_policy_loss_workspace() bytes; required where that is not 0. */
 uint64_t ws_policy_loss_workspace(uint32_t rows);
 int ws_policy_loss(void* stream, uint32_t rows, const ws_policy* p, const float* logprob, const float* entropy, float* sums, float* d_logprob,
                    float* d_entropy, void* workspace, uint64_t workspace_bytes);
 
-/* The loss from the logits, and its gradient by them: what ws_token_logprobs, ws_policy_loss (with weight 0 for rows without a token) and ws_token_logprobs_grad do
- * together, with a row read once where the registers hold it. Rows without a token and rows of weight 0 count for nothing: they are not read, their
- * logprob and entropy are 0, their gradient is zero. Without `weight` every row weighs 1 / rows, those without a token too. entropy: out (may be
- * NULL, entropy_coef must be 0 then). d_logits as in ws_token_logprobs_grad. workspace as above, of
- * ws_policy_loss_rows_workspace() bytes; required. */
+/* The loss from the logits, and its gradient by them: what ws_token_logprobs, ws_policy_loss (with weight 0 for rows without a token)
+ * and ws_token_logprobs_grad do together, with a row read once where the registers hold it. Rows without a token and rows of weight 0 count
+ * for nothing: they are not read, their logprob and entropy are 0, their gradient is zero. Without `weight` every row weighs 1 / rows,
+ * those without a token too. entropy: out (may be NULL, entropy_coef must be 0 then). d_logits as in ws_token_logprobs_grad. workspace as
+ * above, of ws_policy_loss_rows_workspace() bytes; required. */
 uint64_t ws_policy_loss_rows_workspace(const ws_loss_rows* r);
 int ws_policy_loss_rows(void* stream, const ws_loss_rows* r, const ws_policy* p, float* sums, float* logprob, float* entropy, void* d_logits,
                         uint64_t d_stride, void* workspace, uint64_t workspace_bytes);
@@ -629,11 +631,12 @@ int ws_policy_loss_rows(void* stream, const ws_loss_rows* r, const ws_policy* p,
 /* The loss of paired log ratios: answers 2 p (preferred) and 2 p + 1 of pair p are the rows seq_off[2 p] .. seq_off[2 p + 1] and
  * seq_off[2 p + 1] .. seq_off[2 p + 2]; with s their sums of logprob - ref_logprob and h = beta * (s_preferred - s_other)
  *   pair_loss = (1 - label_smoothing) * ln(1 + exp(-h)) + label_smoothing * ln(1 + exp(h)),    loss = sum of weight * pair_loss,
- * reward[p] = beta * s of the two. A term whose factor is 0 is left out. A token whose logprob and ref_logprob are both -inf (neither model can give it: a mask leaves it out)
- * counts for nothing: it adds nothing, its derivative is 0. An answer with another token of logprob -inf has s = -inf, and its pair the limits: the loss 0 or +inf, the
- * derivatives those of h = +-inf. Where both of a pair's s are -inf h has no value, and loss and derivatives are NaN unless the pair weighs 0. Answers may be empty. seq_off ascends; offsets beyond `rows` end there. d_logprob is written for all rows, 0 for those
- * of no answer. A pair of weight 0 counts for nothing. workspace as above, of ws_preference_loss_workspace() bytes; required where that is
- * not 0. */
+ * reward[p] = beta * s of the two. A term whose factor is 0 is left out. A token whose logprob and ref_logprob are both -inf (neither model
+ * can give it: a mask leaves it out) counts for nothing: it adds nothing, its derivative is 0. An answer with another token of logprob -inf
+ * has s = -inf, and its pair the limits: the loss 0 or +inf, the derivatives those of h = +-inf. Where both of a pair's s are -inf h has no
+ * value, and loss and derivatives are NaN unless the pair weighs 0. Answers may be empty. seq_off ascends; offsets beyond `rows` end there.
+ * d_logprob is written for all rows, 0 for those of no answer. A pair of weight 0 counts for nothing. workspace as above, of
+ * ws_preference_loss_workspace() bytes; required where that is not 0. */
 typedef struct ws_preference {
     uint32_t rows, pairs;
     const uint32_t* seq_off;  /* device [2 * pairs + 1] */

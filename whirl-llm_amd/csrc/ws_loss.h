@@ -7,7 +7,8 @@
 // Both directions are one pass over the row: forwards every thread keeps a maximum, a sum and (for H) a sum of products that are
 // scaled down when its maximum grows, backwards every logit gives its own derivative. Exponentials go to base two with the factor
 // t log2(e) split in two floats (a rounded one alone would move every exponent the same way, 1e-6 of a sum); sums are held
-// in 32 bits by a thread, over some hundred terms, and in 64 bits from the wave on; ln S, log p and the loss of a token in 64 bits.
+// in 32 bits by a thread, over some 120 terms at most where a row's workgroups share it (scores without a workspace: over the 4096 that a thread has of the longest row),
+// and in 64 bits from the wave on; ln S, log p and the loss of a token in 64 bits.
 #pragma once
 
 #include "ws_common.h"
@@ -564,7 +565,9 @@ __device__ __forceinline__ RowSlope row_slope(float m, float S, float inv_t, flo
     r.at_id = g * inv_t;
     return r;
 }
-// (bf16 results: the exponent with the factor's first float alone is 2^-23 |d| off relative to its power at most, a thousandth of their rounding)
+// bf16 results take the exponent with the factor's first float alone, which is rounded down: a power is up to 2^-23 ln 2 |d| of itself too large - a thousandth of the results' half step of
+// 2^-8 where the power is 2^-48 and more, a four hundredth at the smallest - for an instruction a logit less (4096 x 262144 747 us, and 740). A factor rounded to nearest takes another register, and the masked
+// build with entropy spills it.
 template <int DT, bool ENT>
 __device__ __forceinline__ float slope_at(float x, const RowSlope& r, const Scale& c) {
     const float d = DT == 0 ? c.of(x - r.m) : __fmul_rn(x - r.m, c.hi), e = exp2_fast(d);
@@ -643,8 +646,8 @@ __global__ void __launch_bounds__(T) grad_rows_kernel(GradArgs A) {
 // read before a look that still finds no words are the logits, and the token's logit goes with the words, not to be read
 // by a part that comes late.) The words stay until every part has seen them: where the rows' terms meet in this launch too (`terms` is NULL), the parts leave a mark each when they are
 // through, and whoever sees all marks of a row breaks its words; else a second launch adds up the terms and breaks the words.
-// What bounds it: memory, and the vector units at 80 % (16.6 instructions a logit, 19.6 with entropy). 2048 x 151936 bf16 with entropy, a fifth of the rows not counting, 214 us = 5.2 TB/s; 4096 x
-// 262144 741 us = 5.8 TB/s; a row in one workgroup of 1024 threads, what its registers do not hold read twice, 282 and 988. Shares of 11, 14, 16 or 19 vectors a thread are up to 8 % slower, workgroups of 512
+// What bounds it: memory, and the vector units at 80 to 85 % (16.7 instructions a logit, 23.6 with entropy and its gradient). 2048 x 151936 bf16 with entropy, a fifth of the rows not counting, 215 to
+// 220 us = 5.3 TB/s; 4096 x 262144 750 to 780 us = 5.7 TB/s; a row in one workgroup of 1024 threads, what its registers do not hold read twice, 282 and 988. Shares of 11, 14, 16 or 19 vectors a thread are up to 8 % slower, workgroups of 512
 // threads 10 to 20 %: a unit then holds fewer of them, and fewer are at another stage than their neighbours.
 struct RowsArgs {
     LossRows R;
