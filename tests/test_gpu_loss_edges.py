@@ -490,3 +490,30 @@ def test_very_small_inverse_temperatures(dtype, masked):
     for d in (m.token_logprobs_grad(dx, ids, stats, d_logprob=g.to(DEV), inv_t=inv, allow=allow), ):
         want, size = lr.grad(r, g.double(), torch.zeros(rows, dtype=torch.float64))
         near(d, want, lr.grad_tol(r, size, want, V, dtype) + size * (2.0 ** -148 / inv_t.double())[:, None] * (1.0 + r["a"].abs()), "gradient")
+
+
+def share_tol(r):
+    """lr.sum_tol for rows that workgroups share: a share is 15 vectors of 8 logits a thread at most (scores with entropy: 1.5 x 2560 vectors over 256 threads; the policy step: 12), and one of the
+    row's ends, 121 terms however long the row."""
+    return lr.EPS * (2.0 * (r["p"] * r["a"].abs()).sum(1) + 2.0 + 121.0 + 40.0)
+
+
+@pytest.mark.parametrize("rows,V", [(2, 1048575), (3, 786409), (9, 262144), (70, 151937)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_long_rows_within_what_a_share_rounds(rows, V, dtype):
+    m = gc.pkg()
+    c = make(rows, V, dtype, 97 + rows, False, 3, 1, sigma=0.5)
+    r = lr.score(c["x"], c["ids"], c["inv_t"])
+    tol = share_tol(r)
+    mean, square = (r["p"] * r["a"].abs()).sum(1), (r["p"] * r["a"] ** 2).sum(1)
+    Htol = tol * (1.0 + 2.0 * mean) + lr.EPS * (2.0 * square + r["H"].abs() + 4.0 * mean)
+    old, adv = torch.full((rows,), -12.0, device=DEV), torch.zeros(rows, device=DEV)
+    for entropy in (False, True):
+        lp, stats, H = m.token_logprobs(c["dx"], c["dids"], inv_t=c["dinv"], want_entropy=entropy)
+        near(stats[:, 1], r["S"], r["S"] * tol, "sum")
+        _, lp2, H2, _ = m.policy_loss_rows(c["dx"], c["dids"], old, adv, inv_t=c["dinv"], want_entropy=entropy, entropy_coef=0.01 if entropy else 0.0)
+        for what, got in (("scores", lp), ("step", lp2)):
+            near(got, r["lp"], tol + lr.EPS * r["lp"].abs(), what)
+        for what, got in (("scores", H), ("step", H2)):
+            if entropy:
+                near(got, r["H"], Htol, what)
