@@ -7,14 +7,16 @@
  * the host before anything was launched. No exceptions cross this boundary. Per-row run-time conditions
  * (all-masked row, candidate overflow, draw within tolerance of a boundary) are reported in device `flags`.
  *
- * Three groups of entry points:
+ * Four groups of entry points:
  *  (1) one launcher per reference kernel, same argument order and output layout as the kernel the reference
  *      resolves by name (citations at each declaration), with the launch geometry chosen here;
  *      the gfx950 code object whirl_sampling_gfx950.co exports the same `extern "C" __global__` names for callers
  *      that use hipModuleGetFunction (block = 1024 threads, grid = rows, no dynamic LDS);
  *  (2) the batched fused sampler and the classic speculative verify, which the reference does not have;
  *  (3) log-probabilities of the tokens a model answered with, and the losses that train it on them, forwards and backwards,
- *      which the reference does not have either.
+ *      which the reference does not have either;
+ *  (4) a decoding cycle whose drafts form a tree: attention of the tree's rows over a paged cache, verification of the drafts from
+ *      the logits, and what becomes of the cache's pages, all without a host round trip (the reference drafts chains).
  */
 #ifndef WHIRL_SAMPLING_ABI_H
 #define WHIRL_SAMPLING_ABI_H
@@ -652,6 +654,144 @@ typedef struct ws_preference {
 } ws_preference;
 uint64_t ws_preference_loss_workspace(uint32_t pairs);
 int ws_preference_loss(void* stream, const ws_preference* p, void* workspace, uint64_t workspace_bytes);
+
+/* ---- (4) a cycle whose drafts form a tree ------------------------------------------------------------------ */
+
+/* A sequence's drafts as a tree: node 0, the root, is the token that goes in next (ws_history), every other node a drafted token behind its parent,
+ * which comes before it. The nodes of all sequences lie one sequence behind the other: those of sequence s are the rows seq_off[s] .. seq_off[s + 1]
+ * of the call's arrays, WS_TREE_MAX of them at most (rows behind these, and behind the last sequence, are neither read nor written). parent counts within
+ * the sequence; a node whose parent is not an earlier one is never reached. NULL: chains, parent = node - 1. seq_off ascends; offsets beyond `rows` end there.
+ * In the sequence's cache node j lies at position length + j, behind the `length` tokens that the model holds. */
+enum { WS_TREE_MAX = 64 };
+
+/* What a cycle's other calls read, from the trees and the device history (ws_history_stage's part for chains): mask[row] = the nodes that the row sees, bit j
+ * for node j of its sequence - itself and the nodes above it -, position[row] = len + levels above it (the text's position), length[s] = len of the sequence as
+ * the cycle begins. Outputs may be NULL. A node that is never reached sees itself alone, at the position len. */
+typedef struct ws_tree_stage_args {
+    uint32_t n_seq, rows;
+    const uint32_t* seq_off; /* device [n_seq + 1] */
+    const int32_t* parent;   /* device [rows] (NULL: chains) */
+    const uint32_t* len;     /* device, ws_history.len (NULL: 0) */
+    const uint32_t* slot;    /* device [n_seq] (NULL: sequence s has slot s) */
+    uint64_t* mask;          /* out, device [rows] */
+    int32_t* position;       /* out, device [rows] */
+    uint32_t* length;        /* out, device [n_seq] */
+} ws_tree_stage_args;
+int ws_tree_stage(void* stream, const ws_tree_stage_args* a);
+
+/* Drafted tokens against the target's probabilities, from given uniforms. Row `r` of ws_loss_rows is node r's: its logits are the target's for the token behind
+ * the node, `ids` the drafted tokens (a root's is not looked at), inv_t and allow per row as there. From the root on, at node i with P = the row's
+ * distribution p, for its children in order, each with its token y:
+ *   accepted, and the walk goes on from it, if u_accept[child] * Q(y) < P(y), in 64 bits; if not,
+ *   P = max(P - Q, 0) / sum, then Q(y) = 0 and Q divided by its sum: the children of a node are drawn without replacement. (A sum of 0 leaves P, or Q, as it is.)
+ * Q is the distribution that the node's children were drawn from, an entry of WS_Q_WORDS words as ws_draft_sample_rows leaves it (more than WS_Q_MAX ids: the first
+ * WS_Q_MAX; an id twice counts with both), at word q_off[row] of q. Where q is NULL or q_off[row] < 0 the children are guesses: Q is 1 at the token being looked at.
+ * Where no child is accepted, a token is drawn from P: the first in id order up to which P adds up to more than u_draw[s] of its sum; the last with any where there is none.
+ *   n_accepted[s], path[s][0 .. n_accepted) = the accepted nodes, -1 behind them (the first `depth` of them), chosen[s] = the token drawn,
+ *   logprob[s][0 .. n_accepted] = ln p of the accepted nodes' tokens and of the chosen one, each under its own row's p, 0 behind (the first depth + 1).
+ * With a history, next and the accepted tokens are appended to the slot, chosen becomes its next and n_gen advances, as ws_accept_sampled does.
+ * status[s]: WS_ACCEPT_HOST where a row on the walk has nothing that can be drawn (nothing allowed, NaN, an infinite logit, an inv_t that is none) or its q
+ * entry lies outside q, or the sequence has no nodes: chosen is -1 then, what was accepted before is reported and the history left as it was;
+ * WS_ACCEPT_HISTORY_FULL (with WS_ACCEPT_HOST) where the slot has no room for what was accepted: n_accepted 0, chosen -1.
+ * Only the rows that the walk meets are read. workspace: device memory of ws_verify_tree_workspace() bytes (0: none is needed), 8-byte aligned, of any contents, nobody else's
+ * until the launch is done (a captured launch may be replayed); the workgroups that share a row meet there. Required where that is not 0. */
+typedef struct ws_verify_tree_args {
+    uint32_t n_seq;
+    const uint32_t* seq_off; /* device [n_seq + 1] */
+    const int32_t* parent;   /* device [rows] (NULL: chains) */
+    const int32_t* q;        /* device [q_words] (NULL: all drafts are guesses) */
+    uint64_t q_words;
+    const int32_t* q_off;    /* device [rows]: word of each row's entry (with q) */
+    const double* u_accept;  /* device [rows], [0, 1): a root's is not looked at */
+    const double* u_draw;    /* device [n_seq], [0, 1) */
+    uint32_t depth;          /* columns of path (1 .. WS_TREE_MAX) */
+    int32_t* n_accepted;     /* out, device [n_seq] */
+    int32_t* path;           /* out, device [n_seq][depth] */
+    int32_t* chosen;         /* out, device [n_seq] */
+    uint32_t* status;        /* out, device [n_seq] */
+    float* logprob;          /* out, device [n_seq][depth + 1] (may be NULL) */
+    ws_history hist;         /* tokens NULL: no device history */
+    uint32_t spins;          /* as ws_policy.spins */
+} ws_verify_tree_args;
+uint64_t ws_verify_tree_workspace(const ws_loss_rows* r, const ws_verify_tree_args* a);
+int ws_verify_tree(void* stream, const ws_loss_rows* r, const ws_verify_tree_args* a, void* workspace, uint64_t workspace_bytes);
+
+/* One layer of a paged cache: K and V [pages][page_tokens][kv_heads][head_dim] of dtype, the dimensions any strides apart (in elements, multiples of 16 bytes, head_dim's
+ * 1), 16-byte aligned; which page holds what: position p of slot s is token p % page_tokens of page table[s][p / page_tokens]. page_tokens: a power of two.
+ * head_dim: a multiple of 8, up to 256. A page outside [0, pages) - -1 by custom - holds nothing. */
+typedef struct ws_cache_layer {
+    const void* k;
+    const void* v;
+    int32_t dtype; /* WS_DTYPE_* */
+    uint32_t pages, page_tokens, kv_heads, head_dim;
+    uint64_t k_page, k_token, k_head; /* strides */
+    uint64_t v_page, v_token, v_head;
+    const int32_t* table; /* device [slots][table_stride] */
+    uint32_t slots, slot_pages;
+    uint64_t table_stride; /* entries between slots (>= slot_pages) */
+} ws_cache_layer;
+
+/* Attention of the rows of trees over a cache: with `heads` query heads, head h reading kv head h / (heads / kv_heads),
+ *   out[row][h] = sum p_t v_t,  p = softmax over the t that the row sees of scale * q[row][h] . k_t,  lse[row][h] = ln sum exp(scale * q . k_t)
+ * where a row of sequence s sees the positions below length[s] and its sequence's node j at position length[s] + j where bit j of mask[row] is set (NULL: itself and the nodes before
+ * it, a chain's). Whose page holds nothing, or lies past slot_pages, is not seen; nor does what lies in unseen places matter, whatever it is. A row that sees nothing gets zeros and
+ * lse -inf. The scores and their sums are held in 32 bits; bf16: p is rounded to bf16 for the product with V (2^-8 a term, of either sign), out once. Results are
+ * the same bits on every run. max_nodes: the most nodes of a sequence where the caller knows it (0: not known; a sequence with more is answered all the same).
+ * workspace: device memory of ws_tree_attention_workspace() bytes, 16-byte aligned, of any contents, nobody else's until the launch is done. Required. */
+typedef struct ws_tree_attention_args {
+    ws_cache_layer cache;
+    uint32_t n_seq, rows, heads;
+    const void* q;           /* device [rows][heads][head_dim] of dtype */
+    uint64_t q_row, q_head;  /* strides, as the cache's */
+    void* out;               /* device [rows][heads][head_dim] of dtype */
+    uint64_t out_row, out_head;
+    float* lse;              /* out, device [rows][heads] (may be NULL) */
+    const uint32_t* seq_off; /* device [n_seq + 1] */
+    const uint32_t* length;  /* device [n_seq] */
+    const uint32_t* slot;    /* device [n_seq] (NULL: sequence s has slot s) */
+    const uint64_t* mask;    /* device [rows] */
+    float scale;             /* > 0 */
+    uint32_t max_nodes;
+} ws_tree_attention_args;
+uint64_t ws_tree_attention_workspace(const ws_tree_attention_args* a);
+int ws_tree_attention(void* stream, const ws_tree_attention_args* a, void* workspace, uint64_t workspace_bytes);
+
+/* A paged cache of all layers, and what its allocator knows: k and v [layers][pages][page_tokens][kv_heads][head_dim], the dimensions any strides apart as above;
+ * table as above, held[slot] = the pages of a slot (its first entries; the others are -1), refs[page] = how many slots hold a page, free[0 .. n_free[0]) = the pages that nobody
+ * holds, taken from the end. An empty cache: table -1, held 0, refs 0, free every page once. The calls below change these in the order of the stream, each for n sequences
+ * (1024 at most, ws_cache_keep any number); they go by what is there as the call begins, and their results do not depend on the order in which the GPU works. status[i]:
+ * WS_CACHE_OK; WS_CACHE_FULL, too few pages are left, or more than slot_pages would be held: nothing was done for i (sequences are served in order: one that
+ * comes behind the first for whom the pages do not suffice gets none either); WS_CACHE_BAD, a slot that does not exist, is named twice, or is not as the call needs it. */
+enum { WS_CACHE_OK = 0, WS_CACHE_FULL = 1, WS_CACHE_BAD = 2, WS_CACHE_MOST = 1024 };
+typedef struct ws_cache {
+    void* k;
+    void* v;
+    int32_t dtype; /* WS_DTYPE_* */
+    uint32_t layers, pages, page_tokens, kv_heads, head_dim;
+    uint64_t k_layer, k_page, k_token, k_head;
+    uint64_t v_layer, v_page, v_token, v_head;
+    int32_t* table; /* device [slots][table_stride] */
+    uint32_t slots, slot_pages;
+    uint64_t table_stride;
+    int32_t* held;   /* device [slots] */
+    int32_t* refs;   /* device [pages] */
+    int32_t* free;   /* device [pages] */
+    int32_t* n_free; /* device [1] */
+} ws_cache;
+
+/* Pages for tokens[i] tokens in all for slot[i]: those that it lacks are taken and appended to its table. A slot never shrinks here. */
+int ws_cache_reserve(void* stream, const ws_cache* c, const int32_t* slot, const int32_t* tokens, uint32_t n, int32_t* status);
+/* Slot dst[i], which holds nothing, becomes a copy of the first length[i] tokens of slot src[i], which holds pages for that many: whole pages are shared, the tokens on the last,
+ * partly filled one are copied to a page of dst[i]'s own. A src may be named several times. (Tokens that either writes from then on go behind the first length[i], into pages of its own.) */
+int ws_cache_fork(void* stream, const ws_cache* c, const int32_t* src, const int32_t* dst, const int32_t* length, uint32_t n, int32_t* status);
+/* Slot slot[i] keeps the pages of its first tokens[i] tokens (0: none) and gives the others back. Pages that nobody holds any more go on top of the free ones, the first of the first slot
+ * uppermost. status may be NULL. */
+int ws_cache_release(void* stream, const ws_cache* c, const int32_t* slot, const int32_t* tokens, uint32_t n, int32_t* status);
+/* After ws_verify_tree: in every layer position length[s] + 1 + i of the sequence's slot becomes what position length[s] + path[s][i] holds, i = 0 .. n_accepted[s] - 1 in this order (the
+ * root stays where it is), so that the accepted tokens lie behind the text as the history has them. Entries of path from the first on that does not
+ * ascend (each is above the one before it, the first above 0) or is not below WS_TREE_MAX are left out, as are positions whose page holds nothing. length: as the cycle began (ws_tree_stage). */
+int ws_cache_keep(void* stream, const ws_cache* c, const int32_t* path, uint32_t depth, const int32_t* n_accepted, const uint32_t* length, const uint32_t* slot /* NULL: sequence s has slot s */,
+                  uint32_t n_seq);
 
 #ifdef __cplusplus
 }

@@ -128,6 +128,41 @@ class Preference(C.Structure):
                 ("reward", C.c_void_p), ("d_logprob", C.c_void_p)]
 
 
+class TreeStage(C.Structure):
+    """ws_tree_stage_args of include/whirl_sampling_abi.h."""
+    _fields_ = [("n_seq", C.c_uint32), ("rows", C.c_uint32), ("seq_off", C.c_void_p), ("parent", C.c_void_p), ("len", C.c_void_p), ("slot", C.c_void_p),
+                ("mask", C.c_void_p), ("position", C.c_void_p), ("length", C.c_void_p)]
+
+
+class VerifyTree(C.Structure):
+    """ws_verify_tree_args of include/whirl_sampling_abi.h."""
+    _fields_ = [("n_seq", C.c_uint32), ("seq_off", C.c_void_p), ("parent", C.c_void_p), ("q", C.c_void_p), ("q_words", C.c_uint64), ("q_off", C.c_void_p),
+                ("u_accept", C.c_void_p), ("u_draw", C.c_void_p), ("depth", C.c_uint32), ("n_accepted", C.c_void_p), ("path", C.c_void_p), ("chosen", C.c_void_p),
+                ("status", C.c_void_p), ("logprob", C.c_void_p), ("hist", History), ("spins", C.c_uint32)]
+
+
+class CacheLayer(C.Structure):
+    """ws_cache_layer of include/whirl_sampling_abi.h."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int32), ("pages", C.c_uint32), ("page_tokens", C.c_uint32), ("kv_heads", C.c_uint32),
+                ("head_dim", C.c_uint32), ("k_page", C.c_uint64), ("k_token", C.c_uint64), ("k_head", C.c_uint64), ("v_page", C.c_uint64), ("v_token", C.c_uint64),
+                ("v_head", C.c_uint64), ("table", C.c_void_p), ("slots", C.c_uint32), ("slot_pages", C.c_uint32), ("table_stride", C.c_uint64)]
+
+
+class TreeAttention(C.Structure):
+    """ws_tree_attention_args of include/whirl_sampling_abi.h."""
+    _fields_ = [("cache", CacheLayer), ("n_seq", C.c_uint32), ("rows", C.c_uint32), ("heads", C.c_uint32), ("q", C.c_void_p), ("q_row", C.c_uint64), ("q_head", C.c_uint64),
+                ("out", C.c_void_p), ("out_row", C.c_uint64), ("out_head", C.c_uint64), ("lse", C.c_void_p), ("seq_off", C.c_void_p), ("length", C.c_void_p),
+                ("slot", C.c_void_p), ("mask", C.c_void_p), ("scale", C.c_float), ("max_nodes", C.c_uint32)]
+
+
+class Cache(C.Structure):
+    """ws_cache of include/whirl_sampling_abi.h."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int32), ("layers", C.c_uint32), ("pages", C.c_uint32), ("page_tokens", C.c_uint32),
+                ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("k_layer", C.c_uint64), ("k_page", C.c_uint64), ("k_token", C.c_uint64), ("k_head", C.c_uint64),
+                ("v_layer", C.c_uint64), ("v_page", C.c_uint64), ("v_token", C.c_uint64), ("v_head", C.c_uint64), ("table", C.c_void_p), ("slots", C.c_uint32),
+                ("slot_pages", C.c_uint32), ("table_stride", C.c_uint64), ("held", C.c_void_p), ("refs", C.c_void_p), ("free", C.c_void_p), ("n_free", C.c_void_p)]
+
+
 # every symbol include/whirl_sampling_abi.h declares: (result type, argument types)
 ABI = {
     "ws_abi_version": (C.c_int, []),
@@ -191,6 +226,15 @@ ABI = {
                                       C.c_uint64, C.c_void_p, C.c_uint64]),
     "ws_preference_loss_workspace": (C.c_uint64, [C.c_uint32]),
     "ws_preference_loss": (C.c_int, [C.c_void_p, C.POINTER(Preference), C.c_void_p, C.c_uint64]),
+    "ws_tree_stage": (C.c_int, [C.c_void_p, C.POINTER(TreeStage)]),
+    "ws_verify_tree_workspace": (C.c_uint64, [C.POINTER(LossRows), C.POINTER(VerifyTree)]),
+    "ws_verify_tree": (C.c_int, [C.c_void_p, C.POINTER(LossRows), C.POINTER(VerifyTree), C.c_void_p, C.c_uint64]),
+    "ws_tree_attention_workspace": (C.c_uint64, [C.POINTER(TreeAttention)]),
+    "ws_tree_attention": (C.c_int, [C.c_void_p, C.POINTER(TreeAttention), C.c_void_p, C.c_uint64]),
+    "ws_cache_reserve": (C.c_int, [C.c_void_p, C.POINTER(Cache), C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p]),
+    "ws_cache_fork": (C.c_int, [C.c_void_p, C.POINTER(Cache), C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p]),
+    "ws_cache_release": (C.c_int, [C.c_void_p, C.POINTER(Cache), C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p]),
+    "ws_cache_keep": (C.c_int, [C.c_void_p, C.POINTER(Cache), C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32]),
 }
 
 _lib = None
@@ -744,6 +788,195 @@ def preference_loss(logprob, seq_off, ref_logprob=None, weight=None, beta=0.1, l
                    pair_loss.data_ptr(), reward.data_ptr(), d_logprob.data_ptr())
     check(call.ws_preference_loss(_stream(), C.byref(a), work, need), "ws_preference_loss")
     return loss if held is not None else loss.resize_(1), pair_loss, reward, d_logprob
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# a cycle whose drafts form a tree: attention over a paged cache, verification, the cache's pages
+
+TREE_MAX = 64
+CACHE_OK, CACHE_FULL, CACHE_BAD, CACHE_MOST = 0, 1, 2, 1024
+_F64, _I64 = torch.float64, torch.int64
+
+
+def _sequences(seq_off):
+    n = seq_off.numel() - 1
+    if n < 0 or n > _MOST_ROWS:
+        raise WsError(f"seq_off: offsets of 0 to {_MOST_ROWS} sequences")
+    return n
+
+
+def tree_stage(seq_off, rows, parent=None, hist=None, slot=None):
+    """What a cycle with trees of drafts begins with (ws_tree_stage). seq_off: int32 [n_seq + 1], the nodes of sequence s are the rows seq_off[s] .. seq_off[s + 1] (64 at
+    most), the first of them the root, the token that goes in next; parent: int32 [rows], each node's parent within its sequence (None: chains); hist, slot: a DeviceHistory and the
+    sequences' slots (None: texts of length 0). Returns (mask int64 [rows] = bit j: the row sees node j, position int32 [rows], length int32 [n_seq]), which
+    tree_attention, the model's positions and PagedCache.keep take."""
+    at, n_seq = _device_of("seq_off", seq_off), _sequences(seq_off)
+    if not 0 <= rows <= _MOST_ROWS:
+        raise WsError(f"rows: 0 to {_MOST_ROWS}")
+    dev = seq_off.device
+    if rows:  # (every row of a sequence is written; the caller may have rows behind the last)
+        mask, position = torch.zeros(rows, dtype=_I64, device=dev), torch.zeros(rows, dtype=_I32, device=dev)
+    else:
+        mask, position = torch.empty(0, dtype=_I64, device=dev), torch.empty(0, dtype=_I32, device=dev)
+    length = torch.empty(n_seq, dtype=_I32, device=dev)
+    a = TreeStage(n_seq, rows, _vector("seq_off", seq_off, _I32, n_seq + 1, at), _vector("parent", parent, _I32, rows, at), _p(hist.len) if hist is not None else None,
+                  _vector("slot", slot, _I32, n_seq, at), mask.data_ptr(), position.data_ptr(), length.data_ptr())
+    check(lib().ws_tree_stage(_stream(), C.byref(a)), "ws_tree_stage")
+    return mask, position, length
+
+
+def verify_tree(logits, ids, seq_off, u_accept, u_draw, parent=None, q=None, q_off=None, inv_t=None, allow=None, depth=TREE_MAX - 1, hist=None, slot=None, spins=0):
+    """Drafted tokens against the target's probabilities, from given uniforms (ws_verify_tree). logits, inv_t, allow: as in token_logprobs, a row a node; ids int32 [rows]: the drafted tokens;
+    seq_off, parent: as in tree_stage. u_accept float64 [rows], u_draw float64 [n_seq]: uniforms from [0, 1). q: the draft distributions' entries, int32 words as draft_sample_rows
+    leaves them, and q_off int32 [rows], the word where the entry of a node's children begins (< 0, or q None: the children are guesses, accepted with their own probability).
+    hist, slot: a DeviceHistory and the sequences' slots; what is kept is appended to it. Returns (n_accepted int32 [n_seq], path int32 [n_seq, depth] = the accepted nodes, chosen int32
+    [n_seq] = the token drawn behind them, status int32 [n_seq] = ACCEPT_* bits, logprob float32 [n_seq, depth + 1] of the accepted tokens and the chosen one)."""
+    r, rows, vocab, at = _loss_rows(logits, _given("ids", ids), inv_t, allow)
+    n_seq, dev = _sequences(seq_off), logits.device
+    if not 1 <= depth <= TREE_MAX or not 0 <= spins <= _MOST_SPINS:
+        raise WsError(f"depth: 1 to {TREE_MAX}; spins: at most {_MOST_SPINS}")
+    if q is not None and (q.dtype is not _I32 or q.get_device() != at or not q.is_contiguous()):
+        raise WsError("q: contiguous int32 tensor on the logits' device")
+    counts = torch.empty((3, n_seq), dtype=_I32, device=dev)
+    path = torch.empty((n_seq, depth), dtype=_I32, device=dev)
+    a = VerifyTree(n_seq, _vector("seq_off", seq_off, _I32, n_seq + 1, at), _vector("parent", parent, _I32, rows, at), _p(q), q.numel() if q is not None else 0,
+                   _vector("q_off", _given("q_off", q_off) if q is not None else None, _I32, rows, at), _vector("u_accept", _given("u_accept", u_accept), _F64, rows, at),
+                   _vector("u_draw", _given("u_draw", u_draw), _F64, n_seq, at), depth, counts.data_ptr(), path.data_ptr(), counts.data_ptr() + 4 * n_seq, counts.data_ptr() + 8 * n_seq)
+    if hist is not None:
+        if slot is not None:
+            _vector("slot", slot, _I32, n_seq, at)
+        a.hist = hist.ref(slot)
+    a.spins = spins
+    call = lib()
+    need = call.ws_verify_tree_workspace(C.byref(r), C.byref(a))
+    logprob, work, held = _with_work(n_seq * (depth + 1), need, dev)
+    a.logprob = logprob.data_ptr()
+    check(call.ws_verify_tree(_stream(), C.byref(r), C.byref(a), work, need), "ws_verify_tree")
+    n_accepted, chosen, status = counts.unbind()
+    return n_accepted, path, chosen, status, logprob.resize_(n_seq, depth + 1)
+
+
+def _pages_of(name, t, dims):
+    """A cache's K or V: its strides, the last dimension's apart."""
+    if t.dim() != dims or t.dtype not in _LOSS_DTYPES or (t.stride(-1) != 1 and t.shape[-1] > 1):
+        raise WsError(f"{name}: {'[layers, ' if dims == 5 else '['}pages, page_tokens, kv_heads, head_dim] float32 / bfloat16 device tensor, unit inner stride")
+    return t.stride()[:-1]
+
+
+def _cache_table(table, at):
+    if table.dim() != 2 or table.dtype is not _I32 or table.get_device() != at or (table.stride(1) != 1 and table.shape[1] > 1):
+        raise WsError("table: [slots, pages of a slot] int32 tensor with unit inner stride on the cache's device")
+    slots, wide = table.shape
+    return slots, wide, table.stride(0) if slots > 1 else wide
+
+
+def tree_attention(q, k, v, table, length, seq_off, mask=None, slot=None, scale=None, out=None, want_lse=False, max_nodes=0):
+    """Attention of trees' rows over one layer of a paged cache (ws_tree_attention). q: [rows, heads, head_dim] float32 / bfloat16; k, v: [pages, page_tokens, kv_heads, head_dim] of its dtype, the
+    dimensions in any order in memory but the last (page_tokens a power of two); table: int32 [slots, pages of a slot]; length: int32 [n_seq], the tokens of each sequence before its nodes, which
+    lie behind them in the cache; seq_off: as in tree_stage; mask: int64 [rows] (None: chains); slot: int32 [n_seq] (None: sequence s has slot s); scale: None = head_dim ** -0.5. One row a sequence: plain
+    decoding. max_nodes: the most nodes of a sequence, where the caller knows it. out: where to write (strides in multiples of 16 bytes); rows behind the last sequence are left as they are.
+    Returns out, or (out, lse float32 [rows, heads]) with want_lse."""
+    at = _device_of("q", q)
+    if q.dim() != 3 or q.dtype not in _LOSS_DTYPES or (q.stride(2) != 1 and q.shape[2] > 1):
+        raise WsError("q: [rows, heads, head_dim] float32 / bfloat16 device tensor, unit inner stride")
+    rows, heads, dim = q.shape
+    n_seq = _sequences(seq_off)
+    ks, vs = _pages_of("k", k, 4), _pages_of("v", v, 4)
+    if k.shape != v.shape or k.dtype is not q.dtype or v.dtype is not q.dtype or k.get_device() != at or v.get_device() != at or k.shape[3] != dim:
+        raise WsError("k, v: of one shape, of q's dtype and head_dim, on its device")
+    pages, page_tokens, kv_heads, _ = k.shape
+    slots, wide, table_stride = _cache_table(table, at)
+    if max(rows, n_seq, heads, pages, page_tokens, kv_heads, slots, wide) >= 1 << 31 or not 0 <= max_nodes < 1 << 31:
+        raise WsError("sizes beyond 31 bits")
+    if slot is None and n_seq > slots:
+        raise WsError(f"slot: missing, and {n_seq} sequences have {slots} slots")
+    if out is None:
+        # (where a caller has rows behind the last sequence, they are left as they are: zeros)
+        out = torch.empty((rows, heads, dim), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != at or (out.stride(2) != 1 and dim > 1):
+        raise WsError("out: of q's shape and dtype, on its device, unit inner stride")
+    else:
+        torch.autograd.graph.increment_version(out)
+    lse = torch.empty((rows, heads), dtype=_F32, device=q.device) if want_lse else None
+    a = TreeAttention(CacheLayer(k.data_ptr(), v.data_ptr(), _LOSS_DTYPES[q.dtype], pages, page_tokens, kv_heads, dim, *ks, *vs, table.data_ptr(), slots, wide, table_stride),
+                      n_seq, rows, heads, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), _p(lse), _vector("seq_off", seq_off, _I32, n_seq + 1, at),
+                      _vector("length", length, _I32, n_seq, at), _vector("slot", slot, _I32, n_seq, at), _vector("mask", mask, _I64, rows, at), dim ** -0.5 if scale is None else scale, max_nodes)
+    call, ref = lib(), C.byref(a)
+    need = call.ws_tree_attention_workspace(ref)
+    work = torch.empty(need, dtype=torch.uint8, device=q.device)
+    check(call.ws_tree_attention(_stream(), ref, work.data_ptr(), need), "ws_tree_attention")
+    return (out, lse) if want_lse else out
+
+
+class PagedCache:
+    """A paged cache of all layers and its allocator's state, on the device (ws_cache): k, v [layers, pages, page_tokens, kv_heads, head_dim] float32 / bfloat16, table int32 [slots, pages of a
+    slot], held int32 [slots], refs int32 [pages], free int32 [pages], n_free int32 [1]. Position p of slot s is token p % page_tokens of page table[s, p // page_tokens]. The calls below change
+    these in the order of the stream and wait for nothing; status int32 [n]: CACHE_OK, CACHE_FULL (too few pages: nothing was done) or CACHE_BAD. At most 1024 slots a call; lists are int32 device tensors."""
+
+    def __init__(self, k, v, table, held, refs, free, n_free):
+        at = _device_of("k", k)
+        ks, vs = _pages_of("k", k, 5), _pages_of("v", v, 5)
+        if k.shape != v.shape or k.dtype is not v.dtype or v.get_device() != at:
+            raise WsError("k, v: of one shape and dtype, on one device")
+        layers, pages, page_tokens, kv_heads, dim = k.shape
+        slots, wide, table_stride = _cache_table(table, at)
+        if max(layers, pages, page_tokens, kv_heads, dim, slots, wide) >= 1 << 31:
+            raise WsError("sizes beyond 31 bits")
+        self.k, self.v, self.table, self.held, self.refs, self.free, self.n_free = k, v, table, held, refs, free, n_free
+        self.page_tokens, self.at = page_tokens, at
+        self.desc = Cache(k.data_ptr(), v.data_ptr(), _LOSS_DTYPES[k.dtype], layers, pages, page_tokens, kv_heads, dim, *ks, *vs, table.data_ptr(), slots, wide, table_stride,
+                          _vector("held", held, _I32, slots, at), _vector("refs", refs, _I32, pages, at), _vector("free", free, _I32, pages, at), _vector("n_free", n_free, _I32, 1, at))
+
+    @classmethod
+    def empty(cls, layers, pages, page_tokens, kv_heads, head_dim, slots, slot_pages, dtype=torch.bfloat16, device="cuda:0"):
+        """One that holds nothing, all pages free (page 0 is the first to be taken)."""
+        k, v = (torch.zeros((layers, pages, page_tokens, kv_heads, head_dim), dtype=dtype, device=device) for _ in range(2))
+        return cls(k, v, torch.full((slots, slot_pages), -1, dtype=_I32, device=device), torch.zeros(slots, dtype=_I32, device=device), torch.zeros(pages, dtype=_I32, device=device),
+                   torch.arange(pages - 1, -1, -1, dtype=_I32, device=device), torch.full((1,), pages, dtype=_I32, device=device))
+
+    def _lists(self, *named):
+        n = named[0][1].numel()
+        if n > CACHE_MOST:
+            raise WsError(f"{named[0][0]}: {n} slots, at most {CACHE_MOST} a call")
+        if self.at != torch._C._cuda_getDevice():
+            raise WsError(f"the cache is on cuda:{self.at}, which is not the current device")
+        return n, [_vector(name, _given(name, t), _I32, n, self.at) for name, t in named]
+
+    def reserve(self, slot, tokens):
+        """Pages for tokens[i] tokens in all for slot[i] (ws_cache_reserve). Returns status."""
+        n, at = self._lists(("slot", slot), ("tokens", tokens))
+        status = torch.empty(n, dtype=_I32, device=slot.device)
+        check(lib().ws_cache_reserve(_stream(), C.byref(self.desc), *at, n, status.data_ptr()), "ws_cache_reserve")
+        return status
+
+    def fork(self, src, dst, length):
+        """The empty slot dst[i] becomes a copy of the first length[i] tokens of slot src[i]: whole pages shared, the last, partly filled one copied (ws_cache_fork). Returns status."""
+        n, at = self._lists(("src", src), ("dst", dst), ("length", length))
+        status = torch.empty(n, dtype=_I32, device=src.device)
+        check(lib().ws_cache_fork(_stream(), C.byref(self.desc), *at, n, status.data_ptr()), "ws_cache_fork")
+        return status
+
+    def release(self, slot, tokens):
+        """Slot slot[i] keeps the pages of its first tokens[i] tokens, the others go back (ws_cache_release). Returns status."""
+        n, at = self._lists(("slot", slot), ("tokens", tokens))
+        status = torch.empty(n, dtype=_I32, device=slot.device)
+        check(lib().ws_cache_release(_stream(), C.byref(self.desc), *at, n, status.data_ptr()), "ws_cache_release")
+        return status
+
+    def keep(self, path, n_accepted, length, slot=None):
+        """After verify_tree: the accepted nodes' keys and values, of all layers, move behind the root, where the text goes on (ws_cache_keep). path, n_accepted: verify_tree's; length: int32
+        [n_seq], the tokens before the root (tree_stage's); slot: int32 [n_seq] (None: sequence s has slot s)."""
+        n_seq = n_accepted.numel()
+        if path.dim() != 2 or path.shape[0] != n_seq or not 1 <= path.shape[1] <= TREE_MAX or n_seq > _MOST_ROWS:
+            raise WsError(f"path: [n_seq, 1 .. {TREE_MAX}] for the n_seq of n_accepted")
+        if self.at != torch._C._cuda_getDevice():
+            raise WsError(f"the cache is on cuda:{self.at}, which is not the current device")
+        check(lib().ws_cache_keep(_stream(), C.byref(self.desc), _vector("path", path, _I32, path.numel(), self.at), path.shape[1], _vector("n_accepted", n_accepted, _I32, n_seq, self.at),
+                                  _vector("length", length, _I32, n_seq, self.at), _vector("slot", slot, _I32, n_seq, self.at), n_seq), "ws_cache_keep")
+
+    def attention(self, layer, q, length, seq_off, **more):
+        """tree_attention over one layer."""
+        return tree_attention(q, self.k[layer], self.v[layer], self.table, length, seq_off, **more)
 
 
 # ---------------------------------------------------------------------------------------------------------------------

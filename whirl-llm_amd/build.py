@@ -24,6 +24,9 @@ SRC_FEW = os.path.join(HERE, "csrc", "ws_few.hip")  # short-list rows shared bet
 SRC_TOP = os.path.join(HERE, "csrc", "ws_top.hip")  # top-k lists and draft draws of few rows, shared the same way
 SRC_LEAN = os.path.join(HERE, "csrc", "ws_lean.hip")  # the lean single-sweep kernel for batches of unsplit rows
 SRC_LOSS = os.path.join(HERE, "csrc", "ws_loss.hip")  # log-probabilities, losses over them and their gradients
+SRC_TREE = os.path.join(HERE, "csrc", "ws_tree.hip")  # trees of drafts: what their rows see, and their verification
+SRC_ATTEND = os.path.join(HERE, "csrc", "ws_attend.hip")  # attention of their rows over a paged cache
+SRC_CACHE = os.path.join(HERE, "csrc", "ws_cache.hip")  # that cache's pages
 # packed FP32 instructions are switched off for every device compile of this repository
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
          # the fused sweep is one fully unrolled loop of ~20 batches (its bin cache must stay in registers)
@@ -52,7 +55,7 @@ def build(verbose=True):
     # the translation units and the bare code object side by side (each takes a minute or two), then the link
     objdir = os.path.join(HERE, "csrc", "obj")
     os.makedirs(objdir, exist_ok=True)
-    srcs = (SRC_LEAN, SRC_FEW, SRC, SRC_FUSED_SHORT, SRC_CODE, SRC_FUSED, SRC_SPLIT, *SRC_KEPT, SRC_SHORT, SRC_TWIN, SRC_TOP, SRC_LOSS)  # the longest first
+    srcs = (SRC_LEAN, SRC_FEW, SRC, SRC_FUSED_SHORT, SRC_CODE, SRC_FUSED, SRC_SPLIT, *SRC_KEPT, SRC_SHORT, SRC_TWIN, SRC_TOP, SRC_LOSS, SRC_TREE, SRC_ATTEND, SRC_CACHE)  # the longest first
     objs = [os.path.join(objdir, os.path.basename(src)[:-4] + ".o") for src in srcs]
     jobs = [[hipcc, *FLAGS, "-fPIC", "-c", "-o", obj, src] for obj, src in zip(objs, srcs)]
     jobs.append([hipcc, *FLAGS, "--genco", "-o", co, SRC])

@@ -11,6 +11,7 @@
 #include "ws_accept.h"
 #include "ws_adjust.h"
 #include "ws_common.h"
+#include "ws_cycle.h"
 #include "ws_draft.h"
 #include "ws_loss.h"
 #include "ws_pick.h"
@@ -524,6 +525,9 @@ int prepare_all() {
     if (const int e = ws::prepare_few(kMaxLds - kStaticFew); e != 0) return e;
     if (const int e = ws::prepare_top(); e != 0) return e;
     if (const int e = ws::prepare_loss(); e != 0) return e;
+    if (const int e = ws::prepare_tree(); e != 0) return e;
+    if (const int e = ws::prepare_attend(); e != 0) return e;
+    if (const int e = ws::prepare_cache(); e != 0) return e;
     return ws::prepare_short(kMaxLds - kStaticShort);
 }
 
@@ -1308,6 +1312,207 @@ int ws_preference_loss(void* stream, const ws_preference* p, void* workspace, ui
     a.meet = static_cast<unsigned long long*>(workspace);
     a.tag = launch_tag();
     return ws::launch_preference(S(stream), a, preference_groups(p->pairs));
+}
+
+// ---- a cycle whose drafts form a tree
+
+namespace {
+constexpr uint32_t kMostTrees = 1048575u;
+static_assert(WS_TREE_MAX == ws::kTreeNodes && WS_Q_MAX == ws::kTreeListed && WS_Q_WORDS == ws::kTreeEntryWords);
+static_assert(WS_CACHE_MOST == ws::kCacheMost && WS_CACHE_MOST == WS_BLOCK);
+
+// Workgroups a sequence of the verification: two a compute unit where sequences are few, of 256 vectors at least; as many as hold the row in registers
+uint32_t verify_parts(const ws_loss_rows* r, uint32_t n_seq) {
+    const uint32_t per = r->dtype == WS_DTYPE_F32 ? 4u : 8u, vectors = (r->vocab + per - 1u) / per, least = (vectors + ws::tree_most_share() - 1u) / ws::tree_most_share();
+    uint32_t parts = n_seq ? 2u * static_cast<uint32_t>(compute_units()) / n_seq : 1u;
+    if (parts > vectors / 256u) parts = vectors / 256u;
+    if (parts < least) parts = least;
+    return parts < 1u ? 1u : (parts > 64u ? 64u : parts);
+}
+bool verify_ok(const ws_loss_rows* r, const ws_verify_tree_args* a) {
+    if (!loss_rows_ok(r) || !a || a->n_seq > kMostTrees || a->depth < 1u || a->depth > WS_TREE_MAX || a->spins > kMostLooks) return false;
+    if (a->n_seq == 0u) return true;
+    if (r->rows && (!r->ids || !a->u_accept || (a->q && !a->q_off))) return false;
+    if (!a->seq_off || !a->u_draw || !a->n_accepted || !a->path || !a->chosen || !a->status) return false;
+    return !a->hist.tokens || a->hist.len;
+}
+
+// strides of 16 bytes and more, at 16-byte addresses, that the GPU's 64 bits hold
+bool strides_ok(const void* at, uint32_t each, std::initializer_list<std::pair<uint64_t, uint64_t>> dims) {
+    if (!aligned(at, 16u)) return false;
+    unsigned __int128 end = 0;
+    for (const auto& [count, stride] : dims) {
+        if (count > 1u && stride * each % 16u != 0u) return false;
+        if (count) end += static_cast<unsigned __int128>(count - 1u) * stride * each;
+    }
+    return end < (static_cast<unsigned __int128>(1) << 62);
+}
+bool page_shape_ok(int32_t dtype, uint32_t pages, uint32_t page_tokens, uint32_t kv_heads, uint32_t head_dim, uint32_t slots, uint32_t slot_pages, uint64_t table_stride) {
+    if (dtype != WS_DTYPE_F32 && dtype != WS_DTYPE_BF16) return false;
+    if (pages == 0 || pages > (1u << 30) || page_tokens == 0 || page_tokens > (1u << 20) || (page_tokens & (page_tokens - 1u)) != 0 || kv_heads == 0 || kv_heads > 65535u) return false;
+    if (head_dim == 0 || head_dim % 8u != 0 || slots == 0 || slots > (1u << 30) || slot_pages == 0 || slot_pages >= (1u << 20)) return false;
+    return static_cast<uint64_t>(slot_pages) * page_tokens < (1ull << 31) && table_stride >= slot_pages;
+}
+uint32_t shift_of(uint32_t power) { return static_cast<uint32_t>(__builtin_ctz(power)); }
+
+bool attention_ok(const ws_tree_attention_args* a) {
+    if (!a) return false;
+    const ws_cache_layer& c = a->cache;
+    if (!page_shape_ok(c.dtype, c.pages, c.page_tokens, c.kv_heads, c.head_dim, c.slots, c.slot_pages, c.table_stride) || c.head_dim > 256u) return false;
+    if (a->heads == 0 || a->heads > 65535u || a->heads % c.kv_heads != 0 || a->n_seq > kMostTrees || a->rows > kMostTrees) return false;
+    if (!(a->scale > 0.f) || a->scale > 1e30f) return false;
+    return true;
+}
+// columns of a tile that the build is chosen by: those of the largest sequence, or of one as large as they are on average
+uint32_t attention_cols(const ws_tree_attention_args* a) {
+    uint32_t nodes = a->max_nodes ? a->max_nodes : (a->n_seq ? (a->rows + a->n_seq - 1u) / a->n_seq : 1u);
+    nodes = nodes < 1u ? 1u : (nodes > WS_TREE_MAX ? WS_TREE_MAX : nodes);
+    return nodes * (a->heads / a->cache.kv_heads);
+}
+ws::AttendPlan attention_plan(const ws_tree_attention_args* a) {
+    return ws::attend_plan(a->cache.dtype, a->cache.head_dim, attention_cols(a), static_cast<uint32_t>(compute_units() > 0 ? compute_units() : 256));
+}
+
+bool cache_ok(const ws_cache* c) {
+    if (!c || !page_shape_ok(c->dtype, c->pages, c->page_tokens, c->kv_heads, c->head_dim, c->slots, c->slot_pages, c->table_stride)) return false;
+    if (c->layers == 0 || c->layers > 65535u || !c->k || !c->v || !c->table || !c->held || !c->refs || !c->free || !c->n_free) return false;
+    const uint32_t e = static_cast<uint32_t>(elem_bytes(c->dtype));
+    return strides_ok(c->k, e, {{c->layers, c->k_layer}, {c->pages, c->k_page}, {c->page_tokens, c->k_token}, {c->kv_heads, c->k_head}}) &&
+           strides_ok(c->v, e, {{c->layers, c->v_layer}, {c->pages, c->v_page}, {c->page_tokens, c->v_token}, {c->kv_heads, c->v_head}});
+}
+ws::CacheRef cache_ref(const ws_cache* c) {
+    const uint64_t e = elem_bytes(c->dtype);
+    ws::CacheRef r{};
+    r.side[0] = ws::CacheSide{static_cast<unsigned char*>(c->k), c->k_layer * e, c->k_page * e, c->k_token * e, c->k_head * e};
+    r.side[1] = ws::CacheSide{static_cast<unsigned char*>(c->v), c->v_layer * e, c->v_page * e, c->v_token * e, c->v_head * e};
+    r.layers = c->layers;
+    r.pages = c->pages;
+    r.page_shift = shift_of(c->page_tokens);
+    r.kv_heads = c->kv_heads;
+    r.head_bytes = static_cast<uint32_t>(c->head_dim * e);
+    r.table = c->table;
+    r.slots = c->slots;
+    r.slot_pages = c->slot_pages;
+    r.table_stride = c->table_stride;
+    r.held = c->held;
+    r.refs = c->refs;
+    r.free = c->free;
+    r.n_free = c->n_free;
+    return r;
+}
+}  // namespace
+
+int ws_tree_stage(void* stream, const ws_tree_stage_args* a) {
+    if (!a || a->n_seq > kMostTrees || a->rows > kMostTrees || (a->n_seq && !a->seq_off)) return WS_E_INVALID;
+    if (a->mask && !aligned(a->mask, 8u)) return WS_E_INVALID;
+    if (a->n_seq == 0) return WS_OK;
+    return ws::launch_tree_stage(S(stream), ws::TreeStageArgs{a->n_seq, a->rows, a->seq_off, a->parent, a->len, a->slot, a->mask, a->position, a->length});
+}
+
+uint64_t ws_verify_tree_workspace(const ws_loss_rows* r, const ws_verify_tree_args* a) {
+    return verify_ok(r, a) && a->n_seq ? meet_bytes(a->n_seq, verify_parts(r, a->n_seq), ws::kTreeWords) : 0u;
+}
+
+int ws_verify_tree(void* stream, const ws_loss_rows* r, const ws_verify_tree_args* a, void* workspace, uint64_t workspace_bytes) {
+    if (!verify_ok(r, a)) return WS_E_INVALID;
+    if (a->n_seq == 0) return WS_OK;
+    if (!workspace_ok(workspace, workspace_bytes, ws_verify_tree_workspace(r, a))) return WS_E_WORKSPACE;
+    ws::TreeVerifyArgs v{};
+    v.R = loss_rows(r);
+    v.n_seq = a->n_seq;
+    v.seq_off = a->seq_off;
+    v.parent = a->parent;
+    v.q = a->q;
+    v.q_words = a->q_words;
+    v.q_off = a->q_off;
+    v.u_accept = a->u_accept;
+    v.u_draw = a->u_draw;
+    v.depth = a->depth;
+    v.n_accepted = a->n_accepted;
+    v.path = a->path;
+    v.chosen = a->chosen;
+    v.status = a->status;
+    v.logprob = a->logprob;
+    v.hist = ws::HistoryRef{a->hist.tokens, a->hist.len, a->hist.n_gen, a->hist.slot, a->hist.cap};
+    const uint32_t per = r->dtype == WS_DTYPE_F32 ? 4u : 8u;
+    v.parts = verify_parts(r, a->n_seq);
+    v.per = share_of((r->vocab + per - 1u) / per, v.parts);
+    v.looks = a->spins ? a->spins : 256u;
+    v.meet = static_cast<unsigned long long*>(workspace);
+    v.tag = launch_tag();
+    return ws::launch_tree_verify(S(stream), r->dtype, v);
+}
+
+uint64_t ws_tree_attention_workspace(const ws_tree_attention_args* a) { return attention_ok(a) && a->n_seq && a->rows ? attention_plan(a).bytes : 0u; }
+
+int ws_tree_attention(void* stream, const ws_tree_attention_args* a, void* workspace, uint64_t workspace_bytes) {
+    if (!attention_ok(a)) return WS_E_INVALID;
+    if (a->n_seq == 0 || a->rows == 0) return WS_OK;
+    const ws_cache_layer& c = a->cache;
+    const uint32_t e = static_cast<uint32_t>(elem_bytes(c.dtype));
+    if (!a->q || !a->out || !a->seq_off || !a->length || !c.k || !c.v || !c.table || (a->mask && !aligned(a->mask, 8u))) return WS_E_INVALID;
+    if (!strides_ok(a->q, e, {{a->rows, a->q_row}, {a->heads, a->q_head}}) || !strides_ok(a->out, e, {{a->rows, a->out_row}, {a->heads, a->out_head}})) return WS_E_INVALID;
+    if (!strides_ok(c.k, e, {{c.pages, c.k_page}, {c.page_tokens, c.k_token}, {c.kv_heads, c.k_head}}) ||
+        !strides_ok(c.v, e, {{c.pages, c.v_page}, {c.page_tokens, c.v_token}, {c.kv_heads, c.v_head}}))
+        return WS_E_INVALID;
+    const ws::AttendPlan plan = attention_plan(a);
+    if (!workspace || workspace_bytes < plan.bytes || !aligned(workspace, 16u)) return WS_E_WORKSPACE;
+    ws::AttendArgs g{};
+    g.k = static_cast<const unsigned char*>(c.k);
+    g.v = static_cast<const unsigned char*>(c.v);
+    g.k_page = c.k_page * e, g.k_token = c.k_token * e, g.k_head = c.k_head * e;
+    g.v_page = c.v_page * e, g.v_token = c.v_token * e, g.v_head = c.v_head * e;
+    g.pages = c.pages;
+    g.page_shift = shift_of(c.page_tokens);
+    g.kv_heads = c.kv_heads;
+    g.head_dim = c.head_dim;
+    g.table = c.table;
+    g.slots = c.slots;
+    g.slot_pages = c.slot_pages;
+    g.table_stride = c.table_stride;
+    g.n_seq = a->n_seq;
+    g.rows = a->rows;
+    g.heads = a->heads;
+    g.group = a->heads / c.kv_heads;
+    g.q = static_cast<const unsigned char*>(a->q);
+    g.q_row = a->q_row * e, g.q_head = a->q_head * e;
+    g.out = static_cast<unsigned char*>(a->out);
+    g.out_row = a->out_row * e, g.out_head = a->out_head * e;
+    g.lse = a->lse;
+    g.seq_off = a->seq_off;
+    g.length = a->length;
+    g.slot = a->slot;
+    g.mask = a->mask;
+    g.scale_log2 = static_cast<float>(static_cast<double>(a->scale) * 1.4426950408889634074);
+    g.groups = plan.groups;
+    g.least = plan.least;
+    g.part = static_cast<float*>(workspace);
+    g.run = reinterpret_cast<ws::AttendRun*>(static_cast<unsigned char*>(workspace) + plan.part_bytes);
+    return ws::launch_attend(S(stream), plan, g);
+}
+
+int ws_cache_reserve(void* stream, const ws_cache* c, const int32_t* slot, const int32_t* tokens, uint32_t n, int32_t* status) {
+    if (!cache_ok(c) || n > WS_CACHE_MOST || (n && (!slot || !tokens || !status))) return WS_E_INVALID;
+    if (n == 0) return WS_OK;
+    return ws::launch_cache_reserve(S(stream), ws::PagesArgs{cache_ref(c), slot, nullptr, tokens, n, status});
+}
+
+int ws_cache_fork(void* stream, const ws_cache* c, const int32_t* src, const int32_t* dst, const int32_t* length, uint32_t n, int32_t* status) {
+    if (!cache_ok(c) || n > WS_CACHE_MOST || (n && (!src || !dst || !length || !status))) return WS_E_INVALID;
+    if (n == 0) return WS_OK;
+    return ws::launch_cache_fork(S(stream), ws::PagesArgs{cache_ref(c), dst, src, length, n, status});
+}
+
+int ws_cache_release(void* stream, const ws_cache* c, const int32_t* slot, const int32_t* tokens, uint32_t n, int32_t* status) {
+    if (!cache_ok(c) || n > WS_CACHE_MOST || (n && (!slot || !tokens))) return WS_E_INVALID;
+    if (n == 0) return WS_OK;
+    return ws::launch_cache_release(S(stream), ws::PagesArgs{cache_ref(c), slot, nullptr, tokens, n, status});
+}
+
+int ws_cache_keep(void* stream, const ws_cache* c, const int32_t* path, uint32_t depth, const int32_t* n_accepted, const uint32_t* length, const uint32_t* slot, uint32_t n_seq) {
+    if (!cache_ok(c) || n_seq > kMostTrees || depth < 1u || depth > WS_TREE_MAX || (n_seq && (!path || !n_accepted || !length))) return WS_E_INVALID;
+    if (n_seq == 0) return WS_OK;
+    return ws::launch_cache_keep(S(stream), ws::KeepArgs{cache_ref(c), path, depth, n_accepted, length, slot, n_seq});
 }
 
 }  // extern "C"

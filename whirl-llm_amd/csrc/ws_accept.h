@@ -15,18 +15,9 @@
 #include <stdint.h>
 
 #include "ws_common.h"
+#include "ws_history.h"
 
 namespace ws {
-
-// A sequence's text on the device: tokens[base .. base + len) are what the model holds, tokens[base + len] is the token
-// that goes in next, behind it the drafts of the running cycle (placed there by history_stage_kernel).
-struct HistoryRef {
-    int32_t* tokens;        // nullptr: no device history
-    uint32_t* len;          // per slot
-    uint64_t* n_gen;        // per slot or nullptr: output tokens so far
-    const uint32_t* slot;   // per sequence: its slot
-    uint32_t cap;           // tokens per slot
-};
 
 // Would the text made of the last `window` tokens of hist[0, n_hist) and then tail[0, n_tail) end in an n-gram it
 // already contains (relax::extendsRepeat, include/whirl/relax_accept.h:72-92)? hist and tail lie one behind the other
@@ -65,8 +56,6 @@ struct AcceptArgs {
     uint32_t* relaxed;      // per sequence, incremented: drafts kept by the typical rule
     HistoryRef hist;
 };
-
-constexpr uint32_t kAcceptHost = 1u, kAcceptNearTypical = 2u, kAcceptHistoryFull = 4u;
 
 // what was accepted goes behind the sequence's text: next, the kept drafts; the chosen token becomes the new `next`
 __device__ __forceinline__ bool history_append(const HistoryRef& h, uint32_t seq, const int32_t* c, int32_t acc, int32_t chosen) {

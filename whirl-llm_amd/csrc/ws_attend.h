@@ -1,0 +1,677 @@
+// Attention of the rows of trees over a paged cache: out_r = sum_t p_rt v_t, p = softmax of scale q_r . k_t over the positions t that row r sees.
+//
+// The rows of a sequence that read the same kv head - its nodes times the heads of a group - are the columns of S^T = K Q^T and of O^T = V^T P^T, both products on the matrix cores with
+// sums in 32 bits. So a column's softmax lies in the lanes that hold it: its maximum and sum never cross to other lanes but where a maximum grows, and P^T is the
+// second product's operand where the first one leaves it. Of V a lane takes 8 tokens' neighbouring elements, which two permutes a pair of tokens turn into 8 tokens of an element.
+//
+// One pass: a column keeps its maximum, sum and O^T; powers are of base two, and a column is scaled down only when its maximum has grown by more than kSlack (powers then
+// reach 2^kSlack, which 32 bits hold as exactly). A wave works on 32 positions at a time. Few columns (WM = 1): the four waves of a workgroup take different positions, K and V go from memory
+// into the registers of their operands. Many (WM = 4): the waves take different columns of the same positions, K and V go through LDS, the next ones' on their way in registers meanwhile.
+//
+// Work: units of kUnit positions of a sequence, a kv head and a tile of columns, numbered through; the workgroups share them evenly, whatever the sequences' lengths, each a run of neighbours.
+// A run that does not hold all units of a tile leaves maximum, sum and O^T in the workspace, and attend_join_kernel joins them. Memory bounds it where there are few columns,
+// from some hundred on the matrix cores and the powers.
+#pragma once
+
+#include "ws_common.h"
+#include "ws_cycle.h"
+
+#include <float.h>
+
+#include <type_traits>
+
+namespace ws {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr uint32_t kUnit = 128u, kAttendThreads = 256u;
+constexpr float kSlack = 8.f;
+
+// a type's operands and their products
+template <int DT>
+struct Mat;
+template <>
+struct Mat<1> {  // bf16
+    static constexpr uint32_t kBytes = 2u, kPer = 8u, kDepth = 32u;  // elements of a 16-byte load, depth of a product
+    typedef bf16x8 Frag;
+    static __device__ __forceinline__ f32x4 mul(const uint4& a, const uint4& b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    // eight tokens' element e, in a word each, times their powers
+    static __device__ __forceinline__ f32x4 mul_tokens(const uint32_t (&word)[8], uint32_t e, const uint4 (&p)[1], f32x4 c) {
+        const uint32_t half = e % 2u ? 0x07060302u : 0x05040100u;
+        return mul(make_uint4(__builtin_amdgcn_perm(word[1], word[0], half), __builtin_amdgcn_perm(word[3], word[2], half), __builtin_amdgcn_perm(word[5], word[4], half),
+                              __builtin_amdgcn_perm(word[7], word[6], half)), p[0], c);
+    }
+    // all bits of the elements of a word that are infinities or NaN: an exponent of ones and one more carry into the sign's place
+    static __device__ __forceinline__ uint32_t special(uint32_t w) {
+        const uint32_t f = ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+        return (f - (f >> 15)) | f;
+    }
+    static __device__ __forceinline__ float element(const unsigned char* at, uint32_t i) { return bf16_to_f32(reinterpret_cast<const uint16_t*>(at)[i]); }
+};
+template <>
+struct Mat<0> {  // fp32: four products of depth 4, lane group g's i-th element in the i-th
+    static constexpr uint32_t kBytes = 4u, kPer = 4u, kDepth = 16u;
+    static __device__ __forceinline__ f32x4 mul(const uint4& a, const uint4& b, f32x4 c) {
+        const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x[i]), __uint_as_float(y[i]), c, 0, 0, 0);
+        return c;
+    }
+    static __device__ __forceinline__ f32x4 mul_tokens(const uint32_t (&word)[8], uint32_t, const uint4 (&p)[2], f32x4 c) {
+        c = mul(make_uint4(word[0], word[1], word[2], word[3]), p[0], c);
+        return mul(make_uint4(word[4], word[5], word[6], word[7]), p[1], c);
+    }
+    static __device__ __forceinline__ uint32_t special(uint32_t w) {
+        const uint32_t f = ((w & 0x7f800000u) + 0x00800000u) & 0x80000000u;
+        return (f - (f >> 31)) | f;
+    }
+    static __device__ __forceinline__ float element(const unsigned char* at, uint32_t i) { return reinterpret_cast<const float*>(at)[i]; }
+};
+
+// A build: DT, DP (head_dim rounded up to 64, 128 or 256), MS tiles of 16 columns a wave, WM waves over columns (4 / WM over positions)
+template <int DT, int DP, int MS, int WM>
+struct AttendShape {
+    static constexpr uint32_t kTileCols = 16u * MS * WM;
+    static constexpr uint32_t kEach = DT == 1 && DP >= 128 ? 8u : 4u;  // elements of V a lane loads together: a lane holds elements kEach c + e of a block of 16 kEach
+    static constexpr uint32_t kBlocks = DP / (16u * kEach);
+    static constexpr uint32_t kOuts = kBlocks * kEach;                 // products' results that make up O^T of 16 columns, 4 floats a lane each
+    static constexpr uint32_t kChunks = DP / Mat<DT>::kDepth;
+    static constexpr uint32_t kSubFloats = 64u * (4u * kOuts + 2u);    // of 16 columns in the workspace: maximum and sum, O^T, as the lanes hold them
+    static constexpr uint32_t kPartFloats = MS * WM * kSubFloats;
+    // through LDS: tokens at a time, bytes of one, its 16-byte pieces, those of a thread
+    static constexpr uint32_t kRow = DP * Mat<DT>::kBytes, kTokens = kRow <= 256u ? 64u : 32u, kPieces = kRow / 16u, kMine = kTokens * kPieces / 256u;
+    static constexpr uint32_t kBuffer = kTokens * kRow;
+    // A token's pieces lie in another order for each of 16 neighbours, so that a piece of all of them, which K's operand takes together, lies in different banks.
+    static __device__ __forceinline__ uint32_t place(uint32_t token, uint32_t piece) { return token * kRow + (piece ^ (kPieces == 8u ? token >> 1 & 7u : token & 15u)) * 16u; }
+};
+
+// which of four positions from `pos` on a row sees: those before `length` and the nodes behind, by its bits. (A select a position, position < length ? true : bit, has been compiled
+// to the bit alone.)
+__device__ __forceinline__ uint32_t sees_four(uint64_t sees, uint32_t pos, uint32_t length) {
+    const int32_t behind = static_cast<int32_t>(pos) - static_cast<int32_t>(length);  // (both below 2^31)
+    const uint32_t before = static_cast<uint32_t>(min(max(-behind, 0), 4));           // of the four
+    const uint32_t nodes = behind >= 0 ? (behind < 64 ? static_cast<uint32_t>(sees >> behind) : 0u) : static_cast<uint32_t>(sees) << before;
+    return ((1u << before) - 1u) | (nodes & 15u);
+}
+
+struct AttendWork {  // a sequence's
+    uint32_t first, nodes, total, length, tiles, units;  // row, nodes, positions, those before the nodes, tiles of columns, units of a tile
+    uint64_t all;                                        // units of all heads and tiles
+};
+__device__ __forceinline__ AttendWork attend_work(const AttendArgs& A, uint32_t s, uint32_t cols) {
+    AttendWork w;
+    const uint32_t a = min(A.seq_off[s], A.rows), b = min(A.seq_off[s + 1u], A.rows);
+    w.first = a;
+    w.nodes = b > a ? min(b - a, kTreeNodes) : 0u;
+    const uint64_t room = static_cast<uint64_t>(A.slot_pages) << A.page_shift;  // (below 2^31)
+    w.length = A.length[s];
+    w.total = static_cast<uint32_t>(min(static_cast<uint64_t>(w.length) + w.nodes, room));
+    w.tiles = (w.nodes * A.group + cols - 1u) / cols;
+    w.units = max((w.total + kUnit - 1u) / kUnit, 1u);
+    w.all = static_cast<uint64_t>(w.tiles) * A.kv_heads * w.units;
+    return w;
+}
+
+// exclusive prefix over the workgroup's 256 threads
+__device__ __forceinline__ uint64_t scan256(uint64_t v, uint64_t* red, uint64_t& total) {
+    const uint64_t inc = wave_incl_scan(v);
+    __syncthreads();
+    if (lane_id() == 63) red[wave_id()] = inc;
+    __syncthreads();
+    uint64_t base = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const uint64_t x = red[w];
+        if (w < wave_id()) base += x;
+        total += x;
+    }
+    return base + inc - v;
+}
+
+struct AttendFind {
+    uint64_t red[4];
+    uint64_t all;       // units of all sequences
+    uint64_t seq_first;  // the first unit of `seq`
+    uint32_t seq;
+};
+// the sequence that holds unit `at`(all sequences' units are added up on the way where `sum`)
+__device__ __forceinline__ void attend_sum(const AttendArgs& A, uint32_t cols, AttendFind& F) {
+    uint64_t sum = 0;
+    for (uint32_t s = threadIdx.x; s < A.n_seq; s += kAttendThreads) sum += attend_work(A, s, cols).all;
+    uint64_t total;
+    scan256(sum, F.red, total);
+    if (threadIdx.x == 0u) F.all = total;
+    __syncthreads();
+}
+__device__ __forceinline__ void attend_find(const AttendArgs& A, uint32_t cols, AttendFind& F, uint64_t at) {
+    uint64_t base = 0;
+    for (uint32_t s0 = 0; s0 < A.n_seq; s0 += kAttendThreads) {
+        const uint32_t s = s0 + threadIdx.x;
+        const uint64_t mine = s < A.n_seq ? attend_work(A, s, cols).all : 0u;
+        uint64_t total;
+        const uint64_t before = base + scan256(mine, F.red, total);
+        if (mine && at >= before && at - before < mine) {
+            F.seq = s;
+            F.seq_first = before;
+        }
+        base += total;
+        if (at < base) break;  // (uniform)
+    }
+    __syncthreads();
+}
+
+// What the products leave out: infinities and NaN in the V of nodes, which must not reach the rows that do not see them (0 times NaN is NaN). Rare, so it is done where a column is
+// written: element d of each such node that the column sees is added to it (an infinity to whatever the others have made: the same sum).
+template <int DT>
+__device__ __forceinline__ float attend_odd(const AttendArgs& A, const unsigned char* v_token, uint32_t d, bool sees) {
+    const float x = d < A.head_dim ? Mat<DT>::element(v_token, d) : 0.f;
+    return sees && !(fabsf(x) <= FLT_MAX) ? x : 0.f;
+}
+
+// the page of a position of the slot whose table row this is; `pages` where there is none
+__device__ __forceinline__ uint32_t attend_page(const AttendArgs& A, const int32_t* row, uint32_t pos) {
+    const uint32_t at = pos >> A.page_shift;
+    const uint32_t page = at < A.slot_pages ? static_cast<uint32_t>(row[at]) : A.pages;
+    return min(page, A.pages);
+}
+
+template <int DT, int DP, int MS, int WM, int OCC>
+__global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
+    typedef AttendShape<DT, DP, MS, WM> H;
+    constexpr uint32_t kWT = 4u / WM, kOuts = H::kOuts, kEach = H::kEach, kBlocks = H::kBlocks, kChunks = H::kChunks, E = Mat<DT>::kBytes;
+    constexpr uint32_t kDump = 4u * kOuts * 64u;  // floats of 16 columns' O^T
+    constexpr bool kStaged = WM > 1;
+    static_assert(WM == 1 || WM == 4);
+    __shared__ AttendFind F;
+    __shared__ uint32_t s_odd;
+    __shared__ float s_part[kWT > 1u ? (kWT / 2u) * MS * (kDump + 128u) : 1u];
+    __shared__ uint4 s_kv[kStaged ? 2u * 2u * H::kBuffer / 16u : 1u];  // two buffers of K, then V
+    __shared__ uint8_t s_here[kStaged ? 2u * H::kTokens : 1u];         // whether a token is there
+    const uint32_t t = threadIdx.x, lane = lane_id(), c = lane & 15u, g = lane >> 4, wave = wave_id(), wm = wave % WM, wt = wave / WM;
+
+    attend_sum(A, H::kTileCols, F);
+    const uint64_t per = max((F.all + A.groups - 1u) / A.groups, static_cast<uint64_t>(A.least));
+    // (neighbouring runs on the same part of the chip: workgroup b runs on XCD b % 8)
+    const uint32_t in_xcd = A.groups / 8u, run_id = blockIdx.x < in_xcd * 8u ? (blockIdx.x & 7u) * in_xcd + (blockIdx.x >> 3) : blockIdx.x;
+    const uint64_t begin = min(per * run_id, F.all), end = min(begin + per, F.all);
+    uint32_t run_odd = 0u;  // (the first thread's)
+    if (t == 0u) A.run[run_id].more = 0u;
+    if (t == 0u) s_odd = 0u;
+    if (begin >= end) return;
+    attend_find(A, H::kTileCols, F, begin);
+    uint32_t s = F.seq;
+    uint64_t seq_first = F.seq_first;
+    AttendWork W = attend_work(A, s, H::kTileCols);
+
+    for (uint64_t at = begin; at < end;) {
+        while (at - seq_first >= W.all) {
+            seq_first += W.all;
+            ++s;  // (there is one: at < all)
+            W = attend_work(A, s, H::kTileCols);
+        }
+        const uint64_t in_seq = at - seq_first;
+        const uint32_t item = static_cast<uint32_t>(in_seq / W.units), u0 = static_cast<uint32_t>(in_seq - static_cast<uint64_t>(item) * W.units);
+        const uint32_t u1 = static_cast<uint32_t>(min(static_cast<uint64_t>(W.units), u0 + (end - at)));
+        const uint32_t head = item / W.tiles, tile = item - head * W.tiles;
+        const uint32_t cols = W.nodes * A.group, col0 = tile * H::kTileCols + wm * (16u * MS);
+        const uint32_t slot = A.slot ? A.slot[s] : s;
+        const int32_t* table = A.table + static_cast<uint64_t>(slot) * A.table_stride;
+        const bool no_slot = slot >= A.slots;
+        const uint32_t total = no_slot ? 0u : W.total, length = min(W.length, total);
+
+        // the columns: Q in its operand's places, what a column sees of the nodes
+        uint4 q[MS][kChunks];
+        uint64_t sees[MS];
+        float top[MS], sum[MS];
+        f32x4 o[MS][kOuts];
+#pragma unroll
+        for (int m = 0; m < MS; ++m) {
+            const uint32_t col = min(col0 + m * 16u + c, cols - 1u), node = col / A.group, h = head * A.group + (col - node * A.group);
+            const unsigned char* at_q = A.q + static_cast<uint64_t>(W.first + node) * A.q_row + static_cast<uint64_t>(h) * A.q_head;
+#pragma unroll
+            for (uint32_t j = 0; j < kChunks; ++j) {
+                const uint32_t d = j * Mat<DT>::kDepth + g * Mat<DT>::kPer;
+                q[m][j] = make_uint4(0u, 0u, 0u, 0u);
+                if (d < A.head_dim) q[m][j] = *reinterpret_cast<const uint4*>(at_q + d * E);
+            }
+            sees[m] = A.mask ? A.mask[W.first + node] : (node < 63u ? (uint64_t{2} << node) - 1u : ~uint64_t{0});
+            top[m] = -FLT_MAX;
+            sum[m] = 0.f;
+#pragma unroll
+            for (uint32_t r = 0; r < kOuts; ++r) o[m][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        const unsigned char* k_base = A.k + static_cast<uint64_t>(head) * A.k_head;
+        const unsigned char* v_base = A.v + static_cast<uint64_t>(head) * A.v_head;
+        const uint32_t in_page = (1u << A.page_shift) - 1u;
+
+        const uint32_t p_end = min(u1 * kUnit, total);
+        // page of the positions whose K this lane loads (tokens c and 16 + c of 32) and whose scores and V it holds (4 g .. and 16 + 4 g ..)
+        uint32_t k_pg[2], v_pg[2];
+        auto pages_of = [&](uint32_t p0) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                k_pg[i] = p0 < p_end ? attend_page(A, table, p0 + 16u * i + c) : 0u;
+                v_pg[i] = p0 < p_end ? attend_page(A, table, p0 + 16u * i + 4u * g) : 0u;
+            }
+        };
+        uint4 kx[2][kChunks];
+        auto load_k = [&](uint32_t p0) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                // (a page that is not there: the first one's, not looked at)
+                const uint64_t page = k_pg[i] < A.pages ? k_pg[i] : 0u;
+                const unsigned char* at_k = k_base + page * A.k_page + static_cast<uint64_t>((p0 + 16u * i + c) & in_page) * A.k_token;
+#pragma unroll
+                for (uint32_t j = 0; j < kChunks; ++j) {
+                    const uint32_t d = j * Mat<DT>::kDepth + g * Mat<DT>::kPer;
+                    kx[i][j] = *reinterpret_cast<const uint4*>(at_k + (d < A.head_dim ? d : 0u) * E);
+                }
+            }
+        };
+        // (8 bf16 or 4 fp32: one load of 16 bytes; 4 bf16: one of 8)
+        uint4 vx[8][kBlocks];
+        // token i of a lane's eight: 4 g + i of the first 16 positions, 4 g + i - 4 of the second
+        auto v_pos = [&](uint32_t p0, uint32_t i) __attribute__((always_inline)) { return p0 + (i < 4u ? 0u : 12u) + 4u * g + i; };
+        auto load_v = [&](uint32_t p0) __attribute__((always_inline)) {
+            const unsigned char* at_v[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i) {
+                const uint64_t page = v_pg[i / 4u] < A.pages ? v_pg[i / 4u] : 0u;
+                at_v[i] = i % 4u ? at_v[i - 1u] + A.v_token : v_base + page * A.v_page + static_cast<uint64_t>(v_pos(p0, i) & in_page) * A.v_token;
+            }
+            if (A.page_shift < 2u) {  // (uniform) fewer than four tokens a page
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; ++i) {
+                    const uint32_t pos = v_pos(p0, i), pg = pos < p_end ? attend_page(A, table, pos) : 0u;
+                    at_v[i] = v_base + static_cast<uint64_t>(pg < A.pages ? pg : 0u) * A.v_page + static_cast<uint64_t>(pos & in_page) * A.v_token;
+                }
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i) {
+#pragma unroll
+                for (uint32_t b = 0; b < kBlocks; ++b) {
+                    const uint32_t d = b * 16u * kEach + c * kEach;
+                    const unsigned char* from = at_v[i] + (d < A.head_dim ? d : 0u) * E;
+                    if constexpr (kEach * E == 16u) {
+                        vx[i][b] = *reinterpret_cast<const uint4*>(from);
+                    } else {
+                        const uint2 two = *reinterpret_cast<const uint2*>(from);
+                        vx[i][b] = make_uint4(two.x, two.y, 0u, 0u);
+                    }
+                }
+            }
+        };
+        // whether token i of the positions from p0 is there
+        auto there = [&](uint32_t p0, uint32_t i) __attribute__((always_inline)) {
+            const uint32_t pos = v_pos(p0, i);
+            if (pos >= p_end) return false;
+            if (A.page_shift < 2u && i % 4u != 0u) return attend_page(A, table, pos) < A.pages;
+            return v_pg[i / 4u] < A.pages;
+        };
+
+        // the word that holds element e of a token's
+        auto element_word = [](const uint4& v, uint32_t e) __attribute__((always_inline)) {
+            const uint32_t w = e * E / 4u;
+            return w == 0u ? v.x : (w == 1u ? v.y : (w == 2u ? v.z : v.w));
+        };
+        constexpr uint32_t kStep = 32u * kWT;
+        uint32_t odd = 0u;
+        uint4 px[MS][DT == 1 ? 1 : 2];
+        // the powers of 32 positions' scores from their K (k_of: piece j of tokens c and 16 + c); here: a bit a token of the lane; `then` is done when K has been read
+        auto powers = [&](uint32_t p0, bool plain, uint32_t here, auto&& k_of, auto&& then) __attribute__((always_inline)) {
+            f32x4 x[MS][2];
+#pragma unroll
+            for (uint32_t j = 0; j < kChunks; ++j)
+#pragma unroll
+                for (uint32_t i = 0; i < 2u; ++i) {
+                    const uint4 k = k_of(i, j);
+#pragma unroll
+                    for (int m = 0; m < MS; ++m) x[m][i] = Mat<DT>::mul(k, q[m][j], j ? x[m][i] : f32x4{0.f, 0.f, 0.f, 0.f});
+                }
+            then();
+            if (!plain) {  // (uniform)
+#pragma unroll
+                for (int m = 0; m < MS; ++m) {
+                    const uint32_t seen = here & (sees_four(sees[m], v_pos(p0, 0u), length) | sees_four(sees[m], v_pos(p0, 4u), length) << 4);
+#pragma unroll
+                    for (uint32_t i = 0; i < 8u; ++i) x[m][i / 4u][i % 4u] = seen >> i & 1u ? x[m][i / 4u][i % 4u] : -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < MS; ++m) {
+                float most = fmaxf(fmaxf(fmaxf(x[m][0][0], x[m][0][1]), fmaxf(x[m][0][2], x[m][0][3])), fmaxf(fmaxf(x[m][1][0], x[m][1][1]), fmaxf(x[m][1][2], x[m][1][3])));
+                most *= A.scale_log2;
+                float p[8];
+                if (__ballot(most > top[m] + kSlack) != 0ull) {  // (uniform) some column's maximum has grown
+                    most = fmaxf(most, __shfl_xor(most, 16));
+                    most = fmaxf(most, __shfl_xor(most, 32));
+                    const float to = fmaxf(top[m], most), down = __builtin_amdgcn_exp2f(top[m] - to);
+                    top[m] = to;
+                    sum[m] *= down;
+#pragma unroll
+                    for (uint32_t r = 0; r < kOuts; ++r) o[m][r] *= down;
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(x[m][i / 4u][i % 4u], A.scale_log2, -top[m]));
+                sum[m] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                if constexpr (DT == 1) {
+                    bf16x8 b;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) b[i] = static_cast<__bf16>(p[i]);
+                    px[m][0] = __builtin_bit_cast(uint4, b);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        px[m][i] = make_uint4(__float_as_uint(p[4 * i]), __float_as_uint(p[4 * i + 1]), __float_as_uint(p[4 * i + 2]), __float_as_uint(p[4 * i + 3]));
+                }
+            }
+        };
+        // V that is not there counts as 0, whatever the place holds; of nodes, which some columns see and others do not, what is no number is left for later
+        auto clean = [&](uint4 v, bool there_, bool node) __attribute__((always_inline)) {
+            const uint32_t keep = there_ ? 0xffffffffu : 0u;
+            v = make_uint4(v.x & keep, v.y & keep, v.z & keep, v.w & keep);
+            if (node) {
+                const uint4 z = make_uint4(Mat<DT>::special(v.x), Mat<DT>::special(v.y), Mat<DT>::special(v.z), Mat<DT>::special(v.w));
+                odd |= z.x | z.y | z.z | z.w;
+                v = make_uint4(v.x & ~z.x, v.y & ~z.y, v.z & ~z.z, v.w & ~z.w);
+            }
+            return v;
+        };
+        auto add_up = [&](auto&& v_of) __attribute__((always_inline)) {  // O^T; v_of: block b of a lane's token i
+#pragma unroll
+            for (uint32_t b = 0; b < kBlocks; ++b) {
+                uint4 v[8];
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; ++i) v[i] = v_of(i, b);
+#pragma unroll
+                for (uint32_t e = 0; e < kEach; ++e) {
+                    uint32_t word[8];
+#pragma unroll
+                    for (uint32_t i = 0; i < 8u; ++i) word[i] = element_word(v[i], e);
+#pragma unroll
+                    for (int m = 0; m < MS; ++m) o[m][b * kEach + e] = Mat<DT>::mul_tokens(word, e, px[m], o[m][b * kEach + e]);
+                }
+            }
+        };
+        if constexpr (!kStaged) {
+            uint32_t p0 = u0 * kUnit + wt * 32u;
+            if (p0 < p_end) {
+                pages_of(p0);
+                load_k(p0);
+            }
+            for (; p0 < p_end; p0 += kStep) {
+                load_v(p0);
+                // all 32 positions there and seen by every column (uniform)
+                const bool plain = p0 + 32u <= min(length, p_end) && A.page_shift >= 2u && __ballot(v_pg[0] >= A.pages || v_pg[1] >= A.pages) == 0ull;
+                uint32_t here = 0u;
+                if (!plain) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 8u; ++i) here |= there(p0, i) ? 1u << i : 0u;
+                }
+                powers(p0, plain, here, [&](uint32_t i, uint32_t j) { return kx[i][j]; }, [&]() {  // the next positions' K while these are worked on
+                    if (p0 + kStep < p_end) {
+                        pages_of(p0 + kStep);
+                        load_k(p0 + kStep);
+                    }
+                });
+                if (!plain) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 8u; ++i)
+#pragma unroll
+                        for (uint32_t b = 0; b < kBlocks; ++b) vx[i][b] = clean(vx[i][b], here >> i & 1u, v_pos(p0, i) >= length);
+                }
+                add_up([&](uint32_t i, uint32_t b) { return vx[i][b]; });
+            }
+        } else {
+            unsigned char* const lds = reinterpret_cast<unsigned char*>(s_kv);
+            u32x4 next_k[H::kMine], next_v[H::kMine];  // (uint4's copies of an array's elements keep it in scratch memory)
+            uint32_t next_here = 0u;  // a bit a piece of the thread
+            auto fetch = [&](uint32_t p) __attribute__((always_inline)) {
+                next_here = 0u;
+#pragma unroll
+                for (uint32_t l = 0; l < H::kMine; ++l) {
+                    const uint32_t at = l * 256u + t, token = at / H::kPieces, d = (at % H::kPieces) * Mat<DT>::kPer, pos = p + token;
+                    const uint32_t pg = pos < p_end ? attend_page(A, table, pos) : A.pages;
+                    next_here |= pg < A.pages ? 1u << l : 0u;
+                    const uint64_t page = pg < A.pages ? pg : 0u, in = pos & in_page;
+                    const uint32_t byte = (d < A.head_dim ? d : 0u) * E;
+                    next_k[l] = *reinterpret_cast<const u32x4*>(k_base + page * A.k_page + in * A.k_token + byte);
+                    next_v[l] = *reinterpret_cast<const u32x4*>(v_base + page * A.v_page + in * A.v_token + byte);
+                }
+            };
+            uint32_t p = u0 * kUnit, buffer = 0u;
+            if (p < p_end) fetch(p);
+            for (; p < p_end; p += H::kTokens, buffer ^= 1u) {  // (the same for the workgroup)
+                unsigned char* const k_lds = lds + buffer * 2u * H::kBuffer;
+                unsigned char* const v_lds = k_lds + H::kBuffer;
+                const bool nodes = p + H::kTokens > length;  // (uniform)
+                const bool short_of = __ballot(next_here != (1u << H::kMine) - 1u) != 0ull;
+                if (short_of || nodes) {
+#pragma unroll
+                    for (uint32_t l = 0; l < H::kMine; ++l) {
+                        const uint32_t token = (l * 256u + t) / H::kPieces;
+                        const uint4 v = clean(make_uint4(next_v[l].x, next_v[l].y, next_v[l].z, next_v[l].w), next_here >> l & 1u, p + token >= length);
+                        next_v[l] = u32x4{v.x, v.y, v.z, v.w};
+                    }
+                }
+#pragma unroll
+                for (uint32_t l = 0; l < H::kMine; ++l) {
+                    const uint32_t at = l * 256u + t, token = at / H::kPieces, piece = at % H::kPieces;
+                    *reinterpret_cast<u32x4*>(k_lds + H::place(token, piece)) = next_k[l];
+                    *reinterpret_cast<u32x4*>(v_lds + H::place(token, piece)) = next_v[l];
+                    if (piece == 0u) s_here[buffer * H::kTokens + token] = next_here >> l & 1u;
+                }
+                __syncthreads();
+                if (p + H::kTokens < p_end) fetch(p + H::kTokens);
+#pragma unroll 1
+                for (uint32_t sub = 0; sub < H::kTokens && p + sub < p_end && col0 < cols; sub += 32u) {
+                    const uint32_t p0 = p + sub;
+                    uint32_t here = 0u;
+#pragma unroll
+                    for (uint32_t i = 0; i < 8u; ++i) here |= s_here[buffer * H::kTokens + (v_pos(p0, i) - p)] != 0u ? 1u << i : 0u;
+                    const bool plain = p0 + 32u <= length && __ballot(here != 0xffu) == 0ull;
+                    powers(p0, plain, here, [&](uint32_t i, uint32_t j) { return *reinterpret_cast<const uint4*>(k_lds + H::place(sub + 16u * i + c, j * 4u + g)); }, []() {});
+                    add_up([&](uint32_t i, uint32_t b) {
+                        const uint32_t token = v_pos(p0, i) - p;
+                        if constexpr (kEach * E == 16u) {
+                            return *reinterpret_cast<const uint4*>(v_lds + H::place(token, b * 16u + c));
+                        } else {
+                            const uint2 two = *reinterpret_cast<const uint2*>(v_lds + H::place(token, b * 8u + c / 2u) + (c & 1u) * 8u);
+                            return make_uint4(two.x, two.y, 0u, 0u);
+                        }
+                    });
+                }
+            }
+        }
+        if (__ballot(odd != 0u) != 0ull && lane == 0u) s_odd = 1u;
+        // a column's sum over its four lanes
+#pragma unroll
+        for (int m = 0; m < MS; ++m) {
+            sum[m] += __shfl_xor(sum[m], 16);
+            sum[m] += __shfl_xor(sum[m], 32);
+        }
+        // the waves of other positions: the upper half leaves what it has, the lower half joins it, and so on
+        auto join = [&](int m, float their_top, float their_sum, auto&& theirs) __attribute__((always_inline)) {
+            const float to = fmaxf(top[m], their_top), a = __builtin_amdgcn_exp2f(top[m] - to), z = __builtin_amdgcn_exp2f(their_top - to);
+            top[m] = to;
+            sum[m] = sum[m] * a + their_sum * z;
+#pragma unroll
+            for (uint32_t r = 0; r < kOuts; ++r) o[m][r] = o[m][r] * a + theirs(r) * z;
+        };
+        if constexpr (kWT > 1u) {
+#pragma unroll
+            for (uint32_t half = kWT / 2u; half >= 1u; half /= 2u) {
+                __syncthreads();
+                if (wt >= half && wt < 2u * half) {
+#pragma unroll
+                    for (int m = 0; m < MS; ++m) {
+                        float* to = s_part + ((wt - half) * MS + m) * (kDump + 128u);
+                        to[lane] = top[m];
+                        to[64u + lane] = sum[m];
+#pragma unroll
+                        for (uint32_t r = 0; r < kOuts; ++r) *reinterpret_cast<f32x4*>(to + 128u + (r * 64u + lane) * 4u) = o[m][r];
+                    }
+                }
+                __syncthreads();
+                if (wt < half) {
+#pragma unroll
+                    for (int m = 0; m < MS; ++m) {
+                        const float* from = s_part + (wt * MS + m) * (kDump + 128u);
+                        join(m, from[lane], from[64u + lane], [&](uint32_t r) { return *reinterpret_cast<const f32x4*>(from + 128u + (r * 64u + lane) * 4u); });
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        const bool any_odd = s_odd != 0u;
+        if (wt == 0u) {
+            if (u0 == 0u && u1 == W.units) {
+                if (any_odd) {  // (uniform)
+#pragma unroll 1
+                    for (uint32_t j = 0; j < W.nodes; ++j) {
+                        const uint32_t pos = W.length + j, pg = W.length < total && pos < total ? attend_page(A, table, pos) : A.pages;
+                        if (pg >= A.pages) continue;
+                        const unsigned char* at_v = v_base + static_cast<uint64_t>(pg) * A.v_page + static_cast<uint64_t>(pos & in_page) * A.v_token;
+#pragma unroll
+                        for (uint32_t r = 0; r < kOuts; ++r) {
+#pragma unroll
+                            for (uint32_t l = 0; l < 4u; ++l)
+#pragma unroll
+                                for (int m = 0; m < MS; ++m)
+                                    o[m][r][l] += attend_odd<DT>(A, at_v, (r / kEach) * 16u * kEach + (4u * g + l) * kEach + r % kEach, (sees[m] >> j & 1u) != 0u);
+                            __builtin_amdgcn_sched_barrier(0);  // (loads of all of them together would take the registers that the products need)
+                        }
+                    }
+                }
+#pragma unroll
+                for (int m = 0; m < MS; ++m) {
+                    const uint32_t col = col0 + m * 16u + c;
+                    if (col >= cols) continue;
+                    const uint32_t node = col / A.group, h = head * A.group + (col - node * A.group);
+                    const float by = sum[m] == 0.f ? 0.f : 1.f / sum[m];
+                    if (A.lse && g == 0u)
+                        A.lse[static_cast<uint64_t>(W.first + node) * A.heads + h] = sum[m] == 0.f ? -INFINITY : (top[m] + __builtin_amdgcn_logf(sum[m])) * 0.69314718f;
+                    unsigned char* to = A.out + static_cast<uint64_t>(W.first + node) * A.out_row + static_cast<uint64_t>(h) * A.out_head;
+#pragma unroll
+                    for (uint32_t b = 0; b < kBlocks; ++b)
+#pragma unroll
+                        for (uint32_t l = 0; l < 4u; ++l) {
+                            const uint32_t d = b * 16u * kEach + (4u * g + l) * kEach;
+                            if (d >= A.head_dim) continue;
+                            if constexpr (DT == 1) {
+                                __bf16 y[kEach];
+#pragma unroll
+                                for (uint32_t e = 0; e < kEach; ++e) y[e] = static_cast<__bf16>(o[m][b * kEach + e][l] * by);
+                                __builtin_memcpy(to + d * 2u, y, kEach * 2u);
+                            } else {
+                                float y[kEach];
+#pragma unroll
+                                for (uint32_t e = 0; e < kEach; ++e) y[e] = o[m][b * kEach + e][l] * by;
+                                __builtin_memcpy(to + d * 4u, y, kEach * 4u);
+                            }
+                        }
+                }
+            } else {
+                float* part = A.part + (static_cast<uint64_t>(run_id) * 2u + (u0 == 0u ? 1u : 0u)) * H::kPartFloats + wm * MS * H::kSubFloats;
+#pragma unroll
+                for (int m = 0; m < MS; ++m) {
+                    float* to = part + m * H::kSubFloats;
+                    to[lane] = top[m];
+                    to[64u + lane] = sum[m];
+#pragma unroll
+                    for (uint32_t r = 0; r < kOuts; ++r) *reinterpret_cast<f32x4*>(to + 128u + (r * 64u + lane) * 4u) = o[m][r];
+                }
+            }
+        }
+        if (t == 0u && u0 != 0u) run_odd = any_odd ? 1u : 0u;
+        if (t == 0u && u0 == 0u && u1 < W.units) {
+            // the workgroups that hold the rest of this tile
+            const uint64_t first = at, last = at + W.units - 1u;
+            AttendRun r;
+            r.seq = s;
+            r.head = head;
+            r.tile = tile;
+            r.more = static_cast<uint32_t>(last / per - first / per);
+            r.odd = 0u;
+            A.run[run_id] = r;
+        }
+        at += u1 - u0;
+        __syncthreads();
+        if (t == 0u) s_odd = 0u;
+    }
+    if (t == 0u) A.run[run_id].odd = run_odd;
+}
+
+// A workgroup joins 16 columns of the tile that begins in run x: the tile's first piece is that run's second part, the others are the first parts of the runs behind it. Every thread has one or
+// more of the lanes' four floats, and goes through the pieces in order.
+template <int DT, int DP, int MS, int WM>
+__global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs A) {
+    typedef AttendShape<DT, DP, MS, WM> H;
+    const uint32_t x = blockIdx.x, sub = blockIdx.y, t = threadIdx.x;
+    const AttendRun R = A.run[x];
+    if (R.more == 0u) return;
+    const AttendWork W = attend_work(A, R.seq, H::kTileCols);
+    const uint32_t cols = W.nodes * A.group, col0 = R.tile * H::kTileCols + sub * 16u;
+    if (col0 >= cols) return;
+    auto piece = [&](uint32_t i) { return A.part + ((static_cast<uint64_t>(x) + i) * 2u + (i == 0u ? 1u : 0u)) * H::kPartFloats + sub * H::kSubFloats; };
+    const uint32_t lane = t & 63u, c = lane & 15u, g = lane >> 4;
+    float top = -FLT_MAX;
+    for (uint32_t i = 0; i <= R.more; ++i) top = fmaxf(top, piece(i)[lane]);  // (NaN in a sum, not in a maximum)
+    constexpr uint32_t kMine = (H::kOuts + 3u) / 4u;
+    f32x4 o[kMine];
+    float sum = 0.f;
+#pragma unroll
+    for (uint32_t r = 0; r < kMine; ++r) o[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (uint32_t i = 0; i <= R.more; ++i) {
+        const float* from = piece(i);
+        const float by = __builtin_amdgcn_exp2f(from[lane] - top);
+        sum = fmaf(from[64u + lane], by, sum);
+#pragma unroll
+        for (uint32_t r = 0; r < kMine; ++r) {
+            const uint32_t out = wave_id() * kMine + r;
+            if (out < H::kOuts) o[r] += *reinterpret_cast<const f32x4*>(from + 128u + (out * 64u + lane) * 4u) * by;
+        }
+    }
+    const uint32_t col = col0 + c;
+    if (col >= cols) return;
+    const uint32_t node = col / A.group, h = R.head * A.group + (col - node * A.group);
+    if (A.run[x + R.more].odd != 0u) {
+        const int32_t* table = A.table + static_cast<uint64_t>(A.slot ? A.slot[R.seq] : R.seq) * A.table_stride;
+        const uint64_t sees = A.mask ? A.mask[W.first + node] : (node < 63u ? (uint64_t{2} << node) - 1u : ~uint64_t{0});
+#pragma unroll 1
+        for (uint32_t j = 0; j < W.nodes && W.length + j < W.total; ++j) {
+            const uint32_t pos = W.length + j, pg = attend_page(A, table, pos);
+            if (pg >= A.pages) continue;
+            const unsigned char* at_v = A.v + static_cast<uint64_t>(pg) * A.v_page + static_cast<uint64_t>(pos & ((1u << A.page_shift) - 1u)) * A.v_token + static_cast<uint64_t>(R.head) * A.v_head;
+#pragma unroll
+            for (uint32_t r = 0; r < kMine; ++r) {
+                const uint32_t out = wave_id() * kMine + r;
+#pragma unroll
+                for (uint32_t l = 0; l < 4u; ++l)
+                    o[r][l] += attend_odd<DT>(A, at_v, (out / H::kEach) * 16u * H::kEach + (4u * g + l) * H::kEach + out % H::kEach, (sees >> j & 1u) != 0u);
+            }
+        }
+    }
+    const float by = sum == 0.f ? 0.f : 1.f / sum;
+    if (A.lse && t < 16u) A.lse[static_cast<uint64_t>(W.first + node) * A.heads + h] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * 0.69314718f;
+    unsigned char* to = A.out + static_cast<uint64_t>(W.first + node) * A.out_row + static_cast<uint64_t>(h) * A.out_head;
+#pragma unroll
+    for (uint32_t r = 0; r < kMine; ++r) {
+        const uint32_t out = wave_id() * kMine + r;
+        if (out >= H::kOuts) continue;
+#pragma unroll
+        for (uint32_t l = 0; l < 4u; ++l) {
+            const uint32_t d = (out / H::kEach) * 16u * H::kEach + (4u * g + l) * H::kEach + out % H::kEach;
+            if (d >= A.head_dim) continue;
+            if constexpr (DT == 1) reinterpret_cast<__bf16*>(to)[d] = static_cast<__bf16>(o[r][l] * by);
+            else reinterpret_cast<float*>(to)[d] = o[r][l] * by;
+        }
+    }
+}
+
+}  // namespace ws

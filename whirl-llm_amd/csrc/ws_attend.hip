@@ -1,0 +1,61 @@
+// The kernels of ws_attend.h, a translation unit of its own.
+#define WS_NO_NAMED_KERNELS
+#include "ws_attend.h"
+
+namespace ws {
+
+namespace {
+struct Build {
+    int dtype;
+    uint32_t dim, cols;  // head_dim and columns up to which it is taken
+    uint32_t each;       // workgroups a compute unit
+    uint64_t part_floats;
+    uint32_t subs;
+    void (*run)(hipStream_t, const AttendArgs&);
+};
+template <int DT, int DP, int MS, int WM, int OCC>
+void launch(hipStream_t s, const AttendArgs& a) {
+    hipLaunchKernelGGL((attend_kernel<DT, DP, MS, WM, OCC>), dim3(a.groups), dim3(kAttendThreads), 0, s, a);
+    hipLaunchKernelGGL((attend_join_kernel<DT, DP, MS, WM>), dim3(a.groups, MS * WM), dim3(kAttendThreads), 0, s, a);
+}
+template <int DT, int DP, int MS, int WM, int OCC>
+constexpr Build build(uint32_t cols) {
+    return Build{DT, DP, cols, OCC, AttendShape<DT, DP, MS, WM>::kPartFloats, MS * WM, &launch<DT, DP, MS, WM, OCC>};
+}
+constexpr uint32_t kAny = 0xffffffffu;
+constexpr Build kBuilds[] = {
+    build<1, 64, 1, 1, 3>(16), build<1, 64, 2, 1, 2>(32), build<1, 64, 1, 4, 2>(64), build<1, 64, 2, 4, 2>(kAny),
+    build<1, 128, 1, 1, 2>(16), build<1, 128, 1, 4, 2>(64), build<1, 128, 2, 4, 2>(128), build<1, 128, 4, 4, 1>(kAny),
+    build<1, 256, 1, 1, 1>(16), build<1, 256, 1, 4, 1>(kAny),
+    build<0, 64, 1, 1, 2>(16), build<0, 64, 1, 4, 2>(64), build<0, 64, 2, 4, 2>(kAny),
+    build<0, 128, 1, 4, 2>(kAny), build<0, 256, 1, 4, 1>(kAny),
+};
+}  // namespace
+
+int prepare_attend() {
+    hipFuncAttributes fa;
+    return static_cast<int>(hipFuncGetAttributes(&fa, reinterpret_cast<const void*>(&attend_kernel<1, 128, 1, 1, 2>)));
+}
+
+AttendPlan attend_plan(int dtype, uint32_t head_dim, uint32_t cols, uint32_t compute_units) {
+    AttendPlan p{};
+    for (const Build& b : kBuilds) {
+        if (b.dtype == dtype && head_dim <= b.dim && cols <= b.cols) {
+            p.build = static_cast<uint32_t>(&b - kBuilds);
+            p.groups = compute_units * b.each;
+            // (what a run leaves in the workspace is at most a quarter of what it reads)
+            p.least = 1u;
+            p.part_bytes = uint64_t{p.groups} * 2u * b.part_floats * 4u;
+            p.bytes = p.part_bytes + uint64_t{p.groups} * sizeof(AttendRun);
+            return p;
+        }
+    }
+    return p;
+}
+
+int launch_attend(hipStream_t stream, const AttendPlan& plan, const AttendArgs& a) {
+    kBuilds[plan.build].run(stream, a);
+    return static_cast<int>(hipGetLastError());
+}
+
+}  // namespace ws
