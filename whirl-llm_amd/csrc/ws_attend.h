@@ -135,34 +135,42 @@ __device__ __forceinline__ uint64_t scan256(uint64_t v, uint64_t* red, uint64_t&
 
 struct AttendFind {
     uint64_t red[4];
-    uint64_t all;       // units of all sequences
-    uint64_t seq_first;  // the first unit of `seq`
+    uint64_t seq_first;  // the first unit of sequence `seq`, which holds the one that is looked for
     uint32_t seq;
+    AttendWork work;
 };
-// the sequence that holds unit `at`(all sequences' units are added up on the way where `sum`)
-__device__ __forceinline__ void attend_sum(const AttendArgs& A, uint32_t cols, AttendFind& F) {
-    uint64_t sum = 0;
-    for (uint32_t s = threadIdx.x; s < A.n_seq; s += kAttendThreads) sum += attend_work(A, s, cols).all;
-    uint64_t total;
-    scan256(sum, F.red, total);
-    if (threadIdx.x == 0u) F.all = total;
-    __syncthreads();
-}
-__device__ __forceinline__ void attend_find(const AttendArgs& A, uint32_t cols, AttendFind& F, uint64_t at) {
+// The units of all sequences, and in `find` the sequence that holds unit first(all): a sequence a thread, 256 at a time.
+template <class Fn>
+__device__ __forceinline__ uint64_t attend_find(const AttendArgs& A, uint32_t cols, AttendFind& F, Fn&& first) {
+    const uint32_t t = threadIdx.x;
+    uint64_t mine = 0, before = 0, all = 0;
+    AttendWork w{};
+    for (uint32_t s = t; s < A.n_seq; s += kAttendThreads) {
+        w = attend_work(A, s, cols);
+        mine += w.all;
+    }
+    before = scan256(mine, F.red, all);
+    const uint64_t at = first(all);
+    if (at >= all) return all;
     uint64_t base = 0;
     for (uint32_t s0 = 0; s0 < A.n_seq; s0 += kAttendThreads) {
-        const uint32_t s = s0 + threadIdx.x;
-        const uint64_t mine = s < A.n_seq ? attend_work(A, s, cols).all : 0u;
-        uint64_t total;
-        const uint64_t before = base + scan256(mine, F.red, total);
-        if (mine && at >= before && at - before < mine) {
-            F.seq = s;
-            F.seq_first = before;
+        if (A.n_seq > kAttendThreads) {  // (the sums above were of several)
+            w = AttendWork{};
+            if (s0 + t < A.n_seq) w = attend_work(A, s0 + t, cols);
+            mine = w.all;
+            uint64_t total;
+            before = base + scan256(mine, F.red, total);
+            base += total;
         }
-        base += total;
+        if (mine && at >= before && at - before < mine) {
+            F.seq = s0 + t;
+            F.seq_first = before;
+            F.work = w;
+        }
         if (at < base) break;  // (uniform)
     }
     __syncthreads();
+    return all;
 }
 
 // What the products leave out: infinities and NaN in the V of nodes, which must not reach the rows that do not see them (0 times NaN is NaN). Rare, so it is done where a column is
@@ -173,11 +181,33 @@ __device__ __forceinline__ float attend_odd(const AttendArgs& A, const unsigned 
     return sees && !(fabsf(x) <= FLT_MAX) ? x : 0.f;
 }
 
-// the page of a position of the slot whose table row this is; `pages` where there is none
-__device__ __forceinline__ uint32_t attend_page(const AttendArgs& A, const int32_t* row, uint32_t pos) {
-    const uint32_t at = pos >> A.page_shift;
-    const uint32_t page = at < A.slot_pages ? static_cast<uint32_t>(row[at]) : A.pages;
-    return min(page, A.pages);
+// a column's results: a lane's 4 kEach-element pieces of each block
+template <int DT, uint32_t EACH, uint32_t BLOCKS>
+__device__ __forceinline__ void attend_write(const AttendArgs& A, unsigned char* to, uint32_t g, const f32x4 (&o)[BLOCKS * EACH], float by) {
+#pragma unroll
+    for (uint32_t b = 0; b < BLOCKS; ++b)
+#pragma unroll
+        for (uint32_t l = 0; l < 4u; ++l) {
+            const uint32_t d = b * 16u * EACH + (4u * g + l) * EACH;
+            if (d >= A.head_dim) continue;
+            if constexpr (DT == 1) {
+                __bf16 y[EACH];
+#pragma unroll
+                for (uint32_t e = 0; e < EACH; ++e) y[e] = static_cast<__bf16>(o[b * EACH + e][l] * by);
+                __builtin_memcpy(__builtin_assume_aligned(to + d * 2u, EACH * 2u), y, EACH * 2u);
+            } else {
+                float y[EACH];
+#pragma unroll
+                for (uint32_t e = 0; e < EACH; ++e) y[e] = o[b * EACH + e][l] * by;
+                __builtin_memcpy(__builtin_assume_aligned(to + d * 4u, EACH * 4u), y, EACH * 4u);
+            }
+        }
+}
+
+// the page of a position of the slot whose table row this is; `pages` where there is none. (No branch: what is loaded behind one is waited for there, and with it everything loaded before.)
+__device__ __forceinline__ uint32_t attend_page(const AttendArgs& A, const int32_t* row, uint32_t pos, uint32_t end) {
+    const uint32_t at = pos >> A.page_shift, page = static_cast<uint32_t>(row[min(at, A.slot_pages - 1u)]);
+    return pos < end && at < A.slot_pages ? min(page, A.pages) : A.pages;
 }
 
 template <int DT, int DP, int MS, int WM, int OCC>
@@ -191,22 +221,23 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
     __shared__ uint32_t s_odd;
     __shared__ float s_part[kWT > 1u ? (kWT / 2u) * MS * (kDump + 128u) : 1u];
     __shared__ uint4 s_kv[kStaged ? 2u * 2u * H::kBuffer / 16u : 1u];  // two buffers of K, then V
-    __shared__ uint8_t s_here[kStaged ? 2u * H::kTokens : 1u];         // whether a token is there
     const uint32_t t = threadIdx.x, lane = lane_id(), c = lane & 15u, g = lane >> 4, wave = wave_id(), wm = wave % WM, wt = wave / WM;
 
-    attend_sum(A, H::kTileCols, F);
-    const uint64_t per = max((F.all + A.groups - 1u) / A.groups, static_cast<uint64_t>(A.least));
     // (neighbouring runs on the same part of the chip: workgroup b runs on XCD b % 8)
     const uint32_t in_xcd = A.groups / 8u, run_id = blockIdx.x < in_xcd * 8u ? (blockIdx.x & 7u) * in_xcd + (blockIdx.x >> 3) : blockIdx.x;
-    const uint64_t begin = min(per * run_id, F.all), end = min(begin + per, F.all);
+    uint64_t per = 0, begin = 0;
+    const uint64_t all = attend_find(A, H::kTileCols, F, [&](uint64_t units) {
+        per = max((units + A.groups - 1u) / A.groups, static_cast<uint64_t>(A.least));
+        return begin = per * run_id;
+    });
     uint32_t run_odd = 0u;  // (the first thread's)
     if (t == 0u) A.run[run_id].more = 0u;
     if (t == 0u) s_odd = 0u;
-    if (begin >= end) return;
-    attend_find(A, H::kTileCols, F, begin);
+    if (begin >= all) return;
+    const uint64_t end = min(begin + per, all);
     uint32_t s = F.seq;
     uint64_t seq_first = F.seq_first;
-    AttendWork W = attend_work(A, s, H::kTileCols);
+    AttendWork W = F.work;
 
     for (uint64_t at = begin; at < end;) {
         while (at - seq_first >= W.all) {
@@ -250,21 +281,21 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
         const uint32_t in_page = (1u << A.page_shift) - 1u;
 
         const uint32_t p_end = min(u1 * kUnit, total);
-        // page of the positions whose K this lane loads (tokens c and 16 + c of 32) and whose scores and V it holds (4 g .. and 16 + 4 g ..)
-        uint32_t k_pg[2], v_pg[2];
-        auto pages_of = [&](uint32_t p0) __attribute__((always_inline)) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                k_pg[i] = p0 < p_end ? attend_page(A, table, p0 + 16u * i + c) : 0u;
-                v_pg[i] = p0 < p_end ? attend_page(A, table, p0 + 16u * i + 4u * g) : 0u;
-            }
-        };
+        // A lane looks up the page of one position of those that are worked on next, and asks the others for theirs: one load ahead of the ones that need it
+        constexpr uint32_t kAhead = kStaged ? H::kTokens : 32u;
+        auto page_of = [&](uint32_t p) __attribute__((always_inline)) { return attend_page(A, table, p + (lane & (kAhead - 1u)), p_end); };
+        auto page_from = [&](uint32_t pg, uint32_t token) __attribute__((always_inline)) { return static_cast<uint32_t>(__shfl(static_cast<int>(pg), static_cast<int>(token))); };
+        uint32_t pg_now = 0u, pg_next = 0u;
         uint4 kx[2][kChunks];
-        auto load_k = [&](uint32_t p0) __attribute__((always_inline)) {
+        uint4 vx[8][kBlocks];
+        // token i of a lane's eight: 4 g + i of the first 16 positions, 4 g + i - 4 of the second
+        auto v_pos = [&](uint32_t p0, uint32_t i) __attribute__((always_inline)) { return p0 + (i < 4u ? 0u : 12u) + 4u * g + i; };
+        auto load_k = [&](uint32_t p0, uint32_t pg) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (uint32_t i = 0; i < 2u; ++i) {
                 // (a page that is not there: the first one's, not looked at)
-                const uint64_t page = k_pg[i] < A.pages ? k_pg[i] : 0u;
+                const uint32_t mine = page_from(pg, 16u * i + c);
+                const uint64_t page = mine < A.pages ? mine : 0u;
                 const unsigned char* at_k = k_base + page * A.k_page + static_cast<uint64_t>((p0 + 16u * i + c) & in_page) * A.k_token;
 #pragma unroll
                 for (uint32_t j = 0; j < kChunks; ++j) {
@@ -274,29 +305,16 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
             }
         };
         // (8 bf16 or 4 fp32: one load of 16 bytes; 4 bf16: one of 8)
-        uint4 vx[8][kBlocks];
-        // token i of a lane's eight: 4 g + i of the first 16 positions, 4 g + i - 4 of the second
-        auto v_pos = [&](uint32_t p0, uint32_t i) __attribute__((always_inline)) { return p0 + (i < 4u ? 0u : 12u) + 4u * g + i; };
-        auto load_v = [&](uint32_t p0) __attribute__((always_inline)) {
-            const unsigned char* at_v[8];
+        auto load_v = [&](uint32_t p0, uint32_t pg) __attribute__((always_inline)) {
 #pragma unroll
             for (uint32_t i = 0; i < 8u; ++i) {
-                const uint64_t page = v_pg[i / 4u] < A.pages ? v_pg[i / 4u] : 0u;
-                at_v[i] = i % 4u ? at_v[i - 1u] + A.v_token : v_base + page * A.v_page + static_cast<uint64_t>(v_pos(p0, i) & in_page) * A.v_token;
-            }
-            if (A.page_shift < 2u) {  // (uniform) fewer than four tokens a page
-#pragma unroll
-                for (uint32_t i = 0; i < 8u; ++i) {
-                    const uint32_t pos = v_pos(p0, i), pg = pos < p_end ? attend_page(A, table, pos) : 0u;
-                    at_v[i] = v_base + static_cast<uint64_t>(pg < A.pages ? pg : 0u) * A.v_page + static_cast<uint64_t>(pos & in_page) * A.v_token;
-                }
-            }
-#pragma unroll
-            for (uint32_t i = 0; i < 8u; ++i) {
+                const uint32_t mine = page_from(pg, v_pos(0u, i));
+                const uint64_t page = mine < A.pages ? mine : 0u;
+                const unsigned char* at_v = v_base + page * A.v_page + static_cast<uint64_t>(v_pos(p0, i) & in_page) * A.v_token;
 #pragma unroll
                 for (uint32_t b = 0; b < kBlocks; ++b) {
                     const uint32_t d = b * 16u * kEach + c * kEach;
-                    const unsigned char* from = at_v[i] + (d < A.head_dim ? d : 0u) * E;
+                    const unsigned char* from = at_v + (d < A.head_dim ? d : 0u) * E;
                     if constexpr (kEach * E == 16u) {
                         vx[i][b] = *reinterpret_cast<const uint4*>(from);
                     } else {
@@ -306,12 +324,9 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
                 }
             }
         };
-        // whether token i of the positions from p0 is there
-        auto there = [&](uint32_t p0, uint32_t i) __attribute__((always_inline)) {
-            const uint32_t pos = v_pos(p0, i);
-            if (pos >= p_end) return false;
-            if (A.page_shift < 2u && i % 4u != 0u) return attend_page(A, table, pos) < A.pages;
-            return v_pg[i / 4u] < A.pages;
+        // a bit for each of a lane's eight tokens, of a bit for each token from `sub` on
+        auto mine_of = [&](uint64_t all, uint32_t sub) __attribute__((always_inline)) {
+            return (static_cast<uint32_t>(all >> (sub + 4u * g)) & 15u) | (static_cast<uint32_t>(all >> (sub + 4u * g + 16u)) & 15u) << 4;
         };
 
         // the word that holds element e of a token's
@@ -401,22 +416,21 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
         if constexpr (!kStaged) {
             uint32_t p0 = u0 * kUnit + wt * 32u;
             if (p0 < p_end) {
-                pages_of(p0);
-                load_k(p0);
+                pg_now = page_of(p0);
+                pg_next = page_of(p0 + kStep);
+                load_k(p0, pg_now);
             }
             for (; p0 < p_end; p0 += kStep) {
-                load_v(p0);
-                // all 32 positions there and seen by every column (uniform)
-                const bool plain = p0 + 32u <= min(length, p_end) && A.page_shift >= 2u && __ballot(v_pg[0] >= A.pages || v_pg[1] >= A.pages) == 0ull;
-                uint32_t here = 0u;
-                if (!plain) {
-#pragma unroll
-                    for (uint32_t i = 0; i < 8u; ++i) here |= there(p0, i) ? 1u << i : 0u;
-                }
+                load_v(p0, pg_now);
+                // which of the 32 positions are there (the upper lanes say the same); whether all are and every column sees them (uniform)
+                const uint64_t have = __ballot(pg_now < A.pages);
+                const bool plain = p0 + 32u <= length && static_cast<uint32_t>(have) == 0xffffffffu;
+                const uint32_t here = mine_of(have, 0u);
                 powers(p0, plain, here, [&](uint32_t i, uint32_t j) { return kx[i][j]; }, [&]() {  // the next positions' K while these are worked on
+                    pg_now = pg_next;
                     if (p0 + kStep < p_end) {
-                        pages_of(p0 + kStep);
-                        load_k(p0 + kStep);
+                        load_k(p0 + kStep, pg_now);
+                        pg_next = page_of(p0 + 2u * kStep);
                     }
                 });
                 if (!plain) {
@@ -430,32 +444,33 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
         } else {
             unsigned char* const lds = reinterpret_cast<unsigned char*>(s_kv);
             u32x4 next_k[H::kMine], next_v[H::kMine];  // (uint4's copies of an array's elements keep it in scratch memory)
-            uint32_t next_here = 0u;  // a bit a piece of the thread
-            auto fetch = [&](uint32_t p) __attribute__((always_inline)) {
-                next_here = 0u;
+            auto fetch = [&](uint32_t p, uint32_t pg) __attribute__((always_inline)) {
 #pragma unroll
                 for (uint32_t l = 0; l < H::kMine; ++l) {
-                    const uint32_t at = l * 256u + t, token = at / H::kPieces, d = (at % H::kPieces) * Mat<DT>::kPer, pos = p + token;
-                    const uint32_t pg = pos < p_end ? attend_page(A, table, pos) : A.pages;
-                    next_here |= pg < A.pages ? 1u << l : 0u;
-                    const uint64_t page = pg < A.pages ? pg : 0u, in = pos & in_page;
+                    const uint32_t at = l * 256u + t, token = at / H::kPieces, d = (at % H::kPieces) * Mat<DT>::kPer;
+                    const uint32_t mine = page_from(pg, token);
+                    const uint64_t page = mine < A.pages ? mine : 0u, in = (p + token) & in_page;
                     const uint32_t byte = (d < A.head_dim ? d : 0u) * E;
                     next_k[l] = *reinterpret_cast<const u32x4*>(k_base + page * A.k_page + in * A.k_token + byte);
                     next_v[l] = *reinterpret_cast<const u32x4*>(v_base + page * A.v_page + in * A.v_token + byte);
                 }
             };
             uint32_t p = u0 * kUnit, buffer = 0u;
-            if (p < p_end) fetch(p);
+            if (p < p_end) {
+                pg_now = page_of(p);
+                pg_next = page_of(p + H::kTokens);
+                fetch(p, pg_now);
+            }
             for (; p < p_end; p += H::kTokens, buffer ^= 1u) {  // (the same for the workgroup)
                 unsigned char* const k_lds = lds + buffer * 2u * H::kBuffer;
                 unsigned char* const v_lds = k_lds + H::kBuffer;
-                const bool nodes = p + H::kTokens > length;  // (uniform)
-                const bool short_of = __ballot(next_here != (1u << H::kMine) - 1u) != 0ull;
-                if (short_of || nodes) {
+                const uint64_t have = __ballot(pg_now < A.pages);  // (of 32 tokens: the upper lanes say the same)
+                const bool nodes = p + H::kTokens > length;        // (uniform)
+                if (have != ~0ull || nodes) {
 #pragma unroll
                     for (uint32_t l = 0; l < H::kMine; ++l) {
                         const uint32_t token = (l * 256u + t) / H::kPieces;
-                        const uint4 v = clean(make_uint4(next_v[l].x, next_v[l].y, next_v[l].z, next_v[l].w), next_here >> l & 1u, p + token >= length);
+                        const uint4 v = clean(make_uint4(next_v[l].x, next_v[l].y, next_v[l].z, next_v[l].w), have >> token & 1u, p + token >= length);
                         next_v[l] = u32x4{v.x, v.y, v.z, v.w};
                     }
                 }
@@ -464,20 +479,20 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
                     const uint32_t at = l * 256u + t, token = at / H::kPieces, piece = at % H::kPieces;
                     *reinterpret_cast<u32x4*>(k_lds + H::place(token, piece)) = next_k[l];
                     *reinterpret_cast<u32x4*>(v_lds + H::place(token, piece)) = next_v[l];
-                    if (piece == 0u) s_here[buffer * H::kTokens + token] = next_here >> l & 1u;
                 }
+                pg_now = pg_next;
                 __syncthreads();
-                if (p + H::kTokens < p_end) fetch(p + H::kTokens);
+                if (p + H::kTokens < p_end) {
+                    fetch(p + H::kTokens, pg_now);
+                    pg_next = page_of(p + 2u * H::kTokens);
+                }
 #pragma unroll 1
                 for (uint32_t sub = 0; sub < H::kTokens && p + sub < p_end && col0 < cols; sub += 32u) {
                     const uint32_t p0 = p + sub;
-                    uint32_t here = 0u;
-#pragma unroll
-                    for (uint32_t i = 0; i < 8u; ++i) here |= s_here[buffer * H::kTokens + (v_pos(p0, i) - p)] != 0u ? 1u << i : 0u;
-                    const bool plain = p0 + 32u <= length && __ballot(here != 0xffu) == 0ull;
-                    powers(p0, plain, here, [&](uint32_t i, uint32_t j) { return *reinterpret_cast<const uint4*>(k_lds + H::place(sub + 16u * i + c, j * 4u + g)); }, []() {});
+                    const bool plain = p0 + 32u <= length && static_cast<uint32_t>(have >> sub) == 0xffffffffu;
+                    powers(p0, plain, mine_of(have, sub), [&](uint32_t i, uint32_t j) { return *reinterpret_cast<const uint4*>(k_lds + H::place(sub + 16u * i + c, j * 4u + g)); }, []() {});
                     add_up([&](uint32_t i, uint32_t b) {
-                        const uint32_t token = v_pos(p0, i) - p;
+                        const uint32_t token = v_pos(sub, i);
                         if constexpr (kEach * E == 16u) {
                             return *reinterpret_cast<const uint4*>(v_lds + H::place(token, b * 16u + c));
                         } else {
@@ -534,7 +549,7 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
                 if (any_odd) {  // (uniform)
 #pragma unroll 1
                     for (uint32_t j = 0; j < W.nodes; ++j) {
-                        const uint32_t pos = W.length + j, pg = W.length < total && pos < total ? attend_page(A, table, pos) : A.pages;
+                        const uint32_t pos = W.length + j, pg = W.length < total && pos < total ? attend_page(A, table, pos, total) : A.pages;
                         if (pg >= A.pages) continue;
                         const unsigned char* at_v = v_base + static_cast<uint64_t>(pg) * A.v_page + static_cast<uint64_t>(pos & in_page) * A.v_token;
 #pragma unroll
@@ -557,24 +572,7 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
                     if (A.lse && g == 0u)
                         A.lse[static_cast<uint64_t>(W.first + node) * A.heads + h] = sum[m] == 0.f ? -INFINITY : (top[m] + __builtin_amdgcn_logf(sum[m])) * 0.69314718f;
                     unsigned char* to = A.out + static_cast<uint64_t>(W.first + node) * A.out_row + static_cast<uint64_t>(h) * A.out_head;
-#pragma unroll
-                    for (uint32_t b = 0; b < kBlocks; ++b)
-#pragma unroll
-                        for (uint32_t l = 0; l < 4u; ++l) {
-                            const uint32_t d = b * 16u * kEach + (4u * g + l) * kEach;
-                            if (d >= A.head_dim) continue;
-                            if constexpr (DT == 1) {
-                                __bf16 y[kEach];
-#pragma unroll
-                                for (uint32_t e = 0; e < kEach; ++e) y[e] = static_cast<__bf16>(o[m][b * kEach + e][l] * by);
-                                __builtin_memcpy(to + d * 2u, y, kEach * 2u);
-                            } else {
-                                float y[kEach];
-#pragma unroll
-                                for (uint32_t e = 0; e < kEach; ++e) y[e] = o[m][b * kEach + e][l] * by;
-                                __builtin_memcpy(to + d * 4u, y, kEach * 4u);
-                            }
-                        }
+                    attend_write<DT, kEach, kBlocks>(A, to, g, o[m], by);
                 }
             } else {
                 float* part = A.part + (static_cast<uint64_t>(run_id) * 2u + (u0 == 0u ? 1u : 0u)) * H::kPartFloats + wm * MS * H::kSubFloats;
@@ -607,71 +605,86 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
     if (t == 0u) A.run[run_id].odd = run_odd;
 }
 
-// A workgroup joins 16 columns of the tile that begins in run x: the tile's first piece is that run's second part, the others are the first parts of the runs behind it. Every thread has one or
-// more of the lanes' four floats, and goes through the pieces in order.
+// A workgroup joins 16 columns of the tile that begins in run x: the tile's first piece is that run's second part, the others are the first parts of the runs behind it. A wave takes every eighth
+// piece, the next while it adds one, and what the waves have is joined through LDS, in an order that does not depend on who comes first.
+constexpr uint32_t kJoinWaves = 8u;
 template <int DT, int DP, int MS, int WM>
-__global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs A) {
+__global__ void __launch_bounds__(64 * kJoinWaves) attend_join_kernel(AttendArgs A) {
     typedef AttendShape<DT, DP, MS, WM> H;
-    const uint32_t x = blockIdx.x, sub = blockIdx.y, t = threadIdx.x;
+    constexpr uint32_t kOuts = H::kOuts, kEach = H::kEach;
+    __shared__ f32x4 s_o[kJoinWaves / 2u][kOuts][64];
+    __shared__ float s_top[kJoinWaves / 2u][64], s_sum[kJoinWaves / 2u][64];
+    const uint32_t x = blockIdx.x, sub = blockIdx.y, t = threadIdx.x, lane = t & 63u, wave = t >> 6, c = lane & 15u, g = lane >> 4;
     const AttendRun R = A.run[x];
     if (R.more == 0u) return;
     const AttendWork W = attend_work(A, R.seq, H::kTileCols);
-    const uint32_t cols = W.nodes * A.group, col0 = R.tile * H::kTileCols + sub * 16u;
-    if (col0 >= cols) return;
+    const uint32_t cols = W.nodes * A.group, col = R.tile * H::kTileCols + sub * 16u + c;
+    if (col - c >= cols) return;
     auto piece = [&](uint32_t i) { return A.part + ((static_cast<uint64_t>(x) + i) * 2u + (i == 0u ? 1u : 0u)) * H::kPartFloats + sub * H::kSubFloats; };
-    const uint32_t lane = t & 63u, c = lane & 15u, g = lane >> 4;
-    float top = -FLT_MAX;
-    for (uint32_t i = 0; i <= R.more; ++i) top = fmaxf(top, piece(i)[lane]);  // (NaN in a sum, not in a maximum)
-    constexpr uint32_t kMine = (H::kOuts + 3u) / 4u;
-    f32x4 o[kMine];
-    float sum = 0.f;
+    float top = -FLT_MAX, sum = 0.f;
+    f32x4 o[kOuts];
 #pragma unroll
-    for (uint32_t r = 0; r < kMine; ++r) o[r] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (uint32_t i = 0; i <= R.more; ++i) {
+    for (uint32_t r = 0; r < kOuts; ++r) o[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float their_top = -FLT_MAX, their_sum = 0.f;
+    f32x4 theirs[kOuts];
+    auto load = [&](uint32_t i) __attribute__((always_inline)) {
         const float* from = piece(i);
-        const float by = __builtin_amdgcn_exp2f(from[lane] - top);
-        sum = fmaf(from[64u + lane], by, sum);
+        their_top = from[lane];
+        their_sum = from[64u + lane];
 #pragma unroll
-        for (uint32_t r = 0; r < kMine; ++r) {
-            const uint32_t out = wave_id() * kMine + r;
-            if (out < H::kOuts) o[r] += *reinterpret_cast<const f32x4*>(from + 128u + (out * 64u + lane) * 4u) * by;
+        for (uint32_t r = 0; r < kOuts; ++r) theirs[r] = *reinterpret_cast<const f32x4*>(from + 128u + (r * 64u + lane) * 4u);
+    };
+    auto join = [&]() __attribute__((always_inline)) {
+        const float to = fmaxf(top, their_top), a = __builtin_amdgcn_exp2f(top - to), z = __builtin_amdgcn_exp2f(their_top - to);
+        top = to;
+        sum = sum * a + their_sum * z;
+#pragma unroll
+        for (uint32_t r = 0; r < kOuts; ++r) o[r] = o[r] * a + theirs[r] * z;
+    };
+    if (wave <= R.more) load(wave);
+    for (uint32_t i = wave; i <= R.more; i += kJoinWaves) {
+        join();
+        if (i + kJoinWaves <= R.more) load(i + kJoinWaves);
+    }
+#pragma unroll
+    for (uint32_t half = kJoinWaves / 2u; half >= 1u; half /= 2u) {
+        __syncthreads();
+        if (wave >= half && wave < 2u * half) {
+            s_top[wave - half][lane] = top;
+            s_sum[wave - half][lane] = sum;
+#pragma unroll
+            for (uint32_t r = 0; r < kOuts; ++r) s_o[wave - half][r][lane] = o[r];
+        }
+        __syncthreads();
+        if (wave < half) {
+            their_top = s_top[wave][lane];
+            their_sum = s_sum[wave][lane];
+#pragma unroll
+            for (uint32_t r = 0; r < kOuts; ++r) theirs[r] = s_o[wave][r][lane];
+            join();
         }
     }
-    const uint32_t col = col0 + c;
-    if (col >= cols) return;
+    if (wave != 0u || col >= cols) return;
     const uint32_t node = col / A.group, h = R.head * A.group + (col - node * A.group);
     if (A.run[x + R.more].odd != 0u) {
         const int32_t* table = A.table + static_cast<uint64_t>(A.slot ? A.slot[R.seq] : R.seq) * A.table_stride;
         const uint64_t sees = A.mask ? A.mask[W.first + node] : (node < 63u ? (uint64_t{2} << node) - 1u : ~uint64_t{0});
 #pragma unroll 1
         for (uint32_t j = 0; j < W.nodes && W.length + j < W.total; ++j) {
-            const uint32_t pos = W.length + j, pg = attend_page(A, table, pos);
+            const uint32_t pos = W.length + j, pg = attend_page(A, table, pos, W.total);
             if (pg >= A.pages) continue;
             const unsigned char* at_v = A.v + static_cast<uint64_t>(pg) * A.v_page + static_cast<uint64_t>(pos & ((1u << A.page_shift) - 1u)) * A.v_token + static_cast<uint64_t>(R.head) * A.v_head;
 #pragma unroll
-            for (uint32_t r = 0; r < kMine; ++r) {
-                const uint32_t out = wave_id() * kMine + r;
+            for (uint32_t r = 0; r < kOuts; ++r) {
 #pragma unroll
-                for (uint32_t l = 0; l < 4u; ++l)
-                    o[r][l] += attend_odd<DT>(A, at_v, (out / H::kEach) * 16u * H::kEach + (4u * g + l) * H::kEach + out % H::kEach, (sees >> j & 1u) != 0u);
+                for (uint32_t l = 0; l < 4u; ++l) o[r][l] += attend_odd<DT>(A, at_v, (r / kEach) * 16u * kEach + (4u * g + l) * kEach + r % kEach, (sees >> j & 1u) != 0u);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
     const float by = sum == 0.f ? 0.f : 1.f / sum;
-    if (A.lse && t < 16u) A.lse[static_cast<uint64_t>(W.first + node) * A.heads + h] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * 0.69314718f;
-    unsigned char* to = A.out + static_cast<uint64_t>(W.first + node) * A.out_row + static_cast<uint64_t>(h) * A.out_head;
-#pragma unroll
-    for (uint32_t r = 0; r < kMine; ++r) {
-        const uint32_t out = wave_id() * kMine + r;
-        if (out >= H::kOuts) continue;
-#pragma unroll
-        for (uint32_t l = 0; l < 4u; ++l) {
-            const uint32_t d = (out / H::kEach) * 16u * H::kEach + (4u * g + l) * H::kEach + out % H::kEach;
-            if (d >= A.head_dim) continue;
-            if constexpr (DT == 1) reinterpret_cast<__bf16*>(to)[d] = static_cast<__bf16>(o[r][l] * by);
-            else reinterpret_cast<float*>(to)[d] = o[r][l] * by;
-        }
-    }
+    if (A.lse && g == 0u) A.lse[static_cast<uint64_t>(W.first + node) * A.heads + h] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * 0.69314718f;
+    attend_write<DT, kEach, H::kBlocks>(A, A.out + static_cast<uint64_t>(W.first + node) * A.out_row + static_cast<uint64_t>(h) * A.out_head, g, o, by);
 }
 
 }  // namespace ws

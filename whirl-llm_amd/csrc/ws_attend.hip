@@ -16,7 +16,7 @@ struct Build {
 template <int DT, int DP, int MS, int WM, int OCC>
 void launch(hipStream_t s, const AttendArgs& a) {
     hipLaunchKernelGGL((attend_kernel<DT, DP, MS, WM, OCC>), dim3(a.groups), dim3(kAttendThreads), 0, s, a);
-    hipLaunchKernelGGL((attend_join_kernel<DT, DP, MS, WM>), dim3(a.groups, MS * WM), dim3(kAttendThreads), 0, s, a);
+    hipLaunchKernelGGL((attend_join_kernel<DT, DP, MS, WM>), dim3(a.groups, MS * WM), dim3(64 * kJoinWaves), 0, s, a);
 }
 template <int DT, int DP, int MS, int WM, int OCC>
 constexpr Build build(uint32_t cols) {
@@ -25,7 +25,7 @@ constexpr Build build(uint32_t cols) {
 constexpr uint32_t kAny = 0xffffffffu;
 constexpr Build kBuilds[] = {
     build<1, 64, 1, 1, 3>(16), build<1, 64, 2, 1, 2>(32), build<1, 64, 1, 4, 2>(64), build<1, 64, 2, 4, 2>(kAny),
-    build<1, 128, 1, 1, 2>(16), build<1, 128, 1, 4, 2>(64), build<1, 128, 2, 4, 2>(128), build<1, 128, 4, 4, 1>(kAny),
+    build<1, 128, 1, 1, 2>(16), build<1, 128, 1, 4, 2>(64), build<1, 128, 2, 4, 2>(kAny),
     build<1, 256, 1, 1, 1>(16), build<1, 256, 1, 4, 1>(kAny),
     build<0, 64, 1, 1, 2>(16), build<0, 64, 1, 4, 2>(64), build<0, 64, 2, 4, 2>(kAny),
     build<0, 128, 1, 4, 2>(kAny), build<0, 256, 1, 4, 1>(kAny),
