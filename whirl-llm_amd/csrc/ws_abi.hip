@@ -1460,8 +1460,12 @@ int ws_tree_attention(void* stream, const ws_tree_attention_args* a, void* works
     ws::AttendArgs g{};
     g.k = static_cast<const unsigned char*>(c.k);
     g.v = static_cast<const unsigned char*>(c.v);
-    g.k_page = c.k_page * e, g.k_token = c.k_token * e, g.k_head = c.k_head * e;
-    g.v_page = c.v_page * e, g.v_token = c.v_token * e, g.v_head = c.v_head * e;
+    // (a stride whose dimension has one entry is never taken)
+    const uint64_t pieces[4] = {c.pages > 1u ? c.k_page * e / 16u : 0u, c.page_tokens > 1u ? c.k_token * e / 16u : 0u, c.pages > 1u ? c.v_page * e / 16u : 0u, c.page_tokens > 1u ? c.v_token * e / 16u : 0u};
+    for (const uint64_t stride : pieces)
+        if (stride >> 32) return WS_E_UNSUPPORTED;
+    g.k_page = static_cast<uint32_t>(pieces[0]), g.k_token = static_cast<uint32_t>(pieces[1]), g.v_page = static_cast<uint32_t>(pieces[2]), g.v_token = static_cast<uint32_t>(pieces[3]);
+    g.k_head = c.k_head * e, g.v_head = c.v_head * e;
     g.pages = c.pages;
     g.page_shift = shift_of(c.page_tokens);
     g.kv_heads = c.kv_heads;

@@ -72,6 +72,10 @@ struct Mat<0> {  // fp32: four products of depth 4, lane group g's i-th element 
     static __device__ __forceinline__ float element(const unsigned char* at, uint32_t i) { return reinterpret_cast<const float*>(at)[i]; }
 };
 
+// The larger of two, as the middle of them and infinity. (Of fmaxf the compiler makes another instruction a value, to quiet NaN; inline assembly may not read what the matrix cores have
+// just written: the compiler does not see to the pause that takes.)
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
+
 // A build: DT, DP (head_dim rounded up to 64, 128 or 256), MS tiles of 16 columns a wave, WM waves over columns (4 / WM over positions)
 template <int DT, int DP, int MS, int WM>
 struct AttendShape {
@@ -204,6 +208,11 @@ __device__ __forceinline__ void attend_write(const AttendArgs& A, unsigned char*
         }
 }
 
+// bytes to a token's piece of 16 bytes, from strides in such pieces: two multiplications of 32 bits, added up in 64
+__device__ __forceinline__ uint64_t attend_offset(uint32_t page, uint32_t page_stride, uint32_t token, uint32_t token_stride, uint32_t piece) {
+    return (static_cast<uint64_t>(page) * page_stride + (static_cast<uint64_t>(token) * token_stride + piece)) << 4;
+}
+
 // the page of a position of the slot whose table row this is; `pages` where there is none. (No branch: what is loaded behind one is waited for there, and with it everything loaded before.)
 __device__ __forceinline__ uint32_t attend_page(const AttendArgs& A, const int32_t* row, uint32_t pos, uint32_t end) {
     const uint32_t at = pos >> A.page_shift, page = static_cast<uint32_t>(row[min(at, A.slot_pages - 1u)]);
@@ -276,8 +285,8 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
 #pragma unroll
             for (uint32_t r = 0; r < kOuts; ++r) o[m][r] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
-        const unsigned char* k_base = A.k + static_cast<uint64_t>(head) * A.k_head;
-        const unsigned char* v_base = A.v + static_cast<uint64_t>(head) * A.v_head;
+        const unsigned char* k_base = A.k + head * A.k_head;
+        const unsigned char* v_base = A.v + head * A.v_head;
         const uint32_t in_page = (1u << A.page_shift) - 1u;
 
         const uint32_t p_end = min(u1 * kUnit, total);
@@ -285,7 +294,13 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
         constexpr uint32_t kAhead = kStaged ? H::kTokens : 32u;
         auto page_of = [&](uint32_t p) __attribute__((always_inline)) { return attend_page(A, table, p + (lane & (kAhead - 1u)), p_end); };
         auto page_from = [&](uint32_t pg, uint32_t token) __attribute__((always_inline)) { return static_cast<uint32_t>(__shfl(static_cast<int>(pg), static_cast<int>(token))); };
-        uint32_t pg_now = 0u, pg_next = 0u;
+        // pg: of the positions that are worked on next; have: a bit for each that is there. (A page that is not: the first one's, not looked at.)
+        uint32_t pg = 0u, pg_next = 0u;
+        uint64_t have = 0ull;
+        auto turn = [&]() __attribute__((always_inline)) {
+            have = __ballot(pg_next < A.pages);  // (of 32 positions: the upper lanes say the same)
+            pg = pg_next < A.pages ? pg_next : 0u;
+        };
         uint4 kx[2][kChunks];
         uint4 vx[8][kBlocks];
         // token i of a lane's eight: 4 g + i of the first 16 positions, 4 g + i - 4 of the second
@@ -293,10 +308,7 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
         auto load_k = [&](uint32_t p0, uint32_t pg) __attribute__((always_inline)) {
 #pragma unroll
             for (uint32_t i = 0; i < 2u; ++i) {
-                // (a page that is not there: the first one's, not looked at)
-                const uint32_t mine = page_from(pg, 16u * i + c);
-                const uint64_t page = mine < A.pages ? mine : 0u;
-                const unsigned char* at_k = k_base + page * A.k_page + static_cast<uint64_t>((p0 + 16u * i + c) & in_page) * A.k_token;
+                const unsigned char* at_k = k_base + attend_offset(page_from(pg, 16u * i + c), A.k_page, (p0 + 16u * i + c) & in_page, A.k_token, 0u);
 #pragma unroll
                 for (uint32_t j = 0; j < kChunks; ++j) {
                     const uint32_t d = j * Mat<DT>::kDepth + g * Mat<DT>::kPer;
@@ -308,9 +320,7 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
         auto load_v = [&](uint32_t p0, uint32_t pg) __attribute__((always_inline)) {
 #pragma unroll
             for (uint32_t i = 0; i < 8u; ++i) {
-                const uint32_t mine = page_from(pg, v_pos(0u, i));
-                const uint64_t page = mine < A.pages ? mine : 0u;
-                const unsigned char* at_v = v_base + page * A.v_page + static_cast<uint64_t>(v_pos(p0, i) & in_page) * A.v_token;
+                const unsigned char* at_v = v_base + attend_offset(page_from(pg, v_pos(0u, i)), A.v_page, v_pos(p0, i) & in_page, A.v_token, 0u);
 #pragma unroll
                 for (uint32_t b = 0; b < kBlocks; ++b) {
                     const uint32_t d = b * 16u * kEach + c * kEach;
@@ -359,7 +369,7 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
             }
 #pragma unroll
             for (int m = 0; m < MS; ++m) {
-                float most = fmaxf(fmaxf(fmaxf(x[m][0][0], x[m][0][1]), fmaxf(x[m][0][2], x[m][0][3])), fmaxf(fmaxf(x[m][1][0], x[m][1][1]), fmaxf(x[m][1][2], x[m][1][3])));
+                float most = larger(larger(larger(x[m][0][0], x[m][0][1]), larger(x[m][0][2], x[m][0][3])), larger(larger(x[m][1][0], x[m][1][1]), larger(x[m][1][2], x[m][1][3])));
                 most *= A.scale_log2;
                 float p[8];
                 if (__ballot(most > top[m] + kSlack) != 0ull) {  // (uniform) some column's maximum has grown
@@ -416,20 +426,20 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
         if constexpr (!kStaged) {
             uint32_t p0 = u0 * kUnit + wt * 32u;
             if (p0 < p_end) {
-                pg_now = page_of(p0);
+                pg_next = page_of(p0);
+                turn();
                 pg_next = page_of(p0 + kStep);
-                load_k(p0, pg_now);
+                load_k(p0, pg);
             }
             for (; p0 < p_end; p0 += kStep) {
-                load_v(p0, pg_now);
-                // which of the 32 positions are there (the upper lanes say the same); whether all are and every column sees them (uniform)
-                const uint64_t have = __ballot(pg_now < A.pages);
+                load_v(p0, pg);
+                // whether all 32 positions are there and every column sees them (uniform)
                 const bool plain = p0 + 32u <= length && static_cast<uint32_t>(have) == 0xffffffffu;
                 const uint32_t here = mine_of(have, 0u);
                 powers(p0, plain, here, [&](uint32_t i, uint32_t j) { return kx[i][j]; }, [&]() {  // the next positions' K while these are worked on
-                    pg_now = pg_next;
                     if (p0 + kStep < p_end) {
-                        load_k(p0 + kStep, pg_now);
+                        turn();
+                        load_k(p0 + kStep, pg);
                         pg_next = page_of(p0 + 2u * kStep);
                     }
                 });
@@ -444,33 +454,32 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
         } else {
             unsigned char* const lds = reinterpret_cast<unsigned char*>(s_kv);
             u32x4 next_k[H::kMine], next_v[H::kMine];  // (uint4's copies of an array's elements keep it in scratch memory)
-            auto fetch = [&](uint32_t p, uint32_t pg) __attribute__((always_inline)) {
+            auto fetch = [&](uint32_t p) __attribute__((always_inline)) {
 #pragma unroll
                 for (uint32_t l = 0; l < H::kMine; ++l) {
                     const uint32_t at = l * 256u + t, token = at / H::kPieces, d = (at % H::kPieces) * Mat<DT>::kPer;
-                    const uint32_t mine = page_from(pg, token);
-                    const uint64_t page = mine < A.pages ? mine : 0u, in = (p + token) & in_page;
-                    const uint32_t byte = (d < A.head_dim ? d : 0u) * E;
-                    next_k[l] = *reinterpret_cast<const u32x4*>(k_base + page * A.k_page + in * A.k_token + byte);
-                    next_v[l] = *reinterpret_cast<const u32x4*>(v_base + page * A.v_page + in * A.v_token + byte);
+                    const uint32_t page = page_from(pg, token), in = (p + token) & in_page, piece = (d < A.head_dim ? d : 0u) * E / 16u;
+                    next_k[l] = *reinterpret_cast<const u32x4*>(k_base + attend_offset(page, A.k_page, in, A.k_token, piece));
+                    next_v[l] = *reinterpret_cast<const u32x4*>(v_base + attend_offset(page, A.v_page, in, A.v_token, piece));
                 }
             };
             uint32_t p = u0 * kUnit, buffer = 0u;
             if (p < p_end) {
-                pg_now = page_of(p);
+                pg_next = page_of(p);
+                turn();
                 pg_next = page_of(p + H::kTokens);
-                fetch(p, pg_now);
+                fetch(p);
             }
             for (; p < p_end; p += H::kTokens, buffer ^= 1u) {  // (the same for the workgroup)
                 unsigned char* const k_lds = lds + buffer * 2u * H::kBuffer;
                 unsigned char* const v_lds = k_lds + H::kBuffer;
-                const uint64_t have = __ballot(pg_now < A.pages);  // (of 32 tokens: the upper lanes say the same)
+                const uint64_t here = have;
                 const bool nodes = p + H::kTokens > length;        // (uniform)
-                if (have != ~0ull || nodes) {
+                if (here != ~0ull || nodes) {
 #pragma unroll
                     for (uint32_t l = 0; l < H::kMine; ++l) {
                         const uint32_t token = (l * 256u + t) / H::kPieces;
-                        const uint4 v = clean(make_uint4(next_v[l].x, next_v[l].y, next_v[l].z, next_v[l].w), have >> token & 1u, p + token >= length);
+                        const uint4 v = clean(make_uint4(next_v[l].x, next_v[l].y, next_v[l].z, next_v[l].w), here >> token & 1u, p + token >= length);
                         next_v[l] = u32x4{v.x, v.y, v.z, v.w};
                     }
                 }
@@ -480,17 +489,17 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
                     *reinterpret_cast<u32x4*>(k_lds + H::place(token, piece)) = next_k[l];
                     *reinterpret_cast<u32x4*>(v_lds + H::place(token, piece)) = next_v[l];
                 }
-                pg_now = pg_next;
                 __syncthreads();
                 if (p + H::kTokens < p_end) {
-                    fetch(p + H::kTokens, pg_now);
+                    turn();
+                    fetch(p + H::kTokens);
                     pg_next = page_of(p + 2u * H::kTokens);
                 }
 #pragma unroll 1
                 for (uint32_t sub = 0; sub < H::kTokens && p + sub < p_end && col0 < cols; sub += 32u) {
                     const uint32_t p0 = p + sub;
-                    const bool plain = p0 + 32u <= length && static_cast<uint32_t>(have >> sub) == 0xffffffffu;
-                    powers(p0, plain, mine_of(have, sub), [&](uint32_t i, uint32_t j) { return *reinterpret_cast<const uint4*>(k_lds + H::place(sub + 16u * i + c, j * 4u + g)); }, []() {});
+                    const bool plain = p0 + 32u <= length && static_cast<uint32_t>(here >> sub) == 0xffffffffu;
+                    powers(p0, plain, mine_of(here, sub), [&](uint32_t i, uint32_t j) { return *reinterpret_cast<const uint4*>(k_lds + H::place(sub + 16u * i + c, j * 4u + g)); }, []() {});
                     add_up([&](uint32_t i, uint32_t b) {
                         const uint32_t token = v_pos(sub, i);
                         if constexpr (kEach * E == 16u) {
@@ -551,7 +560,7 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
                     for (uint32_t j = 0; j < W.nodes; ++j) {
                         const uint32_t pos = W.length + j, pg = W.length < total && pos < total ? attend_page(A, table, pos, total) : A.pages;
                         if (pg >= A.pages) continue;
-                        const unsigned char* at_v = v_base + static_cast<uint64_t>(pg) * A.v_page + static_cast<uint64_t>(pos & in_page) * A.v_token;
+                        const unsigned char* at_v = v_base + attend_offset(pg, A.v_page, pos & in_page, A.v_token, 0u);
 #pragma unroll
                         for (uint32_t r = 0; r < kOuts; ++r) {
 #pragma unroll
@@ -673,7 +682,7 @@ __global__ void __launch_bounds__(64 * kJoinWaves) attend_join_kernel(AttendArgs
         for (uint32_t j = 0; j < W.nodes && W.length + j < W.total; ++j) {
             const uint32_t pos = W.length + j, pg = attend_page(A, table, pos, W.total);
             if (pg >= A.pages) continue;
-            const unsigned char* at_v = A.v + static_cast<uint64_t>(pg) * A.v_page + static_cast<uint64_t>(pos & ((1u << A.page_shift) - 1u)) * A.v_token + static_cast<uint64_t>(R.head) * A.v_head;
+            const unsigned char* at_v = A.v + R.head * A.v_head + attend_offset(pg, A.v_page, pos & ((1u << A.page_shift) - 1u), A.v_token, 0u);
 #pragma unroll
             for (uint32_t r = 0; r < kOuts; ++r) {
 #pragma unroll

@@ -56,7 +56,8 @@ int prepare_tree();
 struct AttendArgs {
     const unsigned char* k;
     const unsigned char* v;
-    uint64_t k_page, k_token, k_head, v_page, v_token, v_head;  // bytes
+    uint32_t k_page, k_token, v_page, v_token;  // pieces of 16 bytes between
+    uint64_t k_head, v_head;                    // bytes
     uint32_t pages, page_shift, kv_heads, head_dim;
     const int32_t* table;
     uint32_t slots, slot_pages;
