@@ -60,15 +60,19 @@ def test_verification_workspaces():
     m = gc.pkg()
     r, a = rows_of(m, vocab=151936, row_stride=151936), verify_of(m)
     need = m.lib().ws_verify_tree_workspace(C.byref(r), C.byref(a))
-    assert need >= 2 * 2 * 80
+    assert need >= 32 + 2 * 2 * 32 + 4 * 16
     for at, size in ((None, need), (AT, need - 1), (AT + 4, need)):
         assert m.lib().ws_verify_tree(None, C.byref(r), C.byref(a), at, size) == m.E_WORKSPACE
     assert m.lib().ws_verify_tree(None, C.byref(r), None, AT, need) == m.lib().ws_verify_tree(None, None, C.byref(a), AT, need) == m.E_INVALID
     assert m.lib().ws_verify_tree(None, C.byref(r), C.byref(verify_of(m, n_seq=0)), None, 0) == 0  # nothing to do
     for dtype in (0, 1):  # the longest rows: as many parts as can meet
         for n_seq in (1, 300, 5000):
-            r = rows_of(m, vocab=1048575, row_stride=1048575, dtype=dtype, logits=AT)
-            parts = m.lib().ws_verify_tree_workspace(C.byref(r), C.byref(verify_of(m, n_seq=n_seq))) / (n_seq * 80)
+            r = rows_of(m, vocab=1048575, row_stride=1048575, dtype=dtype, rows=0)
+            draw = m.lib().ws_verify_tree_workspace(C.byref(r), C.byref(verify_of(m, n_seq=n_seq)))
+            parts = (draw - 32) / (n_seq * 32)
+            assert parts == int(parts) and 2 <= parts <= 64
+            r.rows = 64 * n_seq
+            parts = (m.lib().ws_verify_tree_workspace(C.byref(r), C.byref(verify_of(m, n_seq=n_seq))) - draw - r.rows * 16) / (r.rows * 32)
             assert parts == int(parts) and 2 <= parts <= 64
 
 

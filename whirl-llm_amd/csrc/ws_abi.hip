@@ -1321,13 +1321,30 @@ constexpr uint32_t kMostTrees = 1048575u;
 static_assert(WS_TREE_MAX == ws::kTreeNodes && WS_Q_MAX == ws::kTreeListed && WS_Q_WORDS == ws::kTreeEntryWords);
 static_assert(WS_CACHE_MOST == ws::kCacheMost && WS_CACHE_MOST == WS_BLOCK);
 
-// Workgroups a sequence of the verification: two a compute unit where sequences are few, of 256 vectors at least; as many as hold the row in registers
-uint32_t verify_parts(const ws_loss_rows* r, uint32_t n_seq) {
+// The verification's workgroups. A sequence's draw: two a compute unit where sequences are few, of 256 vectors at least; as many as hold the row in registers. A row's decision: shares of
+// 2048 vectors at least, larger ones where there are many rows, so that fewer workgroups begin at the ends of trips to memory. Parts, us: 64 trees of 16 x 151936 bf16 62: 109, 12: 33.7, 6: 32.1, 3: 35.1, 1: 47.5;
+// 256 of 25 x 50257 fp32, masked, 42: 777, 8: 202, 4: 134, 2: 110, 1: 121; five rows of 151936 bf16 62: 15.6, 37: 13.2, 12: 11.8, 6: 12.5, 1: 22.8. Words: the draw's, the decisions, the rows' sums.
+struct VerifyPlan {
+    uint32_t parts, row_parts, levels;
+    uint64_t meet, decided, bytes;
+};
+VerifyPlan verify_plan(const ws_loss_rows* r, uint32_t n_seq) {
+    VerifyPlan p{};
     const uint32_t per = r->dtype == WS_DTYPE_F32 ? 4u : 8u, vectors = (r->vocab + per - 1u) / per, least = (vectors + ws::tree_most_share() - 1u) / ws::tree_most_share();
     uint32_t parts = n_seq ? 2u * static_cast<uint32_t>(compute_units()) / n_seq : 1u;
     if (parts > vectors / 256u) parts = vectors / 256u;
     if (parts < least) parts = least;
-    return parts < 1u ? 1u : (parts > 64u ? 64u : parts);
+    p.parts = parts < 1u ? 1u : (parts > 64u ? 64u : parts);
+    const uint32_t most = row_vectors(r) / 2048u, rows = r->rows ? r->rows : 1u;
+    p.row_parts = (32u * static_cast<uint32_t>(compute_units()) + rows / 2u) / rows;
+    if (p.row_parts > most) p.row_parts = most;
+    p.row_parts = p.row_parts < 1u ? 1u : (p.row_parts > 64u ? 64u : p.row_parts);
+    p.levels = n_seq ? (r->rows + n_seq - 1u) / n_seq : 1u;  // (as many nodes as a sequence has on average; a larger one's take turns)
+    p.levels = p.levels < 1u ? 1u : (p.levels > WS_TREE_MAX ? WS_TREE_MAX : p.levels);
+    p.meet = 32u + meet_bytes(n_seq, p.parts, ws::kTreeWords);  // (behind the epochs)
+    p.decided = p.meet + uint64_t{r->rows} * 16u;
+    p.bytes = p.decided + meet_bytes(r->rows, p.row_parts, 4u);
+    return p;
 }
 bool verify_ok(const ws_loss_rows* r, const ws_verify_tree_args* a) {
     if (!loss_rows_ok(r) || !a || a->n_seq > kMostTrees || a->depth < 1u || a->depth > WS_TREE_MAX || a->spins > kMostLooks) return false;
@@ -1410,13 +1427,14 @@ int ws_tree_stage(void* stream, const ws_tree_stage_args* a) {
 }
 
 uint64_t ws_verify_tree_workspace(const ws_loss_rows* r, const ws_verify_tree_args* a) {
-    return verify_ok(r, a) && a->n_seq ? meet_bytes(a->n_seq, verify_parts(r, a->n_seq), ws::kTreeWords) : 0u;
+    return verify_ok(r, a) && a->n_seq ? verify_plan(r, a->n_seq).bytes : 0u;
 }
 
 int ws_verify_tree(void* stream, const ws_loss_rows* r, const ws_verify_tree_args* a, void* workspace, uint64_t workspace_bytes) {
     if (!verify_ok(r, a)) return WS_E_INVALID;
     if (a->n_seq == 0) return WS_OK;
-    if (!workspace_ok(workspace, workspace_bytes, ws_verify_tree_workspace(r, a))) return WS_E_WORKSPACE;
+    const VerifyPlan plan = verify_plan(r, a->n_seq);
+    if (!workspace_ok(workspace, workspace_bytes, plan.bytes)) return WS_E_WORKSPACE;
     ws::TreeVerifyArgs v{};
     v.R = loss_rows(r);
     v.n_seq = a->n_seq;
@@ -1435,10 +1453,19 @@ int ws_verify_tree(void* stream, const ws_loss_rows* r, const ws_verify_tree_arg
     v.logprob = a->logprob;
     v.hist = ws::HistoryRef{a->hist.tokens, a->hist.len, a->hist.n_gen, a->hist.slot, a->hist.cap};
     const uint32_t per = r->dtype == WS_DTYPE_F32 ? 4u : 8u;
-    v.parts = verify_parts(r, a->n_seq);
+    unsigned char* const work = static_cast<unsigned char*>(workspace);
+    v.levels = plan.levels;
+    v.row_parts = plan.row_parts;
+    v.row_per = share_of(row_vectors(r), plan.row_parts);
+    // (Whether a row's parent is asked first: where not all rows' workgroups run at once anyway, so that some have decided when others begin.)
+    v.look = uint64_t{r->rows} * plan.row_parts > 8u * static_cast<uint64_t>(compute_units()) ? 1u : 0u;
+    v.decided = reinterpret_cast<unsigned long long*>(work + plan.meet);
+    v.row_meet = reinterpret_cast<unsigned long long*>(work + plan.decided);
+    v.parts = plan.parts;
     v.per = share_of((r->vocab + per - 1u) / per, v.parts);
     v.looks = a->spins ? a->spins : 256u;
-    v.meet = static_cast<unsigned long long*>(workspace);
+    v.epoch = reinterpret_cast<unsigned long long*>(work);
+    v.meet = reinterpret_cast<unsigned long long*>(work + 32u);
     v.tag = launch_tag();
     return ws::launch_tree_verify(S(stream), r->dtype, v);
 }

@@ -40,12 +40,18 @@ struct TreeVerifyArgs {
     uint32_t* status;
     float* logprob;
     HistoryRef hist;
-    uint32_t parts, per, looks;  // workgroups a sequence, vectors each (at most T * NV)
-    unsigned long long* meet;    // parts > 1: [n_seq][kTreeWords][parts]
+    // of the rows' decisions: nodes of a sequence that have workgroups of their own, whether a node asks for its parent's decision first, workgroups a row, vectors each
+    uint32_t levels, look, row_parts, row_per;
+    unsigned long long* row_meet;  // row_parts > 1: [rows][4][row_parts]
+    unsigned long long* decided;   // [rows][2]
+    unsigned long long* epoch;     // [3]
+    // of the draw: workgroups a sequence, vectors each (at most T * NV), how often one looks for the others
+    uint32_t parts, per, looks;
+    unsigned long long* meet;  // parts > 1: [n_seq][kTreeWords][parts]
     unsigned long long tag;
 };
-// 64-bit words a part: two steps' m and S, each twice, and a mark, twice
-constexpr uint32_t kTreeWords = 10u;
+// 64-bit words a part: maximum and sum, each twice
+constexpr uint32_t kTreeWords = 4u;
 
 int launch_tree_stage(hipStream_t stream, const TreeStageArgs& a);
 int launch_tree_verify(hipStream_t stream, int dtype, const TreeVerifyArgs& a);

@@ -2,8 +2,12 @@
 //
 // Verification. With w_v = exp((x_v - m) t) over the allowed tokens of a node's row, S = sum w_v and P = w / S, a child with token y is accepted if u Q(y) < P(y); after
 // a rejection P becomes max(P - Q, 0) divided by its sum Z. Q is 0 but at 32 ids at most (or at one, where the child is a guess), so that outside of them P stays w times one number c:
-// what a walk carries along is c and the P and Q of those ids, a lane each, and the mass outside of them, 1 - sum P at first. No pass over the row is made for a rejection. What is read:
-// the rows that the walk meets, once, for m and S; the one that it ends at a second time, out of the registers that hold it.
+// what is carried along is c and the P and Q of those ids, a lane each, and the mass outside of them, 1 - sum P at first. No pass over the row is made for a rejection.
+//
+// Which child a node passes the walk on to, if any, does not depend on how the walk came to it. So tree_rows_kernel decides all nodes with children at once, one pass over a row, its workgroups meeting
+// without waiting; nodes are numbered level by level as far as the grid can, and one whose parent has decided against it by then is not read. (A kernel that walked, row after row, waited for memory
+// and for its parts at each: 64 trees of 16 nodes 83 us, 256 of 25 237 us, five rows 40 us.) tree_draw_kernel then goes down the tree along what was decided and draws from the row where
+// that ends, which its workgroups hold in registers.
 //
 // Accuracy. The comparisons u Q < P are made in 64 bits, S is added up from powers of 32 bits (1e-8 of S where many tokens count): of ten million drafts one may be judged otherwise than by an
 // exact sum. The token behind the walk is looked for among some 100 000 steps of a cumulative sum, whose places would move by 1e-8 of the sum, a hundredth of a step where tokens are
@@ -131,15 +135,18 @@ struct TreeShare {
             }
         }
     }
-    __device__ __forceinline__ void sums(const Scale& c, Running<false>& a) const {
+    __device__ __forceinline__ float largest() const {
+        float m = -FLT_MAX;
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
             if (static_cast<uint32_t>(u) < rounds) {
                 float x[kPer];
                 unpack<DT>(q[u], x);
-                a.take(x, c);
+#pragma unroll
+                for (uint32_t e = 0; e < kPer; e += 2u) m = max3(m, x[e], x[e + 1u]);
             }
         }
+        return m;
     }
 };
 
@@ -178,21 +185,212 @@ __device__ __forceinline__ void tree_reject(TreeNode& N, uint32_t place) {
     }
 }
 
+// The trees' nodes, a lane each.
+struct TreeLane {
+    int32_t above;   // its parent, -1: none
+    uint32_t token;
+    double u;
+};
+__device__ __forceinline__ TreeLane tree_lane(const TreeVerifyArgs& A, uint32_t first, uint32_t n) {
+    TreeLane L{-1, 0xffffffffu, 0.0};
+    const uint32_t t = lane_id();
+    if (t < n) {
+        L.above = A.parent ? A.parent[first + t] : static_cast<int32_t>(t) - 1;
+        if (t == 0u || L.above >= static_cast<int32_t>(t)) L.above = -1;
+        L.token = static_cast<uint32_t>(A.R.ids[first + t]);
+        L.u = A.u_accept[first + t];
+    }
+    return L;
+}
+// The children of a node and what the distribution they were drawn from names (its entry at word off of q), for a wave; false where the entry lies outside q.
+template <int DT, bool MASK>
+__device__ __forceinline__ bool tree_drafts(const TreeVerifyArgs& A, int32_t off, const unsigned char* base, const uint32_t* allow, const TreeLane& L, uint64_t kids, TreeNode& N, float& x_child) {
+    const uint32_t t = lane_id(), V = A.R.vocab;
+    auto logit = [&](uint32_t id) { return id < V && (!MASK || allowed(allow, id)) ? load_logit<DT>(base, id) : -INFINITY; };
+    N.guess = off < 0;
+    N.drawn = 0.0;
+    x_child = kids >> t & 1u ? logit(L.token) : -INFINITY;
+    if (N.guess) {
+        N.listed = kids >> t & 1u;
+        N.id = L.token;
+        N.x = x_child;
+    } else if (kids == 0ull) {
+        N.listed = false;
+    } else {
+        if (static_cast<uint64_t>(off) + kTreeEntryWords > A.q_words) return false;
+        const int32_t* entry = A.q + off;
+        const int32_t count = entry[0], id = entry[1u + min(t, kTreeListed - 1u)];  // (all at once: one trip to memory)
+        const float q = __int_as_float(entry[33u + min(t, kTreeListed - 1u)]);
+        N.listed = t < kTreeListed && static_cast<int32_t>(t) < count;
+        N.id = static_cast<uint32_t>(id);
+        N.drawn = N.listed ? static_cast<double>(q) : 0.0;
+        N.x = N.listed ? logit(N.id) : -INFINITY;
+    }
+    // an id that is named before counts there
+    for (uint64_t left = __ballot(N.listed); left; left &= left - 1ull) {
+        const uint32_t l = static_cast<uint32_t>(__ffsll(static_cast<long long>(left)) - 1), id = lane_value(N.id, l);
+        const uint64_t same = __ballot(N.listed && N.id == id) & (~0ull << l);
+        if ((same & (same - 1ull)) == 0ull) continue;
+        const double sum = wave_sum((same >> t & 1u) ? N.drawn : 0.0);
+        if (t == l) N.drawn = sum;
+        else if (same >> t & 1u) N.listed = false;
+        left &= ~same | (1ull << l);
+    }
+    return true;
+}
+
+// The words of a launch (ws_loss.h) have a tag that no other launch has, but the replays of a captured one. So the tags also have a number that lies in the workspace, whatever it begins with, and
+// moves with every launch: epoch[0] is the one of the rows' words, epoch[1] the same for the draw to know, epoch[2] the draw's. The rows' kernel moves the last two, the draw's the first: neither one
+// that it reads itself.
+__device__ __forceinline__ unsigned long long tree_tag(const TreeVerifyArgs& A, unsigned long long epoch) { return A.tag ^ mix64(epoch); }
+
+// ---- what each node decides: the child that it passes the walk on to (with the log-probability of that one's token), or none; or that the walk does not come to it, or that its q entry is none
+constexpr uint32_t kDecNone = 64u, kDecNever = 65u, kDecBad = 66u;
+constexpr uint32_t kRowThreads = 256u;
+__device__ __forceinline__ unsigned long long* tree_decision(const TreeVerifyArgs& A, uint32_t row) { return A.decided + 2u * static_cast<size_t>(row); }
+
+template <int DT, bool MASK>
+__global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(TreeVerifyArgs A) {
+    constexpr uint32_t T = kRowThreads, kPer = Elem<DT>::kPer, kU = 4u;  // vectors of a thread on their way together
+    __shared__ float red_m[T / 64];
+    __shared__ double red_s[T / 64], red_t[T / 64];
+    __shared__ uint32_t s_never;
+    const uint32_t y = grid_row(), level = y / A.n_seq, s = y - level * A.n_seq, part = blockIdx.x, t = threadIdx.x, V = A.R.vocab;
+    const unsigned long long epoch = A.epoch[0], tag = tree_tag(A, epoch);
+    if (y == 0u && part == 0u && t == 0u) {
+        A.epoch[1] = epoch;
+        A.epoch[2] += 1ull;
+    }
+    if (level >= A.levels) return;
+    uint32_t n;
+    const uint32_t first = tree_rows(A.seq_off, s, A.R.rows, n);
+    if (level >= n) return;
+    const TreeLane L = tree_lane(A, first, n);
+    for (uint32_t node = level; node < n; node += A.levels) {  // (uniform; one, but of sequences with more nodes than the others)
+        const uint32_t row = first + node;
+        const unsigned char* base = A.R.logits + row * A.R.row_bytes;
+        const uint32_t* allow = MASK ? A.R.allow + row * A.R.allow_stride : nullptr;
+        const RowSpan<DT> span(base, V);
+        const Share<DT, MASK, T> share(base, allow, span, V, part, A.row_per);
+        const uint32_t j0 = share.j0, j1 = share.any() ? share.j1 : share.j0;
+        // whether anybody needs the node's decision: it has children, a parent, and that one has not decided against it
+        uint64_t kids = 0;
+        auto needed = [&]() {
+            kids = __ballot(L.above == static_cast<int32_t>(node));
+            return kids != 0ull && (node == 0u || static_cast<int32_t>(lane_value(static_cast<uint32_t>(L.above), node)) >= 0);
+        };
+        if (A.look) {
+            if (!needed()) continue;
+            if (node > 0u) {
+                if (t == 0u) {
+                    unsigned long long v;
+                    s_never = find_word(tree_decision(A, first + lane_value(static_cast<uint32_t>(L.above), node)), 1u, tag, v) && static_cast<uint32_t>(v & 0xffu) != node ? 1u : 0u;
+                    if (s_never) leave_word(tree_decision(A, row), 1u, kDecNever, tag);
+                }
+                __syncthreads();
+                const bool never = s_never != 0u;
+                __syncthreads();
+                if (never) continue;
+            }
+        }
+        uint4 q[kU];
+        uint32_t bits[kU];
+        if (j0 < j1) {
+#pragma unroll
+            for (uint32_t u = 0; u < kU; ++u) q[u] = share.load(j0 + u * T + t, bits[u]);
+        }
+        const float inv_t32 = A.R.inv_t ? A.R.inv_t[row] : 1.f;
+        const int32_t off = A.q ? A.q_off[row] : -1;
+        if (!A.look && !needed()) continue;  // (few rows: it is read while that is found out)
+        TreeNode N{};
+        float x_child = -INFINITY;
+        bool fine = true;
+        if (t < 64u) fine = tree_drafts<DT, MASK>(A, off, base, allow, L, kids, N, x_child);  // (while the row travels)
+        const Scale c(inv_t32);
+        Running<false> a;
+        for (uint32_t jb = j0; jb < j1; jb += kU * T) {
+            uint4 next[kU];
+            uint32_t next_bits[kU];
+            const bool more = jb + kU * T < j1;
+            if (more) {
+#pragma unroll
+                for (uint32_t u = 0; u < kU; ++u) next[u] = share.load(jb + (kU + u) * T + t, next_bits[u]);
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < kU; ++u) {
+                if (jb + u * T < j1) {  // (uniform)
+                    float x[kPer];
+                    unpack<DT>(share.own(q[u], bits[u], jb + u * T), x);
+                    a.take(x, c);
+                }
+            }
+            if (more) {
+#pragma unroll
+                for (uint32_t u = 0; u < kU; ++u) {
+                    q[u] = next[u];
+                    bits[u] = next_bits[u];
+                }
+            }
+        }
+        if (part == 0u && t < span.rest) {
+            const uint32_t i = span.rest_index(t);
+            if (!MASK || allowed(allow, i)) a.take1(load_logit<DT>(base, i), c);
+        }
+        RowSums r = block_sums<false, T>(a, c, red_m, red_s, red_t);
+        bool mine = t < 64u;
+        if (mine && A.row_parts > 1u) {  // (at most 64) who finds everybody's words decides; several may, and write the same
+            unsigned long long* at = A.row_meet + static_cast<size_t>(row) * A.row_parts * 4u;
+            if (t == 0u) {
+                leave_word(at + part, A.row_parts, __float_as_uint(r.m), tag);
+                leave_word(at + 2u * A.row_parts + part, A.row_parts, static_cast<unsigned long long>(__double_as_longlong(r.s)), tag);
+            }
+            words_arrived();
+            const bool in = t < A.row_parts;
+            unsigned long long wm = 0, ws = 0;
+            bool here = !in;
+            if (in) {
+                here = find_word(at + t, A.row_parts, tag, wm);
+                here = find_word(at + 2u * A.row_parts + t, A.row_parts, tag, ws) && here;
+            }
+            mine = __ballot(!here) == 0ull;
+            r = join_parts<false>(in, PartSums{__uint_as_float(static_cast<uint32_t>(wm)), 0.f, __longlong_as_double(static_cast<long long>(ws)), 0.0}, c);
+        }
+        if (mine) {  // (a wave)
+            const double inv_t = static_cast<double>(inv_t32);
+            uint32_t next = fine ? kDecNone : kDecBad;
+            tree_begin(N, r.m, inv_t, r.s, -1.0);
+            const double w_child = exp64((static_cast<double>(x_child) - static_cast<double>(r.m)) * inv_t) / r.s;
+            for (uint64_t left = fine ? kids : 0ull; left; left &= left - 1ull) {
+                const uint32_t k = static_cast<uint32_t>(__ffsll(static_cast<long long>(left)) - 1), place = tree_find(N, lane_value(L.token, k));
+                const double P = place < 64u ? lane_value(N.P, place) : N.c * lane_value(w_child, k);
+                const double Q = N.guess ? 1.0 : (place < 64u ? lane_value(N.Q, place) : 0.0);
+                if (lane_value(L.u, k) * Q < P) {
+                    next = k;
+                    break;
+                }
+                tree_reject(N, place);
+            }
+            const float lp = static_cast<float>((static_cast<double>(x_child) - static_cast<double>(r.m)) * inv_t - log(r.s));
+            if (t == (next < 64u ? next : 0u)) leave_word(tree_decision(A, row), 1u, (static_cast<unsigned long long>(__float_as_uint(lp)) << 32) | next, tag);
+        }
+        __syncthreads();
+    }
+}
+
+// ---- the walk, and the token behind it
 template <int DT, bool MASK, int T, int NV, int WAVES>
-__global__ void __launch_bounds__(T, WAVES) tree_verify_kernel(TreeVerifyArgs A) {
+__global__ void __launch_bounds__(T, WAVES) tree_draw_kernel(TreeVerifyArgs A) {
     constexpr uint32_t kPer = Elem<DT>::kPer, kW = T / 64u;
     __shared__ float red_m[kW];
-    __shared__ double red_s[kW], red_t[kW];
+    __shared__ double red_t[kW];
     __shared__ float part_m[64];
     __shared__ double part_s[64];
     __shared__ unsigned long long missing;
-    __shared__ uint32_t s_next;
-    __shared__ float s_m;
     __shared__ uint32_t taken_out[T * NV / 4];  // a byte a vector of the share: which of its tokens are listed
     __shared__ uint32_t special_id[64];
     __shared__ double special_w[64];
     __shared__ uint32_t s_part, s_wave, s_token;
-    __shared__ double s_before, s_target, s_wave_before;
+    __shared__ double s_target, s_wave_before;
     __shared__ float s_x;
     __shared__ double round_sum[NV][T];
     const uint32_t s = grid_row();
@@ -202,190 +400,70 @@ __global__ void __launch_bounds__(T, WAVES) tree_verify_kernel(TreeVerifyArgs A)
     const uint32_t first = tree_rows(A.seq_off, s, A.R.rows, n);
     unsigned long long* meet = A.meet + static_cast<size_t>(s) * parts * kTreeWords;
 
-    // what the first wave knows of the nodes, a lane a node, and of the walk, a lane a level
-    int32_t above = -1;
-    uint32_t token = 0xffffffffu;
-    double u = 0.0;
+    const unsigned long long rows_tag = tree_tag(A, A.epoch[1]), tag = tree_tag(A, A.epoch[2]);
+    if (part == 0u && s == 0u && t == 0u) A.epoch[0] = A.epoch[1] + 1ull;
+    const double u_draw = A.u_draw[s];
+    // down the tree, every wave by itself: a lane a node, and a lane a level for what was accepted
+    const TreeLane L = tree_lane(A, first, n);
+    unsigned long long decided = 0ull;
+    const bool known = lane < n && find_word(tree_decision(A, first + lane), 1u, rows_tag, decided);
+    const uint32_t next_of = known ? static_cast<uint32_t>(decided & 0xffu) : kDecBad;
     int32_t path = -1;
     float path_lp = 0.f;
-    uint32_t levels = 0;
-    if (t < n) {
-        above = A.parent ? A.parent[first + t] : static_cast<int32_t>(t) - 1;
-        if (t == 0u || above >= static_cast<int32_t>(t)) above = -1;
-        token = static_cast<uint32_t>(A.R.ids[first + t]);
-        u = A.u_accept[first + t];
-    }
-    TreeShare<DT, MASK, T, NV> share;
-    TreeNode N{};
+    uint32_t levels = 0, cur = 0;
     uint64_t kids = 0;
-    bool bad = n == 0u, own = false;
-    uint32_t cur = 0, step = 0;
-    float m = 0.f;
-    double S = 0.0, inv_t = 1.0;
-    const unsigned char* base = nullptr;
-    const uint32_t* allow = nullptr;
-
-    // everybody's words of this step, two a part, by the first wave: in part_m, part_s, and a bit in `missing` for each that has not come
-    auto meet_parts = [&](float mine_m, double mine_s) {
-        if (t >= 64u) return;
-        unsigned long long* at = meet + (step & 1u) * 4u * parts;
-        const unsigned long long tag = A.tag + (step + 1ull) * 0x9E3779B97F4A7C15ull;
-        if (t == 0u) {
-            leave_word(at + part, parts, __float_as_uint(mine_m), tag);
-            leave_word(at + 2u * parts + part, parts, static_cast<unsigned long long>(__double_as_longlong(mine_s)), tag);
+    bool bad = n == 0u;
+    while (!bad) {
+        kids = __ballot(L.above == static_cast<int32_t>(cur));
+        if (kids == 0ull) break;
+        const uint32_t next = lane_value(next_of, cur);
+        if (next == kDecNone) break;
+        if (next >= 64u || next <= cur) {
+            bad = true;
+            break;
         }
-        words_arrived();
-        bool here = t >= parts;
-        unsigned long long wm = 0, ws = 0;
-        for (uint32_t look = 0; look < A.looks; ++look) {
-            if (!here) {
-                here = find_word(at + t, parts, tag, wm);
-                here = find_word(at + 2u * parts + t, parts, tag, ws) && here;
-            }
-            if (__ballot(!here) == 0ull) break;
-            __builtin_amdgcn_s_sleep(2);
+        const uint32_t lp = lane_value(static_cast<uint32_t>(decided >> 32), cur);
+        if (lane == levels) {
+            path = static_cast<int32_t>(next);
+            path_lp = __uint_as_float(lp);
         }
-        const unsigned long long late = __ballot(!here);
-        part_m[t] = __uint_as_float(static_cast<uint32_t>(wm));
-        part_s[t] = __longlong_as_double(static_cast<long long>(ws));
-        if (t == 0u) missing = late;
-    };
-    // the sums of the share in `share`, in the first wave
-    auto row_sums = [&](const Scale& c) {
-        Running<false> a;
-        share.sums(c, a);
-        return block_sums<false, T>(a, c, red_m, red_s, red_t);
-    };
-
-    while (!bad) {  // a node a turn
-        const uint32_t row = first + cur;
-        base = A.R.logits + row * A.R.row_bytes;
-        allow = MASK ? A.R.allow + row * A.R.allow_stride : nullptr;
-        const float inv_t32 = A.R.inv_t ? A.R.inv_t[row] : 1.f;
-        inv_t = static_cast<double>(inv_t32);
-        float x_child = -INFINITY;
-        bool entry_bad = false;
-        auto drafts = [&]() {  // the first wave's: the node's children and what their distribution names
-            kids = __ballot(above == static_cast<int32_t>(cur));
-            auto logit = [&](uint32_t id) { return id < V && (!MASK || allowed(allow, id)) ? load_logit<DT>(base, id) : -INFINITY; };
-            const int32_t off = A.q ? A.q_off[row] : -1;
-            N.guess = off < 0;
-            N.drawn = 0.0;
-            if (kids >> t & 1u) x_child = logit(token);
-            if (N.guess) {
-                N.listed = kids >> t & 1u;
-                N.id = token;
-                N.x = x_child;
-            } else if (kids == 0ull) {
-                N.listed = false;
-            } else {
-                entry_bad = static_cast<uint64_t>(off) + kTreeEntryWords > A.q_words;
-                const int32_t* entry = A.q + (entry_bad ? 0 : off);
-                const int32_t count = entry_bad ? 0 : entry[0];
-                N.listed = t < kTreeListed && static_cast<int32_t>(t) < count;
-                if (N.listed) {
-                    N.id = static_cast<uint32_t>(entry[1u + t]);
-                    N.drawn = static_cast<double>(__int_as_float(entry[33u + t]));
-                }
-                N.x = N.listed ? logit(N.id) : -INFINITY;
-                if (entry_bad) kids = 0ull;  // (none is looked at)
-            }
-            // an id that is named before counts there
-            const uint64_t names = __ballot(N.listed);
-            for (uint64_t left = names; left; left &= left - 1ull) {
-                const uint32_t l = static_cast<uint32_t>(__ffsll(static_cast<long long>(left)) - 1), id = lane_value(N.id, l);
-                const uint64_t same = __ballot(N.listed && N.id == id) & (~0ull << l);
-                if ((same & (same - 1ull)) == 0ull) continue;
-                const double sum = wave_sum((same >> t & 1u) ? N.drawn : 0.0);
-                if (t == l) N.drawn = sum;
-                else if (same >> t & 1u) N.listed = false;
-                left &= ~same | (1ull << l);
-            }
-        };
-        const Scale c(inv_t32);
-        RowSums r;
-        unsigned long long late = 0;
-        uint32_t p = part;
-        for (bool first_turn = true;; first_turn = false) {  // the own share, then those of workgroups that have not come (in one loop: the code is there once)
-            share.place(V, p, per);
-            share.load(base, allow, V);
-            if (first_turn && t < 64u) drafts();  // (while the row travels)
-            r = row_sums(c);
-            if (parts == 1u) break;
-            if (first_turn) {
-                meet_parts(r.m, r.s);
-            } else if (t == 0u) {
-                part_m[p] = r.m;
-                part_s[p] = r.s;
-            }
-            __syncthreads();
-            late = first_turn ? missing : late & (late - 1ull);
-            if (late == 0ull) break;
-            p = static_cast<uint32_t>(__ffsll(late) - 1);
-        }
-        own = p == part;
-        if (parts > 1u && t < 64u) {
-            __builtin_amdgcn_wave_barrier();
-            r = join_parts<false>(t < parts, PartSums{part_m[t], 0.f, part_s[t], 0.0}, c);
-        }
-        ++step;
-        if (t < 64u) {
-            const double lnS = log(r.s);
-            uint32_t next = 0xffffffffu;
-            tree_begin(N, r.m, inv_t, r.s, -1.0);
-            const double w_child = exp64((static_cast<double>(x_child) - static_cast<double>(r.m)) * inv_t) / r.s;
-            for (uint64_t left = kids; left; left &= left - 1ull) {
-                const uint32_t k = static_cast<uint32_t>(__ffsll(static_cast<long long>(left)) - 1), place = tree_find(N, lane_value(token, k));
-                const double P = place < 64u ? lane_value(N.P, place) : N.c * lane_value(w_child, k);
-                const double Q = N.guess ? 1.0 : (place < 64u ? lane_value(N.Q, place) : 0.0);
-                if (lane_value(u, k) * Q < P) {
-                    next = k;
-                    break;
-                }
-                tree_reject(N, place);
-            }
-            if (next != 0xffffffffu) {
-                const float lp = static_cast<float>((static_cast<double>(__uint_as_float(lane_value(__float_as_uint(x_child), next))) - static_cast<double>(r.m)) * inv_t - lnS);
-                if (t == levels) {
-                    path = static_cast<int32_t>(next);
-                    path_lp = lp;
-                }
-                ++levels;
-            }
-            if (t == 0u) {
-                s_next = entry_bad ? 0xfffffffeu : next;
-                s_m = r.m;
-            }
-        }
-        __syncthreads();
-        const uint32_t next = s_next;
-        m = s_m;
-        __syncthreads();
-        if (next == 0xfffffffeu) bad = true;
-        if (next >= 0xfffffffeu) break;
+        ++levels;
         cur = next;
     }
 
-    // the token behind the walk
-    uint32_t chosen = 0xffffffffu;
-    float chosen_x = 0.f;
-    uint32_t target_part = 0;
+    uint32_t chosen = 0xffffffffu, target_part = 0;
+    float chosen_x = 0.f, m = 0.f;
+    double S = 0.0, inv_t = 1.0;
     if (!bad) {
-        // weights of a share's tokens that are not listed: the sum of each round of a thread, and of the workgroup
+        const uint32_t row = first + cur;
+        const unsigned char* base = A.R.logits + row * A.R.row_bytes;
+        const uint32_t* allow = MASK ? A.R.allow + row * A.R.allow_stride : nullptr;
+        TreeShare<DT, MASK, T, NV> share;
+        TreeNode N{};
+        inv_t = static_cast<double>(A.R.inv_t ? A.R.inv_t[row] : 1.f);
+        const int32_t off = A.q ? A.q_off[row] : -1;
+        const bool no_t = !(inv_t > 0.0 && inv_t < static_cast<double>(INFINITY));
+        float share_m = 0.f;
+        // weights of a share's tokens that are not listed, against the share's own maximum: the sum of each round of a thread, and of the workgroup
         auto weights = [&](uint32_t u_, double (&w)[kPer]) {
             float x[kPer];
             unpack<DT>(share.q[u_], x);
             const uint32_t out = reinterpret_cast<const unsigned char*>(taken_out)[wave_id() * 64u * share.rounds + u_ * 64u + lane];
 #pragma unroll
-            for (uint32_t e = 0; e < kPer; ++e) w[e] = out >> e & 1u ? 0.0 : exp64((static_cast<double>(x[e]) - static_cast<double>(m)) * inv_t);
+            for (uint32_t e = 0; e < kPer; ++e) w[e] = out >> e & 1u ? 0.0 : exp64((static_cast<double>(x[e]) - static_cast<double>(share_m)) * inv_t);
         };
         auto outside_sum = [&]() {
             for (uint32_t i = t; i < T * NV / 4u; i += T) taken_out[i] = 0u;
+            const float mine = wave_max(share.largest());
+            if (lane == 0u) red_m[wave_id()] = mine;
             __syncthreads();
             if (t < 64u && N.listed && N.id < V) {
                 const uint32_t j = N.id / kPer;
                 if (j >= share.j0 && j < share.j1) atomicOr(&taken_out[(j - share.j0) / 4u], 1u << ((j - share.j0) % 4u * 8u + N.id % kPer));
             }
+            share_m = red_m[0];
+#pragma unroll
+            for (uint32_t w = 1; w < kW; ++w) share_m = fmaxf(share_m, red_m[w]);
             __syncthreads();
             double sum = 0.0;
 #pragma unroll
@@ -395,7 +473,7 @@ __global__ void __launch_bounds__(T, WAVES) tree_verify_kernel(TreeVerifyArgs A)
                     weights(v, w);
 #pragma unroll
                     for (uint32_t e = 0; e < kPer; ++e) of_round += w[e];
-                    round_sum[v][t] = of_round;  // (LDS: read again by the wave that the target lies in)
+                    round_sum[v][t] = of_round;  // (read again by the wave that the target lies in)
                     sum += of_round;
                 }
             }
@@ -404,21 +482,42 @@ __global__ void __launch_bounds__(T, WAVES) tree_verify_kernel(TreeVerifyArgs A)
             __syncthreads();
             double all = 0.0;
             for (uint32_t w = 0; w < kW; ++w) all += red_t[w];
-            return all;
+            return no_t ? __builtin_nan("") : all;
         };
         unsigned long long late = 0;
         uint32_t p = part;
         for (bool first_turn = true;; first_turn = false) {  // the own share, those of workgroups that have not come, then the own again where it is no longer there
-            if (!own || !first_turn) {
-                share.place(V, p, per);
-                share.load(base, allow, V);
-                __syncthreads();  // (taken_out and red_t are free)
+            share.place(V, p, per);
+            share.load(base, allow, V);
+            if (first_turn && t < 64u) {  // (while the row travels)
+                float x_child;
+                tree_drafts<DT, MASK>(A, off, base, allow, L, kids, N, x_child);
             }
             const double sum = outside_sum();
-            if (first_turn) {
-                if (parts > 1u) meet_parts(0.f, sum);
-                else if (t == 0u) part_s[0] = sum;
-            } else if (t == 0u && p != part) {
+            if (first_turn && parts > 1u) {
+                if (t < 64u) {  // everybody's maximum and sum
+                    if (t == 0u) {
+                        leave_word(meet + part, parts, __float_as_uint(share_m), tag);
+                        leave_word(meet + 2u * parts + part, parts, static_cast<unsigned long long>(__double_as_longlong(sum)), tag);
+                    }
+                    words_arrived();
+                    bool here = t >= parts;
+                    unsigned long long wm = 0, ws = 0;
+                    for (uint32_t look = 0; look < A.looks; ++look) {
+                        if (!here) {
+                            here = find_word(meet + t, parts, tag, wm);
+                            here = find_word(meet + 2u * parts + t, parts, tag, ws) && here;
+                        }
+                        if (__ballot(!here) == 0ull) break;
+                        __builtin_amdgcn_s_sleep(2);
+                    }
+                    const unsigned long long none = __ballot(!here);
+                    part_m[t] = __uint_as_float(static_cast<uint32_t>(wm));
+                    part_s[t] = __longlong_as_double(static_cast<long long>(ws));
+                    if (t == 0u) missing = none;
+                }
+            } else if (t == 0u && (first_turn || p != part)) {
+                part_m[p] = share_m;
                 part_s[p] = sum;
             }
             __syncthreads();
@@ -430,31 +529,34 @@ __global__ void __launch_bounds__(T, WAVES) tree_verify_kernel(TreeVerifyArgs A)
             p = late ? static_cast<uint32_t>(__ffsll(late) - 1) : part;
         }
         if (t < 64u) {
-            const double outside = t < parts ? part_s[t] : 0.0, out_all = wave_sum(outside);
+            const float mine_m = t < parts ? part_m[t] : -FLT_MAX;
+            m = wave_max(mine_m);
+            const double scale = exp64((static_cast<double>(mine_m) - static_cast<double>(m)) * inv_t);
+            const double outside = t < parts ? part_s[t] * scale : 0.0, out_all = wave_sum(outside);
             const double w = N.listed ? exp64((static_cast<double>(N.x) - static_cast<double>(m)) * inv_t) : 0.0;
             S = out_all + wave_sum(w);
             tree_begin(N, m, inv_t, S, out_all);
             for (uint64_t left = kids; left; left &= left - 1ull)
-                tree_reject(N, tree_find(N, lane_value(token, static_cast<uint32_t>(__ffsll(static_cast<long long>(left)) - 1))));
+                tree_reject(N, tree_find(N, lane_value(L.token, static_cast<uint32_t>(__ffsll(static_cast<long long>(left)) - 1))));
             // in units of the weights outside
             const double special = N.listed && N.id < V ? N.P / N.c * S : 0.0;
-            special_id[t] = special > 0.0 ? N.id : 0xffffffffu;
-            special_w[t] = special;
             double in_part = outside;
             for (uint64_t left = __ballot(special > 0.0); left; left &= left - 1ull) {
                 const uint32_t l = static_cast<uint32_t>(__ffsll(static_cast<long long>(left)) - 1);
                 if (lane_value(N.id, l) / kPer / per == t) in_part += lane_value(special, l);
             }
-            const double upto = wave_incl_scan(in_part), all = last_lane(upto), target = A.u_draw[s] * all;
+            const double upto = wave_incl_scan(in_part), all = last_lane(upto), target = u_draw * all;
             // the first part up to which there is more than the target; else the last with any
             const uint64_t over = __ballot(upto > target && in_part > 0.0), any = __ballot(in_part > 0.0);
-            const uint32_t p = over ? static_cast<uint32_t>(__ffsll(static_cast<long long>(over)) - 1) : (any ? 63u - static_cast<uint32_t>(__clzll(static_cast<long long>(any))) : 0u);
+            const uint32_t at = over ? static_cast<uint32_t>(__ffsll(static_cast<long long>(over)) - 1) : (any ? 63u - static_cast<uint32_t>(__clzll(static_cast<long long>(any))) : 0u);
             const bool none = !(all > 0.0 && all < static_cast<double>(INFINITY));
-            const double before = p ? lane_value(upto, p - 1u) : 0.0;  // (upto of the lane before, not upto - in_part: no rounding of the difference)
+            const double before = at ? lane_value(upto, at - 1u) : 0.0, unit = lane_value(scale, at);
+            // what the part's workgroup goes on with is in its own units
+            special_id[t] = special > 0.0 ? N.id : 0xffffffffu;
+            special_w[t] = special / unit;
             if (t == 0u) {
-                s_part = none ? 0xffffffffu : p;
-                s_before = before;
-                s_target = target;
+                s_part = none ? 0xffffffffu : at;
+                s_target = (target - before) / unit;
             }
         }
         __syncthreads();
@@ -463,13 +565,13 @@ __global__ void __launch_bounds__(T, WAVES) tree_verify_kernel(TreeVerifyArgs A)
         if (!bad && target_part == part) {  // (uniform)
             const double target = s_target;
             const uint32_t wave_vectors = 64u * share.rounds;
-            // what the listed ids of [lo, hi) weigh, a lane each; the same for the whole wave
+            // what the listed ids of [lo, hi) weigh; the same for the whole wave
             auto special_sum = [&](uint32_t lo, uint32_t hi) {
                 const uint32_t id = special_id[lane];
                 return wave_sum(id >= lo && id < hi ? special_w[lane] : 0.0);
             };
             if (t < 64u) {
-                double before = s_before;
+                double before = 0.0;
                 uint32_t at = 0xffffffffu, last = 0;
                 double at_before = before, last_before = before;
                 for (uint32_t w = 0; w < kW; ++w) {
@@ -495,21 +597,18 @@ __global__ void __launch_bounds__(T, WAVES) tree_verify_kernel(TreeVerifyArgs A)
                 double before = s_wave_before, at_before = before, last_before = before;
                 uint32_t at = 0xffffffffu, last = 0;
                 const uint32_t j_wave = share.j0 + wave_id() * wave_vectors;
-#pragma unroll
-                for (uint32_t v = 0; v < NV; ++v) {
-                    if (v < share.rounds) {
-                        const uint32_t lo = j_wave + v * 64u, hi = min(lo + 64u, share.j1);
-                        const double sum = wave_sum(round_sum[v][t]) + (lo < hi ? special_sum(lo * kPer, hi * kPer) : 0.0), upto = before + sum;
-                        if (sum > 0.0) {
-                            last = v;
-                            last_before = before;
-                        }
-                        if (at == 0xffffffffu && upto > target && sum > 0.0) {
-                            at = v;
-                            at_before = before;
-                        }
-                        before = upto;
+                for (uint32_t v = 0; v < share.rounds; ++v) {
+                    const uint32_t lo = j_wave + v * 64u, hi = min(lo + 64u, share.j1);
+                    const double sum = wave_sum(round_sum[v][t]) + (lo < hi ? special_sum(lo * kPer, hi * kPer) : 0.0), upto = before + sum;
+                    if (sum > 0.0) {
+                        last = v;
+                        last_before = before;
                     }
+                    if (at == 0xffffffffu && upto > target && sum > 0.0) {
+                        at = v;
+                        at_before = before;
+                    }
+                    before = upto;
                 }
                 if (at == 0xffffffffu) {
                     at = last;
@@ -525,9 +624,9 @@ __global__ void __launch_bounds__(T, WAVES) tree_verify_kernel(TreeVerifyArgs A)
                     }
                 }
                 const uint32_t id0 = (j_wave + at * 64u + lane) * kPer;
-                for (uint32_t l = 0; l < 64u; ++l) {
-                    const uint32_t id = special_id[l];
-                    if (id == 0xffffffffu) continue;  // (uniform)
+                const uint32_t listed = special_id[lane], of_round = (j_wave + at * 64u) * kPer;
+                for (uint64_t left = __ballot(listed - of_round < 64u * kPer); left; left &= left - 1ull) {  // those of this round
+                    const uint32_t l = static_cast<uint32_t>(__ffsll(static_cast<long long>(left)) - 1), id = lane_value(listed, l);
 #pragma unroll
                     for (uint32_t e = 0; e < kPer; ++e)
                         if (id == id0 + e) w[e] = special_w[l];
@@ -578,7 +677,7 @@ __global__ void __launch_bounds__(T, WAVES) tree_verify_kernel(TreeVerifyArgs A)
                 accepted = 0u;
                 chosen = 0xffffffffu;
             } else {
-                const int32_t kept = __shfl(static_cast<int32_t>(token), max(path, 0));
+                const int32_t kept = __shfl(static_cast<int32_t>(L.token), max(path, 0));
                 if (t < accepted) text[len + 1u + t] = kept;
                 if (t == 0u) {
                     text[len + 1u + accepted] = static_cast<int32_t>(chosen);
@@ -600,19 +699,6 @@ __global__ void __launch_bounds__(T, WAVES) tree_verify_kernel(TreeVerifyArgs A)
             float* to = A.logprob + static_cast<size_t>(s) * (A.depth + 1u);
             if (t <= A.depth) to[t] = lp;
             if (t == 0u && A.depth == 64u) to[64] = 0.f;  // (63 drafts at most are accepted: the chosen one's is in the 64th place)
-        }
-    }
-    if (parts > 1u && n != 0u && t < 64u) {
-        // all words of this part have arrived; who finds everybody's mark breaks the sequence's words, for a captured launch has its tag again at every replay
-        unsigned long long* marks = meet + 8u * parts;
-        words_arrived();
-        if (t == 0u) leave_word(marks + part, parts, 0ull, A.tag);
-        words_arrived();
-        unsigned long long v;
-        const bool here = t >= parts || find_word(marks + t, parts, A.tag, v);
-        if (__ballot(!here) == 0ull && t < parts) {
-#pragma unroll
-            for (uint32_t k = 0; k < 5u; ++k) break_word(meet + 2u * k * parts + t, parts);
         }
     }
 }

@@ -11,10 +11,11 @@ static_assert((1048575u / Elem<0>::kPer + 63u) / 64u + 8u <= kWide);
 
 template <int DT, bool MASK, int T, int NV, int WAVES>
 void verify(hipStream_t s, const TreeVerifyArgs& a) {
-    hipLaunchKernelGGL((tree_verify_kernel<DT, MASK, T, NV, WAVES>), grid_of(a.parts, a.n_seq), dim3(T), 0, s, a);
+    hipLaunchKernelGGL((tree_draw_kernel<DT, MASK, T, NV, WAVES>), grid_of(a.parts, a.n_seq), dim3(T), 0, s, a);
 }
 template <int DT, bool MASK>
 void of_size(hipStream_t s, const TreeVerifyArgs& a) {
+    hipLaunchKernelGGL((tree_rows_kernel<DT, MASK>), grid_of(a.row_parts, a.levels * a.n_seq), dim3(kRowThreads), 0, s, a);
     if (a.per <= kSmall) verify<DT, MASK, 256, 4, 4>(s, a);
     else if (a.per <= kMost) verify<DT, MASK, 256, 12, 2>(s, a);
     else verify<DT, MASK, 512, 9, 2>(s, a);
