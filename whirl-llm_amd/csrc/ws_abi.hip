@@ -1322,8 +1322,8 @@ static_assert(WS_TREE_MAX == ws::kTreeNodes && WS_Q_MAX == ws::kTreeListed && WS
 static_assert(WS_CACHE_MOST == ws::kCacheMost && WS_CACHE_MOST == WS_BLOCK);
 
 // The verification's workgroups. A sequence's draw: two a compute unit where sequences are few, of 256 vectors at least; as many as hold the row in registers. A row's decision: shares of
-// 2048 vectors at least, larger ones where there are many rows, so that fewer workgroups begin at the ends of trips to memory. Parts, us: 64 trees of 16 x 151936 bf16 62: 109, 12: 33.7, 6: 32.1, 3: 35.1, 1: 47.5;
-// 256 of 25 x 50257 fp32, masked, 42: 777, 8: 202, 4: 134, 2: 110, 1: 121; five rows of 151936 bf16 62: 15.6, 37: 13.2, 12: 11.8, 6: 12.5, 1: 22.8. Words: the draw's, the decisions, the rows' sums.
+// 2048 vectors at least, larger ones where there are many rows, so that fewer workgroups begin at the ends of trips to memory. Parts, us: 64 trees of 16 x 151936 bf16 62: 109, 12: 33.7, 6: 31.4, 3: 34.1, 1: 47.3;
+// 256 of 25 x 50257 fp32, masked, 42: 777, 8: 202, 4: 114, 2: 97, 1: 110; five rows of 151936 bf16 62: 15.6, 12: 9.7, 6: 9.7, 3: 11.8, 1: 20.4. Words: the draw's, the decisions, the rows' sums.
 struct VerifyPlan {
     uint32_t parts, row_parts, levels;
     uint64_t meet, decided, bytes;

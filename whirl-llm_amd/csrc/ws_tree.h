@@ -59,25 +59,25 @@ __global__ void __launch_bounds__(64) tree_stage_kernel(TreeStageArgs A) {
     if (A.position) A.position[first + lane] = static_cast<int32_t>(len + __popc(lo) + __popc(hi) - 1u);
 }
 
-// e^y for y <= 0 to 1e-12: y = k ln 2 + r, |r| <= 0.35, the Taylor polynomial of e^r to its tenth power (the next is 0.35^11 / 11! = 2e-13)
-__device__ __forceinline__ double exp64(double y) {
-    const double k = rint(y * 1.4426950408889634074);
-    double r = fma(k, -0x1.62e42f0000000p-1, y);  // (ln 2 in two parts, the first of 25 bits: k times it is exact)
-    r = fma(k, -0x1.df473de6af279p-26, r);
-    double p = 1.0 / 3628800.0;
-    p = fma(p, r, 1.0 / 362880.0);
-    p = fma(p, r, 1.0 / 40320.0);
-    p = fma(p, r, 1.0 / 5040.0);
-    p = fma(p, r, 1.0 / 720.0);
-    p = fma(p, r, 1.0 / 120.0);
-    p = fma(p, r, 1.0 / 24.0);
-    p = fma(p, r, 1.0 / 6.0);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
-    p = fma(p, r, 1.0);
-    const double e = ldexp(p, static_cast<int>(k));
-    return y < -700.0 ? 0.0 : e;  // (-inf too; NaN stays)
+// 2^z for z <= 0 to 1e-11: z = k + f, |f| <= 1/2, and of 2^f = e^(f ln 2) the first ten terms of its series (the next is 0.35^10 / 10! = 7e-12). What lies below 2^-2885, -inf too, is 0. Not
+// for NaN, which is told apart where it is looked for.
+__device__ __forceinline__ double power64(double z) {
+    z = fmax(z, -2885.0);
+    const double k = rint(z), f = z - k;
+    double p = 0x1.b5253d395e7c4p-24;
+    p = fma(p, f, 0x1.62c0223a5c824p-20);
+    p = fma(p, f, 0x1.ffcbfc588b0c7p-17);
+    p = fma(p, f, 0x1.430912f86c787p-13);
+    p = fma(p, f, 0x1.5d87fe78a6731p-10);
+    p = fma(p, f, 0x1.3b2ab6fba4e77p-7);
+    p = fma(p, f, 0x1.c6b08d704a0c0p-5);
+    p = fma(p, f, 0x1.ebfbdff82c58fp-3);
+    p = fma(p, f, 0x1.62e42fefa39efp-1);
+    p = fma(p, f, 0x1.0000000000000p+0);
+    return ldexp(p, static_cast<int>(k));
 }
+// exponents of base two: a row's factor
+__device__ __forceinline__ double tree_factor(float inv_t) { return static_cast<double>(inv_t) * 1.4426950408889634074; }
 
 // part `part` of a row: vectors [j0, j1) of 16 bytes, numbered from the row's first token, wherever that lies; a wave's are neighbours, so that sums go in id order
 template <int DT, bool MASK, int T, int NV>
@@ -135,7 +135,8 @@ struct TreeShare {
             }
         }
     }
-    __device__ __forceinline__ float largest() const {
+    // the largest of its logits; whether one is NaN or they have no largest
+    __device__ __forceinline__ float largest(bool& odd) const {
         float m = -FLT_MAX;
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
@@ -143,9 +144,13 @@ struct TreeShare {
                 float x[kPer];
                 unpack<DT>(q[u], x);
 #pragma unroll
-                for (uint32_t e = 0; e < kPer; e += 2u) m = max3(m, x[e], x[e + 1u]);
+                for (uint32_t e = 0; e < kPer; e += 2u) {
+                    m = max3(m, x[e], x[e + 1u]);
+                    odd = odd || __builtin_isunordered(x[e], x[e + 1u]);
+                }
             }
         }
+        odd = odd || m == INFINITY;
         return m;
     }
 };
@@ -159,8 +164,8 @@ struct TreeNode {
     double out, c;       // that of all that is not listed as the node begins, and what it has been multiplied by
 };
 // the node's probabilities, S and what of it lies outside the listed ids known (out_known < 0: not)
-__device__ __forceinline__ void tree_begin(TreeNode& N, float m, double inv_t, double S, double out_known) {
-    N.P = N.listed ? exp64((static_cast<double>(N.x) - static_cast<double>(m)) * inv_t) / S : 0.0;
+__device__ __forceinline__ void tree_begin(TreeNode& N, float m, double factor, double S, double out_known) {
+    N.P = N.listed ? power64((static_cast<double>(N.x) - static_cast<double>(m)) * factor) / S : 0.0;
     N.Q = N.drawn;
     N.c = 1.0;
     N.out = out_known >= 0.0 ? out_known / S : fmax(1.0 - wave_sum(N.P), 0.0);
@@ -204,7 +209,7 @@ __device__ __forceinline__ TreeLane tree_lane(const TreeVerifyArgs& A, uint32_t 
 }
 // The children of a node and what the distribution they were drawn from names (its entry at word off of q), for a wave; false where the entry lies outside q.
 template <int DT, bool MASK>
-__device__ __forceinline__ bool tree_drafts(const TreeVerifyArgs& A, int32_t off, const unsigned char* base, const uint32_t* allow, const TreeLane& L, uint64_t kids, TreeNode& N, float& x_child) {
+__device__ __forceinline__ bool tree_drafts(const TreeVerifyArgs& A, int32_t off, const unsigned char* base, const uint32_t* allow, const TreeLane& L, uint64_t kids, uint32_t* seen, TreeNode& N, float& x_child) {
     const uint32_t t = lane_id(), V = A.R.vocab;
     auto logit = [&](uint32_t id) { return id < V && (!MASK || allowed(allow, id)) ? load_logit<DT>(base, id) : -INFINITY; };
     N.guess = off < 0;
@@ -226,7 +231,13 @@ __device__ __forceinline__ bool tree_drafts(const TreeVerifyArgs& A, int32_t off
         N.drawn = N.listed ? static_cast<double>(q) : 0.0;
         N.x = N.listed ? logit(N.id) : -INFINITY;
     }
-    // an id that is named before counts there
+    // An id that is named before counts there. Whether there is one: a bit an id, in a table of 8192, is there when it comes (of 32 ids that differ once in 16 times: then they are gone through)
+    const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+    reinterpret_cast<uint4*>(seen)[t] = none;
+    __builtin_amdgcn_wave_barrier();  // (one wave: its LDS stores are done before its atomics)
+    const uint32_t hash = N.id * 2654435761u >> 19;
+    const bool again = N.listed && (atomicOr(&seen[hash >> 5], 1u << (hash & 31u)) >> (hash & 31u) & 1u);
+    if (__ballot(again) == 0ull) return true;
     for (uint64_t left = __ballot(N.listed); left; left &= left - 1ull) {
         const uint32_t l = static_cast<uint32_t>(__ffsll(static_cast<long long>(left)) - 1), id = lane_value(N.id, l);
         const uint64_t same = __ballot(N.listed && N.id == id) & (~0ull << l);
@@ -250,11 +261,12 @@ constexpr uint32_t kRowThreads = 256u;
 __device__ __forceinline__ unsigned long long* tree_decision(const TreeVerifyArgs& A, uint32_t row) { return A.decided + 2u * static_cast<size_t>(row); }
 
 template <int DT, bool MASK>
-__global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(TreeVerifyArgs A) {
+__global__ void __launch_bounds__(kRowThreads, 3) tree_rows_kernel(TreeVerifyArgs A) {
     constexpr uint32_t T = kRowThreads, kPer = Elem<DT>::kPer, kU = 4u;  // vectors of a thread on their way together
     __shared__ float red_m[T / 64];
     __shared__ double red_s[T / 64], red_t[T / 64];
     __shared__ uint32_t s_never;
+    __shared__ __attribute__((aligned(16))) uint32_t s_seen[256];
     const uint32_t y = grid_row(), level = y / A.n_seq, s = y - level * A.n_seq, part = blockIdx.x, t = threadIdx.x, V = A.R.vocab;
     const unsigned long long epoch = A.epoch[0], tag = tree_tag(A, epoch);
     if (y == 0u && part == 0u && t == 0u) {
@@ -305,7 +317,7 @@ __global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(TreeVerifyArgs A
         TreeNode N{};
         float x_child = -INFINITY;
         bool fine = true;
-        if (t < 64u) fine = tree_drafts<DT, MASK>(A, off, base, allow, L, kids, N, x_child);  // (while the row travels)
+        if (t < 64u) fine = tree_drafts<DT, MASK>(A, off, base, allow, L, kids, s_seen, N, x_child);  // (while the row travels)
         const Scale c(inv_t32);
         Running<false> a;
         for (uint32_t jb = j0; jb < j1; jb += kU * T) {
@@ -356,10 +368,10 @@ __global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(TreeVerifyArgs A
             r = join_parts<false>(in, PartSums{__uint_as_float(static_cast<uint32_t>(wm)), 0.f, __longlong_as_double(static_cast<long long>(ws)), 0.0}, c);
         }
         if (mine) {  // (a wave)
-            const double inv_t = static_cast<double>(inv_t32);
+            const double inv_t = static_cast<double>(inv_t32), factor = tree_factor(inv_t32);
             uint32_t next = fine ? kDecNone : kDecBad;
-            tree_begin(N, r.m, inv_t, r.s, -1.0);
-            const double w_child = exp64((static_cast<double>(x_child) - static_cast<double>(r.m)) * inv_t) / r.s;
+            tree_begin(N, r.m, factor, r.s, -1.0);
+            const double w_child = power64((static_cast<double>(x_child) - static_cast<double>(r.m)) * factor) / r.s;
             for (uint64_t left = fine ? kids : 0ull; left; left &= left - 1ull) {
                 const uint32_t k = static_cast<uint32_t>(__ffsll(static_cast<long long>(left)) - 1), place = tree_find(N, lane_value(L.token, k));
                 const double P = place < 64u ? lane_value(N.P, place) : N.c * lane_value(w_child, k);
@@ -393,6 +405,7 @@ __global__ void __launch_bounds__(T, WAVES) tree_draw_kernel(TreeVerifyArgs A) {
     __shared__ double s_target, s_wave_before;
     __shared__ float s_x;
     __shared__ double round_sum[NV][T];
+    __shared__ __attribute__((aligned(16))) uint32_t s_seen[256];
     const uint32_t s = grid_row();
     if (s >= A.n_seq) return;
     const uint32_t part = blockIdx.x, t = threadIdx.x, lane = lane_id(), V = A.R.vocab, per = A.per, parts = A.parts;
@@ -440,7 +453,9 @@ __global__ void __launch_bounds__(T, WAVES) tree_draw_kernel(TreeVerifyArgs A) {
         const uint32_t* allow = MASK ? A.R.allow + row * A.R.allow_stride : nullptr;
         TreeShare<DT, MASK, T, NV> share;
         TreeNode N{};
-        inv_t = static_cast<double>(A.R.inv_t ? A.R.inv_t[row] : 1.f);
+        const float inv_t32 = A.R.inv_t ? A.R.inv_t[row] : 1.f;
+        inv_t = static_cast<double>(inv_t32);
+        const double factor = tree_factor(inv_t32);
         const int32_t off = A.q ? A.q_off[row] : -1;
         const bool no_t = !(inv_t > 0.0 && inv_t < static_cast<double>(INFINITY));
         float share_m = 0.f;
@@ -450,20 +465,29 @@ __global__ void __launch_bounds__(T, WAVES) tree_draw_kernel(TreeVerifyArgs A) {
             unpack<DT>(share.q[u_], x);
             const uint32_t out = reinterpret_cast<const unsigned char*>(taken_out)[wave_id() * 64u * share.rounds + u_ * 64u + lane];
 #pragma unroll
-            for (uint32_t e = 0; e < kPer; ++e) w[e] = out >> e & 1u ? 0.0 : exp64((static_cast<double>(x[e]) - static_cast<double>(share_m)) * inv_t);
+            for (uint32_t e = 0; e < kPer; ++e) {  // (those as if they were not there: a branch around each power would have one wait for the other)
+                const float mine = out >> e & 1u ? -INFINITY : x[e];
+                w[e] = power64((static_cast<double>(mine) - static_cast<double>(share_m)) * factor);
+            }
         };
         auto outside_sum = [&]() {
             for (uint32_t i = t; i < T * NV / 4u; i += T) taken_out[i] = 0u;
-            const float mine = wave_max(share.largest());
-            if (lane == 0u) red_m[wave_id()] = mine;
+            bool odd = no_t;
+            const float mine = wave_max(share.largest(odd));
+            const uint64_t odds = __ballot(odd);
+            if (lane == 0u) red_m[wave_id()] = odds ? __builtin_nanf("") : mine;
             __syncthreads();
             if (t < 64u && N.listed && N.id < V) {
                 const uint32_t j = N.id / kPer;
                 if (j >= share.j0 && j < share.j1) atomicOr(&taken_out[(j - share.j0) / 4u], 1u << ((j - share.j0) % 4u * 8u + N.id % kPer));
             }
-            share_m = red_m[0];
+            share_m = -FLT_MAX;
+            bool any_odd = false;
 #pragma unroll
-            for (uint32_t w = 1; w < kW; ++w) share_m = fmaxf(share_m, red_m[w]);
+            for (uint32_t w = 0; w < kW; ++w) {
+                any_odd = any_odd || red_m[w] != red_m[w];
+                share_m = fmaxf(share_m, red_m[w]);
+            }
             __syncthreads();
             double sum = 0.0;
 #pragma unroll
@@ -482,7 +506,7 @@ __global__ void __launch_bounds__(T, WAVES) tree_draw_kernel(TreeVerifyArgs A) {
             __syncthreads();
             double all = 0.0;
             for (uint32_t w = 0; w < kW; ++w) all += red_t[w];
-            return no_t ? __builtin_nan("") : all;
+            return any_odd ? __builtin_nan("") : all;  // (no sum: nothing can be drawn)
         };
         unsigned long long late = 0;
         uint32_t p = part;
@@ -491,7 +515,7 @@ __global__ void __launch_bounds__(T, WAVES) tree_draw_kernel(TreeVerifyArgs A) {
             share.load(base, allow, V);
             if (first_turn && t < 64u) {  // (while the row travels)
                 float x_child;
-                tree_drafts<DT, MASK>(A, off, base, allow, L, kids, N, x_child);
+                tree_drafts<DT, MASK>(A, off, base, allow, L, kids, s_seen, N, x_child);
             }
             const double sum = outside_sum();
             if (first_turn && parts > 1u) {
@@ -531,11 +555,11 @@ __global__ void __launch_bounds__(T, WAVES) tree_draw_kernel(TreeVerifyArgs A) {
         if (t < 64u) {
             const float mine_m = t < parts ? part_m[t] : -FLT_MAX;
             m = wave_max(mine_m);
-            const double scale = exp64((static_cast<double>(mine_m) - static_cast<double>(m)) * inv_t);
+            const double scale = power64((static_cast<double>(mine_m) - static_cast<double>(m)) * factor);
             const double outside = t < parts ? part_s[t] * scale : 0.0, out_all = wave_sum(outside);
-            const double w = N.listed ? exp64((static_cast<double>(N.x) - static_cast<double>(m)) * inv_t) : 0.0;
+            const double w = N.listed ? power64((static_cast<double>(N.x) - static_cast<double>(m)) * factor) : 0.0;
             S = out_all + wave_sum(w);
-            tree_begin(N, m, inv_t, S, out_all);
+            tree_begin(N, m, factor, S, out_all);
             for (uint64_t left = kids; left; left &= left - 1ull)
                 tree_reject(N, tree_find(N, lane_value(L.token, static_cast<uint32_t>(__ffsll(static_cast<long long>(left)) - 1))));
             // in units of the weights outside
