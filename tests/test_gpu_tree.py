@@ -268,6 +268,44 @@ def test_verify_captured_and_replayed():
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("begin", [0, 64, 4096])
+def test_verify_replayed_where_others_use_the_workspace(begin):
+    """A captured call's workspace belongs to others between its replays: some of it has the same in it each time, the rest what the last replay left. Other logits, other entries (some of them
+    none) each time."""
+    m = gc.pkg()
+    counts = [7, 16, 3]
+    cases = [verify_case(counts, 2, 60000, BF16, 200 + i, guessed=False)[0] for i in range(3)]
+    cases[1]["q_off"][cases[1]["q_off"] >= 0] = cases[1]["q"].numel()  # (entries that lie outside: the sequences are the host's)
+    call = {k: None if v is None else v.clone() for k, v in cases[0].items()}
+    r = m._loss_rows(call["logits"], call["ids"], call["inv_t"], call["allow"])[0]
+    small, logprob = torch.empty(3 * 3 + 3 * 15, dtype=torch.int32, device=DEV), torch.empty(3, 16, device=DEV)
+    at = small.data_ptr()
+    a = m.VerifyTree(3, *(0 if call.get(k) is None else call[k].data_ptr() for k in ("seq_off", "parent", "q")), call["q"].numel(),
+                     *(call[k].data_ptr() for k in ("q_off", "u_accept", "u_draw")), 15, at, at + 36, at + 12, at + 24, logprob.data_ptr())
+    need = m.lib().ws_verify_tree_workspace(r, a)
+    work = torch.empty(need, dtype=torch.uint8, device=DEV)
+    assert need > 4160
+    run = lambda: m.check(m.lib().ws_verify_tree(torch.cuda.current_stream().cuda_stream, r, a, work.data_ptr(), need), "ws_verify_tree")  # noqa: E731
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for i in (0, 1, 2, 1, 0, 2, 0, 0, 1, 1, 2):
+        for k, v in cases[i].items():
+            if v is not None:
+                call[k].copy_(v)
+        want = m.verify_tree(depth=15, **cases[i])
+        for _ in range(2):
+            work[begin:begin + 64] = 0
+            small.fill_(-9)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(small[0:3], want[0]) and torch.equal(small[9:].view(3, 15), want[1]) and torch.equal(small[3:6], want[2]) and torch.equal(small[6:9], want[3])
+            assert torch.equal(logprob, want[4])
+            assert int(want[3].sum()) == (0 if i != 1 else 3)
+
+
 # ---- attention
 
 

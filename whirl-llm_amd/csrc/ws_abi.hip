@@ -1341,7 +1341,7 @@ VerifyPlan verify_plan(const ws_loss_rows* r, uint32_t n_seq) {
     p.row_parts = p.row_parts < 1u ? 1u : (p.row_parts > 64u ? 64u : p.row_parts);
     p.levels = n_seq ? (r->rows + n_seq - 1u) / n_seq : 1u;  // (as many nodes as a sequence has on average; a larger one's take turns)
     p.levels = p.levels < 1u ? 1u : (p.levels > WS_TREE_MAX ? WS_TREE_MAX : p.levels);
-    p.meet = 32u + meet_bytes(n_seq, p.parts, ws::kTreeWords);  // (behind the epochs)
+    p.meet = meet_bytes(n_seq, p.parts, ws::kTreeWords);
     p.decided = p.meet + uint64_t{r->rows} * 16u;
     p.bytes = p.decided + meet_bytes(r->rows, p.row_parts, 4u);
     return p;
@@ -1464,8 +1464,7 @@ int ws_verify_tree(void* stream, const ws_loss_rows* r, const ws_verify_tree_arg
     v.parts = plan.parts;
     v.per = share_of((r->vocab + per - 1u) / per, v.parts);
     v.looks = a->spins ? a->spins : 256u;
-    v.epoch = reinterpret_cast<unsigned long long*>(work);
-    v.meet = reinterpret_cast<unsigned long long*>(work + 32u);
+    v.meet = reinterpret_cast<unsigned long long*>(work);
     v.tag = launch_tag();
     return ws::launch_tree_verify(S(stream), r->dtype, v);
 }

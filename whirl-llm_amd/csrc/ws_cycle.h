@@ -44,7 +44,6 @@ struct TreeVerifyArgs {
     uint32_t levels, look, row_parts, row_per;
     unsigned long long* row_meet;  // row_parts > 1: [rows][4][row_parts]
     unsigned long long* decided;   // [rows][2]
-    unsigned long long* epoch;     // [3]
     // of the draw: workgroups a sequence, vectors each (at most T * NV), how often one looks for the others
     uint32_t parts, per, looks;
     unsigned long long* meet;  // parts > 1: [n_seq][kTreeWords][parts]

@@ -250,10 +250,8 @@ __device__ __forceinline__ bool tree_drafts(const TreeVerifyArgs& A, int32_t off
     return true;
 }
 
-// The words of a launch (ws_loss.h) have a tag that no other launch has, but the replays of a captured one. So the tags also have a number that lies in the workspace, whatever it begins with, and
-// moves with every launch: epoch[0] is the one of the rows' words, epoch[1] the same for the draw to know, epoch[2] the draw's. The rows' kernel moves the last two, the draw's the first: neither one
-// that it reads itself.
-__device__ __forceinline__ unsigned long long tree_tag(const TreeVerifyArgs& A, unsigned long long epoch) { return A.tag ^ mix64(epoch); }
+// The words of a launch (ws_loss.h) have a tag that no other launch has, but the replays of a captured one: so no launch leaves its words behind where its next replay looks for them. The draw's
+// are taken apart by the next rows' kernel, when no draw runs; the rows' and the decisions by the draw's workgroups, when all of a sequence's have read them.
 
 // ---- what each node decides: the child that it passes the walk on to (with the log-probability of that one's token), or none; or that the walk does not come to it, or that its q entry is none
 constexpr uint32_t kDecNone = 64u, kDecNever = 65u, kDecBad = 66u;
@@ -268,12 +266,9 @@ __global__ void __launch_bounds__(kRowThreads, 3) tree_rows_kernel(TreeVerifyArg
     __shared__ uint32_t s_never;
     __shared__ __attribute__((aligned(16))) uint32_t s_seen[256];
     const uint32_t y = grid_row(), level = y / A.n_seq, s = y - level * A.n_seq, part = blockIdx.x, t = threadIdx.x, V = A.R.vocab;
-    const unsigned long long epoch = A.epoch[0], tag = tree_tag(A, epoch);
-    if (y == 0u && part == 0u && t == 0u) {
-        A.epoch[1] = epoch;
-        A.epoch[2] += 1ull;
-    }
+    const unsigned long long tag = A.tag;
     if (level >= A.levels) return;
+    if (level == 0u && part == 0u && A.parts > 1u && t < A.parts) break_word(A.meet + static_cast<size_t>(s) * A.parts * kTreeWords + t, A.parts);
     uint32_t n;
     const uint32_t first = tree_rows(A.seq_off, s, A.R.rows, n);
     if (level >= n) return;
@@ -401,7 +396,7 @@ __global__ void __launch_bounds__(T, WAVES) tree_draw_kernel(TreeVerifyArgs A) {
     __shared__ uint32_t taken_out[T * NV / 4];  // a byte a vector of the share: which of its tokens are listed
     __shared__ uint32_t special_id[64];
     __shared__ double special_w[64];
-    __shared__ uint32_t s_part, s_wave, s_token;
+    __shared__ uint32_t s_part, s_wave, s_token, s_last;
     __shared__ double s_target, s_wave_before;
     __shared__ float s_x;
     __shared__ double round_sum[NV][T];
@@ -413,13 +408,12 @@ __global__ void __launch_bounds__(T, WAVES) tree_draw_kernel(TreeVerifyArgs A) {
     const uint32_t first = tree_rows(A.seq_off, s, A.R.rows, n);
     unsigned long long* meet = A.meet + static_cast<size_t>(s) * parts * kTreeWords;
 
-    const unsigned long long rows_tag = tree_tag(A, A.epoch[1]), tag = tree_tag(A, A.epoch[2]);
-    if (part == 0u && s == 0u && t == 0u) A.epoch[0] = A.epoch[1] + 1ull;
+    const unsigned long long tag = A.tag;
     const double u_draw = A.u_draw[s];
     // down the tree, every wave by itself: a lane a node, and a lane a level for what was accepted
     const TreeLane L = tree_lane(A, first, n);
     unsigned long long decided = 0ull;
-    const bool known = lane < n && find_word(tree_decision(A, first + lane), 1u, rows_tag, decided);
+    const bool known = lane < n && find_word(tree_decision(A, first + lane), 1u, tag, decided);
     const uint32_t next_of = known ? static_cast<uint32_t>(decided & 0xffu) : kDecBad;
     int32_t path = -1;
     float path_lp = 0.f;
@@ -431,7 +425,7 @@ __global__ void __launch_bounds__(T, WAVES) tree_draw_kernel(TreeVerifyArgs A) {
         if (kids == 0ull) break;
         const uint32_t next = lane_value(next_of, cur);
         if (next == kDecNone) break;
-        if (next >= 64u || next <= cur) {
+        if (next >= n || next <= cur) {
             bad = true;
             break;
         }
@@ -442,6 +436,21 @@ __global__ void __launch_bounds__(T, WAVES) tree_draw_kernel(TreeVerifyArgs A) {
         }
         ++levels;
         cur = next;
+    }
+
+    // whether all of the sequence's workgroups have read the decisions: the last of them to leave its words finds everybody's at its first look, others may
+    bool all_read = parts == 1u;
+    if (bad) {
+        __syncthreads();
+        if (t < 64u && parts > 1u) {  // (the words of the draw, that say only that they are there)
+            if (t == 0u) leave_word(meet + part, parts, 0ull, tag);
+            words_arrived();
+            unsigned long long w;
+            const unsigned long long none = __ballot(t < parts && !find_word(meet + t, parts, tag, w));
+            if (t == 0u) s_last = none == 0ull ? 1u : 0u;
+        }
+        __syncthreads();
+        all_read = all_read || s_last != 0u;
     }
 
     uint32_t chosen = 0xffffffffu, target_part = 0;
@@ -527,7 +536,8 @@ __global__ void __launch_bounds__(T, WAVES) tree_draw_kernel(TreeVerifyArgs A) {
                     words_arrived();
                     bool here = t >= parts;
                     unsigned long long wm = 0, ws = 0;
-                    for (uint32_t look = 0; look < A.looks; ++look) {
+                    uint32_t look = 0;
+                    for (; look < A.looks; ++look) {
                         if (!here) {
                             here = find_word(meet + t, parts, tag, wm);
                             here = find_word(meet + 2u * parts + t, parts, tag, ws) && here;
@@ -538,7 +548,10 @@ __global__ void __launch_bounds__(T, WAVES) tree_draw_kernel(TreeVerifyArgs A) {
                     const unsigned long long none = __ballot(!here);
                     part_m[t] = __uint_as_float(static_cast<uint32_t>(wm));
                     part_s[t] = __longlong_as_double(static_cast<long long>(ws));
-                    if (t == 0u) missing = none;
+                    if (t == 0u) {
+                        missing = none;
+                        s_last = look == 0u ? 1u : 0u;
+                    }
                 }
             } else if (t == 0u && (first_turn || p != part)) {
                 part_m[p] = share_m;
@@ -546,7 +559,10 @@ __global__ void __launch_bounds__(T, WAVES) tree_draw_kernel(TreeVerifyArgs A) {
             }
             __syncthreads();
             if (parts == 1u) break;
-            if (first_turn) late = missing;
+            if (first_turn) {
+                late = missing;
+                all_read = s_last != 0u;
+            }
             else if (p == part) break;
             else late &= late - 1ull;
             if (first_turn && late == 0ull) break;
@@ -723,6 +739,15 @@ __global__ void __launch_bounds__(T, WAVES) tree_draw_kernel(TreeVerifyArgs A) {
             float* to = A.logprob + static_cast<size_t>(s) * (A.depth + 1u);
             if (t <= A.depth) to[t] = lp;
             if (t == 0u && A.depth == 64u) to[64] = 0.f;  // (63 drafts at most are accepted: the chosen one's is in the 64th place)
+        }
+    }
+    if (all_read) {  // the rows' words are taken apart, a pair of each (by all of a sequence's workgroups: five rows 11 -> 14.5 us)
+        for (uint32_t i = t; i < n; i += T) break_word(tree_decision(A, first + i), 1u);
+        if (A.row_parts > 1u) {
+            for (uint32_t i = t; i < n * A.row_parts; i += T) {
+                const uint32_t r = i / A.row_parts;
+                break_word(A.row_meet + static_cast<size_t>(first + r) * A.row_parts * 4u + (i - r * A.row_parts), A.row_parts);
+            }
         }
     }
 }
