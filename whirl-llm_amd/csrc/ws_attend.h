@@ -4,8 +4,8 @@
 // sums in 32 bits. So a column's softmax lies in the lanes that hold it: its maximum and sum never cross to other lanes but where a maximum grows, and P^T is the
 // second product's operand where the first one leaves it. Of V a lane takes 8 tokens' neighbouring elements, which two permutes a pair of tokens turn into 8 tokens of an element.
 //
-// One pass: a column keeps its maximum, sum and O^T; powers are of base two, and a column is scaled down only when its maximum has grown by more than kSlack (powers then
-// reach 2^kSlack, which 32 bits hold as exactly). A wave works on 32 positions at a time. Few columns (WM = 1): the four waves of a workgroup take different positions, K and V go from memory
+// One pass: a column keeps its maximum, sum and O^T; powers are of base two, and a column is scaled down only when a lane's eight powers against the maximum so far make more than kMost (32 bits
+// hold what is larger than one as exactly): else no maximum is looked for. A wave works on 32 positions at a time. Few columns (WM = 1): the four waves of a workgroup take different positions, K and V go from memory
 // into the registers of their operands. Many (WM = 4): the waves take different columns of the same positions, K and V go through LDS, the next ones' on their way in registers meanwhile.
 //
 // Work: units of kUnit positions of a sequence, a kv head and a tile of columns, numbered through; the workgroups share them evenly, whatever the sequences' lengths, each a run of neighbours.
@@ -25,9 +25,21 @@ namespace ws {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kUnit = 128u, kAttendThreads = 256u;
-constexpr float kSlack = 8.f;
+constexpr float kMost = 256.f;
+
+// 16 lanes' 8 bytes each in LDS, 4 by 16 elements of 16 bits, the other way round
+__device__ __forceinline__ u32x2 turned(const unsigned char* at) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at));
+}
+
+// 16 bytes a lane from memory into LDS, 1024 neighbouring bytes a wave
+__device__ __forceinline__ void to_lds(const unsigned char* from, unsigned char* wave_to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)wave_to, 16, 0, 0);
+}
 
 // a type's operands and their products
 template <int DT>
@@ -80,7 +92,8 @@ __device__ __forceinline__ float larger(float a, float b) { return __builtin_amd
 template <int DT, int DP, int MS, int WM>
 struct AttendShape {
     static constexpr uint32_t kTileCols = 16u * MS * WM;
-    static constexpr uint32_t kEach = DT == 1 && DP >= 128 ? 8u : 4u;  // elements of V a lane loads together: a lane holds elements kEach c + e of a block of 16 kEach
+    static constexpr bool kTurned = DT == 1 && WM > 1;  // V is turned by its reads from LDS: a lane asks for 4 elements of a token and gets 4 tokens' of an element
+    static constexpr uint32_t kEach = kTurned ? 1u : (DT == 1 && DP >= 128 ? 8u : 4u);  // elements of V a lane loads together: a lane holds elements kEach c + e of a block of 16 kEach
     static constexpr uint32_t kBlocks = DP / (16u * kEach);
     static constexpr uint32_t kOuts = kBlocks * kEach;                 // products' results that make up O^T of 16 columns, 4 floats a lane each
     static constexpr uint32_t kChunks = DP / Mat<DT>::kDepth;
@@ -89,8 +102,12 @@ struct AttendShape {
     // through LDS: tokens at a time, bytes of one, its 16-byte pieces, those of a thread
     static constexpr uint32_t kRow = DP * Mat<DT>::kBytes, kTokens = kRow <= 256u ? 64u : 32u, kPieces = kRow / 16u, kMine = kTokens * kPieces / 256u;
     static constexpr uint32_t kBuffer = kTokens * kRow;
-    // A token's pieces lie in another order for each of 16 neighbours, so that a piece of all of them, which K's operand takes together, lies in different banks.
-    static __device__ __forceinline__ uint32_t place(uint32_t token, uint32_t piece) { return token * kRow + (piece ^ (kPieces == 8u ? token >> 1 & 7u : token & 15u)) * 16u; }
+    // A token's pieces lie in another order for each of 16 neighbours, so that a piece of all of them, which K's operand takes together, lies in different banks, and a pair of pieces of 8 of them,
+    // which half a wave takes of V.
+    static __device__ __forceinline__ uint32_t order(uint32_t token) {
+        return (kPieces == 8u ? token & 6u : (token & 7u) << 1) | (token >> 3 & 1u);
+    }
+    static __device__ __forceinline__ uint32_t place(uint32_t token, uint32_t piece) { return token * kRow + (piece ^ order(token)) * 16u; }
 };
 
 // which of four positions from `pos` on a row sees: those before `length` and the nodes behind, by its bits. (A select a position, position < length ? true : bit, has been compiled
@@ -189,7 +206,17 @@ __device__ __forceinline__ float attend_odd(const AttendArgs& A, const unsigned 
 template <int DT, uint32_t EACH, uint32_t BLOCKS>
 __device__ __forceinline__ void attend_write(const AttendArgs& A, unsigned char* to, uint32_t g, const f32x4 (&o)[BLOCKS * EACH], float by) {
 #pragma unroll
-    for (uint32_t b = 0; b < BLOCKS; ++b)
+    for (uint32_t b = 0; b < BLOCKS; ++b) {
+        if constexpr (EACH == 1u) {
+            static_assert(DT == 1);
+            const uint32_t d = b * 16u + 4u * g;
+            if (d >= A.head_dim) continue;
+            __bf16 y[4];
+#pragma unroll
+            for (uint32_t l = 0; l < 4u; ++l) y[l] = static_cast<__bf16>(o[b][l] * by);
+            __builtin_memcpy(__builtin_assume_aligned(to + d * 2u, 8u), y, 8u);
+            continue;
+        }
 #pragma unroll
         for (uint32_t l = 0; l < 4u; ++l) {
             const uint32_t d = b * 16u * EACH + (4u * g + l) * EACH;
@@ -206,6 +233,7 @@ __device__ __forceinline__ void attend_write(const AttendArgs& A, unsigned char*
                 __builtin_memcpy(__builtin_assume_aligned(to + d * 4u, EACH * 4u), y, EACH * 4u);
             }
         }
+    }
 }
 
 // bytes to a token's piece of 16 bytes, from strides in such pieces: two multiplications of 32 bits, added up in 64
@@ -229,7 +257,8 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
     __shared__ AttendFind F;
     __shared__ uint32_t s_odd;
     __shared__ float s_part[kWT > 1u ? (kWT / 2u) * MS * (kDump + 128u) : 1u];
-    __shared__ uint4 s_kv[kStaged ? 2u * 2u * H::kBuffer / 16u : 1u];  // two buffers of K, then V
+    // two buffers of K, then V. (Two variables: of one that is indexed the compiler has every read wait for what is on its way to the other half.)
+    __shared__ uint4 s_even[kStaged ? 2u * H::kBuffer / 16u : 1u], s_odds[kStaged ? 2u * H::kBuffer / 16u : 1u];
     const uint32_t t = threadIdx.x, lane = lane_id(), c = lane & 15u, g = lane >> 4, wave = wave_id(), wm = wave % WM, wt = wave / WM;
 
     // (neighbouring runs on the same part of the chip: workgroup b runs on XCD b % 8)
@@ -292,14 +321,19 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
         const uint32_t p_end = min(u1 * kUnit, total);
         // A lane looks up the page of one position of those that are worked on next, and asks the others for theirs: one load ahead of the ones that need it
         constexpr uint32_t kAhead = kStaged ? H::kTokens : 32u;
-        auto page_of = [&](uint32_t p) __attribute__((always_inline)) { return attend_page(A, table, p + (lane & (kAhead - 1u)), p_end); };
+        uint32_t pg = 0u, pg_next = 0u, pg_pos = 0u;
+        // (What is loaded is not looked at before the next turn: that waits for all loads before it, too.)
+        auto page_of = [&](uint32_t p) __attribute__((always_inline)) {
+            pg_pos = p + (lane & (kAhead - 1u));
+            pg_next = static_cast<uint32_t>(table[min(pg_pos >> A.page_shift, A.slot_pages - 1u)]);
+        };
         auto page_from = [&](uint32_t pg, uint32_t token) __attribute__((always_inline)) { return static_cast<uint32_t>(__shfl(static_cast<int>(pg), static_cast<int>(token))); };
         // pg: of the positions that are worked on next; have: a bit for each that is there. (A page that is not: the first one's, not looked at.)
-        uint32_t pg = 0u, pg_next = 0u;
         uint64_t have = 0ull;
         auto turn = [&]() __attribute__((always_inline)) {
-            have = __ballot(pg_next < A.pages);  // (of 32 positions: the upper lanes say the same)
-            pg = pg_next < A.pages ? pg_next : 0u;
+            const bool is = pg_pos < p_end && pg_pos >> A.page_shift < A.slot_pages && pg_next < A.pages;
+            have = __ballot(is);  // (of 32 positions: the upper lanes say the same)
+            pg = is ? pg_next : 0u;
         };
         uint4 kx[2][kChunks];
         uint4 vx[8][kBlocks];
@@ -367,12 +401,23 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
                     for (uint32_t i = 0; i < 8u; ++i) x[m][i / 4u][i % 4u] = seen >> i & 1u ? x[m][i / 4u][i % 4u] : -INFINITY;
                 }
             }
+            float p[MS][8], part[MS];
+            auto raise = [&](int m) __attribute__((always_inline)) {
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; ++i) p[m][i] = __builtin_amdgcn_exp2f(fmaf(x[m][i / 4u][i % 4u], A.scale_log2, -top[m]));
+                part[m] = ((p[m][0] + p[m][1]) + (p[m][2] + p[m][3])) + ((p[m][4] + p[m][5]) + (p[m][6] + p[m][7]));
+            };
+            bool grown = false;
 #pragma unroll
             for (int m = 0; m < MS; ++m) {
-                float most = larger(larger(larger(x[m][0][0], x[m][0][1]), larger(x[m][0][2], x[m][0][3])), larger(larger(x[m][1][0], x[m][1][1]), larger(x[m][1][2], x[m][1][3])));
-                most *= A.scale_log2;
-                float p[8];
-                if (__ballot(most > top[m] + kSlack) != 0ull) {  // (uniform) some column's maximum has grown
+                raise(m);
+                grown |= part[m] > kMost;
+            }
+            if (__ballot(grown) != 0ull) {  // (uniform) some column's maximum has grown: only then they are looked for
+#pragma unroll
+                for (int m = 0; m < MS; ++m) {
+                    float most = larger(larger(larger(x[m][0][0], x[m][0][1]), larger(x[m][0][2], x[m][0][3])), larger(larger(x[m][1][0], x[m][1][1]), larger(x[m][1][2], x[m][1][3])));
+                    most *= A.scale_log2;
                     most = fmaxf(most, __shfl_xor(most, 16));
                     most = fmaxf(most, __shfl_xor(most, 32));
                     const float to = fmaxf(top[m], most), down = __builtin_amdgcn_exp2f(top[m] - to);
@@ -380,19 +425,21 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
                     sum[m] *= down;
 #pragma unroll
                     for (uint32_t r = 0; r < kOuts; ++r) o[m][r] *= down;
+                    raise(m);
                 }
+            }
 #pragma unroll
-                for (uint32_t i = 0; i < 8u; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(x[m][i / 4u][i % 4u], A.scale_log2, -top[m]));
-                sum[m] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            for (int m = 0; m < MS; ++m) {
+                sum[m] += part[m];
                 if constexpr (DT == 1) {
                     bf16x8 b;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) b[i] = static_cast<__bf16>(p[i]);
+                    for (int i = 0; i < 8; ++i) b[i] = static_cast<__bf16>(p[m][i]);
                     px[m][0] = __builtin_bit_cast(uint4, b);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 2; ++i)
-                        px[m][i] = make_uint4(__float_as_uint(p[4 * i]), __float_as_uint(p[4 * i + 1]), __float_as_uint(p[4 * i + 2]), __float_as_uint(p[4 * i + 3]));
+                        px[m][i] = make_uint4(__float_as_uint(p[m][4 * i]), __float_as_uint(p[m][4 * i + 1]), __float_as_uint(p[m][4 * i + 2]), __float_as_uint(p[m][4 * i + 3]));
                 }
             }
         };
@@ -426,9 +473,9 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
         if constexpr (!kStaged) {
             uint32_t p0 = u0 * kUnit + wt * 32u;
             if (p0 < p_end) {
-                pg_next = page_of(p0);
+                page_of(p0);
                 turn();
-                pg_next = page_of(p0 + kStep);
+                page_of(p0 + kStep);
                 load_k(p0, pg);
             }
             for (; p0 < p_end; p0 += kStep) {
@@ -440,7 +487,7 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
                     if (p0 + kStep < p_end) {
                         turn();
                         load_k(p0 + kStep, pg);
-                        pg_next = page_of(p0 + 2u * kStep);
+                        page_of(p0 + 2u * kStep);
                     }
                 });
                 if (!plain) {
@@ -452,55 +499,70 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
                 add_up([&](uint32_t i, uint32_t b) { return vx[i][b]; });
             }
         } else {
-            unsigned char* const lds = reinterpret_cast<unsigned char*>(s_kv);
-            u32x4 next_k[H::kMine], next_v[H::kMine];  // (uint4's copies of an array's elements keep it in scratch memory)
-            auto fetch = [&](uint32_t p) __attribute__((always_inline)) {
+            unsigned char* const even = reinterpret_cast<unsigned char*>(s_even);
+            unsigned char* const odds = reinterpret_cast<unsigned char*>(s_odds);
+            // 16 bytes a thread, K's and V's pieces in the places that they have in LDS: who loads which is turned about as they lie there
+            const uint32_t wave_at = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(wave))) * 1024u;
+            auto fetch = [&](uint32_t p, unsigned char* k_lds) __attribute__((always_inline)) {
 #pragma unroll
                 for (uint32_t l = 0; l < H::kMine; ++l) {
-                    const uint32_t at = l * 256u + t, token = at / H::kPieces, d = (at % H::kPieces) * Mat<DT>::kPer;
+                    const uint32_t at = l * 256u + t, token = at / H::kPieces, d = ((at % H::kPieces) ^ H::order(token)) * Mat<DT>::kPer;
                     const uint32_t page = page_from(pg, token), in = (p + token) & in_page, piece = (d < A.head_dim ? d : 0u) * E / 16u;
-                    next_k[l] = *reinterpret_cast<const u32x4*>(k_base + attend_offset(page, A.k_page, in, A.k_token, piece));
-                    next_v[l] = *reinterpret_cast<const u32x4*>(v_base + attend_offset(page, A.v_page, in, A.v_token, piece));
+                    to_lds(k_base + attend_offset(page, A.k_page, in, A.k_token, piece), k_lds + l * 4096u + wave_at);
+                    to_lds(v_base + attend_offset(page, A.v_page, in, A.v_token, piece), k_lds + H::kBuffer + l * 4096u + wave_at);
                 }
             };
-            uint32_t p = u0 * kUnit, buffer = 0u;
+            // where a lane reads: of K piece 4 j + g of tokens c, of V (turned) 4 elements of token 4 g + c / 4; a token's order is the same 16 behind it
+            const uint32_t k_row = c * H::kRow, k_piece = (g ^ H::order(c)) * 16u;
+            const uint32_t v_row = (4u * g + c / 4u) * H::kRow + (c & 1u) * 8u, v_piece = ((c >> 1 & 1u) ^ H::order(4u * g + c / 4u)) * 16u;
+            uint32_t p = u0 * kUnit;
             if (p < p_end) {
-                pg_next = page_of(p);
+                page_of(p);
                 turn();
-                pg_next = page_of(p + H::kTokens);
-                fetch(p);
+                page_of(p + H::kTokens);
+                fetch(p, even);
             }
-            for (; p < p_end; p += H::kTokens, buffer ^= 1u) {  // (the same for the workgroup)
-                unsigned char* const k_lds = lds + buffer * 2u * H::kBuffer;
+            auto chunk = [&](unsigned char* const k_lds, unsigned char* const next_lds) __attribute__((always_inline)) {
                 unsigned char* const v_lds = k_lds + H::kBuffer;
                 const uint64_t here = have;
                 const bool nodes = p + H::kTokens > length;        // (uniform)
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (what is on its way to LDS)
+                __syncthreads();
                 if (here != ~0ull || nodes) {
 #pragma unroll
                     for (uint32_t l = 0; l < H::kMine; ++l) {
                         const uint32_t token = (l * 256u + t) / H::kPieces;
-                        const uint4 v = clean(make_uint4(next_v[l].x, next_v[l].y, next_v[l].z, next_v[l].w), here >> token & 1u, p + token >= length);
-                        next_v[l] = u32x4{v.x, v.y, v.z, v.w};
+                        uint4& v = *reinterpret_cast<uint4*>(v_lds + (l * 256u + t) * 16u);
+                        v = clean(v, here >> token & 1u, p + token >= length);
                     }
+                    __syncthreads();
                 }
-#pragma unroll
-                for (uint32_t l = 0; l < H::kMine; ++l) {
-                    const uint32_t at = l * 256u + t, token = at / H::kPieces, piece = at % H::kPieces;
-                    *reinterpret_cast<u32x4*>(k_lds + H::place(token, piece)) = next_k[l];
-                    *reinterpret_cast<u32x4*>(v_lds + H::place(token, piece)) = next_v[l];
-                }
-                __syncthreads();
                 if (p + H::kTokens < p_end) {
                     turn();
-                    fetch(p + H::kTokens);
-                    pg_next = page_of(p + 2u * H::kTokens);
+                    page_of(p + 2u * H::kTokens);
+                    fetch(p + H::kTokens, next_lds);
                 }
-#pragma unroll 1
-                for (uint32_t sub = 0; sub < H::kTokens && p + sub < p_end && col0 < cols; sub += 32u) {
+                if (col0 >= cols) return;
+#pragma unroll
+                for (uint32_t sub = 0; sub < H::kTokens; sub += 32u) {
                     const uint32_t p0 = p + sub;
+                    if (p0 >= p_end) break;
                     const bool plain = p0 + 32u <= length && static_cast<uint32_t>(here >> sub) == 0xffffffffu;
-                    powers(p0, plain, mine_of(here, sub), [&](uint32_t i, uint32_t j) { return *reinterpret_cast<const uint4*>(k_lds + H::place(sub + 16u * i + c, j * 4u + g)); }, []() {});
-                    add_up([&](uint32_t i, uint32_t b) {
+                    u32x2 v[H::kTurned ? kOuts : 1u][2];
+                    powers(p0, plain, mine_of(here, sub), [&](uint32_t i, uint32_t j) { return *reinterpret_cast<const uint4*>(k_lds + k_row + (k_piece ^ j * 64u) + (sub + 16u * i) * H::kRow); }, [&]() {
+                        if constexpr (H::kTurned) {  // of 4 tokens 16 elements: lane c of 16 asks for 4 elements of token c / 4, gets the tokens' c-th
+#pragma unroll
+                            for (uint32_t r = 0; r < kOuts; ++r)
+#pragma unroll
+                                for (uint32_t i = 0; i < 2u; ++i) v[r][i] = turned(v_lds + v_row + (v_piece ^ r * 32u) + (sub + 16u * i) * H::kRow);
+                        }
+                    });
+                    if constexpr (H::kTurned) {
+#pragma unroll
+                        for (uint32_t r = 0; r < kOuts; ++r)
+#pragma unroll
+                            for (int m = 0; m < MS; ++m) o[m][r] = Mat<1>::mul(make_uint4(v[r][0].x, v[r][0].y, v[r][1].x, v[r][1].y), px[m][0], o[m][r]);
+                    } else add_up([&](uint32_t i, uint32_t b) {
                         const uint32_t token = v_pos(sub, i);
                         if constexpr (kEach * E == 16u) {
                             return *reinterpret_cast<const uint4*>(v_lds + H::place(token, b * 16u + c));
@@ -510,6 +572,12 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
                         }
                     });
                 }
+            };
+            for (; p < p_end; p += H::kTokens) {  // (the same for the workgroup)
+                chunk(even, odds);
+                p += H::kTokens;
+                if (p >= p_end) break;
+                chunk(odds, even);
             }
         }
         if (__ballot(odd != 0u) != 0ull && lane == 0u) s_odd = 1u;
