@@ -837,8 +837,7 @@ def verify_tree(logits, ids, seq_off, u_accept, u_draw, parent=None, q=None, q_o
         raise WsError(f"depth: 1 to {TREE_MAX}; spins: at most {_MOST_SPINS}")
     if q is not None and (q.dtype is not _I32 or q.get_device() != at or not q.is_contiguous()):
         raise WsError("q: contiguous int32 tensor on the logits' device")
-    counts = torch.empty((3, n_seq), dtype=_I32, device=dev)
-    path = torch.empty((n_seq, depth), dtype=_I32, device=dev)
+    counts, path = seq_off.new_empty((3, n_seq)), seq_off.new_empty((n_seq, depth))
     a = VerifyTree(n_seq, _vector("seq_off", seq_off, _I32, n_seq + 1, at), _vector("parent", parent, _I32, rows, at), _p(q), q.numel() if q is not None else 0,
                    _vector("q_off", _given("q_off", q_off) if q is not None else None, _I32, rows, at), _vector("u_accept", _given("u_accept", u_accept), _F64, rows, at),
                    _vector("u_draw", _given("u_draw", u_draw), _F64, n_seq, at), depth, counts.data_ptr(), path.data_ptr(), counts.data_ptr() + 4 * n_seq, counts.data_ptr() + 8 * n_seq)
@@ -891,8 +890,7 @@ def tree_attention(q, k, v, table, length, seq_off, mask=None, slot=None, scale=
     if slot is None and n_seq > slots:
         raise WsError(f"slot: missing, and {n_seq} sequences have {slots} slots")
     if out is None:
-        # (where a caller has rows behind the last sequence, they are left as they are: zeros)
-        out = torch.empty((rows, heads, dim), dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)  # (rows behind the last sequence: whatever the memory held)
     elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != at or (out.stride(2) != 1 and dim > 1):
         raise WsError("out: of q's shape and dtype, on its device, unit inner stride")
     else:
@@ -903,7 +901,7 @@ def tree_attention(q, k, v, table, length, seq_off, mask=None, slot=None, scale=
                       _vector("length", length, _I32, n_seq, at), _vector("slot", slot, _I32, n_seq, at), _vector("mask", mask, _I64, rows, at), dim ** -0.5 if scale is None else scale, max_nodes)
     call, ref = lib(), C.byref(a)
     need = call.ws_tree_attention_workspace(ref)
-    work = torch.empty(need, dtype=torch.uint8, device=q.device)
+    work = length.new_empty((need + 3) // 4)
     check(call.ws_tree_attention(_stream(), ref, work.data_ptr(), need), "ws_tree_attention")
     return (out, lse) if want_lse else out
 
@@ -945,21 +943,21 @@ class PagedCache:
     def reserve(self, slot, tokens):
         """Pages for tokens[i] tokens in all for slot[i] (ws_cache_reserve). Returns status."""
         n, at = self._lists(("slot", slot), ("tokens", tokens))
-        status = torch.empty(n, dtype=_I32, device=slot.device)
+        status = torch.empty_like(slot)
         check(lib().ws_cache_reserve(_stream(), C.byref(self.desc), *at, n, status.data_ptr()), "ws_cache_reserve")
         return status
 
     def fork(self, src, dst, length):
         """The empty slot dst[i] becomes a copy of the first length[i] tokens of slot src[i]: whole pages shared, the last, partly filled one copied (ws_cache_fork). Returns status."""
         n, at = self._lists(("src", src), ("dst", dst), ("length", length))
-        status = torch.empty(n, dtype=_I32, device=src.device)
+        status = torch.empty_like(src)
         check(lib().ws_cache_fork(_stream(), C.byref(self.desc), *at, n, status.data_ptr()), "ws_cache_fork")
         return status
 
     def release(self, slot, tokens):
         """Slot slot[i] keeps the pages of its first tokens[i] tokens, the others go back (ws_cache_release). Returns status."""
         n, at = self._lists(("slot", slot), ("tokens", tokens))
-        status = torch.empty(n, dtype=_I32, device=slot.device)
+        status = torch.empty_like(slot)
         check(lib().ws_cache_release(_stream(), C.byref(self.desc), *at, n, status.data_ptr()), "ws_cache_release")
         return status
 

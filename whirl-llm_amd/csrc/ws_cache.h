@@ -149,6 +149,12 @@ __global__ void __launch_bounds__(WS_BLOCK) cache_fork_kernel(PagesArgs A) {
     if (t == 0u) C.n_free[0] = n_free - static_cast<int32_t>(total);
 }
 
+// What the workgroup's atomics have done is in the memory that all of them see (one compute unit's: no cache is written back or emptied for it, which takes microseconds)
+__device__ __forceinline__ void arrived() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
 // A page that several of the call's sequences give back goes where the first of them has it. Who is that does not depend on the order of the atomics: all take theirs off the count; where
 // it is 0, it becomes the smallest number of an entry (kMark below 0), whose thread then gives the page back and makes the count 0 again.
 constexpr int32_t kMark = -2147483647 - 1;
@@ -176,32 +182,30 @@ __global__ void __launch_bounds__(WS_BLOCK) cache_release_kernel(PagesArgs A) {
     L.first[t] = block_excl_scan(static_cast<uint64_t>(gone), L.red, &total);
     L.at[t] = kept;
     __syncthreads();
+    // From the last entry to the first, so that the first comes to lie uppermost. A thread keeps what it finds of the first round of entries, the only one but of calls that give much back.
     auto entry = [&](uint64_t e) {
         const uint32_t i = sequence_of(L.first, A.n, e);
         return C.table + static_cast<uint64_t>(L.name[i]) * C.table_stride + L.at[i] + (e - L.first[i]);
     };
-    for (uint64_t e = t; e < total; e += WS_BLOCK) {
-        const int32_t page = *entry(e);
+    int32_t* const place0 = t < total ? entry(total - 1u - t) : nullptr;
+    const int32_t page0 = place0 ? *place0 : -1;
+    auto page_of = [&](uint64_t at) { return at == 0u ? page0 : (at + t < total ? *entry(total - 1u - at - t) : -1); };
+    for (uint64_t at = 0; at < total; at += WS_BLOCK) {
+        const int32_t page = page_of(at);
         if (static_cast<uint32_t>(page) < C.pages) atomicSub(&C.refs[page], 1);
     }
-    __threadfence();
-    __syncthreads();
-    for (uint64_t e = t; e < total; e += WS_BLOCK) {
-        const int32_t page = *entry(e);
+    arrived();
+    for (uint64_t at = 0; at < total; at += WS_BLOCK) {
+        const int32_t page = page_of(at);
         if (static_cast<uint32_t>(page) >= C.pages) continue;
         const int32_t left = fresh(&C.refs[page]);
-        if (left == 0 || is_mark(left)) atomicMin(&C.refs[page], kMark + static_cast<int32_t>(e));
+        if (left == 0 || is_mark(left)) atomicMin(&C.refs[page], kMark + static_cast<int32_t>(total - 1u - at - t));
     }
-    __threadfence();
-    __syncthreads();
-    // from the last entry to the first, so that the first comes to lie uppermost
+    arrived();
     uint64_t put = 0;
     for (uint64_t at = 0; at < total; at += WS_BLOCK) {
-        const bool in = at + t < total;
-        const uint64_t e = in ? total - 1u - at - t : 0u;
-        int32_t* place = in ? entry(e) : nullptr;
-        const int32_t page = in ? *place : -1;
-        const bool mine = static_cast<uint32_t>(page) < C.pages && fresh(&C.refs[page]) == kMark + static_cast<int32_t>(e);
+        const int32_t page = page_of(at);
+        const bool mine = static_cast<uint32_t>(page) < C.pages && fresh(&C.refs[page]) == kMark + static_cast<int32_t>(total - 1u - at - t);
         uint64_t all = 0;
         const uint64_t rank = block_excl_scan(static_cast<uint64_t>(mine ? 1u : 0u), L.red, &all);
         if (mine) {
@@ -209,7 +213,7 @@ __global__ void __launch_bounds__(WS_BLOCK) cache_release_kernel(PagesArgs A) {
             if (to < C.pages) C.free[to] = page;
             C.refs[page] = 0;
         }
-        if (in) *place = -1;
+        if (at + t < total) *(at == 0u ? place0 : entry(total - 1u - at - t)) = -1;
         put += all;
         __syncthreads();
     }
