@@ -673,6 +673,7 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
             r.tile = tile;
             r.more = static_cast<uint32_t>(last / per - first / per);
             r.odd = 0u;
+            r.first = W.first, r.nodes = W.nodes, r.length = W.length, r.total = W.total;
             A.run[run_id] = r;
         }
         at += u1 - u0;
@@ -694,14 +695,14 @@ __global__ void __launch_bounds__(64 * kJoinWaves) attend_join_kernel(AttendArgs
     const uint32_t x = blockIdx.x, sub = blockIdx.y, t = threadIdx.x, lane = t & 63u, wave = t >> 6, c = lane & 15u, g = lane >> 4;
     const AttendRun R = A.run[x];
     if (R.more == 0u) return;
-    const AttendWork W = attend_work(A, R.seq, H::kTileCols);
-    const uint32_t cols = W.nodes * A.group, col = R.tile * H::kTileCols + sub * 16u + c;
+    const uint32_t cols = R.nodes * A.group, col = R.tile * H::kTileCols + sub * 16u + c;
     if (col - c >= cols) return;
     auto piece = [&](uint32_t i) { return A.part + ((static_cast<uint64_t>(x) + i) * 2u + (i == 0u ? 1u : 0u)) * H::kPartFloats + sub * H::kSubFloats; };
     float top = -FLT_MAX, sum = 0.f;
     f32x4 o[kOuts];
 #pragma unroll
     for (uint32_t r = 0; r < kOuts; ++r) o[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const bool odd = A.run[x + R.more].odd != 0u;  // (said by the one that has the nodes)
     float their_top = -FLT_MAX, their_sum = 0.f;
     f32x4 theirs[kOuts];
     auto load = [&](uint32_t i) __attribute__((always_inline)) {
@@ -743,12 +744,12 @@ __global__ void __launch_bounds__(64 * kJoinWaves) attend_join_kernel(AttendArgs
     }
     if (wave != 0u || col >= cols) return;
     const uint32_t node = col / A.group, h = R.head * A.group + (col - node * A.group);
-    if (A.run[x + R.more].odd != 0u) {
+    if (odd) {
         const int32_t* table = A.table + static_cast<uint64_t>(A.slot ? A.slot[R.seq] : R.seq) * A.table_stride;
-        const uint64_t sees = A.mask ? A.mask[W.first + node] : (node < 63u ? (uint64_t{2} << node) - 1u : ~uint64_t{0});
+        const uint64_t sees = A.mask ? A.mask[R.first + node] : (node < 63u ? (uint64_t{2} << node) - 1u : ~uint64_t{0});
 #pragma unroll 1
-        for (uint32_t j = 0; j < W.nodes && W.length + j < W.total; ++j) {
-            const uint32_t pos = W.length + j, pg = attend_page(A, table, pos, W.total);
+        for (uint32_t j = 0; j < R.nodes && R.length + j < R.total; ++j) {
+            const uint32_t pos = R.length + j, pg = attend_page(A, table, pos, R.total);
             if (pg >= A.pages) continue;
             const unsigned char* at_v = A.v + R.head * A.v_head + attend_offset(pg, A.v_page, pos & ((1u << A.page_shift) - 1u), A.v_token, 0u);
 #pragma unroll
@@ -760,8 +761,8 @@ __global__ void __launch_bounds__(64 * kJoinWaves) attend_join_kernel(AttendArgs
         }
     }
     const float by = sum == 0.f ? 0.f : 1.f / sum;
-    if (A.lse && g == 0u) A.lse[static_cast<uint64_t>(W.first + node) * A.heads + h] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * 0.69314718f;
-    attend_write<DT, kEach, H::kBlocks>(A, A.out + static_cast<uint64_t>(W.first + node) * A.out_row + static_cast<uint64_t>(h) * A.out_head, g, o, by);
+    if (A.lse && g == 0u) A.lse[static_cast<uint64_t>(R.first + node) * A.heads + h] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * 0.69314718f;
+    attend_write<DT, kEach, H::kBlocks>(A, A.out + static_cast<uint64_t>(R.first + node) * A.out_row + static_cast<uint64_t>(h) * A.out_head, g, o, by);
 }
 
 }  // namespace ws

@@ -85,6 +85,7 @@ struct AttendArgs {
 // what the join needs of a workgroup: the tile that begins in its run and does not end there (`more` workgroups behind it hold the rest)
 struct AttendRun {
     uint32_t seq, head, tile, more;
+    uint32_t first, nodes, length, total;  // of the sequence, as in AttendWork
     uint32_t odd;  // whether its first part (of a tile that began before) has met nodes whose V holds infinities or NaN
 };
 
