@@ -385,6 +385,27 @@ def test_attention(case, mask):
     assert all(torch.equal(x[:rows], y[:rows]) for x, y in zip(a, b))
 
 
+@pytest.mark.parametrize("dtype,dim,heads,n", [(BF16, 128, 4, 40), (BF16, 64, 2, 7), (BF16, 128, 2, 64), (BF16, 256, 8, 64), (F32, 64, 4, 64), (F32, 128, 8, 20), (BF16, 128, 16, 64)])
+@pytest.mark.parametrize("before", [0, 25, 60, 100, 127, 1000])
+def test_attention_nodes_that_workgroups_share(dtype, dim, heads, n, before):
+    """Infinities in the V of nodes that several workgroups' positions hold: seen by those that see the node, whichever workgroup has it."""
+    m = gc.pkg()
+    call, host = attend_case([n], [before], heads, 2, dim, 16, dtype, before + dim + n)
+    clean = m.tree_attention(**call)
+    G = heads // 2
+    for node in sorted({0, 1, 3, 31 - before % 32, 64 - before % 64, n // 2, n - 1}):
+        if not 0 <= node < n:
+            continue
+        t = call["v"].clone()
+        p = before + node
+        t[host["table"][0, p // 16], p % 16, 1, 2] = math.inf
+        got = m.tree_attention(**{**call, "v": t})
+        sees = torch.tensor([bool(int(host["masks"][r]) >> node & 1) for r in range(n)])
+        want = clean.clone()
+        want[sees.to(DEV), G:, 2] = math.inf
+        assert torch.equal(got, want), (node, int((got != want).sum()))
+
+
 def test_attention_unseen_places_do_not_matter():
     """Infinities and NaN in the K and V of nodes that a row does not see leave it alone; those that see them get what the formula gives."""
     m = gc.pkg()

@@ -28,7 +28,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-constexpr uint32_t kUnit = 128u, kAttendThreads = 256u;
+constexpr uint32_t kAttendThreads = 256u;
 constexpr float kMost = 256.f;
 
 // 16 lanes' 8 bytes each in LDS, 4 by 16 elements of 16 bits, the other way round
@@ -102,6 +102,8 @@ struct AttendShape {
     // through LDS: tokens at a time, bytes of one, its 16-byte pieces, those of a thread
     static constexpr uint32_t kRow = DP * Mat<DT>::kBytes, kTokens = kRow <= 256u ? 64u : 32u, kPieces = kRow / 16u, kMine = kTokens * kPieces / 256u;
     static constexpr uint32_t kBuffer = kTokens * kRow;
+    // positions that work is counted in: what a workgroup's waves take together
+    static constexpr uint32_t kUnit = WM > 1 ? kTokens : 128u;
     // A token's pieces lie in another order for each of 16 neighbours, so that a piece of all of them, which K's operand takes together, lies in different banks, and a pair of pieces of 8 of them,
     // which half a wave takes of V.
     static __device__ __forceinline__ uint32_t order(uint32_t token) {
@@ -123,7 +125,7 @@ struct AttendWork {  // a sequence's
     uint32_t first, nodes, total, length, tiles, units;  // row, nodes, positions, those before the nodes, tiles of columns, units of a tile
     uint64_t all;                                        // units of all heads and tiles
 };
-__device__ __forceinline__ AttendWork attend_work(const AttendArgs& A, uint32_t s, uint32_t cols) {
+__device__ __forceinline__ AttendWork attend_work(const AttendArgs& A, uint32_t s, uint32_t cols, uint32_t unit) {
     AttendWork w;
     const uint32_t a = min(A.seq_off[s], A.rows), b = min(A.seq_off[s + 1u], A.rows);
     w.first = a;
@@ -132,7 +134,7 @@ __device__ __forceinline__ AttendWork attend_work(const AttendArgs& A, uint32_t 
     w.length = A.length[s];
     w.total = static_cast<uint32_t>(min(static_cast<uint64_t>(w.length) + w.nodes, room));
     w.tiles = (w.nodes * A.group + cols - 1u) / cols;
-    w.units = max((w.total + kUnit - 1u) / kUnit, 1u);
+    w.units = max((w.total + unit - 1u) / unit, 1u);
     w.all = static_cast<uint64_t>(w.tiles) * A.kv_heads * w.units;
     return w;
 }
@@ -162,12 +164,12 @@ struct AttendFind {
 };
 // The units of all sequences, and in `find` the sequence that holds unit first(all): a sequence a thread, 256 at a time.
 template <class Fn>
-__device__ __forceinline__ uint64_t attend_find(const AttendArgs& A, uint32_t cols, AttendFind& F, Fn&& first) {
+__device__ __forceinline__ uint64_t attend_find(const AttendArgs& A, uint32_t cols, uint32_t unit, AttendFind& F, Fn&& first) {
     const uint32_t t = threadIdx.x;
     uint64_t mine = 0, before = 0, all = 0;
     AttendWork w{};
     for (uint32_t s = t; s < A.n_seq; s += kAttendThreads) {
-        w = attend_work(A, s, cols);
+        w = attend_work(A, s, cols, unit);
         mine += w.all;
     }
     before = scan256(mine, F.red, all);
@@ -177,7 +179,7 @@ __device__ __forceinline__ uint64_t attend_find(const AttendArgs& A, uint32_t co
     for (uint32_t s0 = 0; s0 < A.n_seq; s0 += kAttendThreads) {
         if (A.n_seq > kAttendThreads) {  // (the sums above were of several)
             w = AttendWork{};
-            if (s0 + t < A.n_seq) w = attend_work(A, s0 + t, cols);
+            if (s0 + t < A.n_seq) w = attend_work(A, s0 + t, cols, unit);
             mine = w.all;
             uint64_t total;
             before = base + scan256(mine, F.red, total);
@@ -264,7 +266,7 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
     // (neighbouring runs on the same part of the chip: workgroup b runs on XCD b % 8)
     const uint32_t in_xcd = A.groups / 8u, run_id = blockIdx.x < in_xcd * 8u ? (blockIdx.x & 7u) * in_xcd + (blockIdx.x >> 3) : blockIdx.x;
     uint64_t per = 0, begin = 0;
-    const uint64_t all = attend_find(A, H::kTileCols, F, [&](uint64_t units) {
+    const uint64_t all = attend_find(A, H::kTileCols, H::kUnit, F, [&](uint64_t units) {
         per = max((units + A.groups - 1u) / A.groups, static_cast<uint64_t>(A.least));
         return begin = per * run_id;
     });
@@ -281,7 +283,7 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
         while (at - seq_first >= W.all) {
             seq_first += W.all;
             ++s;  // (there is one: at < all)
-            W = attend_work(A, s, H::kTileCols);
+            W = attend_work(A, s, H::kTileCols, H::kUnit);
         }
         const uint64_t in_seq = at - seq_first;
         const uint32_t item = static_cast<uint32_t>(in_seq / W.units), u0 = static_cast<uint32_t>(in_seq - static_cast<uint64_t>(item) * W.units);
@@ -318,7 +320,7 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
         const unsigned char* v_base = A.v + head * A.v_head;
         const uint32_t in_page = (1u << A.page_shift) - 1u;
 
-        const uint32_t p_end = min(u1 * kUnit, total);
+        const uint32_t p_end = min(u1 * H::kUnit, total);
         // A lane looks up the page of one position of those that are worked on next, and asks the others for theirs: one load ahead of the ones that need it
         constexpr uint32_t kAhead = kStaged ? H::kTokens : 32u;
         uint32_t pg = 0u, pg_next = 0u, pg_pos = 0u;
@@ -471,7 +473,7 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
             }
         };
         if constexpr (!kStaged) {
-            uint32_t p0 = u0 * kUnit + wt * 32u;
+            uint32_t p0 = u0 * H::kUnit + wt * 32u;
             if (p0 < p_end) {
                 page_of(p0);
                 turn();
@@ -515,7 +517,7 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
             // where a lane reads: of K piece 4 j + g of tokens c, of V (turned) 4 elements of token 4 g + c / 4; a token's order is the same 16 behind it
             const uint32_t k_row = c * H::kRow, k_piece = (g ^ H::order(c)) * 16u;
             const uint32_t v_row = (4u * g + c / 4u) * H::kRow + (c & 1u) * 8u, v_piece = ((c >> 1 & 1u) ^ H::order(4u * g + c / 4u)) * 16u;
-            uint32_t p = u0 * kUnit;
+            uint32_t p = u0 * H::kUnit;
             if (p < p_end) {
                 page_of(p);
                 turn();
@@ -663,7 +665,7 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
                 }
             }
         }
-        if (t == 0u && u0 != 0u) run_odd = any_odd ? 1u : 0u;
+        if (t == 0u && any_odd) run_odd |= u0 != 0u ? 1u : 2u;
         if (t == 0u && u0 == 0u && u1 < W.units) {
             // the workgroups that hold the rest of this tile
             const uint64_t first = at, last = at + W.units - 1u;
@@ -702,7 +704,9 @@ __global__ void __launch_bounds__(64 * kJoinWaves) attend_join_kernel(AttendArgs
     f32x4 o[kOuts];
 #pragma unroll
     for (uint32_t r = 0; r < kOuts; ++r) o[r] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const bool odd = A.run[x + R.more].odd != 0u;  // (said by the one that has the nodes)
+    // (by those that have the nodes: three pieces at most, of 32 positions at least)
+    bool odd = R.more < 3u && (R.odd & 2u) != 0u;
+    for (uint32_t i = R.more > 2u ? R.more - 2u : 1u; i <= R.more; ++i) odd = odd || (A.run[x + i].odd & 1u) != 0u;
     float their_top = -FLT_MAX, their_sum = 0.f;
     f32x4 theirs[kOuts];
     auto load = [&](uint32_t i) __attribute__((always_inline)) {

@@ -86,7 +86,7 @@ struct AttendArgs {
 struct AttendRun {
     uint32_t seq, head, tile, more;
     uint32_t first, nodes, length, total;  // of the sequence, as in AttendWork
-    uint32_t odd;  // whether its first part (of a tile that began before) has met nodes whose V holds infinities or NaN
+    uint32_t odd;  // bits: whether its first part (of a tile that began before), its last (of the one that begins) has met nodes whose V holds infinities or NaN
 };
 
 struct AttendPlan {
