@@ -693,8 +693,8 @@ int ws_tree_stage(void* stream, const ws_tree_stage_args* a);
  * status[s]: WS_ACCEPT_HOST where a row on the walk has nothing that can be drawn (nothing allowed, NaN, an infinite logit, an inv_t that is none) or its q
  * entry lies outside q, or the sequence has no nodes: chosen is -1 then, what was accepted before is reported and the history left as it was;
  * WS_ACCEPT_HISTORY_FULL (with WS_ACCEPT_HOST) where the slot has no room for what was accepted: n_accepted 0, chosen -1.
- * Only the rows that the walk meets are read. workspace: device memory of ws_verify_tree_workspace() bytes (0: none is needed), 8-byte aligned, of any contents, nobody else's
- * until the launch is done (a captured launch may be replayed); the workgroups that share a row meet there. Required where that is not 0. */
+ * Rows that the walk does not meet do not matter, but may be read. workspace: device memory of ws_verify_tree_workspace() bytes, 8-byte aligned, of any contents, nobody else's
+ * until the launch is done (a captured launch may be replayed, whatever others have done there meanwhile); the workgroups meet there. Required where that is not 0. */
 typedef struct ws_verify_tree_args {
     uint32_t n_seq;
     const uint32_t* seq_off; /* device [n_seq + 1] */
@@ -711,13 +711,13 @@ typedef struct ws_verify_tree_args {
     uint32_t* status;        /* out, device [n_seq] */
     float* logprob;          /* out, device [n_seq][depth + 1] (may be NULL) */
     ws_history hist;         /* tokens NULL: no device history */
-    uint32_t spins;          /* as ws_policy.spins */
+    uint32_t spins;          /* as ws_policy.spins, of the row that the token is drawn from */
 } ws_verify_tree_args;
 uint64_t ws_verify_tree_workspace(const ws_loss_rows* r, const ws_verify_tree_args* a);
 int ws_verify_tree(void* stream, const ws_loss_rows* r, const ws_verify_tree_args* a, void* workspace, uint64_t workspace_bytes);
 
 /* One layer of a paged cache: K and V [pages][page_tokens][kv_heads][head_dim] of dtype, the dimensions any strides apart (in elements, multiples of 16 bytes, head_dim's
- * 1), 16-byte aligned; which page holds what: position p of slot s is token p % page_tokens of page table[s][p / page_tokens]. page_tokens: a power of two.
+ * 1, a page's and a token's below 2^36 bytes: else WS_E_UNSUPPORTED), 16-byte aligned; which page holds what: position p of slot s is token p % page_tokens of page table[s][p / page_tokens]. page_tokens: a power of two.
  * head_dim: a multiple of 8, up to 256. A page outside [0, pages) - -1 by custom - holds nothing. */
 typedef struct ws_cache_layer {
     const void* k;
@@ -785,7 +785,8 @@ int ws_cache_reserve(void* stream, const ws_cache* c, const int32_t* slot, const
  * partly filled one are copied to a page of dst[i]'s own. A src may be named several times. (Tokens that either writes from then on go behind the first length[i], into pages of its own.) */
 int ws_cache_fork(void* stream, const ws_cache* c, const int32_t* src, const int32_t* dst, const int32_t* length, uint32_t n, int32_t* status);
 /* Slot slot[i] keeps the pages of its first tokens[i] tokens (0: none) and gives the others back. Pages that nobody holds any more go on top of the free ones, the first of the first slot
- * uppermost. status may be NULL. */
+ * uppermost. status may be NULL. (A page that a slot keeps in part may have other holders still, who see what is written there: a slot that forked, or was forked from, and is cut
+ * back to less than they share is not written to before a fork of its own.) */
 int ws_cache_release(void* stream, const ws_cache* c, const int32_t* slot, const int32_t* tokens, uint32_t n, int32_t* status);
 /* After ws_verify_tree: in every layer position length[s] + 1 + i of the sequence's slot becomes what position length[s] + path[s][i] holds, i = 0 .. n_accepted[s] - 1 in this order (the
  * root stays where it is), so that the accepted tokens lie behind the text as the history has them. Entries of path from the first on that does not
