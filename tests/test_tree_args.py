@@ -73,7 +73,7 @@ def test_verification_workspaces():
             assert parts == int(parts) and 2 <= parts <= 64
             r.rows = 64 * n_seq
             parts = (m.lib().ws_verify_tree_workspace(C.byref(r), C.byref(verify_of(m, n_seq=n_seq))) - draw - r.rows * 16) / (r.rows * 32)
-            assert parts == int(parts) and (2 <= parts <= 64 if n_seq == 1 else parts == 0)  # (of many rows each has one workgroup: no words)
+            assert parts == int(parts) and (parts == 0 or 2 <= parts <= 64)  # (where each row has one workgroup there are no words)
 
 
 def test_stages_that_are_refused():

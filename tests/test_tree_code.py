@@ -1,0 +1,51 @@
+"""CPU: the code that the compiler makes of the kernels of a cycle with trees. Nothing may be done to vector registers before the lanes that a branch has switched off come back
+(test_exec_restore.py says why); and the builds of attention that load straight into LDS wait for all their loads right before the meetings behind which LDS is read."""
+import importlib.util
+import os
+import re
+import shutil
+import subprocess
+
+import pytest
+
+import wo
+from test_exec_restore import before_the_lanes_come_back, blocks
+
+
+def listing(tmp_path, source):
+    spec = importlib.util.spec_from_file_location("ws_build", os.path.join(wo.ROOT, "whirl-llm_amd", "build.py"))
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+    if not shutil.which(hipcc):
+        pytest.skip("no hipcc")
+    out = tmp_path / "code.s"
+    subprocess.run([hipcc, *build.FLAGS, "-S", "--cuda-device-only", "-o", str(out), getattr(build, source)], check=True, capture_output=True)
+    return out.read_text()
+
+
+@pytest.mark.parametrize("source,kernels,number", [("SRC_TREE", r"tree_(stage|rows|draw)_kernel", 1 + 4 + 12), ("SRC_ATTEND", r"attend_(join_)?kernel", 2 * 14),
+                                                   ("SRC_CACHE", r"cache_(reserve|fork|copy|release|keep)_kernel", 5)])
+def test_nothing_vector_stands_before_the_lanes_come_back(tmp_path, source, kernels, number):
+    seen, staged = set(), 0
+    text = listing(tmp_path, source)
+    for kernel, block in blocks(text):
+        seen.add(kernel)
+        before = before_the_lanes_come_back(block)
+        assert not before, (kernel, before)
+    assert len([k for k in seen if k and re.search(kernels, k)]) == number
+    if source != "SRC_ATTEND":
+        return
+    for name, body in re.findall(r"^(_Z\w*attend_kernel\w*):(.*?)^\.Lfunc_end", text, re.S | re.M):
+        if "global_load_lds" not in body:
+            continue
+        staged += 1
+        ops = [line.split(";")[0].strip() for line in body.splitlines()]
+        last = max(i for i, op in enumerate(ops) if op.startswith("global_load_lds"))
+        waits = [i for i, op in enumerate(ops) if re.match(r"s_waitcnt vmcnt\(0\)", op)]
+        meetings = [i for i, op in enumerate(ops) if op.startswith("s_barrier")]
+        assert any(b > last for b in meetings), name
+        first = min(i for i, op in enumerate(ops) if op.startswith("global_load_lds"))
+        heads = [b for b in meetings if b > first and any(b - 8 < w < b for w in waits)]  # each half of the loop over two buffers begins with one
+        assert len(heads) >= 2, name
+    assert staged == 9
