@@ -1330,7 +1330,7 @@ struct VerifyPlan {
 };
 VerifyPlan verify_plan(const ws_loss_rows* r, uint32_t n_seq) {
     VerifyPlan p{};
-    const uint32_t per = r->dtype == WS_DTYPE_F32 ? 4u : 8u, vectors = (r->vocab + per - 1u) / per, least = (vectors + ws::tree_most_share() - 1u) / ws::tree_most_share();
+    const uint32_t per = r->dtype == WS_DTYPE_F32 ? 4u : 8u, vectors = (r->vocab + per - 1u) / per, least = (vectors + ws::tree_most_share(r->dtype) - 1u) / ws::tree_most_share(r->dtype);
     uint32_t parts = n_seq ? 2u * static_cast<uint32_t>(compute_units()) / n_seq : 1u;
     if (parts > vectors / 256u) parts = vectors / 256u;
     if (parts < least) parts = least;

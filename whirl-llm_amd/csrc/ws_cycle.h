@@ -54,7 +54,7 @@ constexpr uint32_t kTreeWords = 4u;
 
 int launch_tree_stage(hipStream_t stream, const TreeStageArgs& a);
 int launch_tree_verify(hipStream_t stream, int dtype, const TreeVerifyArgs& a);
-uint32_t tree_most_share();
+uint32_t tree_most_share(int dtype);
 int prepare_tree();
 
 // ---- ws_attend.hip

@@ -385,9 +385,10 @@ __global__ void __launch_bounds__(kRowThreads, 3) tree_rows_kernel(TreeVerifyArg
 }
 
 // ---- the walk, and the token behind it
-template <int DT, bool MASK, int T, int NV, int WAVES>
-__global__ void __launch_bounds__(T, WAVES) tree_draw_kernel(TreeVerifyArgs A) {
-    constexpr uint32_t kPer = Elem<DT>::kPer, kW = T / 64u;
+constexpr uint32_t kDrawThreads = 256u;
+template <int DT, bool MASK, int NV, int WAVES>
+__global__ void __launch_bounds__(kDrawThreads, WAVES) tree_draw_kernel(TreeVerifyArgs A) {
+    constexpr uint32_t T = kDrawThreads, kPer = Elem<DT>::kPer, kW = T / 64u;
     __shared__ float red_m[kW];
     __shared__ double red_t[kW];
     __shared__ float part_m[64];

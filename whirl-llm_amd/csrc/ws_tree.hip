@@ -5,20 +5,23 @@
 namespace ws {
 
 namespace {
-// vectors of a workgroup's share, by its build (the longest rows are 262144 vectors, of 64 parts at most)
-constexpr uint32_t kSmall = 4u * 256u, kMost = 12u * 256u, kWide = 9u * 512u;
-static_assert((1048575u / Elem<0>::kPer + 63u) / 64u + 8u <= kWide);
+// Vectors of a thread of the middle build: as many as leave three workgroups a compute unit (two of bf16, whose vectors have twice the powers). 256 rows of 50257 fp32, masked: 12 (five workgroups a
+// row) 46 us, 17 (three, which all run at once) 41.
+template <int DT>
+constexpr uint32_t kMiddle = DT == 0 ? 17u : 12u;
+// (the longest rows, in 64 parts, fit it)
+static_assert((1048575u / Elem<0>::kPer + 63u) / 64u + 8u <= kMiddle<0> * kDrawThreads && (1048575u / Elem<1>::kPer + 63u) / 64u + 8u <= kMiddle<1> * kDrawThreads);
+constexpr uint32_t kSmall = 4u;
 
-template <int DT, bool MASK, int T, int NV, int WAVES>
-void verify(hipStream_t s, const TreeVerifyArgs& a) {
-    hipLaunchKernelGGL((tree_draw_kernel<DT, MASK, T, NV, WAVES>), grid_of(a.parts, a.n_seq), dim3(T), 0, s, a);
+template <int DT, bool MASK, int NV, int WAVES>
+void draw(hipStream_t s, const TreeVerifyArgs& a) {
+    hipLaunchKernelGGL((tree_draw_kernel<DT, MASK, NV, WAVES>), grid_of(a.parts, a.n_seq), dim3(kDrawThreads), 0, s, a);
 }
 template <int DT, bool MASK>
 void of_size(hipStream_t s, const TreeVerifyArgs& a) {
     hipLaunchKernelGGL((tree_rows_kernel<DT, MASK>), grid_of(a.row_parts, a.levels * a.n_seq), dim3(kRowThreads), 0, s, a);
-    if (a.per <= kSmall) verify<DT, MASK, 256, 4, 4>(s, a);
-    else if (a.per <= kMost) verify<DT, MASK, 256, 12, 2>(s, a);
-    else verify<DT, MASK, 512, 9, 2>(s, a);
+    if (a.per <= kSmall * kDrawThreads) draw<DT, MASK, kSmall, 4>(s, a);
+    else draw<DT, MASK, kMiddle<DT>, DT == 0 ? 3 : 2>(s, a);
 }
 }  // namespace
 
@@ -27,7 +30,7 @@ int prepare_tree() {
     return static_cast<int>(hipFuncGetAttributes(&fa, reinterpret_cast<const void*>(&tree_stage_kernel)));
 }
 
-uint32_t tree_most_share() { return kMost; }
+uint32_t tree_most_share(int dtype) { return kDrawThreads * (dtype == 0 ? kMiddle<0> : kMiddle<1>); }
 
 int launch_tree_stage(hipStream_t stream, const TreeStageArgs& a) {
     hipLaunchKernelGGL(tree_stage_kernel, dim3(a.n_seq), dim3(64), 0, stream, a);
