@@ -154,6 +154,29 @@ def test_keep(dtype, page, kv_heads, dim, layers, layout):
     assert torch.equal(dk.cpu(), k)
 
 
+@pytest.mark.parametrize("strides", [((1 << 27) + 512, (1 << 29) + 1024, 64, 32), (1 << 13, 1 << 14, 1 << 29, 32)])
+def test_caches_beyond_32_bits(strides):
+    """Layers, pages or tokens further apart than 32 bits count: a fork's copy, an accepted path."""
+    m = gc.pkg()
+    layers, pages, page, kv_heads, dim = shape = (2, 5, 4, 2, 32)
+    sides = []
+    for _ in range(2):
+        room = torch.empty(sum((size - 1) * by for size, by in zip(shape, (*strides, 1))) + 1, dtype=F32, device=DEV)
+        sides.append(room.as_strided(shape, (*strides, 1)))
+        assert room.numel() * 4 > 1 << 32
+    e = m.PagedCache.empty(*shape, 2, 4, dtype=F32, device=DEV)
+    c = m.PagedCache(*sides, e.table, e.held, e.refs, e.free, e.n_free)
+    numbered(c)
+    want = [t.contiguous() for t in sides]
+    assert c.reserve(i32([0]), i32([11])).tolist() == [0] and c.table[0].tolist() == [0, 1, 2, -1]
+    assert c.fork(i32([0]), i32([1]), i32([10])).tolist() == [0] and c.table[1].tolist() == [0, 1, 3, -1]
+    c.keep(i32([[2, 3]]), i32([2]), i32([6]))  # slot 0: token 8 to 7, 9 to 8
+    for t, w in zip(sides, want):
+        w[:, 3, :2] = w[:, 2, :2].clone()
+        w[:, 1, 3], w[:, 2, 0] = w[:, 2, 0].clone(), w[:, 2, 1].clone()
+        assert torch.equal(t, w)
+
+
 def test_captured_and_replayed():
     """Fork, room for drafts and release in a graph, replayed with eager calls in between: the lists go through the same calls."""
     m = gc.pkg()

@@ -143,6 +143,15 @@ def test_verify(counts, kids, V, dtype, kind):
     assert sum(len(w.path) for w in walks) > 0 or sum(counts) < 100
 
 
+@pytest.mark.parametrize("V", [1, 2, 3, 5, 8])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_verify_of_the_smallest_vocabularies(V, dtype):
+    m = gc.pkg()
+    for seed, masked in ((1, False), (2, True)):
+        call, walks, ids, _ = verify_case([1, 4, 9, 2], 2, V, dtype, 10 * V + seed, guessed=None, masked=masked, stride=1)
+        check_walks(m.verify_tree(depth=8, **call), walks, 8, V)
+
+
 def test_verify_chains_and_few_columns():
     """No parents: chains. Fewer columns than accepted nodes: the first of them."""
     m = gc.pkg()
@@ -484,6 +493,20 @@ def test_attention_scores_far_apart():
             k = host["k"].clone()
             k[used] = flat.view(39, 16, 2, 64)
             check_attention({**call, "k": k.to(DEV)}, {**host, "k": k}, scale=0.5)
+
+
+@pytest.mark.parametrize("dtype,dim,n,strides", [(BF16, 128, 1, ((1 << 31) + 64, 256, 128)), (BF16, 128, 40, ((1 << 31) + 64, 256, 128)), (F32, 64, 9, (128, 1 << 28, 64)), (BF16, 64, 20, (128, 1 << 28, 64))])
+def test_attention_of_a_cache_beyond_32_bits(dtype, dim, n, strides):
+    """Pages, or a page's tokens, further apart than 32 bits count."""
+    call, host = attend_case([n, n], [30, 3], 8, 2, dim, 16, dtype, n + dim, spare=1)
+    far = {}
+    for side in ("k", "v"):
+        shape = call[side].shape
+        room = torch.empty(sum((size - 1) * by for size, by in zip(shape, strides)) + dim, dtype=dtype, device=DEV)
+        far[side] = room.as_strided(shape, (*strides, 1))
+        far[side].copy_(call[side])
+        assert far[side].numel() * far[side].element_size() < 1 << 24 < 1 << 32 < room.numel() * room.element_size()
+    check_attention({**call, **far}, host)
 
 
 def test_attention_captured_and_replayed():
