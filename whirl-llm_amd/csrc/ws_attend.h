@@ -8,7 +8,7 @@
 // hold what is larger than one as exactly): else no maximum is looked for. A wave works on 32 positions at a time. Few columns (WM = 1): the four waves of a workgroup take different positions, K and V go from memory
 // into the registers of their operands. Many (WM = 4): the waves take different columns of the same positions, K and V go through LDS, the next ones' on their way in registers meanwhile.
 //
-// Work: units of kUnit positions of a sequence, a kv head and a tile of columns, numbered through; the workgroups share them evenly, whatever the sequences' lengths, each a run of neighbours.
+// Work: units of kUnit positions of a sequence, a kv head and a tile of columns; the workgroups share them evenly, whatever the sequences' lengths, each a run of neighbours (AttendSpan).
 // A run that does not hold all units of a tile leaves maximum, sum and O^T in the workspace, and attend_join_kernel joins them. Memory bounds it where there are few columns,
 // from some hundred on the matrix cores and the powers.
 #pragma once
@@ -162,19 +162,38 @@ struct AttendFind {
     uint32_t seq;
     AttendWork work;
 };
-// The units of all sequences, and in `find` the sequence that holds unit first(all): a sequence a thread, 256 at a time.
-template <class Fn>
-__device__ __forceinline__ uint64_t attend_find(const AttendArgs& A, uint32_t cols, uint32_t unit, AttendFind& F, Fn&& first) {
+// What a workgroup works on. All units in a row, sequences behind one another, a head's tiles behind one another, in runs of `per`, that do not end at sequences; or, in gangs: where sequences have
+// several tiles, these read the same K and V, so that as many runs as a sequence has tiles, `apart` in number, take the same positions, each of its own tile, at the same time and on one part of
+// the chip: what one has read the others find in its cache (2 x 64 nodes, 512 columns, over 131072: without, K and V came from memory 3.5 times). Then runs end at sequences, which leaves
+// some a little shorter than others: taken where sequences are few.
+struct AttendSpan {
+    uint64_t per, begin, end;  // units; from the first of all, or of the sequence's
+    uint32_t tile, apart;      // of a gang: the run's tile
+    bool gang;
+};
+// A sequence a thread, 256 at a time. False: there is nothing for this run.
+template <bool GANGS>
+__device__ __forceinline__ bool attend_find(const AttendArgs& A, uint32_t cols, uint32_t unit, uint32_t run, AttendFind& F, AttendSpan& S) {
     const uint32_t t = threadIdx.x;
-    uint64_t mine = 0, before = 0, all = 0;
+    uint64_t mine = 0, tiles = 0, all = 0, all_tiles = 0;
     AttendWork w{};
     for (uint32_t s = t; s < A.n_seq; s += kAttendThreads) {
         w = attend_work(A, s, cols, unit);
         mine += w.all;
+        tiles += w.tiles;
     }
-    before = scan256(mine, F.red, all);
-    const uint64_t at = first(all);
-    if (at >= all) return all;
+    uint64_t before = scan256(mine, F.red, all);
+    if (GANGS) scan256(tiles, F.red, all_tiles);
+    S.gang = GANGS && all_tiles > A.n_seq && all_tiles <= A.groups / 8u;  // (so that there are fewer sequences than threads)
+    const uint64_t runs = A.groups - (S.gang ? all_tiles : 0u);
+    S.per = max((all + runs - 1u) / runs, static_cast<uint64_t>(A.least));
+    uint64_t at = S.per * run;
+    if (S.gang) {  // each sequence has as many runs as it needs: all_tiles more than an even split at most
+        mine = w.tiles * ((static_cast<uint64_t>(A.kv_heads) * w.units + S.per - 1u) / S.per);
+        before = scan256(mine, F.red, all);
+        at = run;
+    }
+    if (at >= all) return false;  // (uniform)
     uint64_t base = 0;
     for (uint32_t s0 = 0; s0 < A.n_seq; s0 += kAttendThreads) {
         if (A.n_seq > kAttendThreads) {  // (the sums above were of several)
@@ -193,7 +212,19 @@ __device__ __forceinline__ uint64_t attend_find(const AttendArgs& A, uint32_t co
         if (at < base) break;  // (uniform)
     }
     __syncthreads();
-    return all;
+    S.tile = 0u;
+    S.apart = 1u;
+    if (S.gang) {
+        const uint32_t in_seq = static_cast<uint32_t>(run - F.seq_first);
+        S.apart = F.work.tiles;
+        S.tile = in_seq % S.apart;
+        S.begin = in_seq / S.apart * S.per;
+        S.end = min(S.begin + S.per, static_cast<uint64_t>(A.kv_heads) * F.work.units);
+    } else {
+        S.begin = at;
+        S.end = min(at + S.per, all);
+    }
+    return true;
 }
 
 // What the products leave out: infinities and NaN in the V of nodes, which must not reach the rows that do not see them (0 times NaN is NaN). Rare, so it is done where a column is
@@ -265,30 +296,26 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
 
     // (neighbouring runs on the same part of the chip: workgroup b runs on XCD b % 8)
     const uint32_t in_xcd = A.groups / 8u, run_id = blockIdx.x < in_xcd * 8u ? (blockIdx.x & 7u) * in_xcd + (blockIdx.x >> 3) : blockIdx.x;
-    uint64_t per = 0, begin = 0;
-    const uint64_t all = attend_find(A, H::kTileCols, H::kUnit, F, [&](uint64_t units) {
-        per = max((units + A.groups - 1u) / A.groups, static_cast<uint64_t>(A.least));
-        return begin = per * run_id;
-    });
+    AttendSpan S;
+    const bool any = attend_find<kStaged>(A, H::kTileCols, H::kUnit, run_id, F, S);
     uint32_t run_odd = 0u;  // (the first thread's)
     if (t == 0u) A.run[run_id].more = 0u;
     if (t == 0u) s_odd = 0u;
-    if (begin >= all) return;
-    const uint64_t end = min(begin + per, all);
+    if (!any) return;
     uint32_t s = F.seq;
     uint64_t seq_first = F.seq_first;
     AttendWork W = F.work;
 
-    for (uint64_t at = begin; at < end;) {
-        while (at - seq_first >= W.all) {
+    for (uint64_t at = S.begin; at < S.end;) {
+        while (!S.gang && at - seq_first >= W.all) {
             seq_first += W.all;
-            ++s;  // (there is one: at < all)
+            ++s;  // (there is one: at < S.end)
             W = attend_work(A, s, H::kTileCols, H::kUnit);
         }
-        const uint64_t in_seq = at - seq_first;
+        const uint64_t in_seq = S.gang ? at : at - seq_first;
         const uint32_t item = static_cast<uint32_t>(in_seq / W.units), u0 = static_cast<uint32_t>(in_seq - static_cast<uint64_t>(item) * W.units);
-        const uint32_t u1 = static_cast<uint32_t>(min(static_cast<uint64_t>(W.units), u0 + (end - at)));
-        const uint32_t head = item / W.tiles, tile = item - head * W.tiles;
+        const uint32_t u1 = static_cast<uint32_t>(min(static_cast<uint64_t>(W.units), u0 + (S.end - at)));
+        const uint32_t head = S.gang ? item : item / W.tiles, tile = S.gang ? S.tile : item - head * W.tiles;
         const uint32_t cols = W.nodes * A.group, col0 = tile * H::kTileCols + wm * (16u * MS);
         const uint32_t slot = A.slot ? A.slot[s] : s;
         const int32_t* table = A.table + static_cast<uint64_t>(slot) * A.table_stride;
@@ -673,7 +700,8 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
             r.seq = s;
             r.head = head;
             r.tile = tile;
-            r.more = static_cast<uint32_t>(last / per - first / per);
+            r.more = static_cast<uint32_t>(last / S.per - first / S.per);
+            r.apart = S.apart;
             r.odd = 0u;
             r.first = W.first, r.nodes = W.nodes, r.length = W.length, r.total = W.total;
             A.run[run_id] = r;
@@ -699,14 +727,14 @@ __global__ void __launch_bounds__(64 * kJoinWaves) attend_join_kernel(AttendArgs
     if (R.more == 0u) return;
     const uint32_t cols = R.nodes * A.group, col = R.tile * H::kTileCols + sub * 16u + c;
     if (col - c >= cols) return;
-    auto piece = [&](uint32_t i) { return A.part + ((static_cast<uint64_t>(x) + i) * 2u + (i == 0u ? 1u : 0u)) * H::kPartFloats + sub * H::kSubFloats; };
+    auto piece = [&](uint32_t i) { return A.part + ((static_cast<uint64_t>(x) + static_cast<uint64_t>(i) * R.apart) * 2u + (i == 0u ? 1u : 0u)) * H::kPartFloats + sub * H::kSubFloats; };
     float top = -FLT_MAX, sum = 0.f;
     f32x4 o[kOuts];
 #pragma unroll
     for (uint32_t r = 0; r < kOuts; ++r) o[r] = f32x4{0.f, 0.f, 0.f, 0.f};
     // (by those that have the nodes: three pieces at most, of 32 positions at least)
     bool odd = R.more < 3u && (R.odd & 2u) != 0u;
-    for (uint32_t i = R.more > 2u ? R.more - 2u : 1u; i <= R.more; ++i) odd = odd || (A.run[x + i].odd & 1u) != 0u;
+    for (uint32_t i = R.more > 2u ? R.more - 2u : 1u; i <= R.more; ++i) odd = odd || (A.run[x + i * R.apart].odd & 1u) != 0u;
     float their_top = -FLT_MAX, their_sum = 0.f;
     f32x4 theirs[kOuts];
     auto load = [&](uint32_t i) __attribute__((always_inline)) {

@@ -82,9 +82,9 @@ struct AttendArgs {
     float* part;       // [groups][2][kPartFloats of the build]
     struct AttendRun* run;  // [groups]
 };
-// what the join needs of a workgroup: the tile that begins in its run and does not end there (`more` workgroups behind it hold the rest)
+// what the join needs of a workgroup: the tile that begins in its run and does not end there (`more` runs behind it, `apart` in number, hold the rest)
 struct AttendRun {
-    uint32_t seq, head, tile, more;
+    uint32_t seq, head, tile, more, apart;
     uint32_t first, nodes, length, total;  // of the sequence, as in AttendWork
     uint32_t odd;  // bits: whether its first part (of a tile that began before), its last (of the one that begins) has met nodes whose V holds infinities or NaN
 };
