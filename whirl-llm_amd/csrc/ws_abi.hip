@@ -1515,7 +1515,6 @@ int ws_tree_attention(void* stream, const ws_tree_attention_args* a, void* works
     g.mask = a->mask;
     g.scale_log2 = static_cast<float>(static_cast<double>(a->scale) * 1.4426950408889634074);
     g.groups = plan.groups;
-    g.least = plan.least;
     g.part = static_cast<float*>(workspace);
     g.run = reinterpret_cast<ws::AttendRun*>(static_cast<unsigned char*>(workspace) + plan.part_bytes);
     return ws::launch_attend(S(stream), plan, g);

@@ -6,11 +6,16 @@
 //
 // One pass: a column keeps its maximum, sum and O^T; powers are of base two, and a column is scaled down only when a lane's eight powers against the maximum so far make more than kMost (32 bits
 // hold what is larger than one as exactly): else no maximum is looked for. A wave works on 32 positions at a time. Few columns (WM = 1): the four waves of a workgroup take different positions, K and V go from memory
-// into the registers of their operands. Many (WM = 4): the waves take different columns of the same positions, K and V go through LDS, the next ones' on their way in registers meanwhile.
+// into the registers of their operands. Many (WM = 4): the waves take different columns of the same positions; K and V go from memory straight into LDS, the next ones' while these are worked on, and
+// bf16's V is turned by the instruction that reads it from there.
 //
 // Work: units of kUnit positions of a sequence, a kv head and a tile of columns; the workgroups share them evenly, whatever the sequences' lengths, each a run of neighbours (AttendSpan).
-// A run that does not hold all units of a tile leaves maximum, sum and O^T in the workspace, and attend_join_kernel joins them. Memory bounds it where there are few columns,
-// from some hundred on the matrix cores and the powers.
+// A run that does not hold all units of a tile leaves maximum, sum and O^T in the workspace, and attend_join_kernel joins them.
+//
+// What bounds it. Few columns: memory (64 rows over 4096 positions at most, 32 heads, 8 of K and V, 128 bf16: 575 MB in 120 us, 4.8 TB/s). Many (2 x 64 nodes over 131072, 32 heads, 4 of K and V: 206 GFLOP in 343 us,
+// 600 TFLOP/s; a matrix product of 8192^3 reaches 1207): matrix cores 35 % and vector units 38 % busy, and the clock, which the card lowers from 2.15 to 1.8 GHz in launches one behind the
+// other (300 us where it does not). Tried there and not faster: 8 waves and 256 columns a workgroup (360 us of then 357); three buffers instead of two (385); K of the next 32 positions read
+// while these are added up (356 to 383); 64 columns a wave (680).
 #pragma once
 
 #include "ws_common.h"
@@ -99,8 +104,9 @@ struct AttendShape {
     static constexpr uint32_t kChunks = DP / Mat<DT>::kDepth;
     static constexpr uint32_t kSubFloats = 64u * (4u * kOuts + 2u);    // of 16 columns in the workspace: maximum and sum, O^T, as the lanes hold them
     static constexpr uint32_t kPartFloats = MS * WM * kSubFloats;
-    // through LDS: tokens at a time, bytes of one, its 16-byte pieces, those of a thread
-    static constexpr uint32_t kRow = DP * Mat<DT>::kBytes, kTokens = kRow <= 256u ? 64u : 32u, kPieces = kRow / 16u, kMine = kTokens * kPieces / 256u;
+    // through LDS: bytes of a token, tokens at a time (32 where 64 would take the registers that two tiles of columns need: 128 columns of 128 bf16 151 us instead of 163), a token's 16-byte
+    // pieces, those of a thread
+    static constexpr uint32_t kRow = DP * Mat<DT>::kBytes, kTokens = kRow * MS <= 256u ? 64u : 32u, kPieces = kRow / 16u, kMine = kTokens * kPieces / 256u;
     static constexpr uint32_t kBuffer = kTokens * kRow;
     // positions that work is counted in: what a workgroup's waves take together
     static constexpr uint32_t kUnit = WM > 1 ? kTokens : 128u;
@@ -186,7 +192,7 @@ __device__ __forceinline__ bool attend_find(const AttendArgs& A, uint32_t cols, 
     if (GANGS) scan256(tiles, F.red, all_tiles);
     S.gang = GANGS && all_tiles > A.n_seq && all_tiles <= A.groups / 8u;  // (so that there are fewer sequences than threads)
     const uint64_t runs = A.groups - (S.gang ? all_tiles : 0u);
-    S.per = max((all + runs - 1u) / runs, static_cast<uint64_t>(A.least));
+    S.per = max((all + runs - 1u) / runs, uint64_t{1});  // (two units at least: one row over 4096 positions 15.4 us instead of 11.5, four 20.6; the join 5.4 and 5.0 instead of 6.8)
     uint64_t at = S.per * run;
     if (S.gang) {  // each sequence has as many runs as it needs: all_tiles more than an even split at most
         mine = w.tiles * ((static_cast<uint64_t>(A.kv_heads) * w.units + S.per - 1u) / S.per);

@@ -44,7 +44,7 @@ struct TreeVerifyArgs {
     uint32_t levels, look, row_parts, row_per;
     unsigned long long* row_meet;  // row_parts > 1: [rows][4][row_parts]
     unsigned long long* decided;   // [rows][2]
-    // of the draw: workgroups a sequence, vectors each (at most T * NV), how often one looks for the others
+    // of the draw: workgroups a sequence, vectors each (at most kDrawThreads * NV), how often one looks for the others
     uint32_t parts, per, looks;
     unsigned long long* meet;  // parts > 1: [n_seq][kTreeWords][parts]
     unsigned long long tag;
@@ -78,7 +78,7 @@ struct AttendArgs {
     const uint32_t* slot;
     const uint64_t* mask;
     float scale_log2;  // scale times log2(e)
-    uint32_t groups, least;  // workgroups; the fewest units of one
+    uint32_t groups;
     float* part;       // [groups][2][kPartFloats of the build]
     struct AttendRun* run;  // [groups]
 };
@@ -90,7 +90,7 @@ struct AttendRun {
 };
 
 struct AttendPlan {
-    uint32_t build, groups, least;
+    uint32_t build, groups;
     uint64_t part_bytes, bytes;
 };
 AttendPlan attend_plan(int dtype, uint32_t head_dim, uint32_t cols, uint32_t compute_units);
