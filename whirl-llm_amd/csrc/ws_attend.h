@@ -12,10 +12,10 @@
 // Work: units of kUnit positions of a sequence, a kv head and a tile of columns; the workgroups share them evenly, whatever the sequences' lengths, each a run of neighbours (AttendSpan).
 // A run that does not hold all units of a tile leaves maximum, sum and O^T in the workspace, and attend_join_kernel joins them.
 //
-// What bounds it. Few columns: memory (64 rows over 4096 positions at most, 32 heads, 8 of K and V, 128 bf16: 575 MB in 120 us, 4.8 TB/s). Many (2 x 64 nodes over 131072, 32 heads, 4 of K and V: 206 GFLOP in 343 us,
-// 600 TFLOP/s; a matrix product of 8192^3 reaches 1207): matrix cores 35 % and vector units 38 % busy, and the clock, which the card lowers from 2.15 to 1.8 GHz in launches one behind the
-// other (300 us where it does not). Tried there and not faster: 8 waves and 256 columns a workgroup (360 us of then 357); three buffers instead of two (385); K of the next 32 positions read
-// while these are added up (356 to 383); 64 columns a wave (680).
+// What bounds it. Few columns: memory (64 rows over 4096 positions at most, 32 heads, 8 of K and V, 128 bf16: 575 MB in 120 us, 4.8 TB/s). Many (2 x 64 nodes over 131072, 32 heads, 4 of K and V: 206 GFLOP in 270 to 332 us,
+// 620 to 760 TFLOP/s; a matrix product of 8192^3 reaches 1207): matrix cores 34 % and vector units 44 % busy, each wave waiting for its own products, LDS and barriers in turn, and the clock, which the card
+// lowers from 2.15 to 1.8 GHz in launches one behind the other. Tried there and not faster: 8 waves and 256 columns a workgroup (360 us of then 357); three buffers instead of two (385); K of
+// the next 32 positions read while these are added up (356 to 383); 64 columns a wave (680).
 #pragma once
 
 #include "ws_common.h"
