@@ -5,12 +5,12 @@
 // what is carried along is c and the P and Q of those ids, a lane each, and the mass outside of them, 1 - sum P at first. No pass over the row is made for a rejection.
 //
 // Which child a node passes the walk on to, if any, does not depend on how the walk came to it. So tree_rows_kernel decides all nodes with children at once, one pass over a row, its workgroups meeting
-// without waiting; nodes are numbered level by level as far as the grid can, and one whose parent has decided against it by then is not read. (A kernel that walked, row after row, waited for memory
+// without waiting for each other; nodes are numbered level by level as far as the grid can, and one whose parent has decided against it by then is not read. (A kernel that walked, row after row, waited for memory
 // and for its parts at each: 64 trees of 16 nodes 83 us, 256 of 25 237 us, five rows 40 us.) tree_draw_kernel then goes down the tree along what was decided and draws from the row where
 // that ends, which its workgroups hold in registers.
-// What bounds them is latency (the same three: 35 + 27, 101 + 42, 9 + 12 us): trips to memory one after the other - offsets, decisions, the row, the q entry and its ids' logits, the parts' words -, and workgroups that
+// What bounds them is latency (the same three: 32 + 27, 95 + 42, 9 + 12 us): trips to memory one after the other - offsets, decisions, the row, the q entry and its ids' logits, the parts' words -, and workgroups that
 // only find that their node is not needed, 2 ns each; vector units are 40 to 50 % busy, memory is read at 2 to 3 TB/s. (Every workgroup of a sequence going where the walk may come to next, reading
-// as it goes, instead of one a node: 37 and 131 us for 35 and 101.)
+// as it goes, instead of one a node: 37 and 131 us for then 35 and 101.)
 //
 // Accuracy. The comparisons u Q < P are made in 64 bits, S is added up from powers of 32 bits (1e-8 of S where many tokens count): of ten million drafts one may be judged otherwise than by an
 // exact sum. The token behind the walk is looked for among some 100 000 steps of a cumulative sum, whose places would move by 1e-8 of the sum, a hundredth of a step where tokens are
@@ -258,11 +258,12 @@ __device__ __forceinline__ bool tree_drafts(const TreeVerifyArgs& A, int32_t off
 
 // ---- what each node decides: the child that it passes the walk on to (with the log-probability of that one's token), or none; or that the walk does not come to it, or that its q entry is none
 constexpr uint32_t kDecNone = 64u, kDecNever = 65u, kDecBad = 66u;
-constexpr uint32_t kRowThreads = 256u;
+constexpr uint32_t kRowThreads = 256u, kParentLooks = 64u;  // (a look: a microsecond)
 __device__ __forceinline__ unsigned long long* tree_decision(const TreeVerifyArgs& A, uint32_t row) { return A.decided + 2u * static_cast<size_t>(row); }
 
+// (Three workgroups a unit with a mask, whose loads take registers: four spill, 101 us for 125. Without, four: 35 us for 32.)
 template <int DT, bool MASK>
-__global__ void __launch_bounds__(kRowThreads, 3) tree_rows_kernel(TreeVerifyArgs A) {
+__global__ void __launch_bounds__(kRowThreads, MASK ? 3 : 4) tree_rows_kernel(TreeVerifyArgs A) {
     constexpr uint32_t T = kRowThreads, kPer = Elem<DT>::kPer, kU = 4u;  // vectors of a thread on their way together
     __shared__ float red_m[T / 64];
     __shared__ double red_s[T / 64], red_t[T / 64];
@@ -292,9 +293,18 @@ __global__ void __launch_bounds__(kRowThreads, 3) tree_rows_kernel(TreeVerifyArg
         if (A.look) {
             if (!needed()) continue;
             if (node > 0u) {
+                // A parent's first child is read before that one has decided, as it will mostly be needed; another waits, bounded. (All waiting 41 and 123 us instead of 32 and 95, none 35 and 101.)
+                const uint32_t up = lane_value(static_cast<uint32_t>(L.above), node);
+                const uint64_t siblings = __ballot(L.above == static_cast<int32_t>(up)) & ((uint64_t{1} << node) - 1ull);
+                const uint32_t looks = siblings == 0ull ? 1u : min(A.looks, kParentLooks);
                 if (t == 0u) {
-                    unsigned long long v;
-                    s_never = find_word(tree_decision(A, first + lane_value(static_cast<uint32_t>(L.above), node)), 1u, tag, v) && static_cast<uint32_t>(v & 0xffu) != node ? 1u : 0u;
+                    unsigned long long v = 0;
+                    bool known = false;
+                    for (uint32_t look = 0; look < looks && !known; ++look) {
+                        if (look != 0u) __builtin_amdgcn_s_sleep(8);
+                        known = find_word(tree_decision(A, first + up), 1u, tag, v);
+                    }
+                    s_never = known && static_cast<uint32_t>(v & 0xffu) != node ? 1u : 0u;
                     if (s_never) leave_word(tree_decision(A, row), 1u, kDecNever, tag);
                 }
                 __syncthreads();
