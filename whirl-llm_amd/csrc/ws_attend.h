@@ -690,6 +690,7 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
                 float* part = A.part + (static_cast<uint64_t>(run_id) * 2u + (u0 == 0u ? 1u : 0u)) * H::kPartFloats + wm * MS * H::kSubFloats;
 #pragma unroll
                 for (int m = 0; m < MS; ++m) {
+                    if (col0 + m * 16u >= cols) continue;  // (a wave's)
                     float* to = part + m * H::kSubFloats;
                     to[lane] = top[m];
                     to[64u + lane] = sum[m];
