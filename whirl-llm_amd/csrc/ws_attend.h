@@ -721,12 +721,14 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
 }
 
 // A workgroup joins 16 columns of the tile that begins in run x: the tile's first piece is that run's second part, the others are the first parts of the runs behind it. A wave takes every eighth
-// piece, the next while it adds one, and what the waves have is joined through LDS, in an order that does not depend on who comes first.
-constexpr uint32_t kJoinWaves = 8u;
+// (fourth, of the builds with many columns) piece, the next while it adds one, and what the waves have is joined through LDS, in an order that does not depend on who comes first.
+// Tiles of many columns lie in few runs, and there are as many workgroups as tiles have 16 columns: 8, 4, 2 waves take 20, 13, 12 us for 16 x 48 over 8192, 14, 12.6, 19 for 2 x 64 over 131072; one row over 4096 7, 8, 12.
+template <int WM>
+constexpr uint32_t kJoinWavesOf = WM > 1 ? 4u : 8u;
 template <int DT, int DP, int MS, int WM>
-__global__ void __launch_bounds__(64 * kJoinWaves) attend_join_kernel(AttendArgs A) {
+__global__ void __launch_bounds__(64 * kJoinWavesOf<WM>) attend_join_kernel(AttendArgs A) {
     typedef AttendShape<DT, DP, MS, WM> H;
-    constexpr uint32_t kOuts = H::kOuts, kEach = H::kEach;
+    constexpr uint32_t kOuts = H::kOuts, kEach = H::kEach, kJoinWaves = kJoinWavesOf<WM>;
     __shared__ f32x4 s_o[kJoinWaves / 2u][kOuts][64];
     __shared__ float s_top[kJoinWaves / 2u][64], s_sum[kJoinWaves / 2u][64];
     const uint32_t x = blockIdx.x, sub = blockIdx.y, t = threadIdx.x, lane = t & 63u, wave = t >> 6, c = lane & 15u, g = lane >> 4;

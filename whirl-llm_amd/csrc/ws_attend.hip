@@ -16,7 +16,7 @@ struct Build {
 template <int DT, int DP, int MS, int WM, int OCC>
 void launch(hipStream_t s, const AttendArgs& a) {
     hipLaunchKernelGGL((attend_kernel<DT, DP, MS, WM, OCC>), dim3(a.groups), dim3(kAttendThreads), 0, s, a);
-    hipLaunchKernelGGL((attend_join_kernel<DT, DP, MS, WM>), dim3(a.groups, MS * WM), dim3(64 * kJoinWaves), 0, s, a);
+    hipLaunchKernelGGL((attend_join_kernel<DT, DP, MS, WM>), dim3(a.groups, MS * WM), dim3(64 * kJoinWavesOf<WM>), 0, s, a);
 }
 template <int DT, int DP, int MS, int WM, int OCC>
 constexpr Build build(uint32_t cols) {
