@@ -875,29 +875,34 @@ def tree_attention(q, k, v, table, length, seq_off, mask=None, slot=None, scale=
     lie behind them in the cache; seq_off: as in tree_stage; mask: int64 [rows] (None: chains); slot: int32 [n_seq] (None: sequence s has slot s); scale: None = head_dim ** -0.5. One row a sequence: plain
     decoding. max_nodes: the most nodes of a sequence, where the caller knows it. out: where to write (strides in multiples of 16 bytes); rows behind the last sequence are left as they are.
     Returns out, or (out, lse float32 [rows, heads]) with want_lse."""
-    at = _device_of("q", q)
-    if q.dim() != 3 or q.dtype not in _LOSS_DTYPES or (q.stride(2) != 1 and q.shape[2] > 1):
+    at, dtype = _device_of("q", q), q.dtype
+    if q.dim() != 3 or dtype not in _LOSS_DTYPES:
         raise WsError("q: [rows, heads, head_dim] float32 / bfloat16 device tensor, unit inner stride")
-    rows, heads, dim = q.shape
+    (rows, heads, dim), (q_row, q_head, inner) = q.shape, q.stride()
+    if inner != 1 and dim > 1:
+        raise WsError("q: [rows, heads, head_dim] float32 / bfloat16 device tensor, unit inner stride")
     n_seq = _sequences(seq_off)
     ks, vs = _pages_of("k", k, 4), _pages_of("v", v, 4)
-    if k.shape != v.shape or k.dtype is not q.dtype or v.dtype is not q.dtype or k.get_device() != at or v.get_device() != at or k.shape[3] != dim:
+    shape = k.shape
+    if shape != v.shape or k.dtype is not dtype or v.dtype is not dtype or k.get_device() != at or v.get_device() != at or shape[3] != dim:
         raise WsError("k, v: of one shape, of q's dtype and head_dim, on its device")
-    pages, page_tokens, kv_heads, _ = k.shape
+    pages, page_tokens, kv_heads, _ = shape
     slots, wide, table_stride = _cache_table(table, at)
-    if max(rows, n_seq, heads, pages, page_tokens, kv_heads, slots, wide) >= 1 << 31 or not 0 <= max_nodes < 1 << 31:
+    if (rows | heads | pages | page_tokens | kv_heads | slots | wide) >> 31 or not 0 <= max_nodes < 1 << 31:
         raise WsError("sizes beyond 31 bits")
     if slot is None and n_seq > slots:
         raise WsError(f"slot: missing, and {n_seq} sequences have {slots} slots")
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)  # (rows behind the last sequence: whatever the memory held)
-    elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != at or (out.stride(2) != 1 and dim > 1):
+        out = torch.empty_like(q) if q_row == heads * dim and q.is_contiguous() else q.new_empty((rows, heads, dim))  # (rows behind the last sequence: whatever the memory held)
+        out_row, out_head = heads * dim, dim
+    elif out.shape != q.shape or out.dtype is not dtype or out.get_device() != at or (out.stride(2) != 1 and dim > 1):
         raise WsError("out: of q's shape and dtype, on its device, unit inner stride")
     else:
         torch.autograd.graph.increment_version(out)
-    lse = torch.empty((rows, heads), dtype=_F32, device=q.device) if want_lse else None
-    a = TreeAttention(CacheLayer(k.data_ptr(), v.data_ptr(), _LOSS_DTYPES[q.dtype], pages, page_tokens, kv_heads, dim, *ks, *vs, table.data_ptr(), slots, wide, table_stride),
-                      n_seq, rows, heads, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), _p(lse), _vector("seq_off", seq_off, _I32, n_seq + 1, at),
+        out_row, out_head, _ = out.stride()
+    lse = q.new_empty((rows, heads), dtype=_F32) if want_lse else None
+    a = TreeAttention(CacheLayer(k.data_ptr(), v.data_ptr(), _LOSS_DTYPES[dtype], pages, page_tokens, kv_heads, dim, *ks, *vs, table.data_ptr(), slots, wide, table_stride),
+                      n_seq, rows, heads, q.data_ptr(), q_row, q_head, out.data_ptr(), out_row, out_head, _p(lse), _vector("seq_off", seq_off, _I32, n_seq + 1, at),
                       _vector("length", length, _I32, n_seq, at), _vector("slot", slot, _I32, n_seq, at), _vector("mask", mask, _I64, rows, at), dim ** -0.5 if scale is None else scale, max_nodes)
     call, ref = lib(), C.byref(a)
     need = call.ws_tree_attention_workspace(ref)
