@@ -1322,8 +1322,8 @@ static_assert(WS_TREE_MAX == ws::kTreeNodes && WS_Q_MAX == ws::kTreeListed && WS
 static_assert(WS_CACHE_MOST == ws::kCacheMost && WS_CACHE_MOST == WS_BLOCK);
 
 // The verification's workgroups. A sequence's draw: two a compute unit where sequences are few, of 256 vectors at least; as many as hold the row in registers. A row's decision: shares of
-// 2048 vectors at least, larger ones where there are many rows, so that fewer workgroups begin at the ends of trips to memory. Parts, us: 64 trees of 16 x 151936 bf16 62: 109, 12: 33.7, 6: 31.4, 3: 34.1, 1: 47.3;
-// 256 of 25 x 50257 fp32, masked, 42: 777, 8: 202, 4: 114, 2: 97, 1: 110; five rows of 151936 bf16 62: 15.6, 12: 9.7, 6: 9.7, 3: 11.8, 1: 20.4. Words: the draw's, the decisions, the rows' sums.
+// 2048 vectors at least, larger ones where there are many rows, so that fewer workgroups begin at the ends of trips to memory. Parts, us: 64 trees of 16 x 151936 bf16 62: 109, 9: 32.0, 7: 29.1, 4: 29.3, 1: 47;
+// 256 of 25 x 50257 fp32, masked, 42: 777, 5: 133, 3: 105, 2: 95.7, 1: 95.4; five rows of 151936 bf16 62: 15.6, 12: 9.7, 9: 9.0, 6: 9.4, 3: 11.8, 1: 20.4. Words: the draw's, the decisions, the rows' sums.
 struct VerifyPlan {
     uint32_t parts, row_parts, levels;
     uint64_t meet, decided, bytes;
@@ -1336,7 +1336,7 @@ VerifyPlan verify_plan(const ws_loss_rows* r, uint32_t n_seq) {
     if (parts < least) parts = least;
     p.parts = parts < 1u ? 1u : (parts > 64u ? 64u : parts);
     const uint32_t most = row_vectors(r) / 2048u, rows = r->rows ? r->rows : 1u;
-    p.row_parts = (32u * static_cast<uint32_t>(compute_units()) + rows / 2u) / rows;
+    p.row_parts = (20u * static_cast<uint32_t>(compute_units()) + rows / 2u) / rows;
     if (p.row_parts > most) p.row_parts = most;
     p.row_parts = p.row_parts < 1u ? 1u : (p.row_parts > 64u ? 64u : p.row_parts);
     p.levels = n_seq ? (r->rows + n_seq - 1u) / n_seq : 1u;  // (as many nodes as a sequence has on average; a larger one's take turns)
