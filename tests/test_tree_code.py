@@ -24,7 +24,7 @@ def listing(tmp_path, source):
     return out.read_text()
 
 
-@pytest.mark.parametrize("source,kernels,number", [("SRC_TREE", r"tree_(stage|rows|draw)_kernel", 1 + 4 + 8), ("SRC_ATTEND", r"attend_(join_)?kernel", 2 * 13),
+@pytest.mark.parametrize("source,kernels,number", [("SRC_TREE", r"tree_(stage|rows|draw)_kernel", 1 + 4 + 8), ("SRC_ATTEND", r"attend_(join_)?kernel", 2 * 12),
                                                    ("SRC_CACHE", r"cache_(reserve|fork|copy|release|keep)_kernel", 5)])
 def test_nothing_vector_stands_before_the_lanes_come_back(tmp_path, source, kernels, number):
     seen, staged = set(), 0
