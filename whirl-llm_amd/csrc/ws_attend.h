@@ -98,7 +98,7 @@ template <int DT, int DP, int MS, int WM>
 struct AttendShape {
     static constexpr uint32_t kTileCols = 16u * MS * WM;
     static constexpr bool kTurned = DT == 1 && WM > 1;  // V is turned by its reads from LDS: a lane asks for 4 elements of a token and gets 4 tokens' of an element
-    static constexpr uint32_t kEach = kTurned ? 1u : (DT == 1 && DP >= 128 ? 8u : 4u);  // elements of V a lane loads together: a lane holds elements kEach c + e of a block of 16 kEach
+    static constexpr uint32_t kEach = kTurned ? 1u : 16u / Mat<DT>::kBytes;  // elements of V a lane loads together: a lane holds elements kEach c + e of a block of 16 kEach
     static constexpr uint32_t kBlocks = DP / (16u * kEach);
     static constexpr uint32_t kOuts = kBlocks * kEach;                 // products' results that make up O^T of 16 columns, 4 floats a lane each
     static constexpr uint32_t kChunks = DP / Mat<DT>::kDepth;
@@ -385,7 +385,6 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
                 }
             }
         };
-        // (8 bf16 or 4 fp32: one load of 16 bytes; 4 bf16: one of 8)
         auto load_v = [&](uint32_t p0, uint32_t pg) __attribute__((always_inline)) {
 #pragma unroll
             for (uint32_t i = 0; i < 8u; ++i) {
@@ -393,13 +392,7 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
 #pragma unroll
                 for (uint32_t b = 0; b < kBlocks; ++b) {
                     const uint32_t d = b * 16u * kEach + c * kEach;
-                    const unsigned char* from = at_v + (d < A.head_dim ? d : 0u) * E;
-                    if constexpr (kEach * E == 16u) {
-                        vx[i][b] = *reinterpret_cast<const uint4*>(from);
-                    } else {
-                        const uint2 two = *reinterpret_cast<const uint2*>(from);
-                        vx[i][b] = make_uint4(two.x, two.y, 0u, 0u);
-                    }
+                    vx[i][b] = *reinterpret_cast<const uint4*>(at_v + (d < A.head_dim ? d : 0u) * E);
                 }
             }
         };
@@ -597,15 +590,9 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
                         for (uint32_t r = 0; r < kOuts; ++r)
 #pragma unroll
                             for (int m = 0; m < MS; ++m) o[m][r] = Mat<1>::mul(make_uint4(v[r][0].x, v[r][0].y, v[r][1].x, v[r][1].y), px[m][0], o[m][r]);
-                    } else add_up([&](uint32_t i, uint32_t b) {
-                        const uint32_t token = v_pos(sub, i);
-                        if constexpr (kEach * E == 16u) {
-                            return *reinterpret_cast<const uint4*>(v_lds + H::place(token, b * 16u + c));
-                        } else {
-                            const uint2 two = *reinterpret_cast<const uint2*>(v_lds + H::place(token, b * 8u + c / 2u) + (c & 1u) * 8u);
-                            return make_uint4(two.x, two.y, 0u, 0u);
-                        }
-                    });
+                    } else {
+                        add_up([&](uint32_t i, uint32_t b) { return *reinterpret_cast<const uint4*>(v_lds + H::place(v_pos(sub, i), b * 16u + c)); });
+                    }
                 }
             };
             for (; p < p_end; p += H::kTokens) {  // (the same for the workgroup)
