@@ -12,8 +12,8 @@
 // Work: units of kUnit positions of a sequence, a kv head and a tile of columns; the workgroups share them evenly, whatever the sequences' lengths, each a run of neighbours (AttendSpan).
 // A run that does not hold all units of a tile leaves maximum, sum and O^T in the workspace, and attend_join_kernel joins them.
 //
-// What bounds it. Few columns: memory (64 rows over 4096 positions at most, 32 heads, 8 of K and V, 128 bf16: 575 MB in 120 us, 4.8 TB/s). Many (2 x 64 nodes over 131072, 32 heads, 4 of K and V: 206 GFLOP in 270 to 332 us,
-// 620 to 760 TFLOP/s; a matrix product of 8192^3 reaches 1207): matrix cores 34 % and vector units 44 % busy, each wave waiting for its own products, LDS and barriers in turn, and the clock, which the card
+// What bounds it. Few columns: memory (64 rows over 4096 positions at most, 32 heads, 8 of K and V, 128 bf16: 575 MB in 120 us, 4.8 TB/s). Many (2 x 64 nodes over 131072, 32 heads, 4 of K and V: 206 GFLOP in 270 to 346 us,
+// 600 to 760 TFLOP/s; a matrix product of 8192^3 reaches 1207): matrix cores 34 % and vector units 44 % busy, each wave waiting for its own products, LDS and barriers in turn, and the clock, which the card
 // lowers from 2.15 to 1.8 GHz in launches one behind the other. Tried there and not faster: 8 waves and 256 columns a workgroup (360 us of then 357); three buffers instead of two (385); K of
 // the next 32 positions read while these are added up (356 to 383); 64 columns a wave (680).
 #pragma once
@@ -709,7 +709,7 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
 
 // A workgroup joins 16 columns of the tile that begins in run x: the tile's first piece is that run's second part, the others are the first parts of the runs behind it. A wave takes every eighth
 // (fourth, of the builds with many columns) piece, the next while it adds one, and what the waves have is joined through LDS, in an order that does not depend on who comes first.
-// Tiles of many columns lie in few runs, and there are as many workgroups as tiles have 16 columns: 8, 4, 2 waves take 20, 13, 12 us for 16 x 48 over 8192, 14, 12.6, 19 for 2 x 64 over 131072; one row over 4096 7, 8, 12.
+// Tiles of many columns lie in few runs, and there are as many workgroups as tiles have 16 columns: 8, 4, 2 waves take 20, 13, 12 us for 16 x 48 over 8192, 14, 12.6, 19 for 2 x 64 over 131072; one row over 4096 7, 8, 12 (16 waves: 7.9).
 template <int WM>
 constexpr uint32_t kJoinWavesOf = WM > 1 ? 4u : 8u;
 template <int DT, int DP, int MS, int WM>

@@ -8,7 +8,7 @@
 // without waiting for each other; nodes are numbered level by level as far as the grid can, and one whose parent has decided against it by then is not read. (A kernel that walked, row after row, waited for memory
 // and for its parts at each: 64 trees of 16 nodes 83 us, 256 of 25 237 us, five rows 40 us.) tree_draw_kernel then goes down the tree along what was decided and draws from the row where
 // that ends, which its workgroups hold in registers.
-// What bounds them is latency (the same three: 32 + 27, 95 + 42, 9 + 12 us): trips to memory one after the other - offsets, decisions, the row, the q entry and its ids' logits, the parts' words -, and workgroups that
+// What bounds them is latency (the same three: 29 + 27, 95 + 41, 8 + 12 us): trips to memory one after the other - offsets, decisions, the row, the q entry and its ids' logits, the parts' words -, and workgroups that
 // only find that their node is not needed, 2 ns each; vector units are 40 to 50 % busy, memory is read at 2 to 3 TB/s. (Every workgroup of a sequence going where the walk may come to next, reading
 // as it goes, instead of one a node: 37 and 131 us for then 35 and 101.)
 //
