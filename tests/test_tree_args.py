@@ -27,7 +27,7 @@ def attention_of(m, cache=None, **change):
     layer = dict(k=AT, v=AT, dtype=1, pages=10, page_tokens=16, kv_heads=2, head_dim=64, k_page=2048, k_token=128, k_head=64, v_page=2048, v_token=128, v_head=64, table=AT, slots=3, slot_pages=4,
                  table_stride=4)
     layer.update(cache or {})
-    a = m.TreeAttention(cache=m.CacheLayer(**layer), n_seq=2, rows=4, heads=8, q=AT, q_row=512, q_head=64, out=AT, out_row=512, out_head=64, lse=AT, seq_off=AT, length=AT, mask=AT, scale=0.125)
+    a = m.TreeAttention(cache=m.CacheLayer(**layer), n_seq=2, rows=4, heads=8, q=AT, q_row=512, q_head=64, out=2 * AT, out_row=512, out_head=64, lse=AT, seq_off=AT, length=AT, mask=AT, scale=0.125)
     for k, v in change.items():
         setattr(a, k, v)
     return a
@@ -85,7 +85,7 @@ def test_stages_that_are_refused():
 
 @pytest.mark.parametrize("change", [dict(q=None), dict(out=None), dict(seq_off=None), dict(length=None), dict(heads=0), dict(heads=7), dict(heads=65536), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
                                     dict(scale=float("inf")), dict(q_row=511), dict(q_head=63), dict(q=AT + 8), dict(out_row=4), dict(out=AT + 2), dict(mask=AT + 4), dict(n_seq=1 << 20), dict(rows=1 << 20),
-                                    dict(q_row=1 << 63)])
+                                    dict(q_row=1 << 63), dict(q=AT, out=AT)])
 def test_attention_that_is_refused(change):
     m = gc.pkg()
     assert m.lib().ws_tree_attention(None, C.byref(attention_of(m, **change)), AT, 1 << 40) == m.E_INVALID

@@ -1476,7 +1476,7 @@ int ws_tree_attention(void* stream, const ws_tree_attention_args* a, void* works
     if (a->n_seq == 0 || a->rows == 0) return WS_OK;
     const ws_cache_layer& c = a->cache;
     const uint32_t e = static_cast<uint32_t>(elem_bytes(c.dtype));
-    if (!a->q || !a->out || !a->seq_off || !a->length || !c.k || !c.v || !c.table || (a->mask && !aligned(a->mask, 8u))) return WS_E_INVALID;
+    if (!a->q || !a->out || a->out == a->q || !a->seq_off || !a->length || !c.k || !c.v || !c.table || (a->mask && !aligned(a->mask, 8u))) return WS_E_INVALID;
     if (!strides_ok(a->q, e, {{a->rows, a->q_row}, {a->heads, a->q_head}}) || !strides_ok(a->out, e, {{a->rows, a->out_row}, {a->heads, a->out_head}})) return WS_E_INVALID;
     if (!strides_ok(c.k, e, {{c.pages, c.k_page}, {c.page_tokens, c.k_token}, {c.kv_heads, c.k_head}}) ||
         !strides_ok(c.v, e, {{c.pages, c.v_page}, {c.page_tokens, c.v_token}, {c.kv_heads, c.v_head}}))
