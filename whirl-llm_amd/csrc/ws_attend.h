@@ -710,6 +710,7 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
 // A workgroup joins 16 columns of the tile that begins in run x: the tile's first piece is that run's second part, the others are the first parts of the runs behind it. A wave takes every eighth
 // (fourth, of the builds with many columns) piece, the next while it adds one, and what the waves have is joined through LDS, in an order that does not depend on who comes first.
 // Tiles of many columns lie in few runs, and there are as many workgroups as tiles have 16 columns: 8, 4, 2 waves take 20, 13, 12 us for 16 x 48 over 8192, 14, 12.6, 19 for 2 x 64 over 131072; one row over 4096 7, 8, 12 (16 waves: 7.9).
+// (Four pieces of a wave on their way instead of two: registers that leave fewer workgroups to find that they have nothing to do, 13 to 17 and 6.2 to 8.8 us for 64 rows.)
 template <int WM>
 constexpr uint32_t kJoinWavesOf = WM > 1 ? 4u : 8u;
 template <int DT, int DP, int MS, int WM>
@@ -728,9 +729,6 @@ __global__ void __launch_bounds__(64 * kJoinWavesOf<WM>) attend_join_kernel(Atte
     f32x4 o[kOuts];
 #pragma unroll
     for (uint32_t r = 0; r < kOuts; ++r) o[r] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // (by those that have the nodes: three pieces at most, of 32 positions at least)
-    bool odd = R.more < 3u && (R.odd & 2u) != 0u;
-    for (uint32_t i = R.more > 2u ? R.more - 2u : 1u; i <= R.more; ++i) odd = odd || (A.run[x + i * R.apart].odd & 1u) != 0u;
     float their_top = -FLT_MAX, their_sum = 0.f;
     f32x4 theirs[kOuts];
     auto load = [&](uint32_t i) __attribute__((always_inline)) {
@@ -748,6 +746,9 @@ __global__ void __launch_bounds__(64 * kJoinWavesOf<WM>) attend_join_kernel(Atte
         for (uint32_t r = 0; r < kOuts; ++r) o[r] = o[r] * a + theirs[r] * z;
     };
     if (wave <= R.more) load(wave);
+    // whether any of those that have the nodes - three pieces at most, of 32 positions at least - has met such (the same entry again where there are fewer)
+    const uint32_t last = x + R.more * R.apart;
+    const uint32_t odd = ((A.run[last].odd | A.run[last - (R.more > 1u ? R.apart : 0u)].odd | A.run[last - (R.more > 2u ? 2u * R.apart : 0u)].odd) & 1u) | (R.more < 3u ? R.odd & 2u : 0u);
     for (uint32_t i = wave; i <= R.more; i += kJoinWaves) {
         join();
         if (i + kJoinWaves <= R.more) load(i + kJoinWaves);
@@ -772,7 +773,7 @@ __global__ void __launch_bounds__(64 * kJoinWavesOf<WM>) attend_join_kernel(Atte
     }
     if (wave != 0u || col >= cols) return;
     const uint32_t node = col / A.group, h = R.head * A.group + (col - node * A.group);
-    if (odd) {
+    if (odd != 0u) {
         const int32_t* table = A.table + static_cast<uint64_t>(A.slot ? A.slot[R.seq] : R.seq) * A.table_stride;
         const uint64_t sees = A.mask ? A.mask[R.first + node] : (node < 63u ? (uint64_t{2} << node) - 1u : ~uint64_t{0});
 #pragma unroll 1
