@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(kRowThreads, MASK ? 3 : 4) tree_rows_kernel(Tr
                 // A parent's first child is read before that one has decided, as it will mostly be needed; another waits, bounded. (All waiting 41 and 123 us instead of 32 and 95, none 35 and 101.)
                 const uint32_t up = lane_value(static_cast<uint32_t>(L.above), node);
                 const uint64_t siblings = __ballot(L.above == static_cast<int32_t>(up)) & ((uint64_t{1} << node) - 1ull);
-                const uint32_t looks = siblings == 0ull ? 1u : min(A.looks, kParentLooks);
+                const uint32_t looks = siblings == 0ull || up % A.levels > level ? 1u : min(A.looks, kParentLooks);  // (a parent of workgroups that come later may not even have begun)
                 if (t == 0u) {
                     unsigned long long v = 0;
                     bool known = false;
