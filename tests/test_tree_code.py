@@ -10,6 +10,8 @@ import pytest
 
 import wo
 from test_exec_restore import before_the_lanes_come_back, blocks
+from test_lds_budget import READELF
+from test_meeting_order import LIB, code_objects
 
 
 def listing(tmp_path, source):
@@ -49,3 +51,19 @@ def test_nothing_vector_stands_before_the_lanes_come_back(tmp_path, source, kern
         heads = [b for b in meetings if b > first and any(b - 8 < w < b for w in waits)]  # each half of the loop over two buffers begins with one
         assert len(heads) >= 2, name
     assert staged == 9
+
+
+def test_verification_kernels_keep_their_registers(tmp_path):
+    if not os.path.exists(READELF):
+        pytest.skip("no llvm-readelf")
+    found = 0
+    for i, blob in enumerate(code_objects(LIB)):
+        path = tmp_path / f"{i}.elf"
+        path.write_bytes(blob)
+        notes = subprocess.run([READELF, "--notes", str(path)], capture_output=True, text=True, check=True).stdout
+        for block in re.split(r"(?=\.agpr_count)", notes):
+            name = re.search(r"\.name: +(\S+)", block)
+            if name and re.search(r"tree_(stage|rows|draw)_kernel", name.group(1)):
+                found += 1
+                assert re.search(r"\.vgpr_spill_count: 0\b", block) and re.search(r"\.private_segment_fixed_size: 0\b", block), name.group(1)
+    assert found == 1 + 4 + 8

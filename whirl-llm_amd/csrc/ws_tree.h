@@ -63,10 +63,10 @@ __global__ void __launch_bounds__(64) tree_stage_kernel(TreeStageArgs A) {
 }
 
 // 2^z for z <= 0 to 1e-11: z = k + f, |f| <= 1/2, and of 2^f = e^(f ln 2) the first ten terms of its series (the next is 0.35^10 / 10! = 7e-12). What lies below 2^-2885, -inf too, is 0. Not
-// for NaN, which is told apart where it is looked for.
+// for NaN, which is told apart where it is looked for. (k by a sum whose last bit is worth one: of rounding and conversion an instruction takes several times as long.)
 __device__ __forceinline__ double power64(double z) {
     z = fmax(z, -2885.0);
-    const double k = rint(z), f = z - k;
+    const double k = z + 0x1.8p52, f = z - (k - 0x1.8p52);
     double p = 0x1.b5253d395e7c4p-24;
     p = fma(p, f, 0x1.62c0223a5c824p-20);
     p = fma(p, f, 0x1.ffcbfc588b0c7p-17);
@@ -77,7 +77,7 @@ __device__ __forceinline__ double power64(double z) {
     p = fma(p, f, 0x1.ebfbdff82c58fp-3);
     p = fma(p, f, 0x1.62e42fefa39efp-1);
     p = fma(p, f, 0x1.0000000000000p+0);
-    return ldexp(p, static_cast<int>(k));
+    return ldexp(p, __double2loint(k));
 }
 // exponents of base two: a row's factor
 __device__ __forceinline__ double tree_factor(float inv_t) { return static_cast<double>(inv_t) * 1.4426950408889634074; }
@@ -486,11 +486,13 @@ __global__ void __launch_bounds__(kDrawThreads, WAVES) tree_draw_kernel(TreeVeri
         auto weights = [&](uint32_t u_, double (&w)[kPer]) {
             float x[kPer];
             unpack<DT>(share.q[u_], x);
+            const double share_at = static_cast<double>(share_m) * factor;
             const uint32_t out = reinterpret_cast<const unsigned char*>(taken_out)[wave_id() * 64u * share.rounds + u_ * 64u + lane];
 #pragma unroll
             for (uint32_t e = 0; e < kPer; ++e) {  // (those as if they were not there: a branch around each power would have one wait for the other)
                 const float mine = out >> e & 1u ? -INFINITY : x[e];
-                w[e] = power64((static_cast<double>(mine) - static_cast<double>(share_m)) * factor);
+                w[e] = power64(fma(static_cast<double>(mine), factor, -share_at));
+                if (e % 4u == 3u) __builtin_amdgcn_sched_barrier(0);  // (more of them together take the registers that the row is in)
             }
         };
         auto outside_sum = [&]() {
