@@ -315,6 +315,42 @@ def test_verify_replayed_where_others_use_the_workspace(begin):
             assert int(want[3].sum()) == (0 if i != 1 else 3)
 
 
+@pytest.mark.parametrize("counts,V,dtype", [([7, 16, 3], 60000, BF16), ([1, 5], 151936, F32), ([2] * 3, 1048575, F32)])
+def test_verify_leaves_no_words_for_its_replays(counts, V, dtype):
+    """The replays of a captured call have one tag: no word of a launch, of a row's maximum or of its sum, may be whole where the next replay looks for it. The rows' words and the decisions are
+    taken apart by the launch that left them, the draw's by the next one (here one whose sequences are empty, so that its draw leaves a maximum's word alone)."""
+    m = gc.pkg()
+    n_seq, rows = len(counts), sum(counts)
+    call = verify_case(counts, 2, V, dtype, 300 + rows, guessed=True)[0]
+    r = m._loss_rows(call["logits"], call["ids"], call["inv_t"], None)[0]
+    small = torch.zeros(3 * n_seq + 15 * n_seq, dtype=torch.int32, device=DEV)
+    at = small.data_ptr()
+    a = m.VerifyTree(n_seq, call["seq_off"].data_ptr(), call["parent"].data_ptr(), None, 0, None, call["u_accept"].data_ptr(), call["u_draw"].data_ptr(), 15, at, at + 12 * n_seq, at + 4 * n_seq, at + 8 * n_seq)
+    need = m.lib().ws_verify_tree_workspace(r, a)
+    r.rows = 0
+    draw = m.lib().ws_verify_tree_workspace(r, a)
+    r.rows = rows
+    parts, row_parts = draw // (32 * n_seq), (need - draw - 16 * rows) // (32 * rows)
+    assert parts > 1 and row_parts > 1 and need == 32 * n_seq * parts + 16 * rows + 32 * rows * row_parts
+    work = torch.full((need // 8,), -1, dtype=torch.int64, device=DEV)
+    run = lambda: m.check(m.lib().ws_verify_tree(torch.cuda.current_stream().cuda_stream, r, a, work.data_ptr(), need), "ws_verify_tree")  # noqa: E731
+    run()
+    left = work.cpu()
+    of_draw, decided, of_rows = left[:draw // 8].view(n_seq, 4, parts), left[draw // 8:draw // 8 + 2 * rows], left[draw // 8 + 2 * rows:].view(rows, 4, row_parts)
+    assert not small[2 * n_seq:3 * n_seq].any() and (of_draw != -1).all()
+    assert not decided.any()
+    read = [sum(counts[:s]) + i for s in range(n_seq) for i in range(counts[s])]
+    assert ((of_rows[read] == 0) | (of_rows[read] == -1)).all()  # (-1: rows of nodes without children)
+    assert (of_rows[[sum(counts[:s]) for s in range(n_seq) if counts[s] > 1]] == 0).all()
+    call["seq_off"].zero_()
+    run()
+    left = work.cpu()[:draw // 8].view(n_seq, 4, parts)
+    assert (small[2 * n_seq:3 * n_seq] == 1).all()
+    tag = left[:, 0] ^ left[:, 1]
+    assert (tag == tag[0, 0]).all() and int(tag[0, 0]) != 0  # (the words that say only that one is there)
+    assert not left[:, 2:].any()
+
+
 # ---- attention
 
 

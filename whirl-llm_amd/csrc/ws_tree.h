@@ -254,7 +254,8 @@ __device__ __forceinline__ bool tree_drafts(const TreeVerifyArgs& A, int32_t off
 }
 
 // The words of a launch (ws_loss.h) have a tag that no other launch has, but the replays of a captured one: so no launch leaves its words behind where its next replay looks for them. The draw's
-// are taken apart by the next rows' kernel, when no draw runs; the rows' and the decisions by the draw's workgroups, when all of a sequence's have read them.
+// are taken apart by the next rows' kernel, when no draw runs; the rows' and the decisions by the draw's workgroups, when all of a sequence's have read them. All of them, a part's maximum and its
+// sum: who looks between the two may find the one from now and the other, were it still whole, from the replay before.
 
 // ---- what each node decides: the child that it passes the walk on to (with the log-probability of that one's token), or none; or that the walk does not come to it, or that its q entry is none
 constexpr uint32_t kDecNone = 64u, kDecNever = 65u, kDecBad = 66u;
@@ -272,7 +273,10 @@ __global__ void __launch_bounds__(kRowThreads, MASK ? 3 : 4) tree_rows_kernel(Tr
     const uint32_t y = grid_row(), level = y / A.n_seq, s = y - level * A.n_seq, part = blockIdx.x, t = threadIdx.x, V = A.R.vocab;
     const unsigned long long tag = A.tag;
     if (level >= A.levels) return;
-    if (level == 0u && part == 0u && A.parts > 1u && t < A.parts) break_word(A.meet + static_cast<size_t>(s) * A.parts * kTreeWords + t, A.parts);
+    if (level == 0u && part == 0u && A.parts > 1u && t < 2u * A.parts) {  // (128 at most) a part's maximum, a part's sum
+        const uint32_t word = t < A.parts ? 0u : 1u;
+        break_word(A.meet + (static_cast<size_t>(s) * kTreeWords + 2u * word) * A.parts + (t - word * A.parts), A.parts);
+    }
     uint32_t n;
     const uint32_t first = tree_rows(A.seq_off, s, A.R.rows, n);
     if (level >= n) return;
@@ -757,12 +761,12 @@ __global__ void __launch_bounds__(kDrawThreads, WAVES) tree_draw_kernel(TreeVeri
             if (t == 0u && A.depth == 64u) to[64] = 0.f;  // (63 drafts at most are accepted: the chosen one's is in the 64th place)
         }
     }
-    if (all_read) {  // the rows' words are taken apart, a pair of each (by all of a sequence's workgroups: five rows 11 -> 14.5 us)
+    if (all_read) {  // the rows' words are taken apart (by all of a sequence's workgroups: five rows 11 -> 14.5 us)
         for (uint32_t i = t; i < n; i += T) break_word(tree_decision(A, first + i), 1u);
         if (A.row_parts > 1u) {
-            for (uint32_t i = t; i < n * A.row_parts; i += T) {
-                const uint32_t r = i / A.row_parts;
-                break_word(A.row_meet + static_cast<size_t>(first + r) * A.row_parts * 4u + (i - r * A.row_parts), A.row_parts);
+            for (uint32_t i = t; i < 2u * n * A.row_parts; i += T) {  // a row's maxima, its sums, the next row's
+                const uint32_t w = i / A.row_parts;
+                break_word(A.row_meet + (static_cast<size_t>(first) * 2u + w) * A.row_parts * 2u + (i - w * A.row_parts), A.row_parts);
             }
         }
     }
