@@ -580,3 +580,21 @@ def test_attention_on_two_streams_at_once():
                 got.append(m.tree_attention(**c))
     torch.cuda.synchronize()
     assert all(torch.equal(g, want[i % 2]) for i, g in enumerate(got))
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (BF16, 256), (F32, 64), (BF16, 64), (F32, 128)])
+def test_attention_infinities_of_some_of_a_workgroups_tiles(dtype, dim):
+    """A workgroup works on several sequences' tiles, one behind the other: infinities in the V of some of the sequences' nodes are those sequences' alone, and none is lost."""
+    m = gc.pkg()
+    n = 2000
+    call, host = attend_case([1] * n, [i % 61 for i in range(n)], 4, 2, dim, 16, dtype, dim)
+    clean = m.tree_attention(**call)
+    t, want = host["v"].clone(), clean.clone()
+    for s in range(0, n, 3):
+        p = host["lengths"][s]
+        t[host["table"][s, p // 16], p % 16, s % 2, 5] = math.inf
+        want[s, 2 * (s % 2):2 * (s % 2) + 2, 5] = math.inf
+    call["v"] = t.to(DEV)
+    for _ in range(3):
+        got = m.tree_attention(**call)
+        assert torch.equal(got, want), int((got != want).sum())

@@ -67,3 +67,63 @@ def test_verification_kernels_keep_their_registers(tmp_path):
                 found += 1
                 assert re.search(r"\.vgpr_spill_count: 0\b", block) and re.search(r"\.private_segment_fixed_size: 0\b", block), name.group(1)
     assert found == 1 + 4 + 8
+
+
+def flow(function):
+    """{block: (instructions, the blocks behind)} of a function in the compiler's intermediate form."""
+    out, name = {}, "entry"
+    for line in function.splitlines()[1:]:
+        label = re.match(r"^(\d+):", line)
+        if label:
+            name = label.group(1)
+        ops, behind = out.setdefault(name, ([], []))
+        op = line.strip()
+        if line.startswith("  "):
+            ops.append(op)
+            if op.startswith("br ") or op.startswith("switch ") or op.startswith("]") or re.match(r"i\d+ \S+, label", op):
+                behind.extend(re.findall(r"label %(\d+)", op))
+    return out
+
+
+def reached_without_meeting(blocks_, first, second):
+    """Whether an instruction of `second` can come behind one of `first` with no meeting of the workgroup between them."""
+    seen, left = set(), [(name, i + 1) for name, (ops, _) in blocks_.items() for i, op in enumerate(ops) if first(op)]
+    assert left
+    while left:
+        name, i = left.pop()
+        ops, behind = blocks_[name]
+        for op in ops[i:]:
+            if "@llvm.amdgcn.s.barrier()" in op:
+                break
+            if second(op):
+                return True
+        else:
+            for to in behind:
+                if to not in seen:
+                    seen.add(to)
+                    left.append((to, 0))
+    return False
+
+
+def test_attention_clears_a_flag_before_a_meeting(tmp_path):
+    """A workgroup's flag for infinities and NaN in the V of nodes (s_odd): between the store that clears it and one of another wave that sets it the waves meet, on every way through the kernel. Else
+    a wave that is late would clear what another one has found."""
+    spec = importlib.util.spec_from_file_location("ws_build", os.path.join(wo.ROOT, "whirl-llm_amd", "build.py"))
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+    if not shutil.which(hipcc):
+        pytest.skip("no hipcc")
+    out = tmp_path / "code.ll"
+    subprocess.run([hipcc, *build.FLAGS, "-S", "-emit-llvm", "--cuda-device-only", "-o", str(out), build.SRC_ATTEND], check=True, capture_output=True)
+    found = 0
+    for function in re.findall(r"^define [^\n]*attend_kernel.*?^}", out.read_text(), re.S | re.M):
+        flag = r"@\w*s_odd\b"
+        places = re.findall(rf"(%\d+) = getelementptr [^\n]*{flag}", function)
+        at = rf"(?:{flag}|{'|'.join(re.escape(p) for p in places)})" if places else flag
+        clears, sets = re.compile(rf"store i32 0, ptr addrspace\(3\) {at}(?:,|$)"), re.compile(rf"store i32 1, ptr addrspace\(3\) {at}(?:,|$)")
+        blocks_ = flow(function)
+        assert sum(bool(sets.match(op)) for ops, _ in blocks_.values() for op in ops) >= 1
+        assert not reached_without_meeting(blocks_, clears.match, sets.match), function[:120]
+        found += 1
+    assert found == 12

@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
     constexpr bool kStaged = WM > 1;
     static_assert(WM == 1 || WM == 4);
     __shared__ AttendFind F;
-    __shared__ uint32_t s_odd;
+    __shared__ uint32_t s_odd[2];  // a tile's and the next one's, in turn: cleared where a meeting lies between that and who sets it, and between that and who has read it
     __shared__ float s_part[kWT > 1u ? (kWT / 2u) * MS * (kDump + 128u) : 1u];
     // two buffers of K, then V. (Two variables: of one that is indexed the compiler has every read wait for what is on its way to the other half.)
     __shared__ uint4 s_even[kStaged ? 2u * H::kBuffer / 16u : 1u], s_odds[kStaged ? 2u * H::kBuffer / 16u : 1u];
@@ -303,15 +303,16 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
     // (neighbouring runs on the same part of the chip: workgroup b runs on XCD b % 8)
     const uint32_t in_xcd = A.groups / 8u, run_id = blockIdx.x < in_xcd * 8u ? (blockIdx.x & 7u) * in_xcd + (blockIdx.x >> 3) : blockIdx.x;
     AttendSpan S;
+    if (t < 2u) s_odd[t] = 0u;  // (attend_find's waves meet)
     const bool any = attend_find<kStaged>(A, H::kTileCols, H::kUnit, run_id, F, S);
     uint32_t run_odd = 0u;  // (the first thread's)
     if (t == 0u) A.run[run_id].more = 0u;
-    if (t == 0u) s_odd = 0u;
     if (!any) return;
     uint32_t s = F.seq;
     uint64_t seq_first = F.seq_first;
     AttendWork W = F.work;
 
+    uint32_t turn_odd = 0u;
     for (uint64_t at = S.begin; at < S.end;) {
         while (!S.gang && at - seq_first >= W.all) {
             seq_first += W.all;
@@ -602,7 +603,7 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
                 chunk(odds, even);
             }
         }
-        if (__ballot(odd != 0u) != 0ull && lane == 0u) s_odd = 1u;
+        if (__ballot(odd != 0u) != 0ull && lane == 0u) s_odd[turn_odd] = 1u;
         // a column's sum over its four lanes
 #pragma unroll
         for (int m = 0; m < MS; ++m) {
@@ -642,7 +643,9 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
             }
         }
         __syncthreads();
-        const bool any_odd = s_odd != 0u;
+        const bool any_odd = s_odd[turn_odd] != 0u;
+        turn_odd ^= 1u;
+        if (t == 0u) s_odd[turn_odd] = 0u;
         if (wt == 0u) {
             if (u0 == 0u && u1 == W.units) {
                 if (any_odd) {  // (uniform)
@@ -702,7 +705,6 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
         }
         at += u1 - u0;
         __syncthreads();
-        if (t == 0u) s_odd = 0u;
     }
     if (t == 0u) A.run[run_id].odd = run_odd;
 }
