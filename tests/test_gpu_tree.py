@@ -598,3 +598,25 @@ def test_attention_infinities_of_some_of_a_workgroups_tiles(dtype, dim):
     for _ in range(3):
         got = m.tree_attention(**call)
         assert torch.equal(got, want), int((got != want).sum())
+
+
+def test_attention_of_a_slot_that_does_not_exist_behind_infinities():
+    """A workgroup that has met infinities in one sequence's nodes begins the text of the next, whose slot does not exist, and others end it: its rows see nothing, whatever lies behind the table."""
+    m = gc.pkg()
+    n, units = 2002, 9  # (2011 units of 128 positions, four a workgroup of 512: the last text begins in the third of one's, and three workgroups share it)
+    lengths = [i % 61 for i in range(n)] + [128 * units - 1]
+    call, host = attend_case([1] * (n + 1), lengths, 1, 1, 128, 16, BF16, 5)
+    t = host["v"].clone()
+    for s in range(n - 4, n + 1):
+        t[host["table"][s, lengths[s] // 16], lengths[s] % 16, 0, 3] = math.inf
+    call["v"] = t.to(DEV)
+    for slot in (n, n + 1, -1):
+        call["slot"] = torch.arange(n + 1, dtype=torch.int32, device=DEV)
+        call["slot"][n] = slot
+        table = torch.cat([host["table"][:n], host["table"][n:].repeat(2, 1)]).to(DEV)
+        got, lse = m.tree_attention(**{**call, "table": table[:n]}, want_lse=True)
+        assert not got[n].any() and float(lse[n, 0]) == -math.inf
+        assert (got[n - 4:n, 0, 3] == math.inf).all() and torch.isfinite(got[:n - 4]).all() and torch.isfinite(lse[:n]).all()
+    call["slot"] = None
+    got = m.tree_attention(**call)
+    assert (got[n - 4:, 0, 3] == math.inf).all() and torch.isfinite(got[n, 0, 4:]).all()

@@ -700,7 +700,7 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
             r.more = static_cast<uint32_t>(last / S.per - first / S.per);
             r.apart = S.apart;
             r.odd = 0u;
-            r.first = W.first, r.nodes = W.nodes, r.length = W.length, r.total = W.total;
+            r.first = W.first, r.nodes = W.nodes, r.length = length, r.total = total;  // (of a slot that does not exist nothing is there: the join reads no table)
             A.run[run_id] = r;
         }
         at += u1 - u0;

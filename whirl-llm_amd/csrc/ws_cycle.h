@@ -85,7 +85,7 @@ struct AttendArgs {
 // what the join needs of a workgroup: the tile that begins in its run and does not end there (`more` runs behind it, `apart` in number, hold the rest)
 struct AttendRun {
     uint32_t seq, head, tile, more, apart;
-    uint32_t first, nodes, length, total;  // of the sequence, as in AttendWork
+    uint32_t first, nodes, length, total;  // of the sequence: row, nodes, positions before the nodes, all positions (0 where its slot does not exist; length no more than that)
     uint32_t odd;  // bits: whether its first part (of a tile that began before), its last (of the one that begins) has met nodes whose V holds infinities or NaN
 };
 
