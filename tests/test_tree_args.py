@@ -165,3 +165,35 @@ def test_pages_by_hand():
     assert p.fork([0, 0], [1, 3], [6, 8]) == [0, 0] and p.table[1] == [0, 3, -1] and p.table[3] == [0, 1, -1] and p.refs[:4] == [3, 2, 1, 1] and p.copies == [(1, 3, 2)]
     assert p.release([0, 1], [0, 0]) == [0, 0] and p.free == [5, 4, 3] and p.refs[:4] == [1, 1, 1, 0]
     assert p.release([3], [0]) == [0] and p.free == [5, 4, 3, 1, 0]
+
+
+def test_histories_that_are_refused(monkeypatch):
+    """Without slots a sequence's slot is its number: a history of fewer would be read, and written, behind its ends. One on another device would be too."""
+    m = gc.pkg()
+
+    class Reached(Exception):
+        pass
+
+    def library():
+        raise Reached
+    monkeypatch.setattr(m, "_device_of", lambda name, t: -1)  # (host tensors stand for device tensors)
+    monkeypatch.setattr(m, "lib", library)
+    n = 5
+    off, ids, u = torch.arange(n + 1, dtype=torch.int32), torch.zeros(n, dtype=torch.int32), torch.zeros(n, dtype=torch.float64)
+    elsewhere = m.DeviceHistory(n, 8, "cpu")
+
+    class Other:
+        device = "cuda:1"
+        get_device = staticmethod(lambda: 1)
+    elsewhere.n_gen = Other
+    for call in (lambda **c: m.tree_stage(off, n, **c), lambda **c: m.verify_tree(torch.zeros(n, 10), ids, off, u, u, **c)):
+        for slots in (0, 1, n - 1):
+            with pytest.raises(m.WsError, match="slot: missing"):
+                call(hist=m.DeviceHistory(slots, 8, "cpu"))
+        with pytest.raises(m.WsError, match="hist: on"):
+            call(hist=elsewhere)
+        with pytest.raises(m.WsError, match="slot: contiguous"):
+            call(hist=m.DeviceHistory(n, 8, "cpu"), slot=ids[:4])
+        for given in ({}, {"hist": m.DeviceHistory(n, 8, "cpu")}, {"hist": m.DeviceHistory(1, 8, "cpu"), "slot": ids}):
+            with pytest.raises(Reached):
+                call(**given)

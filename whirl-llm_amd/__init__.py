@@ -805,10 +805,19 @@ def _sequences(seq_off):
     return n
 
 
+def _history(hist, slot, n_seq, at):
+    """The sequences' slots of a DeviceHistory, which has to be on device number `at` and to have a slot for each where none are named."""
+    if hist.tokens.get_device() != at or hist.len.get_device() != at or hist.n_gen.get_device() != at:
+        raise WsError(f"hist: on {hist.tokens.device}, not on cuda:{at}")
+    if slot is None and n_seq > hist.len.numel():
+        raise WsError(f"slot: missing, and {n_seq} sequences have a history of {hist.len.numel()} slots")
+    return _vector("slot", slot, _I32, n_seq, at)
+
+
 def tree_stage(seq_off, rows, parent=None, hist=None, slot=None):
     """What a cycle with trees of drafts begins with (ws_tree_stage). seq_off: int32 [n_seq + 1], the nodes of sequence s are the rows seq_off[s] .. seq_off[s + 1] (64 at
-    most), the first of them the root, the token that goes in next; parent: int32 [rows], each node's parent within its sequence (None: chains); hist, slot: a DeviceHistory and the
-    sequences' slots (None: texts of length 0). Returns (mask int64 [rows] = bit j: the row sees node j, position int32 [rows], length int32 [n_seq]), which
+    most), the first of them the root, the token that goes in next; parent: int32 [rows], each node's parent within its sequence (None: chains); hist, slot: a DeviceHistory (None: texts of
+    length 0) and the sequences' slots in it (None: sequence s has slot s). Returns (mask int64 [rows] = bit j: the row sees node j, position int32 [rows], length int32 [n_seq]), which
     tree_attention, the model's positions and PagedCache.keep take."""
     at, n_seq = _device_of("seq_off", seq_off), _sequences(seq_off)
     if not 0 <= rows <= _MOST_ROWS:
@@ -820,7 +829,7 @@ def tree_stage(seq_off, rows, parent=None, hist=None, slot=None):
         mask, position = torch.empty(0, dtype=_I64, device=dev), torch.empty(0, dtype=_I32, device=dev)
     length = torch.empty(n_seq, dtype=_I32, device=dev)
     a = TreeStage(n_seq, rows, _vector("seq_off", seq_off, _I32, n_seq + 1, at), _vector("parent", parent, _I32, rows, at), _p(hist.len) if hist is not None else None,
-                  _vector("slot", slot, _I32, n_seq, at), mask.data_ptr(), position.data_ptr(), length.data_ptr())
+                  _history(hist, slot, n_seq, at) if hist is not None else _vector("slot", slot, _I32, n_seq, at), mask.data_ptr(), position.data_ptr(), length.data_ptr())
     check(lib().ws_tree_stage(_stream(), C.byref(a)), "ws_tree_stage")
     return mask, position, length
 
@@ -842,8 +851,7 @@ def verify_tree(logits, ids, seq_off, u_accept, u_draw, parent=None, q=None, q_o
                    _vector("q_off", _given("q_off", q_off) if q is not None else None, _I32, rows, at), _vector("u_accept", _given("u_accept", u_accept), _F64, rows, at),
                    _vector("u_draw", _given("u_draw", u_draw), _F64, n_seq, at), depth, counts.data_ptr(), path.data_ptr(), counts.data_ptr() + 4 * n_seq, counts.data_ptr() + 8 * n_seq)
     if hist is not None:
-        if slot is not None:
-            _vector("slot", slot, _I32, n_seq, at)
+        _history(hist, slot, n_seq, at)
         a.hist = hist.ref(slot)
     a.spins = spins
     call = lib()
