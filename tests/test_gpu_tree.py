@@ -620,3 +620,26 @@ def test_attention_of_a_slot_that_does_not_exist_behind_infinities():
     call["slot"] = None
     got = m.tree_attention(**call)
     assert (got[n - 4:, 0, 3] == math.inf).all() and torch.isfinite(got[n, 0, 4:]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("dim", [8, 24, 40, 64, 72, 80, 96, 112, 128, 136, 200, 248, 256])
+@pytest.mark.parametrize("heads,n", [(2, 1), (2, 24), (8, 40)])
+def test_attention_keys_that_are_infinite(dtype, dim, heads, n):
+    """A key with -inf where the rows' q is above 0 has the score -inf and weight 0, as if its position were not there: whatever the head's dimensions are filled up with."""
+    m = gc.pkg()
+    call, host = attend_case([n, 1], [150, 40], heads, 2, dim, 1, dtype, dim + n)
+    q, k, table = host["q"].clone(), host["k"].clone(), host["table"].clone()
+    gone = [(0, 3), (0, 77), (0, 149), (0, 150 + n // 2), (1, 0), (1, 39)]
+    for i, (s, p) in enumerate(gone):
+        e = (i * 5 + dim // 3) % dim if i % 2 else i
+        q[..., e] = q[..., e].abs() + 0.25
+        k[table[s, p], 0, :, e] = -math.inf
+        table[s, p] = -1
+    call["q"] = q.to(DEV)
+    host.update(q=q, table=table)
+    for nodes in (0, 1, 64):
+        want = check_attention({**call, "table": table.to(DEV)}, host, max_nodes=nodes)
+        got = m.tree_attention(want_lse=True, max_nodes=nodes, **{**call, "k": k.to(DEV)})
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), (nodes, int((a != b).sum()), int(torch.isnan(a).sum()))

@@ -115,6 +115,8 @@ struct AttendShape {
     static __device__ __forceinline__ uint32_t order(uint32_t token) {
         return (kPieces == 8u ? token & 6u : (token & 7u) << 1) | (token >> 3 & 1u);
     }
+    // the piece of a token that the at-th place holds
+    static __device__ __forceinline__ uint32_t piece(uint32_t at) { return (at % kPieces) ^ order(at / kPieces); }
     static __device__ __forceinline__ uint32_t place(uint32_t token, uint32_t piece) { return token * kRow + (piece ^ order(token)) * 16u; }
 };
 
@@ -286,6 +288,18 @@ __device__ __forceinline__ uint32_t attend_page(const AttendArgs& A, const int32
     return pos < end && at < A.slot_pages ? min(page, A.pages) : A.pages;
 }
 
+// Zeros for K and V behind head_dim, which no load overwrites: q is 0 there, but what memory holds may be infinite, and that times 0 is NaN.
+template <typename H, int DT>
+__device__ __forceinline__ void attend_fill(uint32_t head_dim, unsigned char* buffer) {
+#pragma unroll
+    for (uint32_t l = 0; l < H::kMine; ++l) {
+        const uint32_t at = l * 256u + threadIdx.x;
+        if (H::piece(at) * Mat<DT>::kPer < head_dim) continue;
+        *reinterpret_cast<uint4*>(buffer + at * 16u) = make_uint4(0u, 0u, 0u, 0u);
+        *reinterpret_cast<uint4*>(buffer + H::kBuffer + at * 16u) = make_uint4(0u, 0u, 0u, 0u);
+    }
+}
+
 template <int DT, int DP, int MS, int WM, int OCC>
 __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
     typedef AttendShape<DT, DP, MS, WM> H;
@@ -312,6 +326,12 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
     uint64_t seq_first = F.seq_first;
     AttendWork W = F.work;
 
+    if constexpr (kStaged) {
+        if (A.head_dim < DP) {  // (uniform; the waves meet before they read)
+            attend_fill<H, DT>(A.head_dim, reinterpret_cast<unsigned char*>(s_even));
+            attend_fill<H, DT>(A.head_dim, reinterpret_cast<unsigned char*>(s_odds));
+        }
+    }
     uint32_t turn_odd = 0u;
     for (uint64_t at = S.begin; at < S.end;) {
         while (!S.gang && at - seq_first >= W.all) {
@@ -509,6 +529,11 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
             }
             for (; p0 < p_end; p0 += kStep) {
                 load_v(p0, pg);
+                if (A.head_dim < DP) {  // (uniform) what K is filled up with: 0, as q there is (infinity times 0 would be NaN)
+#pragma unroll
+                    for (uint32_t j = 0; j < kChunks; ++j)
+                        if (j * Mat<DT>::kDepth + g * Mat<DT>::kPer >= A.head_dim) kx[0][j] = kx[1][j] = make_uint4(0u, 0u, 0u, 0u);
+                }
                 // whether all 32 positions are there and every column sees them (uniform)
                 const bool plain = p0 + 32u <= length && static_cast<uint32_t>(have) == 0xffffffffu;
                 const uint32_t here = mine_of(have, 0u);
@@ -530,16 +555,22 @@ __global__ void __launch_bounds__(256, OCC) attend_kernel(AttendArgs A) {
         } else {
             unsigned char* const even = reinterpret_cast<unsigned char*>(s_even);
             unsigned char* const odds = reinterpret_cast<unsigned char*>(s_odds);
-            // 16 bytes a thread, K's and V's pieces in the places that they have in LDS: who loads which is turned about as they lie there
+            // 16 bytes a thread, K's and V's pieces in the places that they have in LDS: who loads which is turned about as they lie there. Behind head_dim nothing is loaded: 0 stays there (attend_fill).
             const uint32_t wave_at = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(wave))) * 1024u;
-            auto fetch = [&](uint32_t p, unsigned char* k_lds) __attribute__((always_inline)) {
+            auto fetch_of = [&](uint32_t p, unsigned char* k_lds, auto all) __attribute__((always_inline)) {
 #pragma unroll
                 for (uint32_t l = 0; l < H::kMine; ++l) {
-                    const uint32_t at = l * 256u + t, token = at / H::kPieces, d = ((at % H::kPieces) ^ H::order(token)) * Mat<DT>::kPer;
-                    const uint32_t page = page_from(pg, token), in = (p + token) & in_page, piece = (d < A.head_dim ? d : 0u) * E / 16u;
+                    const uint32_t token = (l * 256u + t) / H::kPieces, piece = H::piece(l * 256u + t);
+                    const uint32_t page = page_from(pg, token), in = (p + token) & in_page;
+                    if (!all() && piece * Mat<DT>::kPer >= A.head_dim) continue;
                     to_lds(k_base + attend_offset(page, A.k_page, in, A.k_token, piece), k_lds + l * 4096u + wave_at);
                     to_lds(v_base + attend_offset(page, A.v_page, in, A.v_token, piece), k_lds + H::kBuffer + l * 4096u + wave_at);
                 }
+            };
+            // (Two copies: lanes switched off and on around each load cost 5 x 9 nodes over 1001 positions of fp32 18.3 instead of 17.9 us, 2 x 64 over 131072 of bf16 286.8 instead of 285.)
+            auto fetch = [&](uint32_t p, unsigned char* k_lds) __attribute__((always_inline)) {
+                if (A.head_dim == DP) fetch_of(p, k_lds, []() { return true; });  // (uniform)
+                else fetch_of(p, k_lds, []() { return false; });
             };
             // where a lane reads: of K piece 4 j + g of tokens c, of V (turned) 4 elements of token 4 g + c / 4; a token's order is the same 16 behind it
             const uint32_t k_row = c * H::kRow, k_piece = (g ^ H::order(c)) * 16u;
