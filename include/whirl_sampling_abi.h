@@ -736,7 +736,7 @@ typedef struct ws_cache_layer {
  * where a row of sequence s sees the positions below length[s] and its sequence's node j at position length[s] + j where bit j of mask[row] is set (NULL: itself and the nodes before
  * it, a chain's). Whose page holds nothing, or lies past slot_pages, is not seen; nor does what lies in unseen places matter, whatever it is. A row that sees nothing gets zeros and
  * lse -inf. The scores and their sums are held in 32 bits; bf16: p is rounded to bf16 for the product with V (2^-8 a term, of either sign), out once. Results are
- * the same bits on every run. max_nodes: the most nodes of a sequence where the caller knows it (0: not known; a sequence with more is answered all the same).
+ * the same bits on every run. max_nodes: the most nodes of a sequence where the caller knows it (WS_TREE_MAX at most; 0: not known; a sequence with more is answered all the same).
  * workspace: device memory of ws_tree_attention_workspace() bytes, 16-byte aligned, of any contents, nobody else's until the launch is done. Required. */
 typedef struct ws_tree_attention_args {
     ws_cache_layer cache;

@@ -197,3 +197,17 @@ def test_histories_that_are_refused(monkeypatch):
         for given in ({}, {"hist": m.DeviceHistory(n, 8, "cpu")}, {"hist": m.DeviceHistory(1, 8, "cpu"), "slot": ids}):
             with pytest.raises(Reached):
                 call(**given)
+
+
+def test_more_nodes_than_a_tree_has_are_refused(monkeypatch):
+    """Who says that a sequence has more than 64 nodes would get rows that nothing has been written to."""
+    m = gc.pkg()
+    for nodes in (65, 1 << 20, (1 << 32) - 1):
+        assert m.lib().ws_tree_attention(None, C.byref(attention_of(m, max_nodes=nodes)), AT, 1 << 40) == m.E_INVALID
+        assert m.lib().ws_tree_attention_workspace(C.byref(attention_of(m, max_nodes=nodes))) == 0
+    assert m.lib().ws_tree_attention_workspace(C.byref(attention_of(m, max_nodes=64))) > 0
+    monkeypatch.setattr(m, "_device_of", lambda name, t: -1)  # (host tensors stand for device tensors)
+    q, k, ids = torch.zeros(3, 4, 64), torch.zeros(2, 16, 2, 64), torch.zeros(3, dtype=torch.int32)
+    for nodes in (-1, 65, 1 << 33):
+        with pytest.raises(m.WsError, match="max_nodes"):
+            m.tree_attention(q, k, k, ids[:2].view(1, 2), ids[:1], torch.tensor([0, 3], dtype=torch.int32), max_nodes=nodes)

@@ -1378,7 +1378,7 @@ bool attention_ok(const ws_tree_attention_args* a) {
     if (!page_shape_ok(c.dtype, c.pages, c.page_tokens, c.kv_heads, c.head_dim, c.slots, c.slot_pages, c.table_stride) || c.head_dim > 256u) return false;
     if (a->heads == 0 || a->heads > 65535u || a->heads % c.kv_heads != 0 || a->n_seq > kMostTrees || a->rows > kMostTrees) return false;
     if (!(a->scale > 0.f) || a->scale > 1e30f) return false;
-    return true;
+    return a->max_nodes <= WS_TREE_MAX;  // (of more than that the rows behind would be left as they were)
 }
 // columns of a tile that the build is chosen by: those of the largest sequence, or of one as large as they are on average
 uint32_t attention_cols(const ws_tree_attention_args* a) {
