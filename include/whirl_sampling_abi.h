@@ -743,7 +743,7 @@ typedef struct ws_tree_attention_args {
     uint32_t n_seq, rows, heads;
     const void* q;           /* device [rows][heads][head_dim] of dtype */
     uint64_t q_row, q_head;  /* strides, as the cache's */
-    void* out;               /* device [rows][heads][head_dim] of dtype, not over q (several workgroups read a row's) */
+    void* out;               /* device [rows][heads][head_dim] of dtype, no place over another or over q, K or V (between the rows or heads of one stride is fine) */
     uint64_t out_row, out_head;
     float* lse;              /* out, device [rows][heads] (may be NULL) */
     const uint32_t* seq_off; /* device [n_seq + 1] */

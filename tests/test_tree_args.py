@@ -211,3 +211,26 @@ def test_more_nodes_than_a_tree_has_are_refused(monkeypatch):
     for nodes in (-1, 65, 1 << 33):
         with pytest.raises(m.WsError, match="max_nodes"):
             m.tree_attention(q, k, k, ids[:2].view(1, 2), ids[:1], torch.tensor([0, 3], dtype=torch.int32), max_nodes=nodes)
+
+
+BIG = 1 << 30
+
+
+@pytest.mark.parametrize("change", [dict(out=BIG), dict(out=BIG + 16), dict(out=BIG + 3 * 1024), dict(out=BIG - 3 * 1024), dict(out=BIG + 512 * 2 - 16), dict(out=2 * BIG), dict(out=2 * BIG + 40960 - 16), dict(out=2 * BIG - 3 * 1024 - 16),
+                                    dict(out=3 * BIG + 4096), dict(out_row=0), dict(out_head=0), dict(out_row=256), dict(out_row=504), dict(out_head=56), dict(out=BIG + 512, q_row=1024, out_row=1024, out_head=128),
+                                    dict(out=BIG + 1024, q_row=1024, out_row=1032), dict(out=BIG + 128, q_row=1024, q_head=128, out_row=1024, out_head=136)])
+def test_attention_whose_out_lies_over_what_it_reads(change):
+    """q at BIG, K at 2 BIG, V at 3 BIG: out over one of them, or over itself, wherever they begin."""
+    m = gc.pkg()
+    a = attention_of(m, cache=dict(k=2 * BIG, v=3 * BIG), q=BIG, **{**dict(out=4 * BIG), **change})
+    assert m.lib().ws_tree_attention(None, C.byref(a), AT, 1 << 40) == m.E_INVALID
+
+
+@pytest.mark.parametrize("change", [dict(out=4 * BIG), dict(out=BIG + 4 * 1024), dict(out=BIG - 4 * 1024), dict(out=BIG + 1024, q_row=1024, out_row=1024), dict(out=BIG - 1024, q_row=1024, out_row=1024),
+                                    dict(out=BIG + 128, q_row=1024, q_head=128, out_row=1024, out_head=128), dict(out=BIG + 512, q_row=64, q_head=512, out_row=64, out_head=512), dict(out_row=64, out_head=256),
+                                    dict(rows=1, out_row=0), dict(q_row=0, q_head=0), dict(out=BIG + 1024, q_row=2048, out_row=1024, rows=1, n_seq=1)])
+def test_outs_that_lie_apart(change):
+    """out between the rows or the heads of q, before it, behind it: what is missing is the workspace."""
+    m = gc.pkg()
+    a = attention_of(m, cache=dict(k=2 * BIG, v=3 * BIG), q=BIG, **{**dict(out=4 * BIG), **change})
+    assert m.lib().ws_tree_attention(None, C.byref(a), None, 0) == m.E_WORKSPACE

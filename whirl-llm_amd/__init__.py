@@ -881,7 +881,7 @@ def tree_attention(q, k, v, table, length, seq_off, mask=None, slot=None, scale=
     """Attention of trees' rows over one layer of a paged cache (ws_tree_attention). q: [rows, heads, head_dim] float32 / bfloat16; k, v: [pages, page_tokens, kv_heads, head_dim] of its dtype, the
     dimensions in any order in memory but the last (page_tokens a power of two); table: int32 [slots, pages of a slot]; length: int32 [n_seq], the tokens of each sequence before its nodes, which
     lie behind them in the cache; seq_off: as in tree_stage; mask: int64 [rows] (None: chains); slot: int32 [n_seq] (None: sequence s has slot s); scale: None = head_dim ** -0.5. One row a sequence: plain
-    decoding. max_nodes: the most nodes of a sequence (64 at most), where the caller knows it (0: not known). out: where to write (strides in multiples of 16 bytes, not over q); rows behind the last sequence are left as they are.
+    decoding. max_nodes: the most nodes of a sequence (64 at most), where the caller knows it (0: not known). out: where to write (strides in multiples of 16 bytes, not over itself, q, k or v); rows behind the last sequence are left as they are.
     Returns out, or (out, lse float32 [rows, heads]) with want_lse."""
     at, dtype = _device_of("q", q), q.dtype
     if q.dim() != 3 or dtype not in _LOSS_DTYPES:

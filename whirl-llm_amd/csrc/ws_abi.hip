@@ -4,9 +4,11 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include <cstring>
+#include <numeric>
 
 #include "ws_accept.h"
 #include "ws_adjust.h"
@@ -1364,6 +1366,39 @@ bool strides_ok(const void* at, uint32_t each, std::initializer_list<std::pair<u
     }
     return end < (static_cast<unsigned __int128>(1) << 62);
 }
+// Places of `width` bytes each, every dimension a stride of bytes apart (what strides_ok has found to fit 62 bits)
+struct Places {
+    uint64_t at, width, reach;                // reach: bytes from the first to behind the last
+    std::pair<uint64_t, uint64_t> dims[3];    // stride, count; the smallest first, of one place left out
+    uint32_t n = 0;
+    uint64_t inner;                           // the reach of what lies within the largest stride
+    bool apart = true;                        // whether no two overlap, as far as strides that contain one another show it
+    Places(const void* first, uint32_t each, uint32_t elements, std::initializer_list<std::pair<uint64_t, uint64_t>> of)
+        : at(reinterpret_cast<uintptr_t>(first)), width(uint64_t{elements} * each), reach(width), inner(width) {
+        for (const auto& [count, stride] : of)
+            if (count > 1u) dims[n++] = {stride * each, count};
+        std::sort(dims, dims + n);
+        for (uint32_t i = 0; i < n; ++i) {
+            apart = apart && dims[i].first >= reach;
+            inner = reach;
+            reach += (dims[i].second - 1u) * dims[i].first;
+        }
+    }
+};
+// Whether none of the one lies over one of the other: one behind the other, or between the other's, as the halves of rows, or of heads, of one matrix do.
+bool lie_apart(const Places& a, const Places& b) {
+    if (a.at + a.reach <= b.at || b.at + b.reach <= a.at) return true;
+    auto between = [&](uint64_t period, uint64_t of_a, uint64_t of_b) {
+        if (period == 0u) return false;
+        const uint64_t behind = a.at < b.at ? (b.at - a.at) % period : period - 1u - (a.at - b.at - 1u) % period;
+        return behind >= of_a && behind + of_b <= period;
+    };
+    if (a.n && b.n && a.dims[a.n - 1u].first == b.dims[b.n - 1u].first && between(a.dims[a.n - 1u].first, a.inner, b.inner)) return true;
+    uint64_t common = 0;
+    for (const Places* p : {&a, &b})
+        for (uint32_t i = 0; i < p->n; ++i) common = std::gcd(common, p->dims[i].first);
+    return between(common, a.width, b.width);
+}
 bool page_shape_ok(int32_t dtype, uint32_t pages, uint32_t page_tokens, uint32_t kv_heads, uint32_t head_dim, uint32_t slots, uint32_t slot_pages, uint64_t table_stride) {
     if (dtype != WS_DTYPE_F32 && dtype != WS_DTYPE_BF16) return false;
     if (pages == 0 || pages > (1u << 30) || page_tokens == 0 || page_tokens > (1u << 20) || (page_tokens & (page_tokens - 1u)) != 0 || kv_heads == 0 || kv_heads > 65535u) return false;
@@ -1476,13 +1511,11 @@ int ws_tree_attention(void* stream, const ws_tree_attention_args* a, void* works
     if (a->n_seq == 0 || a->rows == 0) return WS_OK;
     const ws_cache_layer& c = a->cache;
     const uint32_t e = static_cast<uint32_t>(elem_bytes(c.dtype));
-    if (!a->q || !a->out || a->out == a->q || !a->seq_off || !a->length || !c.k || !c.v || !c.table || (a->mask && !aligned(a->mask, 8u))) return WS_E_INVALID;
+    if (!a->q || !a->out || !a->seq_off || !a->length || !c.k || !c.v || !c.table || (a->mask && !aligned(a->mask, 8u))) return WS_E_INVALID;
     if (!strides_ok(a->q, e, {{a->rows, a->q_row}, {a->heads, a->q_head}}) || !strides_ok(a->out, e, {{a->rows, a->out_row}, {a->heads, a->out_head}})) return WS_E_INVALID;
     if (!strides_ok(c.k, e, {{c.pages, c.k_page}, {c.page_tokens, c.k_token}, {c.kv_heads, c.k_head}}) ||
         !strides_ok(c.v, e, {{c.pages, c.v_page}, {c.page_tokens, c.v_token}, {c.kv_heads, c.v_head}}))
         return WS_E_INVALID;
-    const ws::AttendPlan plan = attention_plan(a);
-    if (!workspace || workspace_bytes < plan.bytes || !aligned(workspace, 16u)) return WS_E_WORKSPACE;
     ws::AttendArgs g{};
     g.k = static_cast<const unsigned char*>(c.k);
     g.v = static_cast<const unsigned char*>(c.v);
@@ -1491,6 +1524,14 @@ int ws_tree_attention(void* stream, const ws_tree_attention_args* a, void* works
     for (const uint64_t stride : pieces)
         if (stride >> 32) return WS_E_UNSUPPORTED;
     g.k_page = static_cast<uint32_t>(pieces[0]), g.k_token = static_cast<uint32_t>(pieces[1]), g.v_page = static_cast<uint32_t>(pieces[2]), g.v_token = static_cast<uint32_t>(pieces[3]);
+    // (several workgroups read a row's q, and all of them K and V, while others write)
+    const Places out(a->out, e, c.head_dim, {{a->rows, a->out_row}, {a->heads, a->out_head}});
+    if (!out.apart || !lie_apart(out, Places(a->q, e, c.head_dim, {{a->rows, a->q_row}, {a->heads, a->q_head}})) ||
+        !lie_apart(out, Places(c.k, e, c.head_dim, {{c.pages, c.k_page}, {c.page_tokens, c.k_token}, {c.kv_heads, c.k_head}})) ||
+        !lie_apart(out, Places(c.v, e, c.head_dim, {{c.pages, c.v_page}, {c.page_tokens, c.v_token}, {c.kv_heads, c.v_head}})))
+        return WS_E_INVALID;
+    const ws::AttendPlan plan = attention_plan(a);
+    if (!workspace || workspace_bytes < plan.bytes || !aligned(workspace, 16u)) return WS_E_WORKSPACE;
     g.k_head = c.k_head * e, g.v_head = c.v_head * e;
     g.pages = c.pages;
     g.page_shift = shift_of(c.page_tokens);
