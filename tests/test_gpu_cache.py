@@ -299,3 +299,29 @@ def test_cycles_with_trees(dtype):
     one = c.attention(0, q, i32([n - 1]), i32([0, 1]), slot=a)
     two = c.attention(0, q, i32([n - 1]), i32([0, 1]), slot=b)
     assert torch.equal(one, two) and not math.isnan(float(one.float().sum()))
+
+
+def test_autograd_sees_what_is_written():
+    """A backward pass that has kept a cache's K or V refuses to go on once a call has written there; the tables and counts that the calls write have another version, too."""
+    m = gc.pkg()
+    one, two, none = i32([0]), i32([20]), i32([0])
+    calls = {"reserve": lambda c: c.reserve(i32([1]), two), "release": lambda c: c.release(one, none), "fork": lambda c: c.fork(one, i32([1]), i32([5])), "keep": lambda c: c.keep(i32([[3, -1]]), i32([1]), i32([5]))}
+    for name, call in calls.items():
+        c = m.PagedCache.empty(1, 8, 16, 1, 16, 2, 3, dtype=F32)
+        assert c.reserve(one, two).cpu().tolist() == [0]
+        w = torch.ones((), device=DEV, requires_grad=True)
+        kept = [(w * t).sum() for t in (c.k, c.v)]
+        lists = [c.table, c.held, c.refs, c.free, c.n_free]
+        before = [t._version for t in lists]
+        call(c)
+        assert all((t._version > b) == (name != "keep") for t, b in zip(lists, before)), name
+        for y in kept:
+            if name in ("fork", "keep"):
+                with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                    y.backward()
+            else:
+                y.backward()
+    with torch.inference_mode():  # (no versions are counted there)
+        c = m.PagedCache.empty(1, 8, 16, 1, 16, 2, 3, dtype=F32)
+        assert c.reserve(one, two).cpu().tolist() == c.fork(one, i32([1]), i32([5])).cpu().tolist() == c.release(one, none).cpu().tolist() == [0]
+        c.keep(i32([[3, -1], [2, -1]]), i32([1, 1]), i32([5, 0]))

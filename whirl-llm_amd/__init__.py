@@ -882,7 +882,7 @@ def tree_attention(q, k, v, table, length, seq_off, mask=None, slot=None, scale=
     dimensions in any order in memory but the last (page_tokens a power of two); table: int32 [slots, pages of a slot]; length: int32 [n_seq], the tokens of each sequence before its nodes, which
     lie behind them in the cache; seq_off: as in tree_stage; mask: int64 [rows] (None: chains); slot: int32 [n_seq] (None: sequence s has slot s); scale: None = head_dim ** -0.5. One row a sequence: plain
     decoding. max_nodes: the most nodes of a sequence (64 at most), where the caller knows it (0: not known). out: where to write (strides in multiples of 16 bytes, not over itself, q, k or v); rows behind the last sequence are left as they are.
-    Returns out, or (out, lse float32 [rows, heads]) with want_lse."""
+    Returns out, or (out, lse float32 [rows, heads]) with want_lse; autograd records nothing of it, whatever q, k and v ask for: neither has a gradient."""
     at, dtype = _device_of("q", q), q.dtype
     if q.dim() != 3 or dtype not in _LOSS_DTYPES:
         raise WsError("q: [rows, heads, head_dim] float32 / bfloat16 device tensor, unit inner stride")
@@ -955,11 +955,16 @@ class PagedCache:
             raise WsError(f"the cache is on cuda:{self.at}, which is not the current device")
         return n, [_vector(name, _given(name, t), _I32, n, self.at) for name, t in named]
 
+    def _written(self, *tensors):
+        """(a backward pass that has kept them has to see that they are overwritten)"""
+        torch.autograd.graph.increment_version((self.table, self.held, self.refs, self.free, self.n_free, *tensors))
+
     def reserve(self, slot, tokens):
         """Pages for tokens[i] tokens in all for slot[i] (ws_cache_reserve). Returns status."""
         n, at = self._lists(("slot", slot), ("tokens", tokens))
         status = torch.empty_like(slot)
         check(lib().ws_cache_reserve(_stream(), C.byref(self.desc), *at, n, status.data_ptr()), "ws_cache_reserve")
+        self._written()
         return status
 
     def fork(self, src, dst, length):
@@ -967,6 +972,7 @@ class PagedCache:
         n, at = self._lists(("src", src), ("dst", dst), ("length", length))
         status = torch.empty_like(src)
         check(lib().ws_cache_fork(_stream(), C.byref(self.desc), *at, n, status.data_ptr()), "ws_cache_fork")
+        self._written(self.k, self.v)
         return status
 
     def release(self, slot, tokens):
@@ -974,6 +980,7 @@ class PagedCache:
         n, at = self._lists(("slot", slot), ("tokens", tokens))
         status = torch.empty_like(slot)
         check(lib().ws_cache_release(_stream(), C.byref(self.desc), *at, n, status.data_ptr()), "ws_cache_release")
+        self._written()
         return status
 
     def keep(self, path, n_accepted, length, slot=None):
@@ -986,6 +993,7 @@ class PagedCache:
             raise WsError(f"the cache is on cuda:{self.at}, which is not the current device")
         check(lib().ws_cache_keep(_stream(), C.byref(self.desc), _vector("path", path, _I32, path.numel(), self.at), path.shape[1], _vector("n_accepted", n_accepted, _I32, n_seq, self.at),
                                   _vector("length", length, _I32, n_seq, self.at), _vector("slot", slot, _I32, n_seq, self.at), n_seq), "ws_cache_keep")
+        torch.autograd.graph.increment_version((self.k, self.v))
 
     def attention(self, layer, q, length, seq_off, **more):
         """tree_attention over one layer."""
