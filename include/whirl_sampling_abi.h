@@ -462,7 +462,7 @@ int ws_history_stage(void* stream, const ws_history_stage_args* a);
  *   WS_FLAG_APPROX_ENTROPY came out within 2 % of its threshold; WS_ACCEPT_HISTORY_FULL (with WS_ACCEPT_HOST) when the
  *   slot's history has no room for what was accepted.
  * With a history, next and the accepted drafts are appended to the slot, chosen becomes its next and n_gen advances. */
-enum { WS_ACCEPT_OK = 0, WS_ACCEPT_HOST = 1, WS_ACCEPT_NEAR_TYPICAL = 2, WS_ACCEPT_HISTORY_FULL = 4 };
+enum { WS_ACCEPT_OK = 0, WS_ACCEPT_HOST = 1, WS_ACCEPT_NEAR_TYPICAL = 2, WS_ACCEPT_HISTORY_FULL = 4, WS_ACCEPT_PATH_FULL = 8 };
 typedef struct ws_accept {
     const int32_t* token;  /* device [rows]: ws_batch.token of the launch that sampled the verify rows */
     const uint32_t* flags; /* device [rows]: ws_batch.flags of that launch */
@@ -692,7 +692,8 @@ int ws_tree_stage(void* stream, const ws_tree_stage_args* a);
  * With a history, next and the accepted tokens are appended to the slot, chosen becomes its next and n_gen advances, as ws_accept_sampled does.
  * status[s]: WS_ACCEPT_HOST where a row on the walk has nothing that can be drawn (nothing allowed, NaN, an infinite logit, an inv_t that is none) or its q
  * entry lies outside q, or the sequence has no nodes: chosen is -1 then, what was accepted before is reported and the history left as it was;
- * WS_ACCEPT_HISTORY_FULL (with WS_ACCEPT_HOST) where the slot has no room for what was accepted: n_accepted 0, chosen -1.
+ * WS_ACCEPT_HISTORY_FULL (with WS_ACCEPT_HOST) where the slot has no room for what was accepted: n_accepted 0, chosen -1; WS_ACCEPT_PATH_FULL (with WS_ACCEPT_HOST), the same, where
+ * there is a history and `path` has no room for it (more than `depth` were accepted), as ws_cache_keep could not move the others. Without a history n_accepted counts them all.
  * Rows that the walk does not meet do not matter, but may be read. workspace: device memory of ws_verify_tree_workspace() bytes, 8-byte aligned, of any contents, nobody else's
  * until the launch is done (a captured launch may be replayed, whatever others have done there meanwhile); the workgroups meet there. Required where that is not 0. */
 typedef struct ws_verify_tree_args {
@@ -704,7 +705,7 @@ typedef struct ws_verify_tree_args {
     const int32_t* q_off;    /* device [rows]: word of each row's entry (with q) */
     const double* u_accept;  /* device [rows], [0, 1): a root's is not looked at */
     const double* u_draw;    /* device [n_seq], [0, 1) */
-    uint32_t depth;          /* columns of path (1 .. WS_TREE_MAX) */
+    uint32_t depth;          /* columns of path (1 .. WS_TREE_MAX): as many levels as the deepest tree has below its root */
     int32_t* n_accepted;     /* out, device [n_seq] */
     int32_t* path;           /* out, device [n_seq][depth] */
     int32_t* chosen;         /* out, device [n_seq] */
@@ -790,7 +791,8 @@ int ws_cache_fork(void* stream, const ws_cache* c, const int32_t* src, const int
 int ws_cache_release(void* stream, const ws_cache* c, const int32_t* slot, const int32_t* tokens, uint32_t n, int32_t* status);
 /* After ws_verify_tree: in every layer position length[s] + 1 + i of the sequence's slot becomes what position length[s] + path[s][i] holds, i = 0 .. n_accepted[s] - 1 in this order (the
  * root stays where it is), so that the accepted tokens lie behind the text as the history has them. Entries of path from the first on that does not
- * ascend (each is above the one before it, the first above 0) or is not below WS_TREE_MAX are left out, as are positions whose page holds nothing. length: as the cycle began (ws_tree_stage). */
+ * ascend (each is above the one before it, the first above 0) or is not below WS_TREE_MAX are left out, as are positions whose page holds nothing; of more than `depth`
+ * accepted nodes only those that path names are moved (ws_verify_tree's depth should be the deepest tree's). length: as the cycle began (ws_tree_stage). */
 int ws_cache_keep(void* stream, const ws_cache* c, const int32_t* path, uint32_t depth, const int32_t* n_accepted, const uint32_t* length, const uint32_t* slot /* NULL: sequence s has slot s */,
                   uint32_t n_seq);
 

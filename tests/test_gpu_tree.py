@@ -643,3 +643,31 @@ def test_attention_keys_that_are_infinite(dtype, dim, heads, n):
         got = m.tree_attention(want_lse=True, max_nodes=nodes, **{**call, "k": k.to(DEV)})
         for a, b in zip(got, want):
             assert torch.equal(a, b), (nodes, int((a != b).sum()), int(torch.isnan(a).sum()))
+
+
+def test_verify_history_and_a_path_without_room():
+    """With a history a walk that `path` cannot hold is the host's: nothing is appended that the cache could not be brought to. One that fits is appended."""
+    m = gc.pkg()
+    call, _, ids, _ = verify_case([6, 3, 4, 1], 1, 500, F32, 2, guessed=True, chain=True)
+    call["u_accept"][:] = 0.0  # (all are accepted: 5, 2, 3 and none)
+    for depth, n_want, status_want in ((5, [5, 2, 3, 0], [0, 0, 0, 0]), (4, [0, 2, 3, 0], [9, 0, 0, 0]), (2, [0, 2, 0, 0], [9, 0, 9, 0]), (1, [0, 0, 0, 0], [9, 9, 9, 0])):
+        hist = m.DeviceHistory(4, 12, DEV)
+        hist.len[:] = torch.tensor([5, 9, 7, 0], device=DEV, dtype=torch.int32)
+        hist.tokens[:] = 77
+        want = list(status_want)
+        want[1] |= 5 if 9 + 2 + 2 > 12 else 0  # (5 + 5 + 2 tokens fit in 12, 9 + 2 + 2 do not)
+        n = [0 if w else k for w, k in zip(want, n_want)]
+        n_accepted, path, chosen, status, logprob = (t.cpu() for t in m.verify_tree(depth=depth, hist=hist, **call))
+        assert status.tolist() == want and n_accepted.tolist() == n, (depth, status.tolist(), n_accepted.tolist())
+        assert [int(c) < 0 for c in chosen] == [w != 0 for w in want]
+        for s in range(4):
+            assert path[s].tolist() == list(range(1, n[s] + 1)) + [-1] * (depth - n[s])
+            before = [5, 9, 7, 0][s]
+            assert int(hist.len[s]) == before + (0 if want[s] else n[s] + 1) and int(hist.n_gen[s]) == (0 if want[s] else n[s] + 1)
+            first = sum([6, 3, 4, 1][:s])
+            text = [77] * 12
+            if not want[s]:
+                text[before + 1:before + 2 + n[s]] = ids[first + 1:first + 1 + n[s]].tolist() + [int(chosen[s])]
+            assert hist.tokens[s].cpu().tolist() == text
+        n_accepted, path, chosen, status, _ = (t.cpu() for t in m.verify_tree(depth=depth, **call))  # without one: all are counted, the first named
+        assert n_accepted.tolist() == [5, 2, 3, 0] and not status.any() and path[0].tolist() == list(range(1, depth + 1))

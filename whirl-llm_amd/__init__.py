@@ -23,7 +23,7 @@ RNG_SPLITMIX, RNG_PHILOX = 0, 1
 MODE_AUTO, MODE_EXACT, MODE_FUSED = 0, 1, 2
 FLAG_NEAR_TOP_P, FLAG_NEAR_MIN_P, FLAG_NEAR_DRAW = 1, 2, 4
 FLAG_ALL_MASKED, FLAG_OVERFLOW, FLAG_BAD_PARAM, FLAG_OPEN, FLAG_APPROX_ENTROPY = 8, 16, 32, 64, 128
-ACCEPT_OK, ACCEPT_HOST, ACCEPT_NEAR_TYPICAL, ACCEPT_HISTORY_FULL = 0, 1, 2, 4
+ACCEPT_OK, ACCEPT_HOST, ACCEPT_NEAR_TYPICAL, ACCEPT_HISTORY_FULL, ACCEPT_PATH_FULL = 0, 1, 2, 4, 8
 FLAG_NEAR = FLAG_NEAR_TOP_P | FLAG_NEAR_MIN_P | FLAG_NEAR_DRAW
 # which way a row went inside the launch (WS_FLAG_ROUTE_*)
 FLAG_ROUTE_HANDED_BACK, FLAG_ROUTE_EXACT, FLAG_ROUTE_REDONE, FLAG_ROUTE_SPLIT_ALONE, FLAG_ROUTE_LEAN, FLAG_ROUTE_SHORT = 0x100, 0x200, 0x400, 0x800, 0x1000, 0x2000
@@ -838,7 +838,8 @@ def verify_tree(logits, ids, seq_off, u_accept, u_draw, parent=None, q=None, q_o
     """Drafted tokens against the target's probabilities, from given uniforms (ws_verify_tree). logits, inv_t, allow: as in token_logprobs, a row a node; ids int32 [rows]: the drafted tokens;
     seq_off, parent: as in tree_stage. u_accept float64 [rows], u_draw float64 [n_seq]: uniforms from [0, 1). q: the draft distributions' entries, int32 words as draft_sample_rows
     leaves them, and q_off int32 [rows], the word where the entry of a node's children begins (< 0, or q None: the children are guesses, accepted with their own probability).
-    hist, slot: a DeviceHistory and the sequences' slots; what is kept is appended to it. Returns (n_accepted int32 [n_seq], path int32 [n_seq, depth] = the accepted nodes, chosen int32
+    hist, slot: a DeviceHistory and the sequences' slots; what is kept is appended to it. depth: columns of path, as many as the
+    deepest tree has levels below its root (of a longer walk only the first are named; with a history it is the host's, ACCEPT_PATH_FULL). Returns (n_accepted int32 [n_seq], path int32 [n_seq, depth] = the accepted nodes, chosen int32
     [n_seq] = the token drawn behind them, status int32 [n_seq] = ACCEPT_* bits, logprob float32 [n_seq, depth + 1] of the accepted tokens and the chosen one)."""
     r, rows, vocab, at = _loss_rows(logits, _given("ids", ids), inv_t, allow)
     n_seq, dev = _sequences(seq_off), logits.device

@@ -15,6 +15,6 @@ struct HistoryRef {
     uint32_t cap;           // tokens per slot
 };
 
-constexpr uint32_t kAcceptHost = 1u, kAcceptNearTypical = 2u, kAcceptHistoryFull = 4u;
+constexpr uint32_t kAcceptHost = 1u, kAcceptNearTypical = 2u, kAcceptHistoryFull = 4u, kAcceptPathFull = 8u;
 
 }  // namespace ws

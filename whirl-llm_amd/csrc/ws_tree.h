@@ -732,8 +732,10 @@ __global__ void __launch_bounds__(kDrawThreads, WAVES) tree_draw_kernel(TreeVeri
             const uint32_t slot = A.hist.slot ? A.hist.slot[s] : s;
             int32_t* text = A.hist.tokens + static_cast<size_t>(slot) * A.hist.cap;
             const uint32_t len = A.hist.len[slot];
-            if (static_cast<uint64_t>(len) + accepted + 2u > A.hist.cap) {
-                status = kAcceptHistoryFull | kAcceptHost;
+            // (a path without room: the cache could not be brought to what the history would say)
+            const uint32_t full = (static_cast<uint64_t>(len) + accepted + 2u > A.hist.cap ? kAcceptHistoryFull : 0u) | (accepted > A.depth ? kAcceptPathFull : 0u);
+            if (full) {
+                status = full | kAcceptHost;
                 accepted = 0u;
                 chosen = 0xffffffffu;
             } else {
