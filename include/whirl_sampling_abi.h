@@ -757,7 +757,8 @@ typedef struct ws_tree_attention_args {
 uint64_t ws_tree_attention_workspace(const ws_tree_attention_args* a);
 int ws_tree_attention(void* stream, const ws_tree_attention_args* a, void* workspace, uint64_t workspace_bytes);
 
-/* A paged cache of all layers, and what its allocator knows: k and v [layers][pages][page_tokens][kv_heads][head_dim], the dimensions any strides apart as above;
+/* A paged cache of all layers, and what its allocator knows: k and v [layers][pages][page_tokens][kv_heads][head_dim], the dimensions any strides apart as above, a page's tokens 2^34 bytes
+ * at most in each;
  * table as above, held[slot] = the pages of a slot (its first entries; the others are -1), refs[page] = how many slots hold a page, free[0 .. n_free[0]) = the pages that nobody
  * holds, taken from the end. An empty cache: table -1, held 0, refs 0, free every page once. The calls below change these in the order of the stream, each for n sequences
  * (1024 at most, ws_cache_keep any number); they go by what is there as the call begins, and their results do not depend on the order in which the GPU works. status[i]:

@@ -234,3 +234,11 @@ def test_outs_that_lie_apart(change):
     m = gc.pkg()
     a = attention_of(m, cache=dict(k=2 * BIG, v=3 * BIG), q=BIG, **{**dict(out=4 * BIG), **change})
     assert m.lib().ws_tree_attention(None, C.byref(a), None, 0) == m.E_WORKSPACE
+
+
+@pytest.mark.parametrize("change", [dict(page_tokens=1 << 20, kv_heads=128, head_dim=128), dict(kv_heads=65535, head_dim=(1 << 32) - 8, page_tokens=1 << 10), dict(head_dim=1 << 31, page_tokens=4),
+                                    dict(page_tokens=1 << 20, slot_pages=1, table_stride=1, kv_heads=65528, head_dim=256)])
+def test_pages_of_more_pieces_than_32_bits_count(change):
+    m = gc.pkg()
+    lib, c = m.lib(), C.byref(cache_of(m, **{**dict(k_token=0, v_token=0, k_head=0, v_head=0), **change}))
+    assert lib.ws_cache_fork(None, c, AT, AT, AT, 1, AT) == lib.ws_cache_reserve(None, c, AT, AT, 1, AT) == lib.ws_cache_keep(None, c, AT, 3, AT, AT, None, 1) == m.E_INVALID

@@ -1429,6 +1429,7 @@ bool cache_ok(const ws_cache* c) {
     if (!c || !page_shape_ok(c->dtype, c->pages, c->page_tokens, c->kv_heads, c->head_dim, c->slots, c->slot_pages, c->table_stride)) return false;
     if (c->layers == 0 || c->layers > 65535u || !c->k || !c->v || !c->table || !c->held || !c->refs || !c->free || !c->n_free) return false;
     const uint32_t e = static_cast<uint32_t>(elem_bytes(c->dtype));
+    if (static_cast<unsigned __int128>(c->page_tokens) * c->kv_heads * c->head_dim * e > (uint64_t{1} << 34)) return false;  // (a page's pieces of 16 bytes are counted in 32 bits)
     return strides_ok(c->k, e, {{c->layers, c->k_layer}, {c->pages, c->k_page}, {c->page_tokens, c->k_token}, {c->kv_heads, c->k_head}}) &&
            strides_ok(c->v, e, {{c->layers, c->v_layer}, {c->pages, c->v_page}, {c->page_tokens, c->v_token}, {c->kv_heads, c->v_head}});
 }
