@@ -671,3 +671,75 @@ def test_verify_history_and_a_path_without_room():
             assert hist.tokens[s].cpu().tolist() == text
         n_accepted, path, chosen, status, _ = (t.cpu() for t in m.verify_tree(depth=depth, **call))  # without one: all are counted, the first named
         assert n_accepted.tolist() == [5, 2, 3, 0] and not status.any() and path[0].tolist() == list(range(1, depth + 1))
+
+
+EXACT = [  # nodes, lengths, heads, kv heads, dim, page, dtype
+    ([1], [8191], 8, 2, 128, 16, BF16), ([1, 1, 1], [4096, 5003, 129], 32, 8, 128, 16, BF16), ([1], [8001], 4, 1, 64, 64, BF16), ([1], [6000], 4, 2, 256, 16, BF16), ([24], [6001], 4, 2, 128, 32, BF16),
+    ([64, 5], [8200, 3333], 8, 2, 128, 16, BF16), ([64, 64], [16000, 15001], 16, 4, 128, 16, BF16), ([40], [5001], 4, 1, 64, 16, BF16), ([33], [4097], 4, 2, 256, 16, BF16), ([20, 3], [5000, 4500], 8, 2, 80, 1, BF16),
+    ([1], [8000], 8, 2, 64, 16, F32), ([1], [5001], 4, 2, 128, 16, F32), ([1], [4097], 4, 2, 256, 16, F32), ([40, 2], [6001, 40], 4, 1, 64, 16, F32), ([64], [4100], 4, 2, 128, 8, F32), ([9], [3001], 4, 2, 256, 16, F32)]
+
+
+@pytest.mark.parametrize("case", EXACT, ids=[f"{len(c[0])}x{max(c[0])}_{max(c[1])}_{c[2]}h{c[3]}_{c[4]}_{str(c[6])[6:]}" for c in EXACT])
+@pytest.mark.parametrize("mask", ["tree", "any"])
+def test_attention_takes_every_position_once(case, mask):
+    """q = 0, so that every weight is 1 and a row's sums are counts, which 32 bits hold: element d of V is 1 at the positions that are d modulo head_dim, so that one position more or less, of 126
+    at most, shows in bf16 as well; and lse is the logarithm of how many are seen."""
+    m = gc.pkg()
+    counts, lengths, heads, kv_heads, dim, page, dtype = case
+    call, host = attend_case(counts, lengths, heads, kv_heads, dim, page, dtype, 7 * dim + sum(counts), mask=mask)
+    v = host["v"].clone()
+    for s, (n, c) in enumerate(zip(lengths, counts)):
+        p = torch.arange(n + c)
+        pg = host["table"][s, p // page].long()
+        v[pg, p % page] = 0.0
+        for h in range(kv_heads):
+            v[pg, p % page, h, (p + 3 * h) % dim] = 1.0
+    call["v"], call["q"] = v.to(DEV), torch.zeros_like(call["q"])
+    got, lse = (t.cpu().double() for t in m.tree_attention(want_lse=True, **call))
+    G = heads // kv_heads
+    for r, (s, see) in enumerate(tr.visible(lengths, counts, host["masks"])):
+        at = see.nonzero()[:, 0]
+        n = at.numel()
+        for h in range(kv_heads):
+            have = torch.bincount((at + 3 * h) % dim, minlength=dim).double()
+            # 1 / n, its product, and the result: half a step each (2^-24, 2^-24, the type's); a count that is off by one is off by 1 / count
+            tol = have / n * (2.0 ** -23 + tr.HALF[dtype]) * 1.01
+            assert 1.0 / float(have.max()) > 2.0 * 1.01 * (2.0 ** -23 + tr.HALF[dtype])  # (so that it shows, rounded either way)
+            mine = got[r, h * G:(h + 1) * G]
+            assert ((mine - have / n).abs() <= tol).all(), (r, h)
+        # the logarithm to base two by one instruction (a step), its factor and product (half a step each) of a number of 14 at most
+        assert ((lse[r] - math.log(n)).abs() <= 2.0 ** -22 * max(1.0, math.log(n))).all() and 1.0 / n > 2.0 ** -20 * math.log(n), r
+
+
+def test_attention_replayed_with_other_tables_masks_and_offsets():
+    """A captured call: other tables, masks, offsets, lengths and rows than it was captured with, the eager call's answer each time."""
+    m = gc.pkg()
+    cases = [attend_case(c, n, 8, 2, 128, 16, BF16, 70 + i, mask=k)[0] for i, (c, n, k) in enumerate([
+        ([12, 1, 33], [900, 5, 77], "tree"), ([1, 44, 1], [20, 600, 300], "any"), ([20, 20, 6], [0, 1, 850], "tree"), ([46, 0, 0], [910, 3, 3], "any")])]
+    pages, wide = max(c["k"].shape[0] for c in cases), max(c["table"].shape[1] for c in cases)
+    call = dict(q=torch.zeros_like(cases[0]["q"]), k=torch.zeros((pages, 16, 2, 128), dtype=BF16, device=DEV), v=torch.zeros((pages, 16, 2, 128), dtype=BF16, device=DEV), table=torch.full((3, wide), -1, dtype=torch.int32, device=DEV),
+                length=torch.zeros(3, dtype=torch.int32, device=DEV), seq_off=torch.zeros(4, dtype=torch.int32, device=DEV), mask=torch.zeros(46, dtype=torch.int64, device=DEV))
+
+    def put(c):
+        call["table"].fill_(-1)
+        for k, v in c.items():
+            if v is not None:
+                call[k][tuple(slice(0, n) for n in v.shape)].copy_(v)
+    put(cases[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        m.tree_attention(want_lse=True, **call)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = m.tree_attention(want_lse=True, **call)
+    for i in (1, 0, 2, 3, 3, 1, 2, 0):
+        put(cases[i])
+        want = m.tree_attention(want_lse=True, **cases[i])  # (its own table and pages, as wide as they are)
+        for _ in range(3):
+            for t in got:
+                t.fill_(7.0)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), i
