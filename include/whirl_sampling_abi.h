@@ -688,8 +688,9 @@ int ws_tree_stage(void* stream, const ws_tree_stage_args* a);
  * WS_Q_MAX; an id twice counts with both), at word q_off[row] of q. Where q is NULL or q_off[row] < 0 the children are guesses: Q is 1 at the token being looked at.
  * Where no child is accepted, a token is drawn from P: the first in id order up to which P adds up to more than u_draw[s] of its sum; the last with any where there is none.
  *   n_accepted[s], path[s][0 .. n_accepted) = the accepted nodes, -1 behind them (the first `depth` of them), chosen[s] = the token drawn,
- *   logprob[s][0 .. n_accepted] = ln p of the accepted nodes' tokens and of the chosen one, each under its own row's p, 0 behind (the first depth + 1).
- * With a history, next and the accepted tokens are appended to the slot, chosen becomes its next and n_gen advances, as ws_accept_sampled does.
+ *   logprob[s][0 .. n_accepted] = ln p of the accepted nodes' tokens and of the chosen one, each under its own row's p, 0 behind (the first depth + 1). A row's
+ *   sum is added up from powers of 32 bits: off by no more than 2^-21, and by 2^-23 of itself (its own rounding).
+ * With a history (a slot for each sequence, none twice), next and the accepted tokens are appended to the slot, chosen becomes its next and n_gen advances, as ws_accept_sampled does.
  * status[s]: WS_ACCEPT_HOST where a row on the walk has nothing that can be drawn (nothing allowed, NaN, an infinite logit, an inv_t that is none) or its q
  * entry lies outside q, or the sequence has no nodes: chosen is -1 then, what was accepted before is reported and the history left as it was;
  * WS_ACCEPT_HISTORY_FULL (with WS_ACCEPT_HOST) where the slot has no room for what was accepted: n_accepted 0, chosen -1; WS_ACCEPT_PATH_FULL (with WS_ACCEPT_HOST), the same, where
@@ -735,7 +736,7 @@ typedef struct ws_cache_layer {
 /* Attention of the rows of trees over a cache: with `heads` query heads, head h reading kv head h / (heads / kv_heads),
  *   out[row][h] = sum p_t v_t,  p = softmax over the t that the row sees of scale * q[row][h] . k_t,  lse[row][h] = ln sum exp(scale * q . k_t)
  * where a row of sequence s sees the positions below length[s] and its sequence's node j at position length[s] + j where bit j of mask[row] is set (NULL: itself and the nodes before
- * it, a chain's). Whose page holds nothing, or lies past slot_pages, is not seen; nor does what lies in unseen places matter, whatever it is. A row that sees nothing gets zeros and
+ * it, a chain's). Whose page holds nothing, or lies past slot_pages, is not seen; nor does what lies in unseen places matter, whatever it is. A row that sees nothing, or nothing but scores of -inf, gets zeros and
  * lse -inf. The scores and their sums are held in 32 bits; bf16: p is rounded to bf16 for the product with V (2^-8 a term, of either sign), out once. Results are
  * the same bits on every run. max_nodes: the most nodes of a sequence where the caller knows it (WS_TREE_MAX at most; 0: not known; a sequence with more is answered all the same).
  * workspace: device memory of ws_tree_attention_workspace() bytes, 16-byte aligned, of any contents, nobody else's until the launch is done. Required. */
@@ -791,7 +792,7 @@ int ws_cache_fork(void* stream, const ws_cache* c, const int32_t* src, const int
  * back to less than they share is not written to before a fork of its own.) */
 int ws_cache_release(void* stream, const ws_cache* c, const int32_t* slot, const int32_t* tokens, uint32_t n, int32_t* status);
 /* After ws_verify_tree: in every layer position length[s] + 1 + i of the sequence's slot becomes what position length[s] + path[s][i] holds, i = 0 .. n_accepted[s] - 1 in this order (the
- * root stays where it is), so that the accepted tokens lie behind the text as the history has them. Entries of path from the first on that does not
+ * root stays where it is), so that the accepted tokens lie behind the text as the history has them. A slot is named once. Entries of path from the first on that does not
  * ascend (each is above the one before it, the first above 0) or is not below WS_TREE_MAX are left out, as are positions whose page holds nothing; of more than `depth`
  * accepted nodes only those that path names are moved (ws_verify_tree's depth should be the deepest tree's). length: as the cycle began (ws_tree_stage). */
 int ws_cache_keep(void* stream, const ws_cache* c, const int32_t* path, uint32_t depth, const int32_t* n_accepted, const uint32_t* length, const uint32_t* slot /* NULL: sequence s has slot s */,

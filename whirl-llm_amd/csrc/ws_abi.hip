@@ -1325,7 +1325,9 @@ static_assert(WS_CACHE_MOST == ws::kCacheMost && WS_CACHE_MOST == WS_BLOCK);
 
 // The verification's workgroups. A sequence's draw: two a compute unit where sequences are few, of 256 vectors at least; as many as hold the row in registers. A row's decision: shares of
 // 2048 vectors at least, larger ones where there are many rows, so that fewer workgroups begin at the ends of trips to memory. Parts, us: 64 trees of 16 x 151936 bf16 62: 109, 9: 32.0, 7: 29.1, 4: 29.3, 1: 47;
-// 256 of 25 x 50257 fp32, masked, 42: 777, 5: 133, 3: 105, 2: 95.7, 1: 95.4; five rows of 151936 bf16 62: 15.6, 12: 9.7, 9: 9.0, 6: 9.4, 3: 11.8, 1: 20.4. Words: the draw's, the decisions, the rows' sums.
+// 256 of 25 x 50257 fp32, masked, 42: 777, 5: 133, 3: 105, 2: 95.7, 1: 95.4; five rows of 151936 bf16 62: 15.6, 12: 9.7, 9: 9.0, 6: 9.4, 3: 11.8, 1: 20.4. Whole calls in between:
+// 16 rows of it 1: 34, 4: 23.5, 9 (taken): 21.6, 18: 21.4; 64 rows 1: 36, 4: 26.5, 9 (taken): 25.9, 30: 29; 144 1: 54, 7: 32.2, 9 (taken): 32.1, 30: 42; 288 1: 53, 4: 44.5, 9 (taken): 45.6, 18: 52;
+// 384 of 50257 fp32 1: 35, 4: 31, 6 (taken): 34, 13: 43; 768 of 32000 bf16 1 (taken): 29.9, 4: 32, 13: 46. Words: the draw's, the decisions, the rows' sums.
 struct VerifyPlan {
     uint32_t parts, row_parts, levels;
     uint64_t meet, decided, bytes;

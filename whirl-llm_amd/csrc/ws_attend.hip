@@ -26,7 +26,9 @@ constexpr uint32_t kAny = 0xffffffffu;
 // Which build, by the columns of a sequence's kv head: the quickest of those below. us, 16 sequences of 8192 positions, 8 kv heads, four waves apart / one tile of columns / two tiles:
 //   128 bf16: 16 columns 117 / 121 / 141, 20 143 / 121 / 141, 64 205 / 125 / 146, 68 464 / 155 / 146, 256 - / 269 / 202;  64 bf16: 16 52 / 55 / 58, 20 65 / 56 / 59, 64 145 / 56 / 62, 68 209 / 80 / 64
 //   (4 columns of 64 sequences of 2200 59 / 55, of 256 of 1000 116 / 102, of one of 4096 15.2 / 14.7: no waves apart);
-//   256 bf16: 16 192 / 232, 32 210 / 237, 36 529 / 241;  64 fp32: 16 116 / 118 / 182, 32 145 / 167 / 182, 36 299 / 170 / 288, 68 472 / 336 / 293
+//   256 bf16: 16 192 / 232, 32 210 / 237, 36 529 / 241;  64 fp32: 16 116 / 118 / 182, 32 145 / 167 / 182, 36 299 / 170 / 288, 68 472 / 336 / 293;
+//   128 fp32: 4 and 16 columns 189 / 200, 32 268 / 305, 64 - / 315, 4 of one sequence of 4096 24 / 27 (four waves apart take a unit's registers alone: a build more for a twentieth, not kept);
+//   256 fp32: 4 to 16 columns 823 / 701, 32 1469 / 708 (four waves apart spill 275 registers)
 constexpr Build kBuilds[] = {
     build<1, 64, 1, 4, 2>(64), build<1, 64, 2, 4, 2>(kAny),
     build<1, 128, 1, 1, 2>(16), build<1, 128, 1, 4, 2>(64), build<1, 128, 2, 4, 2>(kAny),

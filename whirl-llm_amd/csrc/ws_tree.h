@@ -1,4 +1,4 @@
-// A cycle's drafts as trees: what a row sees and where it stands (tree_stage_kernel), and the drafts' verification against the target's logits (tree_verify_kernel).
+// A cycle's drafts as trees: what a row sees and where it stands (tree_stage_kernel), and the drafts' verification against the target's logits (tree_rows_kernel, tree_draw_kernel).
 //
 // Verification. With w_v = exp((x_v - m) t) over the allowed tokens of a node's row, S = sum w_v and P = w / S, a child with token y is accepted if u Q(y) < P(y); after
 // a rejection P becomes max(P - Q, 0) divided by its sum Z. Q is 0 but at 32 ids at most (or at one, where the child is a guess), so that outside of them P stays w times one number c:
@@ -8,13 +8,13 @@
 // without waiting for each other; nodes are numbered level by level as far as the grid can, and one whose parent has decided against it by then is not read. (A kernel that walked, row after row, waited for memory
 // and for its parts at each: 64 trees of 16 nodes 83 us, 256 of 25 237 us, five rows 40 us.) tree_draw_kernel then goes down the tree along what was decided and draws from the row where
 // that ends, which its workgroups hold in registers.
-// What bounds them is latency (the same three: 29 + 27, 95 + 41, 8 + 12 us): trips to memory one after the other - offsets, decisions, the row, the q entry and its ids' logits, the parts' words -, and workgroups that
-// only find that their node is not needed, 2 ns each; vector units are 40 to 50 % busy, memory is read at 2 to 3 TB/s. (Every workgroup of a sequence going where the walk may come to next, reading
+// What bounds them is latency (the same three: 30 + 26, 96 + 40, 8 + 13 us): trips to memory one after the other - offsets, decisions, the row, the q entry and its ids' logits, the parts' words -, and workgroups that
+// only find that their node is not needed, 2 ns each; vector units are 40 to 65 % busy, memory is read at 2 to 3 TB/s. (Every workgroup of a sequence going where the walk may come to next, reading
 // as it goes, instead of one a node: 37 and 131 us for then 35 and 101.)
 //
 // Accuracy. The comparisons u Q < P are made in 64 bits, S is added up from powers of 32 bits (1e-8 of S where many tokens count): of ten million drafts one may be judged otherwise than by an
 // exact sum. The token behind the walk is looked for among some 100 000 steps of a cumulative sum, whose places would move by 1e-8 of the sum, a hundredth of a step where tokens are
-// unlikely: there the powers are taken in 64 bits (to 1e-12), and S, Z and the P of the listed ids once more from them.
+// unlikely: there the powers are taken in 64 bits (to 1e-11), and S, Z and the P of the listed ids once more from them.
 #pragma once
 
 #include "ws_cycle.h"
@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(64) tree_stage_kernel(TreeStageArgs A) {
     if (A.position) A.position[first + lane] = static_cast<int32_t>(len + __popc(lo) + __popc(hi) - 1u);
 }
 
-// 2^z for z <= 0 to 1e-11: z = k + f, |f| <= 1/2, and of 2^f = e^(f ln 2) the first ten terms of its series (the next is 0.35^10 / 10! = 7e-12). What lies below 2^-2885, -inf too, is 0. Not
+// 2^z for z <= 0 to 1e-11: z = k + f, |f| <= 1/2, and of 2^f = e^(f ln 2) the first ten terms of its series (the next is 0.35^10 / 10! = 7e-12). What lies below 2^-1075, -inf too, is 0 (ldexp; k stays in what it takes as z is cut at -2885). Not
 // for NaN, which is told apart where it is looked for. (k by a sum whose last bit is worth one: of rounding and conversion an instruction takes several times as long.)
 __device__ __forceinline__ double power64(double z) {
     z = fmax(z, -2885.0);
