@@ -986,7 +986,8 @@ class PagedCache:
 
     def keep(self, path, n_accepted, length, slot=None):
         """After verify_tree: the accepted nodes' keys and values, of all layers, move behind the root, where the text goes on (ws_cache_keep). path, n_accepted: verify_tree's; length: int32
-        [n_seq], the tokens before the root (tree_stage's); slot: int32 [n_seq] (None: sequence s has slot s)."""
+        [n_seq], the tokens before the root (tree_stage's); slot: int32 [n_seq] (None: sequence s has slot s), none twice. Of more accepted nodes than path has columns only those that it names
+        are moved."""
         n_seq = n_accepted.numel()
         if path.dim() != 2 or path.shape[0] != n_seq or not 1 <= path.shape[1] <= TREE_MAX or n_seq > _MOST_ROWS:
             raise WsError(f"path: [n_seq, 1 .. {TREE_MAX}] for the n_seq of n_accepted")
